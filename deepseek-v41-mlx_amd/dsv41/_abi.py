@@ -112,10 +112,15 @@ _SIGNATURES = {
                                     _i32, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_indexer_topk_mxq_fp8": [_c_p, _c_p, _c_p, _f32, _c_p, _i64, _c_p, _i64, _i32, _c_p, _c_p, _i32, _i32,
                                    _i32, _i32, _i32, _i32, _i32, _i32, _i32, _c_p, _sz, _c_p],
+    "dsv41_adapter_add_workspace_bytes": [_i64, _i32],
+    "dsv41_adapter_add": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _sz, _i64, _i32, _i32, _i32, _i32, _i32,
+                          _i32, _c_p],
+    "dsv41_cache_move": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _c_p, _c_p, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_version": [],
     "dsv41_last_error_string": [],
 }
 _RESTYPES = {
+    "dsv41_adapter_add_workspace_bytes": _sz,
     "dsv41_sparse_mla_workspace_bytes": _sz,
     "dsv41_linear_rows_workspace_bytes": _sz,
     "dsv41_linear_f32_pair_workspace_bytes": _sz,
@@ -1251,3 +1256,97 @@ def sparse_mla_fp8(q, win_kv, chunk_kv, comp8, comp_scale, scale_rb, n_comp, att
               sc_bstride, scale_rb, _ptr(attn_sink), _ptr(idx), k, _ptr(o), b, n, h, d, window, start_pos,
               float(softmax_scale), *tail)
     return o
+
+
+# ---------------------------------------------------------------------------- adapters
+
+
+def _call_on(device, name: str, *args) -> None:
+    """_call with `device` as the current one: a kernel launches on the current device, whatever stream it is given."""
+    if device.type != "cuda" or torch.cuda.current_device() == device.index:
+        _call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _call(name, *args)
+
+
+def _one_device(name: str, *tensors) -> torch.device:
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: tensors on {device} and {t.device}")
+    return device
+
+
+def _adapter_args(name, x, a, b, scale, ids, n):
+    """Checks one bank (a [slots, rank, k], b [slots, n, rank], scale [slots]) and the sequences' ids against x
+    [sequences, (tokens,) k]; returns (rows, tokens, k, rank, slots)."""
+    _gpu(name, x, a, b, scale, ids)
+    _contig(name, x, a, b, scale, ids)
+    _one_device(name, x, a, b, scale, ids)
+    if x.dim() < 2:
+        raise ValueError(f"{name}: x must be [sequences, (tokens,) channels], got {tuple(x.shape)}")
+    k = x.shape[-1]
+    if a.dim() != 3 or b.dim() != 3 or a.shape[2] != k or b.shape != (a.shape[0], n, a.shape[1]):
+        raise ValueError(f"{name}: a {tuple(a.shape)} and b {tuple(b.shape)} are no adapters of [{n}, {k}]")
+    if a.dtype != x.dtype or b.dtype != x.dtype:
+        raise ValueError(f"{name}: adapters of {a.dtype} and {b.dtype} on x of {x.dtype}")
+    _vec(name, "scale", scale, a.shape[0])
+    if ids.dtype != torch.int32 or ids.shape != (x.shape[0],):
+        raise ValueError(f"{name}: ids must be int32 [{x.shape[0]}], got {ids.dtype} {list(ids.shape)}")
+    rows = x.numel() // k if k else 0
+    return rows, (rows // x.shape[0] if x.shape[0] else 1), k, a.shape[1], a.shape[0]
+
+
+def adapter_add(x, a, b, scale, ids, y, out=None, workspace=None):
+    """y + scale[t] ((x a[t]^T) b[t]^T) with t = ids[sequence] (none outside the slots): dsv41_adapter_add."""
+    name = "dsv41_adapter_add"
+    _gpu(name, y, out)
+    _contig(name, y)
+    rows, tokens, k, rank, slots = _adapter_args(name, x, a, b, scale, ids, y.shape[-1])
+    if y.dtype != x.dtype or y.shape[:-1] != x.shape[:-1] or y.device != x.device:
+        raise ValueError(f"{name}: y {y.dtype} {tuple(y.shape)} does not go with x {x.dtype} {tuple(x.shape)}")
+    out = _out(name, out, y.shape, y.dtype, y.device)
+    if rows == 0:
+        return out
+    need = lib().dsv41_adapter_add_workspace_bytes(rows, rank)
+    ws = _ws(name, workspace, need, x.device)
+    _call_on(x.device, name, _ptr(x), _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), _ptr(y), _ptr(out), _ptr(ws), need, rows,
+             tokens, k, y.shape[-1], rank, slots, dtype_code(x, name), _stream(x))
+    return out
+
+
+# ---------------------------------------------------------------------------- cached sequences
+
+
+def _move_index(name, what, index, device, moves=None):
+    if not isinstance(index, torch.Tensor) or index.dtype != torch.int32 or index.dim() != 1 or not index.is_contiguous():
+        raise ValueError(f"{name}: {what} must be a contiguous int32 vector")
+    if index.device != device or (moves is not None and index.numel() != moves):
+        raise ValueError(f"{name}: {what} must hold {moves if moves is not None else 'the'} moves on {device}")
+
+
+def cache_move(buffers, order, rows, src_rows, dst_rows, same):
+    """dsv41_cache_move over `buffers`: (source tensor, destination tensor, bytes of a sequence, fill word) each, batch
+    first. The caller has checked that a row of either tensor holds that many bytes."""
+    name = "dsv41_cache_move"
+    if not buffers:
+        return
+    device = buffers[0][1].device
+    _move_index(name, "order", order, device)
+    if rows is not None:
+        _move_index(name, "rows", rows, device, order.numel())
+    _gpu(name, order, rows)
+    n = len(buffers)
+    table = (ctypes.c_int64 * (5 * n))()
+    fills = (ctypes.c_uint32 * n)()
+    for i, (s, d, nbytes, fill) in enumerate(buffers):
+        if s.device != device or d.device != device:
+            raise ValueError(f"{name}: buffers on {s.device} and {d.device}")
+        size = s.element_size()
+        table[i], table[n + i] = s.data_ptr(), d.data_ptr()
+        table[2 * n + i], table[3 * n + i], table[4 * n + i] = s.stride(0) * size, d.stride(0) * size, nbytes
+        fills[i] = fill
+    at = ctypes.addressof(table)
+    _call_on(device, name, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n, ctypes.addressof(fills), n,
+             _ptr(order), _ptr(rows), order.numel(), src_rows, dst_rows, int(same), _stream(order))

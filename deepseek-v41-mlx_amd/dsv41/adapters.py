@@ -1,0 +1,92 @@
+"""Low-rank adapters of many sequences beside the shared projections (wq_a, wkv, wq_b and wo_b of
+attention.py:114-122 and :179).
+
+A bank holds the adapters of one projection, one per slot; a call gives every sequence of the batch its own slot, or
+none:
+
+    y = x w^T + scale[t] (x A[t]^T) B[t]^T,   t = ids[sequence], t outside the slots: y = x w^T
+
+``ids`` is an int32 device tensor, read by the kernels, so a captured HIP graph replays with whatever it then holds.
+The rank-wide product and all sums are float32; the result is rounded once where the projection itself runs here, and
+once more where it is torch's (float32 activations, widths the matrix-core kernels do not take, a module with hooks).
+Inference only: a call that autograd would have to follow is refused.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _abi
+from .layers import decode_linear, decode_linear_pair
+
+
+class AdapterBank:
+    """The adapters of one projection: ``a`` [slots, rank, in], ``b`` [slots, out, rank], ``scale`` [slots] float32,
+    all zero (a slot that changes nothing) until loaded. Ranks are stored in multiples of 8, zero padded."""
+
+    def __init__(self, slots: int, in_features: int, out_features: int, rank: int, dtype=torch.bfloat16,
+                 device="cuda"):
+        if slots < 1 or in_features < 1 or out_features < 1 or rank < 1:
+            raise ValueError(f"AdapterBank: slots {slots}, in {in_features}, out {out_features} and rank {rank} must be "
+                             "positive")
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"AdapterBank: dtype {dtype} not supported (float32 or bfloat16)")
+        self.slots, self.in_features, self.out_features, self.rank = slots, in_features, out_features, rank
+        held = -(-rank // 8) * 8
+        self.a = torch.zeros(slots, held, in_features, dtype=dtype, device=device)
+        self.b = torch.zeros(slots, out_features, held, dtype=dtype, device=device)
+        self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
+
+    def _slot(self, slot: int) -> int:
+        if not 0 <= slot < self.slots:
+            raise ValueError(f"AdapterBank: slot {slot} of {self.slots}")
+        return slot
+
+    def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
+        """Puts the adapter a [r, in], b [out, r] (r at most the bank's rank) into a slot."""
+        slot = self._slot(slot)
+        if (a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[1] or a.shape[1] != self.in_features
+                or b.shape[0] != self.out_features or a.shape[0] > self.rank):
+            raise ValueError(f"AdapterBank: a {tuple(a.shape)} and b {tuple(b.shape)} are no adapter of rank at most "
+                             f"{self.rank} of [{self.out_features}, {self.in_features}]")
+        r = a.shape[0]
+        self.a[slot, :r].copy_(a)
+        self.a[slot, r:].zero_()
+        self.b[slot, :, :r].copy_(b)
+        self.b[slot, :, r:].zero_()
+        self.scale[slot] = scale
+
+    def clear(self, slot: int) -> None:
+        """Empties a slot: sequences under it get the plain projection."""
+        slot = self._slot(slot)
+        self.a[slot].zero_()
+        self.b[slot].zero_()
+        self.scale[slot] = 0.0
+
+
+def _check(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank, ids: torch.Tensor) -> None:
+    if (bank.out_features, bank.in_features) != tuple(lin.weight.shape):
+        raise ValueError(f"adapters of [{bank.out_features}, {bank.in_features}] on a projection of "
+                         f"{list(lin.weight.shape)}")
+    if torch.is_grad_enabled() and (x.requires_grad or lin.weight.requires_grad):
+        raise ValueError("adapter projections are not differentiable: call them under torch.no_grad()")
+
+
+def adapter_linear(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank | None, ids: torch.Tensor | None,
+                   wide_only: bool = False) -> torch.Tensor:
+    """lin(x) with every sequence's own adapter: x [sequences, (tokens,) in], ids int32 [sequences]. Without a bank or
+    ids it is decode_linear(lin, x, wide_only)."""
+    if bank is None or ids is None:
+        return decode_linear(lin, x, wide_only)
+    _check(lin, x, bank, ids)
+    y = lin(x)
+    return _abi.adapter_add(x.contiguous(), bank.a, bank.b, bank.scale, ids, y.contiguous())
+
+
+def adapter_linear_pair(lin0: torch.nn.Linear, lin1: torch.nn.Linear, x: torch.Tensor, bank0: AdapterBank | None,
+                        bank1: AdapterBank | None, ids: torch.Tensor | None):
+    """(adapter_linear(lin0, x, bank0, ids), adapter_linear(lin1, x, bank1, ids)); without any bank or ids it is
+    decode_linear_pair."""
+    if ids is None or (bank0 is None and bank1 is None):
+        return decode_linear_pair(lin0, lin1, x)
+    return adapter_linear(lin0, x, bank0, ids), adapter_linear(lin1, x, bank1, ids)

@@ -38,10 +38,14 @@ from __future__ import annotations
 import torch
 
 from . import _abi, fakequant
+from .adapters import AdapterBank, adapter_linear, adapter_linear_pair
 from .compressor import Compressor
 from .config import ModelArgs
 from .indexer import Indexer
-from .layers import RMSNorm, decode_linear, decode_linear_pair, yarn_inv_freqs
+from .layers import RMSNorm, yarn_inv_freqs
+
+# the projections that take low-rank adapters (Attention.add_adapters)
+ADAPTED = ("wq_a", "wkv", "wq_b", "wo_b")
 
 
 # multiply-adds from which fp32 activations take the batched GEMM for wo_a (the release shape
@@ -102,11 +106,23 @@ class Attention(torch.nn.Module):
         self._cos = None
         self._sin = None
         self._workspace = None
+        self.adapters = {}                  # projection name -> AdapterBank (add_adapters)
         self.requires_grad_(False)
 
         # test hooks (negative controls), attention.py:95-97
         self._break_rope_inverse = False
         self._break_sink = False
+
+    def add_adapters(self, slots: int, rank: int, names=ADAPTED) -> dict:
+        """Banks of `slots` empty adapters for the named projections, kept in self.adapters and returned; a forward
+        whose shared.adapter_ids names a slot per sequence applies them."""
+        for name in names:
+            if name not in ADAPTED:
+                raise ValueError(f"adapters go on {ADAPTED}, not on {name!r}")
+        for name in names:
+            w = getattr(self, name).weight
+            self.adapters[name] = AdapterBank(slots, w.shape[1], w.shape[0], rank, w.dtype, w.device)
+        return self.adapters
 
     def _freqs(self, upto: int):
         """Device (cos, sin) tables covering positions < upto; grown geometrically."""
@@ -157,11 +173,16 @@ class Attention(torch.nn.Module):
         cos, sin = self._freqs(end_pos)
         x = x.contiguous()
 
+        # the batch's adapters, one slot (or none) per sequence
+        ids = getattr(shared, "adapter_ids", None)
+        banks = self.adapters if ids is not None else {}
+
         # wq_a and wkv read the same rows: one launch at decode row counts
-        qa, kv_raw = decode_linear_pair(self.wq_a, self.wkv, x)
+        qa, kv_raw = adapter_linear_pair(self.wq_a, self.wkv, x, banks.get("wq_a"), banks.get("wkv"), ids)
         # queries: q's rope tail (attention.py:117) is applied by the attention launch as it loads q
         qr = self.q_norm(qa)
-        q = decode_linear(self.wq_b, qr, wide_only=True).view(bsz, n, self.n_heads, self.head_dim).contiguous()
+        q = adapter_linear(self.wq_b, qr, banks.get("wq_b"), ids, wide_only=True)
+        q = q.view(bsz, n, self.n_heads, self.head_dim).contiguous()
 
         # this chunk's window KV
         kv = self._kv_prologue(kv_raw.contiguous(), cos, sin, start_pos)
@@ -230,7 +251,7 @@ class Attention(torch.nn.Module):
         # grouped block-diagonal wo_a, fp32 sums cast to x's dtype, then wo_b (attention.py:176-179)
         # wo_b at 33-64 rows: 128-row tiles over 4 contraction ranges and their reduce (24.4 + 4.5
         # us at 64 rows against 28.9 us for the library; the 40-layer token 5.748 against 5.78 ms)
-        return decode_linear(self.wo_b, self._wo_a(o.view(bsz, n, -1), x.dtype), wide_only=True)
+        return adapter_linear(self.wo_b, self._wo_a(o.view(bsz, n, -1), x.dtype), banks.get("wo_b"), ids, wide_only=True)
 
     def _wo_a(self, o, out_dtype):
         g, r = self.n_groups, self.o_lora_rank

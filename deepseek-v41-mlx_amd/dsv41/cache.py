@@ -208,3 +208,106 @@ def restore(cache: ModelCache, snap) -> None:
     if eng is not None:
         cache.engram_ids[...] = eng
 
+
+# ---------------------------------------------------------------------------- sequences of a batch
+
+_MINUS_INF = 0xFF800000
+
+
+def _row_buffers(cache: ModelCache, offset: int):
+    """(layer, name, tensor, visible bytes of a sequence, the word an emptied row holds) of every buffer, for `offset`
+    positions: the ring slots and compressed rows written by then and the open group's state."""
+    for i, lc in enumerate(cache.layers):
+        wp = min(offset, lc.window)
+        groups = offset // lc.ratio if lc.is_kv_source else 0
+        blocks = -(-groups // lc.fp8_rb)
+        for name in _BUFFERS:
+            t = getattr(lc, name)
+            if t is None:
+                continue
+            rows = wp if name in ("win_kv", "win_kv8") else blocks if name in ("comp_ks", "index_k8s") else groups
+            if rows > t.shape[1]:
+                raise ValueError(f"layer {i}: {name} holds {t.shape[1]} of the {rows} rows that {offset} positions take")
+            yield i, name, t, rows * t.shape[2] * t.element_size(), 0
+        if lc.comp_state is not None:
+            for name, fill in (("kv_state", 0), ("score_state", _MINUS_INF)):
+                t = getattr(lc.comp_state, name)
+                yield i, name, t, t.shape[1] * t.shape[2] * t.element_size(), fill
+
+
+def _index(what: str, values, rows: int, low: int, device) -> torch.Tensor:
+    """order or rows as an int32 device vector; entries of a host sequence are checked here, those of a device tensor
+    by the kernel."""
+    if isinstance(values, torch.Tensor) and values.is_cuda:
+        return values
+    values = [int(v) for v in values]
+    if any(not low <= v < rows for v in values):
+        raise ValueError(f"{what} must lie in [{low}, {rows}), got {values}")
+    return torch.tensor(values, dtype=torch.int32, device=device)
+
+
+def _batch_rows(what: str, buffers) -> int:
+    n = buffers[0][2].shape[0]
+    for i, name, t, _, _ in buffers:
+        if t.shape[0] != n or t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+            raise ValueError(f"{what}: layer {i}'s {name} {tuple(t.shape)} must be [{n}, rows, channels] with dense rows")
+    return n
+
+
+def _move(what: str, dst: ModelCache, src: ModelCache, order, rows) -> None:
+    same = dst is src
+    theirs = list(_row_buffers(src, src.offset))
+    ours = theirs if same else list(_row_buffers(dst, src.offset))
+    if [(i, n, t.dtype, t.shape[2], w) for i, n, t, w, _ in ours] != [(i, n, t.dtype, t.shape[2], w)
+                                                                     for i, n, t, w, _ in theirs]:
+        raise ValueError(f"{what}: the caches differ in layers, formats or widths")
+    if not same and any(a.ratio != b.ratio or a.window != b.window or a.fp8_rb != b.fp8_rb
+                        for a, b in zip(dst.layers, src.layers)):
+        raise ValueError(f"{what}: the caches differ in ratios, windows or scale blocks")
+    if (dst.engram_ids is None) != (src.engram_ids is None):
+        raise ValueError(f"{what}: one of the caches keeps engram ids")
+    dst_rows = _batch_rows(what, ours)
+    src_rows = dst_rows if same else _batch_rows(what, theirs)
+    device = ours[0][2].device
+    order = _index(f"{what}: order", order, src_rows, -1, device)
+    if rows is not None:
+        rows = _index(f"{what}: rows", rows, dst_rows, 0, device)
+    if rows is None and order.numel() > dst_rows:
+        raise ValueError(f"{what}: {order.numel()} rows into a cache of {dst_rows}")
+    whole = rows is None and order.numel() == dst_rows
+    if dst.offset != src.offset and not whole:
+        raise ValueError(f"{what}: a cache at position {src.offset} gives single rows to one at {dst.offset}")
+    if dst.engram_ids is not None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what}: engram ids live on the host, their order cannot be captured")
+        if src.offset > dst.engram_ids.shape[1]:
+            raise ValueError(f"{what}: {src.offset} positions into engram ids of {dst.engram_ids.shape[1]}")
+    _abi.cache_move([(s[2], d[2], s[3], s[4]) for s, d in zip(theirs, ours)], order, rows, src_rows, dst_rows, same)
+    if dst.engram_ids is not None:         # host memory: this waits for order and rows
+        o = order.cpu().numpy()
+        r = np.arange(len(o)) if rows is None else rows.cpu().numpy()
+        old = src.engram_ids[:, :src.offset].copy()
+        for s, d in zip(o, r):
+            if 0 <= d < dst_rows:
+                dst.engram_ids[d, :src.offset] = old[s] if 0 <= s < src_rows else 0
+    dst.offset = src.offset
+
+
+def reorder_sequences(cache: ModelCache, order, rows=None) -> None:
+    """Sequence rows[i] of the batch (row i without rows) becomes what sequence order[i] was, in every buffer of every
+    layer, in place: beams that follow a survivor, a fork inside the batch, finished sequences' rows filled from the
+    end. All rows are read before any is written. -1 (any order outside the batch) empties the row: its visible part is
+    what a new cache holds. Rows that are not named keep theirs.
+
+    order and rows are int32 device tensors, read by the kernel (a rows entry outside the batch then moves nothing), or
+    host sequences, checked here. Of several moves to one row the last counts. Only what cache.offset positions have
+    written moves; the offset stays."""
+    _move("reorder_sequences", cache, cache, order, rows)
+
+
+def copy_sequences(dst: ModelCache, src: ModelCache, order, rows=None) -> None:
+    """Row rows[i] of dst (row i without rows) becomes sequence order[i] of src, as reorder_sequences moves rows: a
+    prompt computed once and forked into a batch, a sequence admitted into a running batch. Both caches have one
+    configuration and format; batch sizes and capacities may differ. Either both are at one position, or the move names
+    every row of dst (no rows, as many orders as rows) and dst takes src's position."""
+    _move("copy_sequences", dst, src, order, rows)

@@ -12,7 +12,7 @@ from __future__ import annotations
 import torch
 
 from . import _abi
-from .attention import Attention
+from .attention import ADAPTED, Attention
 from .cache import ModelCache
 from .config import ModelArgs
 from .layers import RMSNorm
@@ -32,6 +32,7 @@ class SharedState:
         self.index_src_cache = None
         self.topk_idxs = None
         self.candidates = None
+        self.adapter_ids = None            # the batch's adapter slots, int32 [b] (-1: none)
 
 
 class AttentionStack(torch.nn.Module):
@@ -54,10 +55,16 @@ class AttentionStack(torch.nn.Module):
         return ModelCache(self.args, bsz, max_seq_len, self.dtype if dtype is None else dtype, self.device,
                           index_format, cache_format, fp8_block_rows)
 
-    def forward(self, h: torch.Tensor, cache: ModelCache) -> torch.Tensor:
-        """h [b, n, dim] continues the sequence at cache.offset; advances the cache."""
+    def add_adapters(self, slots: int, rank: int, names=ADAPTED) -> list:
+        """Attention.add_adapters on every layer; the layers' banks."""
+        return [attn.add_adapters(slots, rank, names) for attn in self.layers]
+
+    def forward(self, h: torch.Tensor, cache: ModelCache, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
+        """h [b, n, dim] continues the sequence at cache.offset; advances the cache. adapter_ids [b] int32: every
+        sequence's slot in the layers' adapter banks (-1: none)."""
         start_pos = cache.offset
         shared = SharedState()
+        shared.adapter_ids = adapter_ids
         # each block's residual add is fused with the next block's attn_norm (dsv41_add_rmsnorm):
         # the same two ops, bit for bit, in one pass over h, which is updated in place (a copy of
         # the caller's tensor)
@@ -67,6 +74,7 @@ class AttentionStack(torch.nn.Module):
             use = shared
             if self._break_sharing and not attn.is_kv_source and attn.ratio:
                 use = SharedState()
+                use.adapter_ids = shared.adapter_ids
                 use.kv_src_cache = shared.kv_src_cache
                 use.index_src_cache = shared.index_src_cache
                 use.topk_idxs = (torch.full_like(shared.topk_idxs, -1)

@@ -561,6 +561,39 @@ int dsv41_linear_rows_pair(const void* x, const void* w0, const void* w1, void* 
                            void* workspace, size_t workspace_bytes, int32_t rows, int32_t k, int32_t n0,
                            int32_t n1, int32_t splits, int32_t dtype, hipStream_t stream);
 
+/* ---------------------------------------------------------------- adapters --
+ * Low-rank adapters of many sequences beside one shared projection (nn.Linear, y = x @ w^T). Row m of
+ * x [rows, k] belongs to sequence m / tokens, whose adapter is t = ids[m / tokens] (int32 on the
+ * device, rows / tokens of them). For t in [0, slots):
+ *   y[m] = x[m] @ w^T + scale[t] * ((x[m] @ a[t]^T) @ b[t]^T),   a [slots, rank, k], b [slots, n, rank],
+ * and y[m] = x[m] @ w^T for any other t (-1: no adapter), whatever the slots hold. Sums and the
+ * rank-wide intermediate are fp32, in a fixed order: deterministic.
+ */
+
+/* The adapters' part on top of a projection already computed: out = y + scale (x a^T) b^T, y and out
+ * [rows, n] in dtype (F32 or BF16; y == out allowed); any k, n and rank. */
+size_t dsv41_adapter_add_workspace_bytes(int64_t rows, int32_t rank);
+int dsv41_adapter_add(const void* x, const void* a, const void* b, const float* scale, const int32_t* ids,
+                      const void* y, void* out, void* workspace, size_t workspace_bytes, int64_t rows,
+                      int32_t tokens, int32_t k, int32_t n, int32_t rank, int32_t slots, int32_t dtype,
+                      hipStream_t stream);
+
+/* ---------------------------------------------------------------- cached sequences --
+ */
+
+/* Moves of sequences (batch rows) between the buffers of one cache or of two: for each move i < moves,
+ * row rows[i] (rows NULL: row i) of every destination buffer takes the first bytes[b] bytes of row
+ * order[i] of its source buffer. Every row is read before any is written, so src and dst may be the
+ * same buffers (same != 0 says so: a row onto itself is left alone). An order entry outside
+ * [0, src_rows) empties the row: its bytes[b] bytes become the word fill[b] (low byte first). A rows
+ * entry outside [0, dst_rows) moves nothing; of several moves to one row the last counts. order and
+ * rows: int32 on the device. src, dst, the strides (bytes between sequences), bytes and fill: host
+ * arrays of `buffers` entries, read during the call. moves and dst_rows at most 4,096. */
+int dsv41_cache_move(const void* const* src, void* const* dst, const int64_t* src_stride,
+                     const int64_t* dst_stride, const int64_t* bytes, const uint32_t* fill, int32_t buffers,
+                     const int32_t* order, const int32_t* rows, int32_t moves, int32_t src_rows,
+                     int32_t dst_rows, int32_t same, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
