@@ -54,6 +54,410 @@ __global__ __launch_bounds__(256) void adapter_expand_plain_kernel(const T* y, c
   io<T>::st(out + i, fmaf(scale[t], s, io<T>::ld(y + i)));
 }
 
+// ------------------------------------------------------------------ matrix cores (bf16)
+
+// One projection's adapters as the kernels see them.
+struct Bank {
+  const bf16_t* a;       // [slots, rank, k]
+  const bf16_t* b;       // [slots, n, rank]
+  const float* scale;    // [slots]
+  float* h;              // x A^T per contraction chunk: [chunks, rows, rank]
+  int rank, slots;       // rank a multiple of 8, at most kMaxRank; slots 0: no bank
+};
+
+constexpr int kMaxRank = 128;
+
+struct AdapterArgs {
+  WoaArgs t;             // the projection itself: split form, t.groups contraction ranges of t.d channels, weight rows
+                         // [t.r0, t.r) in t.w1 when there are two; t.out: float32 parts or the result
+  Bank bank[2];          // of weight rows [0, t.r0) and [t.r0, t.r)
+  const int32_t* ids;    // [rows / tokens]
+  int tokens, k;
+  int chunk, chunks;     // channels of one partial h, and how many
+  bf16_t* y;             // [rows, t.r0]
+  bf16_t* y1;            // [rows, t.r - t.r0]
+};
+
+// The adapter of row m: -1 for none.
+__device__ __forceinline__ int row_adapter(const AdapterArgs& a, const Bank& bk, int m) {
+  const int t = m < a.t.rows ? a.ids[m / a.tokens] : -1;
+  return (uint32_t)t < (uint32_t)bk.slots ? t : -1;
+}
+
+// The next adapter that occurs in a tile of 16 rows (lane l holds row l % 16's): takes its rows out of `todo`.
+__device__ __forceinline__ int next_adapter(uint32_t& todo, int id) {
+  const int t = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
+  todo &= ~(uint32_t)__ballot(id == t);
+  return t;
+}
+
+// Partial x A^T of 16 rows, one chunk of channels, 16 ranks: the chunk's 32-channel steps in turn over the workgroup's
+// four waves. Rows are the MFMA's columns, so every adapter of the tile multiplies all 16 of them and each lane keeps
+// the product with its own row's: nothing another row's adapter holds can reach it. Up to U adapters at once keep that
+// many loads in flight.
+template <int U>
+__device__ __forceinline__ void shrink_steps(const bf16_t* xp, const bf16_t* const (&ap)[U], int first, int steps,
+                                             f32x4 (&acc)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s = first; s < steps; s += 4) {
+    const bf16x8 xf = ld_bf16x8(xp + 32 * s);
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc[u] = mfma16x16x32(ld_bf16x8(ap[u] + 32 * s), xf, acc[u]);
+  }
+  settle(acc);
+}
+
+__device__ __forceinline__ int shrink_items(const AdapterArgs& a, const Bank& bk) {
+  return bk.slots ? (a.t.rows + 15) / 16 * a.chunks * ((bk.rank + 15) / 16) : 0;
+}
+
+__device__ __forceinline__ void shrink_item(const AdapterArgs& a, const Bank& bk, int item, float* red) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int ranks = (bk.rank + 15) / 16;
+  const int rq = item % ranks, chunk = item / ranks % a.chunks, tile = item / ranks / a.chunks;
+  const int id = row_adapter(a, bk, tile * 16 + l16);
+  const int k0 = chunk * a.chunk, steps = min(a.chunk, a.k - k0) / 32;
+  const bf16_t* xp = a.t.o + (int64_t)min(tile * 16 + l16, a.t.rows - 1) * a.k + k0 + 8 * g;
+  const int64_t arow = (int64_t)min(rq * 16 + l16, bk.rank - 1) * a.k + k0 + 8 * g;   // ranks past the end: not stored
+  const int64_t slot = (int64_t)bk.rank * a.k;
+  f32x4 res = {0.f, 0.f, 0.f, 0.f};
+  uint32_t todo = (uint32_t)__ballot(id >= 0) & 0xFFFFu;
+  while (todo) {
+    int t[4];
+    t[0] = next_adapter(todo, id);
+    if (todo == 0) {
+      f32x4 acc[1];
+      const bf16_t* const ap[1] = {bk.a + t[0] * slot + arow};
+      shrink_steps<1>(xp, ap, wave, steps, acc);
+      res = id == t[0] ? acc[0] : res;
+      break;
+    }
+#pragma unroll
+    for (int u = 1; u < 4; ++u) t[u] = todo ? next_adapter(todo, id) : t[0];
+    f32x4 acc[4];
+    const bf16_t* const ap[4] = {bk.a + t[0] * slot + arow, bk.a + t[1] * slot + arow, bk.a + t[2] * slot + arow,
+                                 bk.a + t[3] * slot + arow};
+    shrink_steps<4>(xp, ap, wave, steps, acc);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) res = id == t[u] ? acc[u] : res;
+  }
+  // the four waves' sums, in order; lane (g, l16) holds ranks 4 g .. 4 g + 3 of row l16
+  *reinterpret_cast<f32x4*>(red + (wave * 16 + l16) * 16 + 4 * g) = res;
+  __syncthreads();
+  const int row = threadIdx.x >> 4, r = rq * 16 + (threadIdx.x & 15), m = tile * 16 + row;
+  if (m < a.t.rows && r < bk.rank) {
+    float s = red[threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) s += red[w * 256 + threadIdx.x];
+    bk.h[((int64_t)chunk * a.t.rows + m) * bk.rank + r] = s;
+  }
+  __syncthreads();
+}
+
+__global__ __launch_bounds__(256) void adapter_shrink_kernel(AdapterArgs a) {
+  __shared__ __align__(16) float red[4 * 256];
+  shrink_item(a, a.bank[0], blockIdx.x, red);
+}
+
+// acc[i] += scale (h B^T) for 16 rows (lane l16's, adapter id) and WR tiles of 16 output columns from col on. hval(c, v)
+// gives scale times ranks 8 c .. 8 c + 7 of the lane's row. They go into the MFMA as the sum of two bf16 values - the
+// upper 8 bits, cut off, and the next 8, rounded - so that 16 bits of the intermediate count (2^-17 of it is lost, far
+// below the result's own rounding); each is multiplied with the same bf16 B, exactly. An infinite value has no lower
+// part. Rows are columns of the MFMA again: every adapter of the tile multiplies all of them, each lane keeps its own.
+template <int WR, typename H>
+__device__ __forceinline__ void expand_tile(f32x4 (&acc)[WR], const Bank& bk, int n, int col, int id, H hval) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int r8 = bk.rank >> 3;
+  uint32_t todo = (uint32_t)__ballot(id >= 0) & 0xFFFFu;
+  while (todo) {
+    const int t = next_adapter(todo, id);
+    const bf16_t* bp = bk.b + ((int64_t)t * n + col + l16) * bk.rank;
+    f32x4 sum[WR];
+#pragma unroll
+    for (int i = 0; i < WR; ++i) sum[i] = acc[i];
+    for (int q = 0; q < 2 * r8; q += 4) {
+      const int s = q + g;                             // upper parts of the rank chunks, then lower parts
+      const bool live = s < 2 * r8, low = s >= r8;
+      const int c = live ? (low ? s - r8 : s) : 0;
+      float v[8];
+      hval(c, v);
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t u0 = __float_as_uint(v[2 * e]), u1 = __float_as_uint(v[2 * e + 1]);
+        const uint32_t h0 = u0 & 0xFFFF0000u, h1 = u1 & 0xFFFF0000u;
+        const float l0 = h0 << 1 == 0xFF000000u ? 0.0f : v[2 * e] - __uint_as_float(h0);
+        const float l1 = h1 << 1 == 0xFF000000u ? 0.0f : v[2 * e + 1] - __uint_as_float(h1);
+        w[e] = low ? pack2_bf16(l0, l1) : (h0 >> 16) | h1;
+        if (!live) w[e] = 0u;
+      }
+      const bf16x8 hf = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
+#pragma unroll
+      for (int i = 0; i < WR; ++i) {
+        uint4 b = *reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank + 8 * c);
+        if (!live) b = make_uint4(0, 0, 0, 0);
+        sum[i] = mfma16x16x32(as_bf16x8(b), hf, sum[i]);
+      }
+    }
+    settle(sum);
+#pragma unroll
+    for (int i = 0; i < WR; ++i) acc[i] = id == t ? sum[i] : acc[i];
+  }
+}
+
+// The projection's tiles. DIRECT: the adapters' part is added to the float32 sums in registers and the result stored,
+// rounded once (h complete before the launch). Else the sums of one contraction range go to t.out in float32, and the
+// workgroups also compute h, each its share while its first copies are on their way.
+template <int WR, int WM, int GR, int GM, int BK, int NS, bool DIRECT>
+__global__ __launch_bounds__(64 * GR * GM, (TileCfg<WR, WM, GR, GM, BK, NS>::LDS <= 72 * 1024) ? 2 : 1) void
+adapter_tiles_kernel(AdapterArgs a) {
+  using C = TileCfg<WR, WM, GR, GM, BK, NS>;
+  __shared__ __align__(16) uint8_t lds[C::LDS];
+  const int mtiles = (a.t.rows + C::TM - 1) / C::TM, rtiles = a.t.r / C::TR;
+  // consecutive tiles on one XCD, the weight tile fastest, as the output projection's
+  const int total = (int)gridDim.x;
+  const int tile = total % 8 ? (int)blockIdx.x : ((int)blockIdx.x % 8) * (total / 8) + (int)blockIdx.x / 8;
+  const int rt = tile % rtiles, mt = (tile / rtiles) % mtiles, grp = tile / (rtiles * mtiles);
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wr = (wave % GR) * 16 * WR, wm = (wave / GR) * 16 * WM;   // this wave's block
+  f32x4 acc[WR][WM];
+  if constexpr (DIRECT) {
+    tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc);
+#pragma unroll
+    for (int i = 0; i < WR; ++i) settle(acc[i]);
+    const Bank& bk = a.bank[0];
+    const int col = rt * C::TR + wr;
+#pragma unroll
+    for (int j = 0; j < WM; ++j) {
+      const int m = mt * C::TM + wm + 16 * j + l16;
+      const int id = row_adapter(a, bk, m);
+      const float scale = id < 0 ? 0.0f : bk.scale[id];
+      const float* hp = bk.h + (int64_t)min(m, a.t.rows - 1) * bk.rank;
+      f32x4 s[WR];
+#pragma unroll
+      for (int i = 0; i < WR; ++i) s[i] = acc[i][j];
+      expand_tile<WR>(s, bk, a.t.r, col, id, [&](int c, float* v) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+        for (int p = 0; p < a.chunks; ++p) {
+          const f32x4* from = reinterpret_cast<const f32x4*>(hp + (int64_t)p * a.t.rows * bk.rank + 8 * c);
+          const f32x4 v0 = from[0], v1 = from[1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            v[e] += v0[e];
+            v[4 + e] += v1[e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= scale;
+      });
+      if (m < a.t.rows)
+#pragma unroll
+        for (int i = 0; i < WR; ++i) store4<bf16_t>(a.y + (int64_t)m * a.t.r + col + 16 * i + 4 * g, s[i]);
+    }
+  } else {
+    static_assert(GR * GM == 4, "a partial h is the work of four waves");
+    __shared__ __align__(16) float red[4 * 256];
+    tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc, [&]() {
+      const int items0 = shrink_items(a, a.bank[0]), items = items0 + shrink_items(a, a.bank[1]);
+      for (int it = blockIdx.x; it < items; it += total)
+        if (it < items0) shrink_item(a, a.bank[0], it, red);
+        else shrink_item(a, a.bank[1], it - items0, red);
+      // the ring's waits count its own copies only
+      if ((int)blockIdx.x < items) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    });
+    const int64_t ostride = (int64_t)a.t.groups * a.t.r;
+    float* out = reinterpret_cast<float*>(a.t.out);
+#pragma unroll
+    for (int j = 0; j < WM; ++j) {
+      const int m = mt * C::TM + wm + 16 * j + l16;
+      if (m >= a.t.rows) continue;
+#pragma unroll
+      for (int i = 0; i < WR; ++i)
+        store4<float>(out + m * ostride + (int64_t)grp * a.t.r + rt * C::TR + wr + 16 * i + 4 * g, acc[i][j]);
+    }
+  }
+}
+
+// The contraction ranges' parts summed in order, plus the adapters' part, rounded once: a workgroup per 16 rows and
+// 64 WR columns, a wave per 16 WR of them. h is summed over its chunks into LDS first.
+template <int WR>
+__global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
+  constexpr int kStride = kMaxRank + 4;
+  __shared__ __align__(16) float hs[2][16 * kStride];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int ctiles = (a.t.r + 64 * WR - 1) / (64 * WR);
+  const int col0 = (int)(blockIdx.x % ctiles) * 64 * WR, m0 = (int)(blockIdx.x / ctiles) * 16;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const Bank& bk = a.bank[s];
+    if (bk.slots == 0 || (s == 0 ? col0 >= a.t.r0 : col0 + 64 * WR <= a.t.r0)) continue;
+    for (int i = threadIdx.x; i < 16 * bk.rank; i += 256) {
+      const int row = i / bk.rank, r = i - row * bk.rank, m = m0 + row;
+      const int id = row_adapter(a, bk, m);
+      float v = 0.0f;
+      if (id >= 0) {
+        const float* hp = bk.h + (int64_t)m * bk.rank + r;
+        for (int p = 0; p < a.chunks; ++p) v += hp[(int64_t)p * a.t.rows * bk.rank];
+        v *= bk.scale[id];
+      }
+      hs[s][row * kStride + r] = v;
+    }
+  }
+  __syncthreads();
+  const int m = m0 + l16, col = col0 + wave * 16 * WR;
+  const float* part = reinterpret_cast<const float*>(a.t.out) + (int64_t)min(m, a.t.rows - 1) * a.t.groups * a.t.r + 4 * g;
+#pragma unroll
+  for (int i0 = 0; i0 < WR; ++i0) {
+    // 16 columns at a time where a wave's block may end or cross from the first projection to the second
+    constexpr int kOne = 1;
+    const int c = col + 16 * i0;
+    if (c >= a.t.r) continue;
+    f32x4 acc[kOne];
+    acc[0] = *reinterpret_cast<const f32x4*>(part + c);
+    for (int p = 1; p < a.t.groups; ++p) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(part + (int64_t)p * a.t.r + c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[0][e] = acc[0][e] + v[e];
+    }
+    const int s = c >= a.t.r0, n = s ? a.t.r - a.t.r0 : a.t.r0, at = s ? c - a.t.r0 : c;
+    const Bank& bk = a.bank[s];
+    if (bk.slots)
+      expand_tile<kOne>(acc, bk, n, at, row_adapter(a, bk, m), [&](int c8, float* v) {
+        const float* from = hs[s] + l16 * kStride + 8 * c8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = from[e];
+      });
+    if (m < a.t.rows) store4<bf16_t>((s ? a.y1 : a.y) + (int64_t)m * n + at + 4 * g, acc[0]);
+  }
+}
+
+// ------------------------------------------------------------------ plan
+
+enum AdapterTile { kRows32, kRows64, kRows64Deep, kRows96, kRows128, kWide128, kWide160, kTile256, kTile128, kTile128Deep,
+                   kTile64, kTile32 };
+
+struct AdapterPlan {
+  AdapterTile tile;
+  int tr, tm;            // the tile's weight rows and query rows
+  int splits;            // contraction ranges; 1 with direct
+  bool direct;
+  int chunk, chunks;
+};
+
+// Ranges for decode row counts, by the rule of the decode-row projections: at 33-64 rows the ranges whose wide tiles
+// make the most workgroups when some do, otherwise the most that keep n / 32 x ranges workgroups within 256.
+static int decode_splits(int rows, int k, int n) {
+  int best = 0;
+  int64_t most = 0;
+  for (int s = 1; s <= 64; ++s) {
+    if (k % (64 * s)) continue;
+    const int tr = wide_split_tile(rows, k / s, n, s);
+    if (tr && (int64_t)(n / tr) * s >= most) {
+      most = (int64_t)(n / tr) * s;
+      best = s;
+    }
+  }
+  if (best) return best;
+  best = 1;
+  for (int s = 1; s <= 64; ++s)
+    if (k % (64 * s) == 0 && (int64_t)(n / 32) * s <= 256) best = s;
+  return best;
+}
+
+// n0: weight rows of the first of two projections (n of one).
+static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
+  AdapterPlan p;
+  p.splits = 1;
+  p.direct = false;
+  if (rows <= 128) {
+    p.splits = decode_splits(rows, k, n);
+    const int wide = wide_split_tile(rows, k / p.splits, n, p.splits);
+    if (wide && n0 % wide == 0) {
+      p.tile = wide == 160 ? kWide160 : kWide128;
+      p.tr = wide;
+      p.tm = 64;
+    } else {
+      const int q = (rows + 31) / 32;
+      p.tile = q == 1 ? kRows32 : q == 2 ? ((int64_t)(n / 32) * p.splits > 256 ? kRows64 : kRows64Deep) : q == 3 ? kRows96 : kRows128;
+      p.tr = 32;
+      p.tm = 32 * q;
+    }
+    p.chunk = 256;
+  } else {
+    auto tiles = [&](int tr, int tm) { return n % tr ? 0 : (int64_t)(n / tr) * ((rows + tm - 1) / tm); };
+    p.tm = 128;
+    if (tiles(256, 256) >= 192) {
+      p.tile = kTile256;
+      p.tr = p.tm = 256;
+    } else if (tiles(128, 128) > 256) {
+      p.tile = kTile128;
+      p.tr = 128;
+    } else if (n % 128 == 0) {
+      p.tile = kTile128Deep;
+      p.tr = 128;
+    } else if (n % 64 == 0) {
+      p.tile = kTile64;
+      p.tr = 64;
+    } else {
+      p.tile = kTile32;
+      p.tr = 32;
+    }
+    const int64_t t = tiles(p.tr, p.tm);
+    for (int s = 2; s <= 16; ++s)
+      if (t * s <= 256 && k % (64 * s) == 0 && k / s >= 256) p.splits = s;
+    p.direct = p.splits == 1;
+    // partial h: enough workgroups to fill the chip, at most 8 of them for the next kernel to sum
+    const int64_t items = (int64_t)((rows + 15) / 16) * ((rank + 15) / 16);
+    const int parts = (int)(items >= 768 ? 1 : (768 + items - 1) / items > 8 ? 8 : (768 + items - 1) / items);
+    p.chunk = ((k + parts - 1) / parts + 127) / 128 * 128;
+  }
+  p.chunks = (k + p.chunk - 1) / p.chunk;
+  return p;
+}
+
+static size_t pad256(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+
+static size_t plan_bytes(const AdapterPlan& p, int rows, int n, int rank0, int rank1) {
+  const size_t parts = p.direct ? 0 : (size_t)rows * p.splits * n * sizeof(float);
+  return pad256(parts) + pad256((size_t)p.chunks * rows * rank0 * sizeof(float)) +
+         pad256((size_t)p.chunks * rows * rank1 * sizeof(float));
+}
+
+template <int WR, int WM, int GR, int GM, int BK, int NS, bool DIRECT>
+static void launch_adapter_tiles(const AdapterArgs& a, int64_t tiles, hipStream_t stream) {
+  hipLaunchKernelGGL((adapter_tiles_kernel<WR, WM, GR, GM, BK, NS, DIRECT>), dim3((unsigned)tiles), dim3(64 * GR * GM), 0,
+                     stream, a);
+}
+
+static void launch_projection(const AdapterArgs& a, const AdapterPlan& p, hipStream_t stream) {
+  const int64_t tiles = (int64_t)(a.t.r / p.tr) * ((a.t.rows + p.tm - 1) / p.tm) * p.splits;
+  switch (p.tile) {
+    case kRows32: launch_adapter_tiles<1, 1, 2, 2, 64, 8, false>(a, tiles, stream); break;
+    case kRows64: launch_adapter_tiles<1, 2, 2, 2, 64, 6, false>(a, tiles, stream); break;
+    case kRows64Deep: launch_adapter_tiles<1, 2, 2, 2, 64, 8, false>(a, tiles, stream); break;
+    case kRows96: launch_adapter_tiles<1, 3, 2, 2, 64, 8, false>(a, tiles, stream); break;
+    case kRows128: launch_adapter_tiles<1, 4, 2, 2, 64, 4, false>(a, tiles, stream); break;
+    case kWide128: launch_adapter_tiles<4, 2, 2, 2, 64, 4, false>(a, tiles, stream); break;
+    case kWide160: launch_adapter_tiles<5, 2, 2, 2, 64, 4, false>(a, tiles, stream); break;
+    case kTile256: launch_adapter_tiles<8, 4, 2, 4, 64, 2, true>(a, tiles, stream); break;
+    case kTile128: launch_adapter_tiles<4, 4, 2, 2, 64, 2, true>(a, tiles, stream); break;
+    case kTile128Deep:
+      if (p.direct) launch_adapter_tiles<4, 4, 2, 2, 64, 4, true>(a, tiles, stream);
+      else launch_adapter_tiles<4, 4, 2, 2, 64, 4, false>(a, tiles, stream);
+      break;
+    case kTile64:
+      if (p.direct) launch_adapter_tiles<2, 4, 2, 2, 64, 3, true>(a, tiles, stream);
+      else launch_adapter_tiles<2, 4, 2, 2, 64, 3, false>(a, tiles, stream);
+      break;
+    case kTile32:
+      if (p.direct) launch_adapter_tiles<1, 4, 2, 2, 64, 4, true>(a, tiles, stream);
+      else launch_adapter_tiles<1, 4, 2, 2, 64, 4, false>(a, tiles, stream);
+      break;
+  }
+}
+
 }  // namespace dsv41
 
 using namespace dsv41;
@@ -93,4 +497,108 @@ extern "C" int dsv41_adapter_add(const void* x, const void* a, const void* b, co
   if (dtype == DSV41_BF16) launch_add<bf16_t>(x, a, b, scale, ids, y, out, h, rows, tokens, k, n, rank, slots, stream);
   else launch_add<float>(x, a, b, scale, ids, y, out, h, rows, tokens, k, n, rank, slots, stream);
   return check_launch(what);
+}
+
+// ------------------------------------------------------------------ the projection and its adapters
+
+static bool projection_sizes(int64_t rows, int32_t k, int32_t n0, int32_t n1, int32_t rank0, int32_t rank1) {
+  return rows > 0 && rows < (1ll << 31) && k > 0 && k % 64 == 0 && n0 > 0 && n1 >= 0 && n0 % 32 == 0 && n1 % 32 == 0 &&
+         (int64_t)n0 + n1 < (1ll << 30) && rank0 >= 0 && rank1 >= 0 && rank0 <= kMaxRank && rank1 <= kMaxRank &&
+         rank0 % 8 == 0 && rank1 % 8 == 0 && (n1 == 0 || rows <= 128);
+}
+
+extern "C" size_t dsv41_adapter_linear_workspace_bytes(int64_t rows, int32_t k, int32_t n0, int32_t n1, int32_t rank0,
+                                                       int32_t rank1) {
+  if (!projection_sizes(rows, k, n0, n1, rank0, rank1)) return 0;
+  const int most = rank0 > rank1 ? rank0 : rank1;
+  return plan_bytes(adapter_plan((int)rows, k, n0 + n1, n0, most), (int)rows, n0 + n1, rank0, rank1);
+}
+
+static int run_adapter_linear(const char* what, const void* x, const void* w0, const void* w1, const Bank* banks,
+                              const int32_t* ids, void* y0, void* y1, void* workspace, size_t workspace_bytes,
+                              int64_t rows, int32_t tokens, int32_t k, int32_t n0, int32_t n1, int32_t dtype,
+                              hipStream_t stream) {
+  DSV41_REQUIRE(dtype == DSV41_BF16, DSV41_E_DTYPE, "%s: bf16 only (dtype %d)", what, dtype);
+  DSV41_REQUIRE(rows >= 0 && rows < (1ll << 31) && tokens > 0 && rows % tokens == 0 && k > 0 && n0 > 0 && n1 >= 0 &&
+                    (int64_t)n0 + n1 < (1ll << 30),
+                DSV41_E_ARG, "%s: rows %lld of %d tokens, k %d, n %d + %d", what, (long long)rows, tokens, k, n0, n1);
+  for (int s = 0; s < 2; ++s) {
+    const Bank& b = banks[s];
+    DSV41_REQUIRE(b.slots >= 0 && (b.slots == 0 || (b.rank > 0 && b.a && b.b && b.scale)), DSV41_E_ARG,
+                  "%s: bank %d of %d slots, rank %d", what, s, b.slots, b.rank);
+    DSV41_REQUIRE(b.slots == 0 || (b.rank % 8 == 0 && b.rank <= kMaxRank), DSV41_E_SHAPE,
+                  "%s: rank %d must be a multiple of 8, at most %d", what, b.rank, kMaxRank);
+    DSV41_REQUIRE(b.slots == 0 || (aligned16(b.a) && aligned16(b.b)), DSV41_E_ARG,
+                  "%s: adapters must be 16-byte aligned", what);
+  }
+  DSV41_REQUIRE(k % 64 == 0 && n0 % 32 == 0 && n1 % 32 == 0, DSV41_E_SHAPE,
+                "%s: k = %d must be a multiple of 64, n = %d (+ %d) of 32", what, k, n0, n1);
+  DSV41_REQUIRE(n1 == 0 || rows <= 128, DSV41_E_SHAPE, "%s: two projections of %lld rows (at most 128)", what,
+                (long long)rows);
+  if (rows == 0) return 0;
+  DSV41_REQUIRE(x && w0 && y0 && ids && (n1 == 0 || (w1 && y1)), DSV41_E_ARG, "%s: null tensor", what);
+  DSV41_REQUIRE(aligned16(x) && aligned16(w0) && aligned16(y0) && (n1 == 0 || (aligned16(w1) && aligned16(y1))),
+                DSV41_E_ARG, "%s: tensors must be 16-byte aligned", what);
+  const int rank0 = banks[0].slots ? banks[0].rank : 0, rank1 = banks[1].slots ? banks[1].rank : 0, n = n0 + n1;
+  const AdapterPlan p = adapter_plan((int)rows, k, n, n0, rank0 > rank1 ? rank0 : rank1);
+  const int64_t tiles = (int64_t)(n / p.tr) * ((rows + p.tm - 1) / p.tm) * p.splits;
+  const int64_t shrinks = (rows + 15) / 16 * p.chunks * ((rank0 + 15) / 16);
+  const int64_t reduces = (rows + 15) / 16 * ((n + 63) / 64);
+  DSV41_REQUIRE(tiles < (1ll << 31) && shrinks < (1ll << 31) && reduces < (1ll << 31), DSV41_E_ARG, "%s: too many tiles",
+                what);
+  const size_t need = plan_bytes(p, (int)rows, n, rank0, rank1);
+  DSV41_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))), DSV41_E_WORKSPACE,
+                "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
+  AdapterArgs a;
+  a.t = WoaArgs{static_cast<const bf16_t*>(x), static_cast<const bf16_t*>(w0), workspace, (int)rows, p.splits,
+                k / p.splits, n, 1, static_cast<const bf16_t*>(n1 ? w1 : nullptr), n0};
+  a.bank[0] = banks[0];
+  a.bank[1] = banks[1];
+  uint8_t* at = static_cast<uint8_t*>(workspace) + (p.direct ? 0 : pad256((size_t)rows * p.splits * n * sizeof(float)));
+  a.bank[0].h = reinterpret_cast<float*>(at);
+  a.bank[1].h = reinterpret_cast<float*>(at + pad256((size_t)p.chunks * rows * rank0 * sizeof(float)));
+  a.ids = ids;
+  a.tokens = tokens;
+  a.k = k;
+  a.chunk = p.chunk;
+  a.chunks = p.chunks;
+  a.y = static_cast<bf16_t*>(y0);
+  a.y1 = static_cast<bf16_t*>(y1);
+  if (p.direct && shrinks)
+    hipLaunchKernelGGL(adapter_shrink_kernel, dim3((unsigned)shrinks), dim3(256), 0, stream, a);
+  launch_projection(a, p, stream);
+  if (!p.direct) {
+    // 256 columns per workgroup where that still gives every CU two of them, 64 otherwise
+    if ((rows + 15) / 16 * ((n + 255) / 256) >= 512)
+      hipLaunchKernelGGL(adapter_reduce_kernel<4>, dim3((unsigned)((rows + 15) / 16 * ((n + 255) / 256))), dim3(256), 0,
+                         stream, a);
+    else hipLaunchKernelGGL(adapter_reduce_kernel<1>, dim3((unsigned)reduces), dim3(256), 0, stream, a);
+  }
+  return check_launch(what);
+}
+
+extern "C" int dsv41_adapter_linear(const void* x, const void* w, const void* a, const void* b, const float* scale,
+                                    const int32_t* ids, void* y, void* workspace, size_t workspace_bytes, int64_t rows,
+                                    int32_t tokens, int32_t k, int32_t n, int32_t rank, int32_t slots, int32_t dtype,
+                                    hipStream_t stream) {
+  const char* what = "dsv41_adapter_linear";
+  DSV41_REQUIRE(slots > 0, DSV41_E_ARG, "%s: %d slots", what, slots);
+  const Bank banks[2] = {{static_cast<const bf16_t*>(a), static_cast<const bf16_t*>(b), scale, nullptr, rank, slots}, {}};
+  return run_adapter_linear(what, x, w, nullptr, banks, ids, y, nullptr, workspace, workspace_bytes, rows, tokens, k, n, 0,
+                            dtype, stream);
+}
+
+extern "C" int dsv41_adapter_linear_pair(const void* x, const void* w0, const void* w1, const void* a0, const void* b0,
+                                         const float* scale0, const void* a1, const void* b1, const float* scale1,
+                                         const int32_t* ids, void* y0, void* y1, void* workspace, size_t workspace_bytes,
+                                         int64_t rows, int32_t tokens, int32_t k, int32_t n0, int32_t n1, int32_t rank0,
+                                         int32_t rank1, int32_t slots0, int32_t slots1, int32_t dtype,
+                                         hipStream_t stream) {
+  const char* what = "dsv41_adapter_linear_pair";
+  DSV41_REQUIRE(n1 > 0, DSV41_E_ARG, "%s: the second weight is missing", what);
+  DSV41_REQUIRE(slots0 > 0 || slots1 > 0, DSV41_E_ARG, "%s: %d and %d slots", what, slots0, slots1);
+  const Bank banks[2] = {{static_cast<const bf16_t*>(a0), static_cast<const bf16_t*>(b0), scale0, nullptr, rank0, slots0},
+                         {static_cast<const bf16_t*>(a1), static_cast<const bf16_t*>(b1), scale1, nullptr, rank1, slots1}};
+  return run_adapter_linear(what, x, w0, w1, banks, ids, y0, y1, workspace, workspace_bytes, rows, tokens, k, n0, n1, dtype,
+                            stream);
 }

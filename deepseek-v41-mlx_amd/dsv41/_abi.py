@@ -115,12 +115,18 @@ _SIGNATURES = {
     "dsv41_adapter_add_workspace_bytes": [_i64, _i32],
     "dsv41_adapter_add": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _sz, _i64, _i32, _i32, _i32, _i32, _i32,
                           _i32, _c_p],
+    "dsv41_adapter_linear_workspace_bytes": [_i64, _i32, _i32, _i32, _i32, _i32],
+    "dsv41_adapter_linear": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _sz, _i64, _i32, _i32, _i32, _i32, _i32,
+                             _i32, _c_p],
+    "dsv41_adapter_linear_pair": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _sz,
+                                  _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_cache_move": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _c_p, _c_p, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_version": [],
     "dsv41_last_error_string": [],
 }
 _RESTYPES = {
     "dsv41_adapter_add_workspace_bytes": _sz,
+    "dsv41_adapter_linear_workspace_bytes": _sz,
     "dsv41_sparse_mla_workspace_bytes": _sz,
     "dsv41_linear_rows_workspace_bytes": _sz,
     "dsv41_linear_f32_pair_workspace_bytes": _sz,
@@ -1314,6 +1320,65 @@ def adapter_add(x, a, b, scale, ids, y, out=None, workspace=None):
     _call_on(x.device, name, _ptr(x), _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), _ptr(y), _ptr(out), _ptr(ws), need, rows,
              tokens, k, y.shape[-1], rank, slots, dtype_code(x, name), _stream(x))
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1) -> int:
+    return lib().dsv41_adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1)
+
+
+def _adapter_weight(name, x, w):
+    _gpu(name, w)
+    _contig(name, w)
+    if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
+        raise ValueError(f"{name}: x and w must be bfloat16")
+    if w.dim() != 2 or w.shape[1] != x.shape[-1] or w.device != x.device:
+        raise ValueError(f"{name}: x {tuple(x.shape)} and w {tuple(w.shape)} do not contract")
+
+
+def adapter_linear(x, w, a, b, scale, ids, out=None, workspace=None):
+    """x w^T + scale[t] ((x a[t]^T) b[t]^T) with t = ids[sequence] (none outside the slots), bf16, rounded once:
+    dsv41_adapter_linear."""
+    name = "dsv41_adapter_linear"
+    rows, tokens, k, rank, slots = _adapter_args(name, x, a, b, scale, ids, w.shape[0])
+    _adapter_weight(name, x, w)
+    n = w.shape[0]
+    out = _out(name, out, (*x.shape[:-1], n), x.dtype, x.device)
+    if rows == 0:
+        return out
+    need = adapter_linear_workspace_bytes(rows, k, n, 0, rank, 0)
+    ws = _ws(name, workspace, need, x.device)
+    _call_on(x.device, name, _ptr(x), _ptr(w), _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), _ptr(out), _ptr(ws), need, rows,
+             tokens, k, n, rank, slots, dtype_code(x, name), _stream(x))
+    return out
+
+
+def adapter_linear_pair(x, w0, w1, bank0, bank1, ids, out0=None, out1=None, workspace=None):
+    """Two projections of the same rows in one call, each with its own adapters under the same ids; bank0 and bank1 are
+    (a, b, scale) or None, not both: dsv41_adapter_linear_pair."""
+    name = "dsv41_adapter_linear_pair"
+    if bank0 is None and bank1 is None:
+        raise ValueError(f"{name}: no adapters")
+    sizes = []
+    for w, bank in ((w0, bank0), (w1, bank1)):
+        _adapter_weight(name, x, w)
+        if bank is not None:
+            sizes.append(_adapter_args(name, x, *bank, ids, w.shape[0]))
+    rows, tokens, k = sizes[0][:3]
+    (rank0, slots0) = sizes[0][3:] if bank0 is not None else (0, 0)
+    (rank1, slots1) = sizes[-1][3:] if bank1 is not None else (0, 0)
+    n0, n1 = w0.shape[0], w1.shape[0]
+    out0 = _out(name, out0, (*x.shape[:-1], n0), x.dtype, x.device)
+    out1 = _out(name, out1, (*x.shape[:-1], n1), x.dtype, x.device)
+    if rows == 0:
+        return out0, out1
+    need = adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1)
+    ws = _ws(name, workspace, need, x.device)
+    p0 = [t.data_ptr() for t in bank0] if bank0 is not None else [None] * 3
+    p1 = [t.data_ptr() for t in bank1] if bank1 is not None else [None] * 3
+    _call_on(x.device, name, _ptr(x), _ptr(w0), _ptr(w1), *p0, *p1, _ptr(ids), _ptr(out0), _ptr(out1), _ptr(ws), need,
+             rows, tokens, k, n0, n1, rank0, rank1, slots0, slots1, dtype_code(x, name), _stream(x))
+    return out0, out1
 
 
 # ---------------------------------------------------------------------------- cached sequences

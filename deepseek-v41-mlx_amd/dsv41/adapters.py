@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _abi
-from .layers import decode_linear, decode_linear_pair
+from .layers import DECODE_ROWS, _only_the_product, decode_linear, decode_linear_pair
 
 
 class AdapterBank:
@@ -72,6 +72,15 @@ def _check(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank, ids: torch.
         raise ValueError("adapter projections are not differentiable: call them under torch.no_grad()")
 
 
+def _fused_ok(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank | None) -> bool:
+    """Whether the projection runs with its adapters in dsv41_adapter_linear: bf16 in whole 64-channel steps and 32-row
+    weight tiles, ranks up to 128, and a module whose call is the product alone."""
+    w = lin.weight
+    return (x.dtype == torch.bfloat16 == w.dtype and x.is_cuda and lin.bias is None and w.is_contiguous()
+            and w.shape[1] % 64 == 0 and w.shape[0] % 32 == 0 and (bank is None or bank.a.shape[1] <= 128)
+            and _only_the_product(lin, x))
+
+
 def adapter_linear(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank | None, ids: torch.Tensor | None,
                    wide_only: bool = False) -> torch.Tensor:
     """lin(x) with every sequence's own adapter: x [sequences, (tokens,) in], ids int32 [sequences]. Without a bank or
@@ -79,14 +88,23 @@ def adapter_linear(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank | No
     if bank is None or ids is None:
         return decode_linear(lin, x, wide_only)
     _check(lin, x, bank, ids)
+    if _fused_ok(lin, x, bank):
+        return _abi.adapter_linear(x.contiguous(), lin.weight, bank.a, bank.b, bank.scale, ids)
     y = lin(x)
     return _abi.adapter_add(x.contiguous(), bank.a, bank.b, bank.scale, ids, y.contiguous())
 
 
 def adapter_linear_pair(lin0: torch.nn.Linear, lin1: torch.nn.Linear, x: torch.Tensor, bank0: AdapterBank | None,
                         bank1: AdapterBank | None, ids: torch.Tensor | None):
-    """(adapter_linear(lin0, x, bank0, ids), adapter_linear(lin1, x, bank1, ids)); without any bank or ids it is
-    decode_linear_pair."""
+    """(adapter_linear(lin0, x, bank0, ids), adapter_linear(lin1, x, bank1, ids)), at decode row counts in one call;
+    without any bank or ids it is decode_linear_pair."""
     if ids is None or (bank0 is None and bank1 is None):
         return decode_linear_pair(lin0, lin1, x)
+    for lin, bank in ((lin0, bank0), (lin1, bank1)):
+        if bank is not None:
+            _check(lin, x, bank, ids)
+    if (x.numel() <= DECODE_ROWS * x.shape[-1] and lin0.weight.shape[1] == lin1.weight.shape[1]
+            and _fused_ok(lin0, x, bank0) and _fused_ok(lin1, x, bank1)):
+        pair = [None if bank is None else (bank.a, bank.b, bank.scale) for bank in (bank0, bank1)]
+        return _abi.adapter_linear_pair(x.contiguous(), lin0.weight, lin1.weight, *pair, ids)
     return adapter_linear(lin0, x, bank0, ids), adapter_linear(lin1, x, bank1, ids)

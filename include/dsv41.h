@@ -578,6 +578,25 @@ int dsv41_adapter_add(const void* x, const void* a, const void* b, const float* 
                       int32_t tokens, int32_t k, int32_t n, int32_t rank, int32_t slots, int32_t dtype,
                       hipStream_t stream);
 
+/* The projection and its adapters in one call, bf16: y [rows, n] rounded once. k a multiple of 64, n of 32, rank of
+ * 8 and at most 128, 16-byte aligned tensors; any number of rows. */
+size_t dsv41_adapter_linear_workspace_bytes(int64_t rows, int32_t k, int32_t n0, int32_t n1, int32_t rank0,
+                                            int32_t rank1);
+int dsv41_adapter_linear(const void* x, const void* w, const void* a, const void* b, const float* scale,
+                         const int32_t* ids, void* y, void* workspace, size_t workspace_bytes, int64_t rows,
+                         int32_t tokens, int32_t k, int32_t n, int32_t rank, int32_t slots, int32_t dtype,
+                         hipStream_t stream);
+
+/* Two projections of the same rows (at most 128), each with adapters of its own under the same ids, in one call:
+ * y0 [rows, n0] and y1 [rows, n1] as two dsv41_adapter_linear calls give them, up to the order of fp32 additions.
+ * A bank of 0 slots (its pointers unused) has no adapters; one of the two must have some. The workspace of both calls
+ * is dsv41_adapter_linear_workspace_bytes (n1, rank1 0 for the single projection, rank 0 for no bank). */
+int dsv41_adapter_linear_pair(const void* x, const void* w0, const void* w1, const void* a0, const void* b0,
+                              const float* scale0, const void* a1, const void* b1, const float* scale1,
+                              const int32_t* ids, void* y0, void* y1, void* workspace, size_t workspace_bytes,
+                              int64_t rows, int32_t tokens, int32_t k, int32_t n0, int32_t n1, int32_t rank0,
+                              int32_t rank1, int32_t slots0, int32_t slots1, int32_t dtype, hipStream_t stream);
+
 /* ---------------------------------------------------------------- cached sequences --
  */
 

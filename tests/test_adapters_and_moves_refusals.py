@@ -78,6 +78,41 @@ def test_adapter_add_checks_its_tensors(host_abi):
     _refused(call(ids=ids.to("meta")), "tensors on")
 
 
+def test_adapter_linear_checks_its_tensors(host_abi):
+    A, b, c = host_abi, _bank(), _bank(slots=2, n=96, rank=16)
+    x, w, ids = torch.zeros(2, 5, 64, dtype=BF), torch.zeros(32, 64, dtype=BF), torch.zeros(2, dtype=torch.int32)
+    w1 = torch.zeros(96, 64, dtype=BF)
+
+    def call(**kw):
+        args = dict(x=x, w=w, a=b.a, b=b.b, scale=b.scale, ids=ids)
+        args.update(kw)
+        return lambda: A.adapter_linear(**args)
+
+    _reaches(call())
+    _reaches(call(out=torch.zeros(2, 5, 32, dtype=BF), workspace=torch.zeros(1 << 20, dtype=torch.uint8)))
+    assert A.adapter_linear(x[:0], w, b.a, b.b, b.scale, ids[:0]).shape == (0, 5, 32)
+    _refused(call(w=w.float()), "bfloat16")
+    _refused(call(w=w1), "no adapters")
+    _refused(call(w=torch.zeros(32, 128, dtype=BF)), "contract")
+    _refused(call(w=torch.zeros(64, 32, dtype=BF).t()), "contiguous")
+    _refused(call(ids=ids[:1]), "ids must be int32")
+    _refused(call(out=torch.zeros(2, 5, 32)), "out must be")
+    _refused(call(workspace=torch.zeros(64)), "workspace")
+
+    def pair(**kw):
+        args = dict(x=x, w0=w, w1=w1, bank0=(b.a, b.b, b.scale), bank1=(c.a, c.b, c.scale), ids=ids)
+        args.update(kw)
+        return lambda: A.adapter_linear_pair(**args)
+
+    _reaches(pair())
+    _reaches(pair(bank0=None))
+    _reaches(pair(bank1=None))
+    _refused(pair(bank0=None, bank1=None), "no adapters")
+    _refused(pair(bank1=(b.a, b.b, b.scale)), "no adapters")
+    _refused(pair(w1=w1.float()), "bfloat16")
+    _refused(pair(out1=torch.zeros(2, 5, 32, dtype=BF)), "out must be")
+
+
 def test_cpu_tensors_are_refused():
     from dsv41 import _abi
     b = _bank()
@@ -173,6 +208,38 @@ def test_c_entry_points_refuse_bad_sizes():
     assert add(bytes=4 * 2 * 4 - 1) == -4 and add(ws=None) == -4 and add(ws=ctypes.c_void_p(4100)) == -4
     assert lib.dsv41_adapter_add_workspace_bytes(4, 2) == 32
     assert lib.dsv41_adapter_add_workspace_bytes(0, 2) == 0
+
+    def linear(**kw):
+        a = dict(x=p, w=p, a=p, b=p, scale=p, ids=p, y=p, ws=p, bytes=1 << 30, rows=4, tokens=2, k=64, n=32, rank=8,
+                 slots=1, dtype=_abi.BF16)
+        a.update(kw)
+        return lib.dsv41_adapter_linear(*a.values(), None)
+
+    assert linear(rows=0) == 0
+    for bad in (dict(rows=-1), dict(rows=5), dict(tokens=0), dict(k=0), dict(n=0), dict(rank=0), dict(slots=0),
+                dict(slots=-1)):
+        assert linear(**bad) == -1, bad
+    for name in ("x", "w", "a", "b", "scale", "ids", "y"):
+        assert linear(**{name: None}) == -1, name
+    for name in ("x", "w", "a", "b", "y"):
+        assert linear(**{name: ctypes.c_void_p(4104)}) == -1, name
+    assert linear(dtype=_abi.F32) == -2
+    for bad in (dict(k=96), dict(n=48), dict(rank=12), dict(rank=136)):
+        assert linear(**bad) == -3, bad
+    need = lib.dsv41_adapter_linear_workspace_bytes(4, 64, 32, 0, 8, 0)
+    assert need > 0 and linear(bytes=need - 1) == -4 and linear(ws=None) == -4
+    assert lib.dsv41_adapter_linear_workspace_bytes(0, 64, 32, 0, 8, 0) == 0
+
+    def pair(**kw):
+        a = dict(x=p, w0=p, w1=p, a0=p, b0=p, s0=p, a1=p, b1=p, s1=p, ids=p, y0=p, y1=p, ws=p, bytes=1 << 30, rows=4,
+                 tokens=1, k=64, n0=32, n1=32, rank0=8, rank1=8, slots0=1, slots1=1, dtype=_abi.BF16)
+        a.update(kw)
+        return lib.dsv41_adapter_linear_pair(*a.values(), None)
+
+    assert pair(rows=0) == 0
+    assert pair(slots0=0, slots1=0) == -1 and pair(n1=0) == -1 and pair(w1=None) == -1 and pair(y1=None) == -1
+    assert pair(a1=None) == -1 and pair(rank1=0) == -1 and pair(rank1=4) == -3 and pair(rows=129) == -3
+    assert pair(slots0=0, a0=None, b0=None, s0=None, rank0=0, rows=0) == 0
 
     ptrs = (ctypes.c_void_p * 1)(4096)
     i64 = lambda v: (ctypes.c_int64 * 1)(v)      # noqa: E731
