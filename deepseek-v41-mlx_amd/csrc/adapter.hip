@@ -155,61 +155,260 @@ __device__ __forceinline__ void shrink_item(const AdapterArgs& a, const Bank& bk
   __syncthreads();
 }
 
-__global__ __launch_bounds__(256) void adapter_shrink_kernel(AdapterArgs a) {
-  __shared__ __align__(16) float red[4 * 256];
-  shrink_item(a, a.bank[0], blockIdx.x, red);
+// Ranks 8 c .. 8 c + 7 of scale h as an operand of the second product: it takes the sum of two bf16 values - the upper
+// 8 bits, cut off, and the next 8, rounded - so that 16 bits of the intermediate count (2^-17 of it is lost, far below
+// the result's own rounding); each is multiplied with the same bf16 B, exactly. An infinite value has no lower part.
+__device__ __forceinline__ uint4 half_of(const float* v, bool low) {
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t h0 = __float_as_uint(v[2 * e]) & 0xFFFF0000u, h1 = __float_as_uint(v[2 * e + 1]) & 0xFFFF0000u;
+    const float l0 = h0 << 1 == 0xFF000000u ? 0.0f : v[2 * e] - __uint_as_float(h0);
+    const float l1 = h1 << 1 == 0xFF000000u ? 0.0f : v[2 * e + 1] - __uint_as_float(h1);
+    w[e] = low ? pack2_bf16(l0, l1) : (h0 >> 16) | h1;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// acc[i] += scale (h B^T) for 16 rows (lane l16's, adapter id) and WR tiles of 16 output columns from col on. hval(c, v)
-// gives scale times ranks 8 c .. 8 c + 7 of the lane's row. They go into the MFMA as the sum of two bf16 values - the
-// upper 8 bits, cut off, and the next 8, rounded - so that 16 bits of the intermediate count (2^-17 of it is lost, far
-// below the result's own rounding); each is multiplied with the same bf16 B, exactly. An infinite value has no lower
-// part. Rows are columns of the MFMA again: every adapter of the tile multiplies all of them, each lane keeps its own.
-template <int WR, typename H>
-__device__ __forceinline__ void expand_tile(f32x4 (&acc)[WR], const Bank& bk, int n, int col, int id, H hval) {
-  const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int r8 = bk.rank >> 3;
-  uint32_t todo = (uint32_t)__ballot(id >= 0) & 0xFFFFu;
-  while (todo) {
-    const int t = next_adapter(todo, id);
-    const bf16_t* bp = bk.b + ((int64_t)t * n + col + l16) * bk.rank;
-    f32x4 sum[WR];
+// The rank chunk of 8 that lane group g supplies to MFMA step q (the upper parts of the r8 chunks, then the lower ones;
+// past them nothing).
+struct RankSlot {
+  int c;
+  bool low, live;
+  __device__ __forceinline__ RankSlot(int q, int r8) {
+    const int s = q + ((threadIdx.x >> 4) & 3);
+    live = s < 2 * r8;
+    low = s >= r8;
+    c = live ? (low ? s - r8 : s) : 0;
+  }
+};
+
+__device__ __forceinline__ bf16x8 or_zero(uint4 v, bool live) {
+  return as_bf16x8(live ? v : make_uint4(0, 0, 0, 0));
+}
+
+// The whole first product of 16 MT rows and 16 RT ranks: the channels in 64-wide steps in turn over NW waves, each
+// step's x rows read once for all ranks and each adapter row once for all x rows; the waves' sums meet in LDS. Writes
+// the second product's operand: per row the upper halves of scale h's ranks, then the lower ones ([rows, 2 rank] bf16).
+// A tile whose rows name several adapters repeats the channels for each and keeps every row's own.
+template <int MT, int RT, int NW>
+__global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(AdapterArgs a) {
+  __shared__ __align__(16) float red[NW][MT * RT * 256];
+  const Bank& bk = a.bank[0];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int rtiles = (bk.rank + 16 * RT - 1) / (16 * RT);
+  const int r0 = (int)(blockIdx.x % rtiles) * 16 * RT, m0 = (int)(blockIdx.x / rtiles) * 16 * MT;
+  int id[MT];
+  const bf16_t* xp[MT];
+  uint32_t todo[MT];
 #pragma unroll
-    for (int i = 0; i < WR; ++i) sum[i] = acc[i];
-    for (int q = 0; q < 2 * r8; q += 4) {
-      const int s = q + g;                             // upper parts of the rank chunks, then lower parts
-      const bool live = s < 2 * r8, low = s >= r8;
-      const int c = live ? (low ? s - r8 : s) : 0;
-      float v[8];
-      hval(c, v);
-      uint32_t w[4];
+  for (int j = 0; j < MT; ++j) {
+    const int m = m0 + 16 * j + l16;
+    id[j] = row_adapter(a, bk, m);
+    xp[j] = a.t.o + (int64_t)min(m, a.t.rows - 1) * a.k + 8 * g;
+    todo[j] = (uint32_t)__ballot(id[j] >= 0) & 0xFFFFu;
+  }
+  f32x4 res[MT][RT];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t u0 = __float_as_uint(v[2 * e]), u1 = __float_as_uint(v[2 * e + 1]);
-        const uint32_t h0 = u0 & 0xFFFF0000u, h1 = u1 & 0xFFFF0000u;
-        const float l0 = h0 << 1 == 0xFF000000u ? 0.0f : v[2 * e] - __uint_as_float(h0);
-        const float l1 = h1 << 1 == 0xFF000000u ? 0.0f : v[2 * e + 1] - __uint_as_float(h1);
-        w[e] = low ? pack2_bf16(l0, l1) : (h0 >> 16) | h1;
-        if (!live) w[e] = 0u;
+  for (int j = 0; j < MT; ++j)
+#pragma unroll
+    for (int i = 0; i < RT; ++i) res[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (;;) {
+    int t = -1;
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+      if (t < 0 && todo[j]) t = __builtin_amdgcn_readlane(id[j], __builtin_ctz(todo[j]));
+    if (t < 0) break;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) todo[j] &= ~(uint32_t)__ballot(id[j] == t);
+    const bf16_t* ap[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)   // ranks past the end: not stored
+      ap[i] = bk.a + ((int64_t)t * bk.rank + min(r0 + 16 * i + l16, bk.rank - 1)) * a.k + 8 * g;
+    f32x4 acc[MT][RT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int i = 0; i < RT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int k = 64 * wave; k < a.k; k += 64 * NW) {
+      bf16x8 xf[2][MT], af[2][RT];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < MT; ++j) xf[h][j] = ld_bf16x8(xp[j] + k + 32 * h);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) af[h][i] = ld_bf16x8(ap[i] + k + 32 * h);
       }
-      const bf16x8 hf = as_bf16x8(make_uint4(w[0], w[1], w[2], w[3]));
 #pragma unroll
-      for (int i = 0; i < WR; ++i) {
-        uint4 b = *reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank + 8 * c);
-        if (!live) b = make_uint4(0, 0, 0, 0);
-        sum[i] = mfma16x16x32(as_bf16x8(b), hf, sum[i]);
-      }
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < MT; ++j)
+#pragma unroll
+          for (int i = 0; i < RT; ++i) acc[j][i] = mfma16x16x32(af[h][i], xf[h][j], acc[j][i]);
     }
-    settle(sum);
 #pragma unroll
-    for (int i = 0; i < WR; ++i) acc[i] = id == t ? sum[i] : acc[i];
+    for (int j = 0; j < MT; ++j) {
+      settle(acc[j]);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) res[j][i] = id[j] == t ? acc[j][i] : res[j][i];
+    }
+  }
+  // lane (g, l16) holds ranks 4 g .. 4 g + 3 of row l16 of every tile
+#pragma unroll
+  for (int j = 0; j < MT; ++j)
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+      *reinterpret_cast<f32x4*>(&red[wave][((j * 16 + l16) * RT + i) * 16 + 4 * g]) = res[j][i];
+  __syncthreads();
+  uint16_t* hl = reinterpret_cast<uint16_t*>(bk.h);
+  for (int q = threadIdx.x; q < MT * RT * 32; q += 64 * NW) {          // 8 ranks of one row each
+    const int row = q / (2 * RT), c = q % (2 * RT), m = m0 + row, r = r0 + 8 * c;
+    if (m >= a.t.rows || r >= bk.rank) continue;
+    const int t = row_adapter(a, bk, m);
+    const float scale = t < 0 ? 0.0f : bk.scale[t];
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float sum = red[0][q * 8 + e];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) sum += red[w][q * 8 + e];
+      v[e] = sum * scale;
+    }
+    uint16_t* to = hl + (int64_t)m * 2 * bk.rank + r;
+    *reinterpret_cast<uint4*>(to) = half_of(v, false);
+    *reinterpret_cast<uint4*>(to + bk.rank) = half_of(v, true);
   }
 }
 
-// The projection's tiles. DIRECT: the adapters' part is added to the float32 sums in registers and the result stored,
+// One MFMA step of acc[i] += h B^T for WR tiles of 16 output columns and U adapters of a tile of 16 rows. Rows are the
+// MFMA's columns: each adapter multiplies all of them, a lane keeps its own row's.
+template <int WR, int U>
+__device__ __forceinline__ void expand_step(f32x4 (&acc)[WR], const bf16_t* bp, int64_t slot, int rank, bool live,
+                                            bf16x8 hf, int id, const int (&t)[U]) {
+  uint4 b[U][WR];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < WR; ++i) b[u][i] = *reinterpret_cast<const uint4*>(bp + t[u] * slot + (int64_t)16 * i * rank);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < WR; ++i) {
+      const f32x4 sum = mfma16x16x32(or_zero(b[u][i], live), hf, acc[i]);
+      acc[i] = id == t[u] && (u == 0 || t[u] != t[0]) ? sum : acc[i];
+    }
+}
+
+// acc[i] += scale (h B^T) for 16 rows (lane l16's, adapter id) and the output columns col + 16 i + l16. hval(c, v)
+// gives scale times ranks 8 c .. 8 c + 7 of the lane's row. Up to four adapters' B are in flight at once.
+template <int WR, typename H>
+__device__ __forceinline__ void expand_tile(f32x4 (&acc)[WR], const Bank& bk, int n, int col, int id, H hval) {
+  const int r8 = bk.rank >> 3;
+  const int64_t slot = (int64_t)n * bk.rank;
+  const uint32_t named = (uint32_t)__ballot(id >= 0) & 0xFFFFu;
+  if (named == 0) return;
+  for (int q = 0; q < 2 * r8; q += 4) {
+    const RankSlot at(q, r8);
+    float v[8];
+    hval(at.c, v);
+    const bf16x8 hf = or_zero(half_of(v, at.low), at.live);
+    const bf16_t* bp = bk.b + (int64_t)(col + (threadIdx.x & 15)) * bk.rank + 8 * at.c;
+    uint32_t todo = named;
+    while (todo) {
+      int t[4];
+      t[0] = next_adapter(todo, id);
+      if (todo == 0) {
+        const int one[1] = {t[0]};
+        expand_step<WR, 1>(acc, bp, slot, bk.rank, at.live, hf, id, one);
+        break;
+      }
+#pragma unroll
+      for (int u = 1; u < 4; ++u) t[u] = todo ? next_adapter(todo, id) : t[0];
+      expand_step<WR, 4>(acc, bp, slot, bk.rank, at.live, hf, id, t);
+    }
+  }
+}
+
+// acc[i][j] += scale (h B^T) for a wave's block of 16 WM rows from m0 on and 16 WR columns from col on, h from the
+// finished first product. One adapter for all rows that are stored: its products go straight into the sums. Several:
+// each multiplies all rows and every lane keeps its own row's, one result beside the sums at a time (they fill the
+// registers). ONE: the sequences are whole blocks, so the second kind is never met.
+template <int WR, int WM, bool ONE>
+__device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const AdapterArgs& a, int m0, int col) {
+  const Bank& bk = a.bank[0];
+  const int l16 = threadIdx.x & 15, r8 = bk.rank >> 3;
+  int id[WM];
+  uint32_t todo[WM];
+  const uint16_t* hp[WM];
+  int t = -1;
+#pragma unroll
+  for (int j = 0; j < WM; ++j) {
+    const int m = m0 + 16 * j + l16;
+    id[j] = row_adapter(a, bk, m);
+    todo[j] = (uint32_t)__ballot(id[j] >= 0) & 0xFFFFu;
+    if (t < 0 && todo[j]) t = __builtin_amdgcn_readlane(id[j], __builtin_ctz(todo[j]));
+    hp[j] = reinterpret_cast<const uint16_t*>(bk.h) + (int64_t)min(m, a.t.rows - 1) * 2 * bk.rank;
+  }
+  if (t < 0) return;
+  bool one = true;
+#pragma unroll
+  for (int j = 0; j < WM && !ONE; ++j) one = one && __ballot(id[j] != t && m0 + 16 * j + l16 < a.t.rows) == 0;
+  const bf16_t* b0 = bk.b + (int64_t)(col + l16) * bk.rank;
+  const int64_t slot = (int64_t)a.t.r * bk.rank;
+  if (ONE || one) {
+    for (int q = 0; q < 2 * r8; q += 4) {
+      const RankSlot at(q, r8);
+      const int from = 8 * at.c + (at.low ? bk.rank : 0);
+      const bf16_t* bp = b0 + t * slot + 8 * at.c;
+      bf16x8 hf[WM], bf[WR];
+#pragma unroll
+      for (int i = 0; i < WR; ++i) bf[i] = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), at.live);
+#pragma unroll
+      for (int j = 0; j < WM; ++j) hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + from), at.live);
+#pragma unroll
+      for (int j = 0; j < WM; ++j)
+#pragma unroll
+        for (int i = 0; i < WR; ++i) acc[i][j] = mfma16x16x32(bf[i], hf[j], acc[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < WR; ++i) settle(acc[i]);
+    return;
+  }
+  while (t >= 0) {
+#pragma unroll
+    for (int j = 0; j < WM; ++j) todo[j] &= ~(uint32_t)__ballot(id[j] == t);
+    for (int q = 0; q < 2 * r8; q += 4) {
+      const RankSlot at(q, r8);
+      const int from = 8 * at.c + (at.low ? bk.rank : 0);
+      const bf16_t* bp = b0 + t * slot + 8 * at.c;
+      bf16x8 hf[WM];
+#pragma unroll
+      for (int j = 0; j < WM; ++j) hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + from), at.live);
+#pragma unroll
+      for (int i = 0; i < WR; ++i) {
+        const bf16x8 bf = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), at.live);
+#pragma unroll
+        for (int j = 0; j < WM; ++j) {
+          const f32x4 sum = mfma16x16x32(bf, hf[j], acc[i][j]);
+          acc[i][j] = id[j] == t ? sum : acc[i][j];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    t = -1;
+#pragma unroll
+    for (int j = 0; j < WM; ++j)
+      if (t < 0 && todo[j]) t = __builtin_amdgcn_readlane(id[j], __builtin_ctz(todo[j]));
+  }
+}
+
+// The projection's tiles. kExpand*: the adapters' part is added to the float32 sums in registers and the result stored,
 // rounded once (h complete before the launch). Else the sums of one contraction range go to t.out in float32, and the
 // workgroups also compute h, each its share while its first copies are on their way.
-template <int WR, int WM, int GR, int GM, int BK, int NS, bool DIRECT>
+enum AdapterPart { kSplitSums, kExpandOne, kExpandAny };
+
+template <int WR, int WM, int GR, int GM, int BK, int NS, AdapterPart PART>
 __global__ __launch_bounds__(64 * GR * GM, (TileCfg<WR, WM, GR, GM, BK, NS>::LDS <= 72 * 1024) ? 2 : 1) void
 adapter_tiles_kernel(AdapterArgs a) {
   using C = TileCfg<WR, WM, GR, GM, BK, NS>;
@@ -222,39 +421,18 @@ adapter_tiles_kernel(AdapterArgs a) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wr = (wave % GR) * 16 * WR, wm = (wave / GR) * 16 * WM;   // this wave's block
   f32x4 acc[WR][WM];
-  if constexpr (DIRECT) {
+  if constexpr (PART != kSplitSums) {
     tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc);
 #pragma unroll
     for (int i = 0; i < WR; ++i) settle(acc[i]);
-    const Bank& bk = a.bank[0];
     const int col = rt * C::TR + wr;
+    expand_block<WR, WM, PART == kExpandOne>(acc, a, mt * C::TM + wm, col);
 #pragma unroll
     for (int j = 0; j < WM; ++j) {
       const int m = mt * C::TM + wm + 16 * j + l16;
-      const int id = row_adapter(a, bk, m);
-      const float scale = id < 0 ? 0.0f : bk.scale[id];
-      const float* hp = bk.h + (int64_t)min(m, a.t.rows - 1) * bk.rank;
-      f32x4 s[WR];
+      if (m >= a.t.rows) continue;
 #pragma unroll
-      for (int i = 0; i < WR; ++i) s[i] = acc[i][j];
-      expand_tile<WR>(s, bk, a.t.r, col, id, [&](int c, float* v) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-        for (int p = 0; p < a.chunks; ++p) {
-          const f32x4* from = reinterpret_cast<const f32x4*>(hp + (int64_t)p * a.t.rows * bk.rank + 8 * c);
-          const f32x4 v0 = from[0], v1 = from[1];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            v[e] += v0[e];
-            v[4 + e] += v1[e];
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= scale;
-      });
-      if (m < a.t.rows)
-#pragma unroll
-        for (int i = 0; i < WR; ++i) store4<bf16_t>(a.y + (int64_t)m * a.t.r + col + 16 * i + 4 * g, s[i]);
+      for (int i = 0; i < WR; ++i) store4<bf16_t>(a.y + (int64_t)m * a.t.r + col + 16 * i + 4 * g, acc[i][j]);
     }
   } else {
     static_assert(GR * GM == 4, "a partial h is the work of four waves");
@@ -281,7 +459,8 @@ adapter_tiles_kernel(AdapterArgs a) {
 }
 
 // The contraction ranges' parts summed in order, plus the adapters' part, rounded once: a workgroup per 16 rows and
-// 64 WR columns, a wave per 16 WR of them. h is summed over its chunks into LDS first.
+// 64 WR columns, a wave per 16 WR of them (whole blocks of one projection: n0 and n are multiples of 16 WR). h is
+// summed over its chunks into LDS, while the parts are on their way.
 template <int WR>
 __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
   constexpr int kStride = kMaxRank + 4;
@@ -289,48 +468,59 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int ctiles = (a.t.r + 64 * WR - 1) / (64 * WR);
   const int col0 = (int)(blockIdx.x % ctiles) * 64 * WR, m0 = (int)(blockIdx.x / ctiles) * 16;
+  const int m = m0 + l16, col = col0 + wave * 16 * WR;
+  const bool cols = col < a.t.r;
+  f32x4 acc[WR];
+  if (cols) {
+    const float* part = reinterpret_cast<const float*>(a.t.out) + (int64_t)min(m, a.t.rows - 1) * a.t.groups * a.t.r + col + 4 * g;
+#pragma unroll
+    for (int i = 0; i < WR; ++i) acc[i] = *reinterpret_cast<const f32x4*>(part + 16 * i);
+    for (int p = 1; p < a.t.groups; ++p)
+#pragma unroll
+      for (int i = 0; i < WR; ++i) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(part + (int64_t)p * a.t.r + 16 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][e] = acc[i][e] + v[e];
+      }
+  }
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const Bank& bk = a.bank[s];
     if (bk.slots == 0 || (s == 0 ? col0 >= a.t.r0 : col0 + 64 * WR <= a.t.r0)) continue;
-    for (int i = threadIdx.x; i < 16 * bk.rank; i += 256) {
-      const int row = i / bk.rank, r = i - row * bk.rank, m = m0 + row;
-      const int id = row_adapter(a, bk, m);
-      float v = 0.0f;
+    const int quads = bk.rank >> 2;
+    for (int i = threadIdx.x; i < 16 * quads; i += 256) {
+      const int row = i / quads, r = (i - row * quads) * 4;
+      const int id = row_adapter(a, bk, m0 + row);
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
       if (id >= 0) {
-        const float* hp = bk.h + (int64_t)m * bk.rank + r;
-        for (int p = 0; p < a.chunks; ++p) v += hp[(int64_t)p * a.t.rows * bk.rank];
-        v *= bk.scale[id];
+        const float* hp = bk.h + (int64_t)(m0 + row) * bk.rank + r;
+        const int64_t step = (int64_t)a.t.rows * bk.rank;
+        const float scale = bk.scale[id];
+#pragma unroll 8
+        for (int p = 0; p < a.chunks; ++p) {
+          const f32x4 h = *reinterpret_cast<const f32x4*>(hp + p * step);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] += h[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= scale;
       }
-      hs[s][row * kStride + r] = v;
+      *reinterpret_cast<f32x4*>(hs[s] + row * kStride + r) = v;
     }
   }
   __syncthreads();
-  const int m = m0 + l16, col = col0 + wave * 16 * WR;
-  const float* part = reinterpret_cast<const float*>(a.t.out) + (int64_t)min(m, a.t.rows - 1) * a.t.groups * a.t.r + 4 * g;
+  if (!cols) return;
+  const int s = col >= a.t.r0, n = s ? a.t.r - a.t.r0 : a.t.r0, at = s ? col - a.t.r0 : col;
+  const Bank& bk = a.bank[s];
+  if (bk.slots)
+    expand_tile<WR>(acc, bk, n, at, row_adapter(a, bk, m), [&](int c, float* v) {
+      const float* from = hs[s] + l16 * kStride + 8 * c;
 #pragma unroll
-  for (int i0 = 0; i0 < WR; ++i0) {
-    // 16 columns at a time where a wave's block may end or cross from the first projection to the second
-    constexpr int kOne = 1;
-    const int c = col + 16 * i0;
-    if (c >= a.t.r) continue;
-    f32x4 acc[kOne];
-    acc[0] = *reinterpret_cast<const f32x4*>(part + c);
-    for (int p = 1; p < a.t.groups; ++p) {
-      const f32x4 v = *reinterpret_cast<const f32x4*>(part + (int64_t)p * a.t.r + c);
+      for (int e = 0; e < 8; ++e) v[e] = from[e];
+    });
+  if (m < a.t.rows)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[0][e] = acc[0][e] + v[e];
-    }
-    const int s = c >= a.t.r0, n = s ? a.t.r - a.t.r0 : a.t.r0, at = s ? c - a.t.r0 : c;
-    const Bank& bk = a.bank[s];
-    if (bk.slots)
-      expand_tile<kOne>(acc, bk, n, at, row_adapter(a, bk, m), [&](int c8, float* v) {
-        const float* from = hs[s] + l16 * kStride + 8 * c8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = from[e];
-      });
-    if (m < a.t.rows) store4<bf16_t>((s ? a.y1 : a.y) + (int64_t)m * n + at + 4 * g, acc[0]);
-  }
+    for (int i = 0; i < WR; ++i) store4<bf16_t>((s ? a.y1 : a.y) + (int64_t)m * n + at + 16 * i + 4 * g, acc[i]);
 }
 
 // ------------------------------------------------------------------ plan
@@ -408,10 +598,10 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
     for (int s = 2; s <= 16; ++s)
       if (t * s <= 256 && k % (64 * s) == 0 && k / s >= 256) p.splits = s;
     p.direct = p.splits == 1;
-    // partial h: enough workgroups to fill the chip, at most 8 of them for the next kernel to sum
+    // beside split sums: enough shares of h to fill the chip, at most 8 of them for the next kernel to sum
     const int64_t items = (int64_t)((rows + 15) / 16) * ((rank + 15) / 16);
     const int parts = (int)(items >= 768 ? 1 : (768 + items - 1) / items > 8 ? 8 : (768 + items - 1) / items);
-    p.chunk = ((k + parts - 1) / parts + 127) / 128 * 128;
+    p.chunk = p.direct ? k : ((k + parts - 1) / parts + 127) / 128 * 128;
   }
   p.chunks = (k + p.chunk - 1) / p.chunk;
   return p;
@@ -425,35 +615,52 @@ static size_t plan_bytes(const AdapterPlan& p, int rows, int n, int rank0, int r
          pad256((size_t)p.chunks * rows * rank1 * sizeof(float));
 }
 
-template <int WR, int WM, int GR, int GM, int BK, int NS, bool DIRECT>
+template <int WR, int WM, int GR, int GM, int BK, int NS, AdapterPart PART>
 static void launch_adapter_tiles(const AdapterArgs& a, int64_t tiles, hipStream_t stream) {
-  hipLaunchKernelGGL((adapter_tiles_kernel<WR, WM, GR, GM, BK, NS, DIRECT>), dim3((unsigned)tiles), dim3(64 * GR * GM), 0,
+  hipLaunchKernelGGL((adapter_tiles_kernel<WR, WM, GR, GM, BK, NS, PART>), dim3((unsigned)tiles), dim3(64 * GR * GM), 0,
                      stream, a);
+}
+
+// Rows and ranks per workgroup of the finished first product.
+static void launch_shrink(const AdapterArgs& a, hipStream_t stream) {
+  const int rank = a.bank[0].rank;
+  auto blocks = [&](int mt, int rt) {
+    return dim3((unsigned)(((a.t.rows + 16 * mt - 1) / (16 * mt)) * ((rank + 16 * rt - 1) / (16 * rt))));
+  };
+  if (rank <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<1, 1, 8>), blocks(1, 1), dim3(512), 0, stream, a);
+  else if (rank <= 32) hipLaunchKernelGGL((adapter_shrink_kernel<2, 2, 8>), blocks(2, 2), dim3(512), 0, stream, a);
+  else hipLaunchKernelGGL((adapter_shrink_kernel<2, 4, 8>), blocks(2, 4), dim3(512), 0, stream, a);
+}
+
+template <int WR, int WM, int GR, int GM, int BK, int NS>
+static void launch_direct_tiles(const AdapterArgs& a, int64_t tiles, hipStream_t stream) {
+  if (a.tokens % (16 * WM) == 0 || a.tokens == a.t.rows) launch_adapter_tiles<WR, WM, GR, GM, BK, NS, kExpandOne>(a, tiles, stream);
+  else launch_adapter_tiles<WR, WM, GR, GM, BK, NS, kExpandAny>(a, tiles, stream);
 }
 
 static void launch_projection(const AdapterArgs& a, const AdapterPlan& p, hipStream_t stream) {
   const int64_t tiles = (int64_t)(a.t.r / p.tr) * ((a.t.rows + p.tm - 1) / p.tm) * p.splits;
   switch (p.tile) {
-    case kRows32: launch_adapter_tiles<1, 1, 2, 2, 64, 8, false>(a, tiles, stream); break;
-    case kRows64: launch_adapter_tiles<1, 2, 2, 2, 64, 6, false>(a, tiles, stream); break;
-    case kRows64Deep: launch_adapter_tiles<1, 2, 2, 2, 64, 8, false>(a, tiles, stream); break;
-    case kRows96: launch_adapter_tiles<1, 3, 2, 2, 64, 8, false>(a, tiles, stream); break;
-    case kRows128: launch_adapter_tiles<1, 4, 2, 2, 64, 4, false>(a, tiles, stream); break;
-    case kWide128: launch_adapter_tiles<4, 2, 2, 2, 64, 4, false>(a, tiles, stream); break;
-    case kWide160: launch_adapter_tiles<5, 2, 2, 2, 64, 4, false>(a, tiles, stream); break;
-    case kTile256: launch_adapter_tiles<8, 4, 2, 4, 64, 2, true>(a, tiles, stream); break;
-    case kTile128: launch_adapter_tiles<4, 4, 2, 2, 64, 2, true>(a, tiles, stream); break;
+    case kRows32: launch_adapter_tiles<1, 1, 2, 2, 64, 8, kSplitSums>(a, tiles, stream); break;
+    case kRows64: launch_adapter_tiles<1, 2, 2, 2, 64, 6, kSplitSums>(a, tiles, stream); break;
+    case kRows64Deep: launch_adapter_tiles<1, 2, 2, 2, 64, 8, kSplitSums>(a, tiles, stream); break;
+    case kRows96: launch_adapter_tiles<1, 3, 2, 2, 64, 8, kSplitSums>(a, tiles, stream); break;
+    case kRows128: launch_adapter_tiles<1, 4, 2, 2, 64, 4, kSplitSums>(a, tiles, stream); break;
+    case kWide128: launch_adapter_tiles<4, 2, 2, 2, 64, 4, kSplitSums>(a, tiles, stream); break;
+    case kWide160: launch_adapter_tiles<5, 2, 2, 2, 64, 4, kSplitSums>(a, tiles, stream); break;
+    case kTile256: launch_direct_tiles<8, 4, 2, 4, 64, 2>(a, tiles, stream); break;
+    case kTile128: launch_direct_tiles<4, 4, 2, 2, 64, 2>(a, tiles, stream); break;
     case kTile128Deep:
-      if (p.direct) launch_adapter_tiles<4, 4, 2, 2, 64, 4, true>(a, tiles, stream);
-      else launch_adapter_tiles<4, 4, 2, 2, 64, 4, false>(a, tiles, stream);
+      if (p.direct) launch_direct_tiles<4, 4, 2, 2, 64, 4>(a, tiles, stream);
+      else launch_adapter_tiles<4, 4, 2, 2, 64, 4, kSplitSums>(a, tiles, stream);
       break;
     case kTile64:
-      if (p.direct) launch_adapter_tiles<2, 4, 2, 2, 64, 3, true>(a, tiles, stream);
-      else launch_adapter_tiles<2, 4, 2, 2, 64, 3, false>(a, tiles, stream);
+      if (p.direct) launch_direct_tiles<2, 4, 2, 2, 64, 3>(a, tiles, stream);
+      else launch_adapter_tiles<2, 4, 2, 2, 64, 3, kSplitSums>(a, tiles, stream);
       break;
     case kTile32:
-      if (p.direct) launch_adapter_tiles<1, 4, 2, 2, 64, 4, true>(a, tiles, stream);
-      else launch_adapter_tiles<1, 4, 2, 2, 64, 4, false>(a, tiles, stream);
+      if (p.direct) launch_direct_tiles<1, 4, 2, 2, 64, 4>(a, tiles, stream);
+      else launch_adapter_tiles<1, 4, 2, 2, 64, 4, kSplitSums>(a, tiles, stream);
       break;
   }
 }
@@ -564,12 +771,11 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   a.chunks = p.chunks;
   a.y = static_cast<bf16_t*>(y0);
   a.y1 = static_cast<bf16_t*>(y1);
-  if (p.direct && shrinks)
-    hipLaunchKernelGGL(adapter_shrink_kernel, dim3((unsigned)shrinks), dim3(256), 0, stream, a);
+  if (p.direct && rank0) launch_shrink(a, stream);
   launch_projection(a, p, stream);
   if (!p.direct) {
     // 256 columns per workgroup where that still gives every CU two of them, 64 otherwise
-    if ((rows + 15) / 16 * ((n + 255) / 256) >= 512)
+    if (n0 % 64 == 0 && n1 % 64 == 0 && (rows + 15) / 16 * ((n + 255) / 256) >= 512)
       hipLaunchKernelGGL(adapter_reduce_kernel<4>, dim3((unsigned)((rows + 15) / 16 * ((n + 255) / 256))), dim3(256), 0,
                          stream, a);
     else hipLaunchKernelGGL(adapter_reduce_kernel<1>, dim3((unsigned)reduces), dim3(256), 0, stream, a);
