@@ -120,12 +120,14 @@ _SIGNATURES = {
                              _i32, _c_p],
     "dsv41_adapter_linear_pair": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _sz,
                                   _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _c_p],
-    "dsv41_cache_move": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _c_p, _c_p, _i32, _i32, _i32, _i32, _c_p],
+    "dsv41_cache_move_workspace_bytes": [_i32, _i32],
+    "dsv41_cache_move": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _c_p, _c_p, _i32, _i32, _i32, _i32, _c_p, _sz, _c_p],
     "dsv41_version": [],
     "dsv41_last_error_string": [],
 }
 _RESTYPES = {
     "dsv41_adapter_add_workspace_bytes": _sz,
+    "dsv41_cache_move_workspace_bytes": _sz,
     "dsv41_adapter_linear_workspace_bytes": _sz,
     "dsv41_sparse_mla_workspace_bytes": _sz,
     "dsv41_linear_rows_workspace_bytes": _sz,
@@ -1384,34 +1386,25 @@ def adapter_linear_pair(x, w0, w1, bank0, bank1, ids, out0=None, out1=None, work
 # ---------------------------------------------------------------------------- cached sequences
 
 
-def _move_index(name, what, index, device, moves=None):
-    if not isinstance(index, torch.Tensor) or index.dtype != torch.int32 or index.dim() != 1 or not index.is_contiguous():
-        raise ValueError(f"{name}: {what} must be a contiguous int32 vector")
-    if index.device != device or (moves is not None and index.numel() != moves):
-        raise ValueError(f"{name}: {what} must hold {moves if moves is not None else 'the'} moves on {device}")
+def _move_index(name, what, index, device, moves):
+    if (not isinstance(index, torch.Tensor) or index.dtype != torch.int32 or index.dim() != 1 or index.numel() != moves
+            or not index.is_contiguous() or index.device != device):
+        raise ValueError(f"{name}: {what} must be a contiguous int32 vector of {moves} moves on {device}")
 
 
-def cache_move(buffers, order, rows, src_rows, dst_rows, same):
-    """dsv41_cache_move over `buffers`: (source tensor, destination tensor, bytes of a sequence, fill word) each, batch
-    first. The caller has checked that a row of either tensor holds that many bytes."""
+def cache_move(src, dst, src_strides, dst_strides, nbytes, fills, order, rows, src_rows, dst_rows, same, device):
+    """dsv41_cache_move over host tables (ctypes arrays, one entry per buffer): pointers and bytes between sequences of
+    both sides, bytes of a sequence that move, the word an emptied row holds. The caller has checked that the buffers
+    hold src_rows and dst_rows sequences of that many bytes."""
     name = "dsv41_cache_move"
-    if not buffers:
-        return
-    device = buffers[0][1].device
-    _move_index(name, "order", order, device)
+    moves = order.numel()
+    _move_index(name, "order", order, device, moves)
     if rows is not None:
-        _move_index(name, "rows", rows, device, order.numel())
+        _move_index(name, "rows", rows, device, moves)
     _gpu(name, order, rows)
-    n = len(buffers)
-    table = (ctypes.c_int64 * (5 * n))()
-    fills = (ctypes.c_uint32 * n)()
-    for i, (s, d, nbytes, fill) in enumerate(buffers):
-        if s.device != device or d.device != device:
-            raise ValueError(f"{name}: buffers on {s.device} and {d.device}")
-        size = s.element_size()
-        table[i], table[n + i] = s.data_ptr(), d.data_ptr()
-        table[2 * n + i], table[3 * n + i], table[4 * n + i] = s.stride(0) * size, d.stride(0) * size, nbytes
-        fills[i] = fill
-    at = ctypes.addressof(table)
-    _call_on(device, name, at, at + 8 * n, at + 16 * n, at + 24 * n, at + 32 * n, ctypes.addressof(fills), n,
-             _ptr(order), _ptr(rows), order.numel(), src_rows, dst_rows, int(same), _stream(order))
+    n = len(nbytes)
+    need = lib().dsv41_cache_move_workspace_bytes(n, moves)
+    ws = _workspace(need, device)
+    at = ctypes.addressof
+    _call_on(device, name, at(src), at(dst), at(src_strides), at(dst_strides), at(nbytes), at(fills), n, _ptr(order),
+             _ptr(rows), moves, src_rows, dst_rows, int(same), _ptr(ws), need, _stream(order))

@@ -42,6 +42,8 @@ reference does (attention.py:127, 163, 166); a cache in the activation dtype is 
 
 from __future__ import annotations
 
+import ctypes
+
 import numpy as np
 import torch
 
@@ -214,25 +216,70 @@ def restore(cache: ModelCache, snap) -> None:
 _MINUS_INF = 0xFF800000
 
 
-def _row_buffers(cache: ModelCache, offset: int):
-    """(layer, name, tensor, visible bytes of a sequence, the word an emptied row holds) of every buffer, for `offset`
-    positions: the ring slots and compressed rows written by then and the open group's state."""
-    for i, lc in enumerate(cache.layers):
-        wp = min(offset, lc.window)
-        groups = offset // lc.ratio if lc.is_kv_source else 0
-        blocks = -(-groups // lc.fp8_rb)
-        for name in _BUFFERS:
-            t = getattr(lc, name)
-            if t is None:
-                continue
-            rows = wp if name in ("win_kv", "win_kv8") else blocks if name in ("comp_ks", "index_k8s") else groups
-            if rows > t.shape[1]:
-                raise ValueError(f"layer {i}: {name} holds {t.shape[1]} of the {rows} rows that {offset} positions take")
-            yield i, name, t, rows * t.shape[2] * t.element_size(), 0
-        if lc.comp_state is not None:
-            for name, fill in (("kv_state", 0), ("score_state", _MINUS_INF)):
-                t = getattr(lc.comp_state, name)
-                yield i, name, t, t.shape[1] * t.shape[2] * t.element_size(), fill
+class _RowTable:
+    """A cache's buffers as moves of sequences take them: one entry per buffer, in layer order. Kept on the ModelCache
+    and built again when one of the buffers is another tensor or lies elsewhere."""
+
+    def __init__(self, cache: ModelCache):
+        self.at, self.tensors, self.layout, self.rows, self.width, fills = [], [], [], [], [], []
+        self.need = {}                     # (what the rows count, ratio, rows per scale) -> fewest rows of such a buffer
+        for i, lc in enumerate(cache.layers):
+            for name in _BUFFERS + ("kv_state", "score_state"):
+                holder = lc.comp_state if name.endswith("_state") else lc
+                t = getattr(holder, name) if holder is not None else None
+                if t is None:
+                    continue
+                if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+                    raise ValueError(f"layer {i}: {name} {tuple(t.shape)} must be [sequences, rows, channels] with dense rows")
+                kind = ("state", t.shape[1], 1) if name.endswith("_state") else ("ring", lc.window, 1) if name.startswith(
+                    "win") else ("comp", lc.ratio, lc.fp8_rb if name in ("comp_ks", "index_k8s") else 1)
+                self.at.append((holder, name))
+                self.tensors.append(t)
+                self.layout.append((i, name, t.dtype, t.shape[2], kind))
+                self.rows.append(kind)
+                self.width.append(t.shape[2] * t.element_size())
+                self.need[kind] = min(self.need.get(kind, t.shape[1]), t.shape[1])
+                fills.append(_MINUS_INF if name == "score_state" else 0)
+        if not self.tensors:
+            raise ValueError("a cache without buffers")
+        self.batch, self.device = self.tensors[0].shape[0], self.tensors[0].device
+        for (i, name, *_), t in zip(self.layout, self.tensors):
+            if t.shape[0] != self.batch or t.device != self.device:
+                raise ValueError(f"layer {i}: {name} {tuple(t.shape)} on {t.device} in a cache of {self.batch} sequences on "
+                                 f"{self.device}")
+        self.where = [(t.data_ptr(), t.numel()) for t in self.tensors]
+        n = len(self.tensors)
+        self.pointers = (ctypes.c_int64 * n)(*(p for p, _ in self.where))
+        self.strides = (ctypes.c_int64 * n)(*(t.stride(0) * t.element_size() for t in self.tensors))
+        self.fills = (ctypes.c_uint32 * n)(*fills)
+
+    def current(self) -> bool:
+        return (all(getattr(o, n) is t for (o, n), t in zip(self.at, self.tensors))
+                and [(t.data_ptr(), t.numel()) for t in self.tensors] == self.where)
+
+    def check(self, offset: int) -> dict:
+        """Rows that `offset` positions have written, by kind of buffer: ring slots, compressed rows (or their scale
+        blocks), the open group's state."""
+        rows = {}
+        for kind, held in self.need.items():
+            what, per, block = kind
+            n = per if what == "state" else min(offset, per) if what == "ring" else -(-(offset // per) // block)
+            if n > held:
+                raise ValueError(f"a buffer holds {held} of the {n} rows that {offset} positions take")
+            rows[kind] = n
+        return rows
+
+    def visible(self, offset: int):
+        """Bytes of a sequence that move, buffer by buffer."""
+        rows = self.check(offset)
+        return (ctypes.c_int64 * len(self.rows))(*[rows[k] * w for k, w in zip(self.rows, self.width)])
+
+
+def _row_table(cache: ModelCache) -> _RowTable:
+    table = cache.__dict__.get("_row_table")
+    if table is None or not table.current():
+        table = cache._row_table = _RowTable(cache)
+    return table
 
 
 def _index(what: str, values, rows: int, low: int, device) -> torch.Tensor:
@@ -246,50 +293,41 @@ def _index(what: str, values, rows: int, low: int, device) -> torch.Tensor:
     return torch.tensor(values, dtype=torch.int32, device=device)
 
 
-def _batch_rows(what: str, buffers) -> int:
-    n = buffers[0][2].shape[0]
-    for i, name, t, _, _ in buffers:
-        if t.shape[0] != n or t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
-            raise ValueError(f"{what}: layer {i}'s {name} {tuple(t.shape)} must be [{n}, rows, channels] with dense rows")
-    return n
-
-
 def _move(what: str, dst: ModelCache, src: ModelCache, order, rows) -> None:
     same = dst is src
-    theirs = list(_row_buffers(src, src.offset))
-    ours = theirs if same else list(_row_buffers(dst, src.offset))
-    if [(i, n, t.dtype, t.shape[2], w) for i, n, t, w, _ in ours] != [(i, n, t.dtype, t.shape[2], w)
-                                                                     for i, n, t, w, _ in theirs]:
-        raise ValueError(f"{what}: the caches differ in layers, formats or widths")
-    if not same and any(a.ratio != b.ratio or a.window != b.window or a.fp8_rb != b.fp8_rb
-                        for a, b in zip(dst.layers, src.layers)):
-        raise ValueError(f"{what}: the caches differ in ratios, windows or scale blocks")
-    if (dst.engram_ids is None) != (src.engram_ids is None):
-        raise ValueError(f"{what}: one of the caches keeps engram ids")
-    dst_rows = _batch_rows(what, ours)
-    src_rows = dst_rows if same else _batch_rows(what, theirs)
-    device = ours[0][2].device
-    order = _index(f"{what}: order", order, src_rows, -1, device)
+    theirs = _row_table(src)
+    ours = theirs if same else _row_table(dst)
+    if not same:
+        if ours.layout != theirs.layout:
+            raise ValueError(f"{what}: the caches differ in layers, formats, widths or ratios")
+        if ours.device != theirs.device:
+            raise ValueError(f"{what}: caches on {ours.device} and {theirs.device}")
+        if (dst.engram_ids is None) != (src.engram_ids is None):
+            raise ValueError(f"{what}: one of the caches keeps engram ids")
+        ours.check(src.offset)
+    visible = theirs.visible(src.offset)
+    order = _index(f"{what}: order", order, theirs.batch, -1, ours.device)
     if rows is not None:
-        rows = _index(f"{what}: rows", rows, dst_rows, 0, device)
-    if rows is None and order.numel() > dst_rows:
-        raise ValueError(f"{what}: {order.numel()} rows into a cache of {dst_rows}")
-    whole = rows is None and order.numel() == dst_rows
-    if dst.offset != src.offset and not whole:
+        rows = _index(f"{what}: rows", rows, ours.batch, 0, ours.device)
+    elif order.numel() > ours.batch:
+        raise ValueError(f"{what}: {order.numel()} rows into a cache of {ours.batch}")
+    if dst.offset != src.offset and (rows is not None or order.numel() != ours.batch):
         raise ValueError(f"{what}: a cache at position {src.offset} gives single rows to one at {dst.offset}")
-    if dst.engram_ids is not None:
+    engram = dst.engram_ids is not None
+    if engram:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{what}: engram ids live on the host, their order cannot be captured")
         if src.offset > dst.engram_ids.shape[1]:
             raise ValueError(f"{what}: {src.offset} positions into engram ids of {dst.engram_ids.shape[1]}")
-    _abi.cache_move([(s[2], d[2], s[3], s[4]) for s, d in zip(theirs, ours)], order, rows, src_rows, dst_rows, same)
-    if dst.engram_ids is not None:         # host memory: this waits for order and rows
+    _abi.cache_move(theirs.pointers, ours.pointers, theirs.strides, ours.strides, visible, ours.fills, order, rows,
+                    theirs.batch, ours.batch, same, ours.device)
+    if engram:                             # host memory: this waits for order and rows
         o = order.cpu().numpy()
         r = np.arange(len(o)) if rows is None else rows.cpu().numpy()
         old = src.engram_ids[:, :src.offset].copy()
         for s, d in zip(o, r):
-            if 0 <= d < dst_rows:
-                dst.engram_ids[d, :src.offset] = old[s] if 0 <= s < src_rows else 0
+            if 0 <= d < ours.batch:
+                dst.engram_ids[d, :src.offset] = old[s] if 0 <= s < theirs.batch else 0
     dst.offset = src.offset
 
 

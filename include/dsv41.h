@@ -607,11 +607,14 @@ int dsv41_adapter_linear_pair(const void* x, const void* w0, const void* w1, con
  * [0, src_rows) empties the row: its bytes[b] bytes become the word fill[b] (low byte first). A rows
  * entry outside [0, dst_rows) moves nothing; of several moves to one row the last counts. order and
  * rows: int32 on the device. src, dst, the strides (bytes between sequences), bytes and fill: host
- * arrays of `buffers` entries, read during the call. moves and dst_rows at most 4,096. */
+ * arrays of `buffers` entries, read during the call. moves and dst_rows at most 4,096. The workspace holds
+ * the call's table and list until its kernels have run. */
+size_t dsv41_cache_move_workspace_bytes(int32_t buffers, int32_t moves);
 int dsv41_cache_move(const void* const* src, void* const* dst, const int64_t* src_stride,
                      const int64_t* dst_stride, const int64_t* bytes, const uint32_t* fill, int32_t buffers,
                      const int32_t* order, const int32_t* rows, int32_t moves, int32_t src_rows,
-                     int32_t dst_rows, int32_t same, hipStream_t stream);
+                     int32_t dst_rows, int32_t same, void* workspace, size_t workspace_bytes,
+                     hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -245,9 +245,14 @@ def test_c_entry_points_refuse_bad_sizes():
     i64 = lambda v: (ctypes.c_int64 * 1)(v)      # noqa: E731
     fill = (ctypes.c_uint32 * 1)(0)
 
-    def move(src=ptrs, dst=ptrs, nbytes=16, buffers=1, order=p, rows=None, moves=1, src_rows=1, dst_rows=1):
+    def move(src=ptrs, dst=ptrs, nbytes=16, buffers=1, order=p, rows=None, moves=1, src_rows=1, dst_rows=1, ws=p,
+             size=1 << 20):
         return lib.dsv41_cache_move(src, dst, i64(16), i64(16), i64(nbytes), fill, buffers, order, rows, moves, src_rows,
-                                    dst_rows, 1, None)
+                                    dst_rows, 1, ws, size, None)
+
+    need = lib.dsv41_cache_move_workspace_bytes(1, 1)
+    assert need > 0 and move(size=need - 1) == -4 and move(ws=None) == -4 and move(ws=ctypes.c_void_p(4104)) == -4
+    assert lib.dsv41_cache_move_workspace_bytes(0, 1) == lib.dsv41_cache_move_workspace_bytes(1, 0) == 0
 
     assert move(buffers=0) == 0 and move(moves=0) == 0 and move(nbytes=0) == 0
     for bad in (dict(buffers=-1), dict(moves=-1), dict(src_rows=0), dict(dst_rows=0), dict(nbytes=-1), dict(order=None),
