@@ -409,20 +409,34 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
 enum AdapterPart { kSplitSums, kExpandOne, kExpandAny };
 
 template <int WR, int WM, int GR, int GM, int BK, int NS, AdapterPart PART>
-__global__ __launch_bounds__(64 * GR * GM, (TileCfg<WR, WM, GR, GM, BK, NS>::LDS <= 72 * 1024) ? 2 : 1) void
+__global__ __launch_bounds__(64 * GR * GM, (TileCfg<WR, WM, GR, GM, BK, NS>::LDS <= 73 * 1024) ? 2 : 1) void
 adapter_tiles_kernel(AdapterArgs a) {
   using C = TileCfg<WR, WM, GR, GM, BK, NS>;
   __shared__ __align__(16) uint8_t lds[C::LDS];
-  const int mtiles = (a.t.rows + C::TM - 1) / C::TM, rtiles = a.t.r / C::TR;
-  // consecutive tiles on one XCD, the weight tile fastest, as the output projection's
-  const int total = (int)gridDim.x;
-  const int tile = total % 8 ? (int)blockIdx.x : ((int)blockIdx.x % 8) * (total / 8) + (int)blockIdx.x / 8;
-  const int rt = tile % rtiles, mt = (tile / rtiles) % mtiles, grp = tile / (rtiles * mtiles);
+  const int mtiles = (a.t.rows + C::TM - 1) / C::TM, rtiles = a.t.r / C::TR, total = (int)gridDim.x;
+  int rt, mt, grp = 0;
+  if constexpr (PART == kSplitSums) {
+    // consecutive tiles on one XCD, the weight tile fastest, as the output projection's
+    const int tile = total % 8 ? (int)blockIdx.x : ((int)blockIdx.x % 8) * (total / 8) + (int)blockIdx.x / 8;
+    rt = tile % rtiles;
+    mt = (tile / rtiles) % mtiles;
+    grp = tile / (rtiles * mtiles);
+  } else {
+    // consecutive tiles on one XCD, in bands of 4 query tiles: 32 CUs work on 4 x 8 tiles and share their 12 operand
+    // panels in the XCD's L2, where 1 x 32 tiles read 33 (TIMING)
+    constexpr int kBand = 4;
+    const int xcd = (int)blockIdx.x % 8, per = total / 8, more = total % 8;
+    const int tile = xcd * per + min(xcd, more) + (int)blockIdx.x / 8;
+    const int band = tile / (kBand * rtiles), in = tile - band * kBand * rtiles, width = min(kBand, mtiles - band * kBand);
+    rt = in / width;
+    mt = band * kBand + in - rt * width;
+  }
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wr = (wave % GR) * 16 * WR, wm = (wave / GR) * 16 * WM;   // this wave's block
   f32x4 acc[WR][WM];
   if constexpr (PART != kSplitSums) {
-    tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc);
+    if constexpr (BK == 64 && NS == 2) tile_sums_ahead<WR, WM, GR, GM>(a.t, lds, rt, mt, grp, acc);
+    else tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc);
 #pragma unroll
     for (int i = 0; i < WR; ++i) settle(acc[i]);
     const int col = rt * C::TR + wr;
@@ -430,21 +444,31 @@ adapter_tiles_kernel(AdapterArgs a) {
 #pragma unroll
     for (int j = 0; j < WM; ++j) {
       const int m = mt * C::TM + wm + 16 * j + l16;
-      if (m >= a.t.rows) continue;
+      bf16_t* to = a.y + (int64_t)m * a.t.r + col;
+      // the swaps of a pair need every lane: a row past the end gives the store up after them
 #pragma unroll
-      for (int i = 0; i < WR; ++i) store4<bf16_t>(a.y + (int64_t)m * a.t.r + col + 16 * i + 4 * g, acc[i][j]);
+      for (int i = 0; i + 1 < WR; i += 2) {
+        uint4 v = pair_of(acc[i][j], acc[i + 1][j]);
+        if (m < a.t.rows) *reinterpret_cast<uint4*>(to + 16 * i + 16 * (g & 1) + 8 * (g >> 1)) = v;
+      }
+      if constexpr (WR % 2 != 0)
+        if (m < a.t.rows) store4<bf16_t>(to + 16 * (WR - 1) + 4 * g, acc[WR - 1][j]);
     }
   } else {
     static_assert(GR * GM == 4, "a partial h is the work of four waves");
     __shared__ __align__(16) float red[4 * 256];
-    tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc, [&]() {
+    auto beside = [&]() {
       const int items0 = shrink_items(a, a.bank[0]), items = items0 + shrink_items(a, a.bank[1]);
       for (int it = blockIdx.x; it < items; it += total)
         if (it < items0) shrink_item(a, a.bank[0], it, red);
         else shrink_item(a, a.bank[1], it - items0, red);
       // the ring's waits count its own copies only
       if ((int)blockIdx.x < items) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    });
+    };
+    if constexpr (BK == 64 && NS == 2) tile_sums_ahead<WR, WM, GR, GM>(a.t, lds, rt, mt, grp, acc, beside);
+    else tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc, beside);
+#pragma unroll
+    for (int i = 0; i < WR; ++i) settle(acc[i]);
     const int64_t ostride = (int64_t)a.t.groups * a.t.r;
     float* out = reinterpret_cast<float*>(a.t.out);
 #pragma unroll
@@ -525,7 +549,7 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
 
 // ------------------------------------------------------------------ plan
 
-enum AdapterTile { kRows32, kRows64, kRows64Deep, kRows96, kRows128, kWide128, kWide160, kTile256, kTile128, kTile128Deep,
+enum AdapterTile { kRows32, kRows64, kRows64Deep, kRows96, kRows128, kWide128, kWide160, kTile256, kTile160, kTile128,
                    kTile64, kTile32 };
 
 struct AdapterPlan {
@@ -576,27 +600,42 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
     }
     p.chunk = 256;
   } else {
-    auto tiles = [&](int tr, int tm) { return n % tr ? 0 : (int64_t)(n / tr) * ((rows + tm - 1) / tm); };
-    p.tm = 128;
-    if (tiles(256, 256) >= 192) {
-      p.tile = kTile256;
-      p.tr = p.tm = 256;
-    } else if (tiles(128, 128) > 256) {
-      p.tile = kTile128;
-      p.tr = 128;
-    } else if (n % 128 == 0) {
-      p.tile = kTile128Deep;
-      p.tr = 128;
-    } else if (n % 64 == 0) {
-      p.tile = kTile64;
-      p.tr = 64;
-    } else {
-      p.tile = kTile32;
-      p.tr = 32;
+    // The shape and ranges whose estimate is the least. A tile's time is fixed us (prologue, first loads, epilogue) and
+    // us per 64-channel step, alone on its CU or as one of two; measured on 4096 rows of 1280 -> 32768 (20 steps), 8192
+    // of 8192 -> 5120 (128) and single tiles of 5120 channels (80).
+    struct Shape {
+      AdapterTile tile;
+      int tr, tm;
+      double fixed, alone, paired;     // paired 0: one per CU
+      bool split;
+    };
+    static const Shape shapes[] = {{kTile256, 256, 256, 15.0, 1.65, 0.0, false},
+                                   {kTile160, 160, 128, 8.0, 0.80, 1.29, true},
+                                   {kTile128, 128, 128, 7.6, 0.71, 1.04, true},
+                                   {kTile64, 64, 128, 4.3, 0.51, 0.67, true},
+                                   {kTile32, 32, 128, 4.0, 0.45, 0.45, true}};
+    double best = 1e30;
+    for (const Shape& s : shapes) {
+      if (n % s.tr) continue;
+      const int64_t tiles = (int64_t)(n / s.tr) * ((rows + s.tm - 1) / s.tm);
+      for (int splits = 1; splits <= (s.split ? 16 : 1); ++splits) {
+        if (k % (64 * splits) || (splits > 1 && tiles * splits > 512)) continue;
+        const int64_t t = tiles * splits;
+        const double steps = k / 64 / splits;
+        const int64_t full = s.paired > 0 ? t / 512 : t / 256, left = t - full * (s.paired > 0 ? 512 : 256);
+        double us = full * (s.fixed + steps * (s.paired > 0 ? s.paired : s.alone));
+        if (left) us += s.fixed + steps * (left > 256 ? s.paired : s.alone);
+        // apart: the finished first product before the tiles, or the parts' way through memory after them
+        us += splits == 1 ? 8.0 : 6.0 + (double)rows * n * splits * 8e-6 / 4.5;
+        if (us < best) {
+          best = us;
+          p.tile = s.tile;
+          p.tr = s.tr;
+          p.tm = s.tm;
+          p.splits = splits;
+        }
+      }
     }
-    const int64_t t = tiles(p.tr, p.tm);
-    for (int s = 2; s <= 16; ++s)
-      if (t * s <= 256 && k % (64 * s) == 0 && k / s >= 256) p.splits = s;
     p.direct = p.splits == 1;
     // beside split sums: enough shares of h to fill the chip, at most 8 of them for the next kernel to sum
     const int64_t items = (int64_t)((rows + 15) / 16) * ((rank + 15) / 16);
@@ -649,10 +688,13 @@ static void launch_projection(const AdapterArgs& a, const AdapterPlan& p, hipStr
     case kWide128: launch_adapter_tiles<4, 2, 2, 2, 64, 4, kSplitSums>(a, tiles, stream); break;
     case kWide160: launch_adapter_tiles<5, 2, 2, 2, 64, 4, kSplitSums>(a, tiles, stream); break;
     case kTile256: launch_direct_tiles<8, 4, 2, 4, 64, 2>(a, tiles, stream); break;
-    case kTile128: launch_direct_tiles<4, 4, 2, 2, 64, 2>(a, tiles, stream); break;
-    case kTile128Deep:
-      if (p.direct) launch_direct_tiles<4, 4, 2, 2, 64, 4>(a, tiles, stream);
-      else launch_adapter_tiles<4, 4, 2, 2, 64, 4, kSplitSums>(a, tiles, stream);
+    case kTile160:
+      if (p.direct) launch_direct_tiles<5, 4, 2, 2, 64, 2>(a, tiles, stream);
+      else launch_adapter_tiles<5, 4, 2, 2, 64, 2, kSplitSums>(a, tiles, stream);
+      break;
+    case kTile128:
+      if (p.direct) launch_direct_tiles<4, 4, 2, 2, 64, 2>(a, tiles, stream);
+      else launch_adapter_tiles<4, 4, 2, 2, 64, 2, kSplitSums>(a, tiles, stream);
       break;
     case kTile64:
       if (p.direct) launch_direct_tiles<2, 4, 2, 2, 64, 3>(a, tiles, stream);

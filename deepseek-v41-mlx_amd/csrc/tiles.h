@@ -17,6 +17,15 @@ struct WoaArgs {
   int r0;              // (two weights applied to the same rows; r0 a multiple of the tile's rows)
 };
 
+// Two 16 x 16 tiles of results side by side (lane (g, l16): columns 4 g .. 4 g + 3 of row l16 of each) as bf16: after two
+// row swaps a lane holds columns 8 (g / 2) .. + 7 of tile g % 2, so that a row's 32 columns are one 64-byte store of its
+// four lanes. Swaps use every lane.
+__device__ __forceinline__ uint4 pair_of(f32x4 v0, f32x4 v1) {
+  const auto lo = __builtin_amdgcn_permlane16_swap(pack2_bf16(v0[0], v0[1]), pack2_bf16(v1[0], v1[1]), false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(pack2_bf16(v0[2], v0[3]), pack2_bf16(v1[2], v1[3]), false, false);
+  return make_uint4(lo[0], hi[0], lo[1], hi[1]);
+}
+
 // Four consecutive outputs of one query row.
 template <typename TO>
 __device__ __forceinline__ void store4(TO* p, f32x4 v);
@@ -184,6 +193,90 @@ __device__ __forceinline__ void tile_sums(const WoaArgs& a, uint8_t* lds, int rt
 #pragma unroll
         for (int j = 0; j < WM; ++j) acc[i][j] = mfma16x16x32(af[i], bf[j], acc[i][j]);
     }
+  }
+}
+
+// tile_sums for large tiles of one projection (the split form, w1 null; two ring stages of 64 channels): the fragments of each
+// 32-channel half step are read while the half before is multiplied, across the step's barrier too. Half way through a
+// step every wave has its second half in registers, so the barrier there frees the step's stage for the copies of the
+// step after next, which then have a whole step to land. Same order of additions as tile_sums.
+template <int WR, int WM, int GR, int GM, typename Beside = NothingBeside>
+__device__ __forceinline__ void tile_sums_ahead(const WoaArgs& a, uint8_t* lds, int rt, int mt, int grp,
+                                                f32x4 (&acc)[WR][WM], Beside beside = Beside()) {
+  using C = TileCfg<WR, WM, GR, GM, 64, 2>;
+  constexpr int kRowsW = C::TR / C::NWV, kRowsO = C::TM / C::NWV;   // tile rows that a wave copies, 8 at a time
+  static_assert(kRowsW % 8 == 0 && kRowsO % 8 == 0, "whole copy instructions per wave");
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int wr = (wave % GR) * 16 * WR, wm = (wave / GR) * 16 * WM;
+  const uint32_t row_bytes = (uint32_t)a.groups * (uint32_t)a.d * 2;
+  // copy sources: a wave-uniform base per copy, the lane's row and swizzled chunk (tile_swz of 8 rows from a multiple
+  // of 8: the row's low bits and the multiple's parity) as a 32-bit offset
+  uint32_t woff[2], ooff[C::NO];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    woff[j] = (uint32_t)(lane >> 3) * row_bytes + 16u * (uint32_t)((lane & 7) ^ (lane >> 3) ^ ((wave * (kRowsW / 8) + j) & 1));
+#pragma unroll
+  for (int j = 0; j < C::NO; ++j) {
+    const int row = wave * kRowsO + 8 * j + (lane >> 3);
+    ooff[j] = (uint32_t)min(row, a.rows - 1 - mt * C::TM) * row_bytes + 16u * (uint32_t)((lane & 7) ^ tile_swz<64>(row));
+  }
+  const int uwave = __builtin_amdgcn_readfirstlane(wave);
+  const uint64_t range = (uint64_t)grp * a.d * 2;
+  const uint64_t wbase = reinterpret_cast<uint64_t>(a.w) + range + ((uint64_t)rt * C::TR + (uint64_t)uwave * kRowsW) * row_bytes;
+  const uint64_t obase = reinterpret_cast<uint64_t>(a.o) + range + (uint64_t)mt * C::TM * row_bytes;
+  const uint32_t lds0 = lds_offset(lds);
+  auto issue = [&](int stage, int kt) {
+    const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + (uint32_t)(stage * C::STAGE)));
+    const uint64_t kb = (uint64_t)kt * C::RB;
+#pragma unroll
+    for (int j = 0; j < C::NW; ++j)
+      dma16_sgpr(wbase + kb + (uint64_t)(8 * j) * row_bytes, woff[j & 1], at + (uint32_t)((uwave * kRowsW + 8 * j) * C::RB));
+#pragma unroll
+    for (int j = 0; j < C::NO; ++j)
+      dma16_sgpr(obase + kb, ooff[j], at + (uint32_t)(C::TR * C::RB + (uwave * kRowsO + 8 * j) * C::RB));
+  };
+  const int swz = (l16 & 7) ^ (l16 >> 3);
+  const uint8_t* wl = lds + (wr + l16) * C::RB;
+  const uint8_t* ol = lds + C::TR * C::RB + (wm + l16) * C::RB;
+  auto read = [&](int stage, int half, bf16x8 (&af)[WR], bf16x8 (&bf)[WM]) {
+    const int at = stage * C::STAGE + (((4 * half + g) ^ swz) << 4);
+#pragma unroll
+    for (int i = 0; i < WR; ++i) af[i] = as_bf16x8(*reinterpret_cast<const uint4*>(wl + at + 16 * i * C::RB));
+#pragma unroll
+    for (int j = 0; j < WM; ++j) bf[j] = as_bf16x8(*reinterpret_cast<const uint4*>(ol + at + 16 * j * C::RB));
+  };
+  auto multiply = [&](const bf16x8 (&af)[WR], const bf16x8 (&bf)[WM]) {
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < WR; ++i)
+#pragma unroll
+      for (int j = 0; j < WM; ++j) acc[i][j] = mfma16x16x32(af[i], bf[j], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+#pragma unroll
+  for (int i = 0; i < WR; ++i)
+#pragma unroll
+    for (int j = 0; j < WM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  const int nk = a.d / 64;
+  bf16x8 a0[WR], b0[WM], a1[WR], b1[WM];
+  issue(0, 0);
+  if (nk > 1) issue(1, 1);
+  beside();
+  if (nk > 1) wait_vmcnt<C::NW + C::NO>();
+  else wait_vmcnt<0>();
+  __syncthreads();
+  read(0, 0, a0, b0);
+  for (int kt = 0; kt < nk; ++kt) {
+    const int stage = kt & 1;
+    read(stage, 1, a1, b1);
+    multiply(a0, b0);
+    // step kt + 1, issued a step ago, has landed, and this wave has read stage `stage`; then every wave's
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (kt + 2 < nk) issue(stage, kt + 2);
+    if (kt + 1 < nk) read(stage ^ 1, 0, a0, b0);
+    multiply(a1, b1);
   }
 }
 
