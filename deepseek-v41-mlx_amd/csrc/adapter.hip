@@ -74,6 +74,7 @@ struct AdapterArgs {
   const int32_t* ids;    // [rows / tokens]
   int tokens, k;
   int chunk, chunks;     // channels of one partial h, and how many
+  int sub;               // rows of a share of it: 4 or 16
   bf16_t* y;             // [rows, t.r0]
   bf16_t* y1;            // [rows, t.r - t.r0]
 };
@@ -91,38 +92,54 @@ __device__ __forceinline__ int next_adapter(uint32_t& todo, int id) {
   return t;
 }
 
-// Partial x A^T of 16 rows, one chunk of channels, 16 ranks: the chunk's 32-channel steps in turn over the workgroup's
-// four waves. Rows are the MFMA's columns, so every adapter of the tile multiplies all 16 of them and each lane keeps
-// the product with its own row's: nothing another row's adapter holds can reach it. Up to U adapters at once keep that
-// many loads in flight.
+__device__ __forceinline__ bf16x8 or_zero(uint4 v, bool live) {
+  return as_bf16x8(live ? v : make_uint4(0, 0, 0, 0));
+}
+
+// Partial x A^T of `sub` rows (4 or 16), one chunk of channels, 16 ranks: the chunk's 32-channel steps in turn over the
+// workgroup's four waves. Rows are the MFMA's columns, so every adapter of the tile multiplies all of them and each lane
+// keeps the product with its own row's: nothing another row's adapter holds can reach it. U adapters and four steps at
+// once keep that many loads in flight; a step past the end multiplies nothing.
 template <int U>
 __device__ __forceinline__ void shrink_steps(const bf16_t* xp, const bf16_t* const (&ap)[U], int first, int steps,
                                              f32x4 (&acc)[U]) {
 #pragma unroll
   for (int u = 0; u < U; ++u) acc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int s = first; s < steps; s += 4) {
-    const bf16x8 xf = ld_bf16x8(xp + 32 * s);
+  for (int s = first; s < steps; s += 16) {
+    uint4 xf[4], af[4][U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) acc[u] = mfma16x16x32(ld_bf16x8(ap[u] + 32 * s), xf, acc[u]);
+    for (int e = 0; e < 4; ++e) {
+      const int at = 32 * min(s + 4 * e, steps - 1);
+      xf[e] = *reinterpret_cast<const uint4*>(xp + at);
+#pragma unroll
+      for (int u = 0; u < U; ++u) af[e][u] = *reinterpret_cast<const uint4*>(ap[u] + at);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool live = s + 4 * e < steps;
+#pragma unroll
+      for (int u = 0; u < U; ++u) acc[u] = mfma16x16x32(or_zero(af[e][u], live), or_zero(xf[e], live), acc[u]);
+    }
   }
   settle(acc);
 }
 
 __device__ __forceinline__ int shrink_items(const AdapterArgs& a, const Bank& bk) {
-  return bk.slots ? (a.t.rows + 15) / 16 * a.chunks * ((bk.rank + 15) / 16) : 0;
+  return bk.slots ? (a.t.rows + a.sub - 1) / a.sub * a.chunks * ((bk.rank + 15) / 16) : 0;
 }
 
 __device__ __forceinline__ void shrink_item(const AdapterArgs& a, const Bank& bk, int item, float* red) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int ranks = (bk.rank + 15) / 16;
   const int rq = item % ranks, chunk = item / ranks % a.chunks, tile = item / ranks / a.chunks;
-  const int id = row_adapter(a, bk, tile * 16 + l16);
+  const int m0 = tile * a.sub + (l16 & (a.sub - 1));       // 4 rows: each four times
+  const int id = row_adapter(a, bk, m0);
   const int k0 = chunk * a.chunk, steps = min(a.chunk, a.k - k0) / 32;
-  const bf16_t* xp = a.t.o + (int64_t)min(tile * 16 + l16, a.t.rows - 1) * a.k + k0 + 8 * g;
+  const bf16_t* xp = a.t.o + (int64_t)min(m0, a.t.rows - 1) * a.k + k0 + 8 * g;
   const int64_t arow = (int64_t)min(rq * 16 + l16, bk.rank - 1) * a.k + k0 + 8 * g;   // ranks past the end: not stored
   const int64_t slot = (int64_t)bk.rank * a.k;
   f32x4 res = {0.f, 0.f, 0.f, 0.f};
-  uint32_t todo = (uint32_t)__ballot(id >= 0) & 0xFFFFu;
+  uint32_t todo = (uint32_t)__ballot(id >= 0) & ((1u << a.sub) - 1u);
   while (todo) {
     int t[4];
     t[0] = next_adapter(todo, id);
@@ -145,8 +162,8 @@ __device__ __forceinline__ void shrink_item(const AdapterArgs& a, const Bank& bk
   // the four waves' sums, in order; lane (g, l16) holds ranks 4 g .. 4 g + 3 of row l16
   *reinterpret_cast<f32x4*>(red + (wave * 16 + l16) * 16 + 4 * g) = res;
   __syncthreads();
-  const int row = threadIdx.x >> 4, r = rq * 16 + (threadIdx.x & 15), m = tile * 16 + row;
-  if (m < a.t.rows && r < bk.rank) {
+  const int row = threadIdx.x >> 4, r = rq * 16 + (threadIdx.x & 15), m = tile * a.sub + row;
+  if (row < a.sub && m < a.t.rows && r < bk.rank) {
     float s = red[threadIdx.x];
 #pragma unroll
     for (int w = 1; w < 4; ++w) s += red[w * 256 + threadIdx.x];
@@ -182,10 +199,6 @@ struct RankSlot {
     c = live ? (low ? s - r8 : s) : 0;
   }
 };
-
-__device__ __forceinline__ bf16x8 or_zero(uint4 v, bool live) {
-  return as_bf16x8(live ? v : make_uint4(0, 0, 0, 0));
-}
 
 // The whole first product of 16 MT rows and 16 RT ranks: the channels in 64-wide steps in turn over NW waves, each
 // step's x rows read once for all ranks and each adapter row once for all x rows; the waves' sums meet in LDS. Writes
@@ -281,54 +294,73 @@ __global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(AdapterArgs a) 
   }
 }
 
-// One MFMA step of acc[i] += h B^T for WR tiles of 16 output columns and U adapters of a tile of 16 rows. Rows are the
-// MFMA's columns: each adapter multiplies all of them, a lane keeps its own row's.
+// The second product for 16 rows (lane l16's, adapter id) and WR tiles of 16 output columns, in steps of one rank group
+// (32 of the 2 rank operands) and up to U adapters, each step's B loaded a step ahead; the first one's before the
+// caller has h at all. Rows are the MFMA's columns: each adapter multiplies all of them, a lane keeps its own row's.
 template <int WR, int U>
-__device__ __forceinline__ void expand_step(f32x4 (&acc)[WR], const bf16_t* bp, int64_t slot, int rank, bool live,
-                                            bf16x8 hf, int id, const int (&t)[U]) {
-  uint4 b[U][WR];
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int i = 0; i < WR; ++i) b[u][i] = *reinterpret_cast<const uint4*>(bp + t[u] * slot + (int64_t)16 * i * rank);
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-#pragma unroll
-    for (int i = 0; i < WR; ++i) {
-      const f32x4 sum = mfma16x16x32(or_zero(b[u][i], live), hf, acc[i]);
-      acc[i] = id == t[u] && (u == 0 || t[u] != t[0]) ? sum : acc[i];
-    }
-}
+struct Expand {
+  const bf16_t* b;       // slot 0, the lane's first output column
+  int64_t slot;
+  int rank, id;
+  uint32_t named, todo;  // rows with an adapter; those whose adapter is still to come in this rank group
+  int q;                 // the rank group
+  int t[U];
+  uint4 next[U][WR];
 
-// acc[i] += scale (h B^T) for 16 rows (lane l16's, adapter id) and the output columns col + 16 i + l16. hval(c, v)
-// gives scale times ranks 8 c .. 8 c + 7 of the lane's row. Up to four adapters' B are in flight at once.
-template <int WR, typename H>
-__device__ __forceinline__ void expand_tile(f32x4 (&acc)[WR], const Bank& bk, int n, int col, int id, H hval) {
-  const int r8 = bk.rank >> 3;
-  const int64_t slot = (int64_t)n * bk.rank;
-  const uint32_t named = (uint32_t)__ballot(id >= 0) & 0xFFFFu;
-  if (named == 0) return;
-  for (int q = 0; q < 2 * r8; q += 4) {
-    const RankSlot at(q, r8);
-    float v[8];
-    hval(at.c, v);
-    const bf16x8 hf = or_zero(half_of(v, at.low), at.live);
-    const bf16_t* bp = bk.b + (int64_t)(col + (threadIdx.x & 15)) * bk.rank + 8 * at.c;
-    uint32_t todo = named;
-    while (todo) {
-      int t[4];
-      t[0] = next_adapter(todo, id);
-      if (todo == 0) {
-        const int one[1] = {t[0]};
-        expand_step<WR, 1>(acc, bp, slot, bk.rank, at.live, hf, id, one);
-        break;
-      }
+  __device__ __forceinline__ void load() {
+    t[0] = next_adapter(todo, id);
 #pragma unroll
-      for (int u = 1; u < 4; ++u) t[u] = todo ? next_adapter(todo, id) : t[0];
-      expand_step<WR, 4>(acc, bp, slot, bk.rank, at.live, hf, id, t);
+    for (int u = 1; u < U; ++u) t[u] = todo ? next_adapter(todo, id) : t[0];
+    const bf16_t* p = b + 8 * RankSlot(q, rank >> 3).c;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < WR; ++i) next[u][i] = *reinterpret_cast<const uint4*>(p + t[u] * slot + (int64_t)16 * i * rank);
+  }
+  __device__ __forceinline__ Expand(const Bank& bk, int n, int col, int id_, uint32_t named_)
+      : b(bk.b + (int64_t)(col + (threadIdx.x & 15)) * bk.rank), slot((int64_t)n * bk.rank), rank(bk.rank), id(id_),
+        named(named_), todo(named_), q(0) {
+    load();
+  }
+  // hval(c, v) gives scale times ranks 8 c .. 8 c + 7 of the lane's row
+  template <typename H>
+  __device__ __forceinline__ void add(f32x4 (&acc)[WR], H hval) {
+    const int end = 2 * (rank >> 3);
+    bf16x8 hf;
+    bool fresh = true;
+    for (;;) {
+      const RankSlot at(q, rank >> 3);
+      if (fresh) {
+        float v[8];
+        hval(at.c, v);
+        hf = or_zero(half_of(v, at.low), at.live);
+      }
+      int now[U];
+      uint4 cur[U][WR];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        now[u] = t[u];
+#pragma unroll
+        for (int i = 0; i < WR; ++i) cur[u][i] = next[u][i];
+      }
+      fresh = todo == 0;
+      if (fresh) {
+        q += 4;
+        todo = named;
+      }
+      const bool more = q < end;
+      if (more) load();
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < WR; ++i) {
+          const f32x4 sum = mfma16x16x32(or_zero(cur[u][i], at.live), hf, acc[i]);
+          acc[i] = id == now[u] && (u == 0 || now[u] != now[0]) ? sum : acc[i];
+        }
+      if (!more) return;
     }
   }
-}
+};
 
 // acc[i][j] += scale (h B^T) for a wave's block of 16 WM rows from m0 on and 16 WR columns from col on, h from the
 // finished first product. One adapter for all rows that are stored: its products go straight into the sums. Several:
@@ -382,15 +414,17 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
       const RankSlot at(q, r8);
       const int from = 8 * at.c + (at.low ? bk.rank : 0);
       const bf16_t* bp = b0 + t * slot + 8 * at.c;
-      bf16x8 hf[WM];
+      bf16x8 hf[WM], bf[WR];
+#pragma unroll
+      for (int i = 0; i < WR; ++i) bf[i] = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), at.live);
 #pragma unroll
       for (int j = 0; j < WM; ++j) hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + from), at.live);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < WR; ++i) {
-        const bf16x8 bf = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), at.live);
 #pragma unroll
         for (int j = 0; j < WM; ++j) {
-          const f32x4 sum = mfma16x16x32(bf, hf[j], acc[i][j]);
+          const f32x4 sum = mfma16x16x32(bf[i], hf[j], acc[i][j]);
           acc[i][j] = id[j] == t ? sum : acc[i][j];
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -435,12 +469,13 @@ adapter_tiles_kernel(AdapterArgs a) {
   const int wr = (wave % GR) * 16 * WR, wm = (wave / GR) * 16 * WM;   // this wave's block
   f32x4 acc[WR][WM];
   if constexpr (PART != kSplitSums) {
-    if constexpr (BK == 64 && NS == 2) tile_sums_ahead<WR, WM, GR, GM>(a.t, lds, rt, mt, grp, acc);
-    else tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc);
+    const int col = rt * C::TR + wr;
+    // the adapters' part first, while the ring's first copies are on their way
+    auto beside = [&]() { expand_block<WR, WM, PART == kExpandOne>(acc, a, mt * C::TM + wm, col); };
+    if constexpr (BK == 64 && NS == 2) tile_sums_ahead<WR, WM, GR, GM>(a.t, lds, rt, mt, grp, acc, beside);
+    else tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc, beside);
 #pragma unroll
     for (int i = 0; i < WR; ++i) settle(acc[i]);
-    const int col = rt * C::TR + wr;
-    expand_block<WR, WM, PART == kExpandOne>(acc, a, mt * C::TM + wm, col);
 #pragma unroll
     for (int j = 0; j < WM; ++j) {
       const int m = mt * C::TM + wm + 16 * j + l16;
@@ -483,8 +518,8 @@ adapter_tiles_kernel(AdapterArgs a) {
 }
 
 // The contraction ranges' parts summed in order, plus the adapters' part, rounded once: a workgroup per 16 rows and
-// 64 WR columns, a wave per 16 WR of them (whole blocks of one projection: n0 and n are multiples of 16 WR). h is
-// summed over its chunks into LDS, while the parts are on their way.
+// 64 WR columns, a wave per 16 WR of them (whole blocks of one projection: n0 and n are multiples of 16 WR). The parts
+// and the first adapters' B are on their way while h is summed over its chunks into LDS.
 template <int WR>
 __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
   constexpr int kStride = kMaxRank + 4;
@@ -492,11 +527,15 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int ctiles = (a.t.r + 64 * WR - 1) / (64 * WR);
   const int col0 = (int)(blockIdx.x % ctiles) * 64 * WR, m0 = (int)(blockIdx.x / ctiles) * 16;
-  const int m = m0 + l16, col = col0 + wave * 16 * WR;
-  const bool cols = col < a.t.r;
+  const int m = m0 + l16, col = min(col0 + wave * 16 * WR, a.t.r - 16 * WR);   // a wave past the end repeats the last
+  const int sel = col >= a.t.r0, n = sel ? a.t.r - a.t.r0 : a.t.r0, at = sel ? col - a.t.r0 : col;
+  const Bank& bk = a.bank[sel];
+  const int id = row_adapter(a, bk, m);
+  const uint32_t named = (uint32_t)__ballot(id >= 0) & 0xFFFFu;
+  const float* part = reinterpret_cast<const float*>(a.t.out) + (int64_t)min(m, a.t.rows - 1) * a.t.groups * a.t.r + col + 4 * g;
   f32x4 acc[WR];
-  if (cols) {
-    const float* part = reinterpret_cast<const float*>(a.t.out) + (int64_t)min(m, a.t.rows - 1) * a.t.groups * a.t.r + col + 4 * g;
+
+  auto sum_parts = [&]() {
 #pragma unroll
     for (int i = 0; i < WR; ++i) acc[i] = *reinterpret_cast<const f32x4*>(part + 16 * i);
     for (int p = 1; p < a.t.groups; ++p)
@@ -506,45 +545,57 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][e] = acc[i][e] + v[e];
       }
-  }
+  };
+  auto sum_h = [&]() {
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const Bank& bk = a.bank[s];
-    if (bk.slots == 0 || (s == 0 ? col0 >= a.t.r0 : col0 + 64 * WR <= a.t.r0)) continue;
-    const int quads = bk.rank >> 2;
-    for (int i = threadIdx.x; i < 16 * quads; i += 256) {
-      const int row = i / quads, r = (i - row * quads) * 4;
-      const int id = row_adapter(a, bk, m0 + row);
-      f32x4 v = {0.f, 0.f, 0.f, 0.f};
-      if (id >= 0) {
-        const float* hp = bk.h + (int64_t)(m0 + row) * bk.rank + r;
-        const int64_t step = (int64_t)a.t.rows * bk.rank;
-        const float scale = bk.scale[id];
+    for (int s = 0; s < 2; ++s) {
+      const Bank& bs = a.bank[s];
+      if (bs.slots == 0 || (s == 0 ? col0 >= a.t.r0 : col0 + 64 * WR <= a.t.r0)) continue;
+      const int quads = bs.rank >> 2;
+      for (int i = threadIdx.x; i < 16 * quads; i += 256) {
+        const int row = i / quads, r = (i - row * quads) * 4, t = row_adapter(a, bs, m0 + row);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (t >= 0) {
+          const float* hp = bs.h + (int64_t)(m0 + row) * bs.rank + r;
+          const int64_t step = (int64_t)a.t.rows * bs.rank;
+          const float scale = bs.scale[t];
 #pragma unroll 8
-        for (int p = 0; p < a.chunks; ++p) {
-          const f32x4 h = *reinterpret_cast<const f32x4*>(hp + p * step);
+          for (int p = 0; p < a.chunks; ++p) {
+            const f32x4 h = *reinterpret_cast<const f32x4*>(hp + p * step);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] += h[e];
+            for (int e = 0; e < 4; ++e) v[e] += h[e];
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= scale;
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= scale;
+        *reinterpret_cast<f32x4*>(hs[s] + row * kStride + r) = v;
       }
-      *reinterpret_cast<f32x4*>(hs[s] + row * kStride + r) = v;
     }
-  }
-  __syncthreads();
-  if (!cols) return;
-  const int s = col >= a.t.r0, n = s ? a.t.r - a.t.r0 : a.t.r0, at = s ? col - a.t.r0 : col;
-  const Bank& bk = a.bank[s];
-  if (bk.slots)
-    expand_tile<WR>(acc, bk, n, at, row_adapter(a, bk, m), [&](int c, float* v) {
-      const float* from = hs[s] + l16 * kStride + 8 * c;
+    __syncthreads();
+  };
+  auto hval = [&](int c, float* v) {
+    const float* from = hs[sel] + l16 * kStride + 8 * c;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = from[e];
-    });
+    for (int e = 0; e < 8; ++e) v[e] = from[e];
+  };
+  const bool one = named == 0 || __ballot(id >= 0 && id != __builtin_amdgcn_readlane(id, __builtin_ctz(named | 0x10000u))) == 0;
+  if (named == 0) {
+    sum_parts();
+    sum_h();
+  } else if (one) {
+    Expand<WR, 1> ex(bk, n, at, id, named);
+    sum_parts();
+    sum_h();
+    ex.add(acc, hval);
+  } else {
+    Expand<WR, 4> ex(bk, n, at, id, named);
+    sum_parts();
+    sum_h();
+    ex.add(acc, hval);
+  }
   if (m < a.t.rows)
 #pragma unroll
-    for (int i = 0; i < WR; ++i) store4<bf16_t>((s ? a.y1 : a.y) + (int64_t)m * n + at + 16 * i + 4 * g, acc[i]);
+    for (int i = 0; i < WR; ++i) store4<bf16_t>((sel ? a.y1 : a.y) + (int64_t)m * n + at + 16 * i + 4 * g, acc[i]);
 }
 
 // ------------------------------------------------------------------ plan
@@ -557,7 +608,7 @@ struct AdapterPlan {
   int tr, tm;            // the tile's weight rows and query rows
   int splits;            // contraction ranges; 1 with direct
   bool direct;
-  int chunk, chunks;
+  int chunk, chunks, sub;
 };
 
 // Ranges for decode row counts, by the rule of the decode-row projections: at 33-64 rows the ranges whose wide tiles
@@ -598,8 +649,13 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
       p.tr = 32;
       p.tm = 32 * q;
     }
-    p.chunk = 256;
+    // partial h: one share per CU, of 512 to 1024 channels (4 to 8 steps of each wave)
+    p.sub = 4;
+    const int64_t tiles = (int64_t)((rows + 3) / 4) * ((rank + 15) / 16);
+    const int64_t chunk = ((int64_t)k * tiles / 256 + 127) / 128 * 128;
+    p.chunk = (int)(chunk < 512 ? 512 : chunk > 1024 ? 1024 : chunk);
   } else {
+    p.sub = 16;
     // The shape and ranges whose estimate is the least. A tile's time is fixed us (prologue, first loads, epilogue) and
     // us per 64-channel step, alone on its CU or as one of two; measured on 4096 rows of 1280 -> 32768 (20 steps), 8192
     // of 8192 -> 5120 (128) and single tiles of 5120 channels (80).
@@ -660,13 +716,17 @@ static void launch_adapter_tiles(const AdapterArgs& a, int64_t tiles, hipStream_
                      stream, a);
 }
 
-// Rows and ranks per workgroup of the finished first product.
+// Rows and ranks per workgroup of the finished first product: 16 rows and 16 waves while the rows do not fill the chip
+// (latency: 999 rows of 1280 channels at rank 32 TIMING2), 32 rows beyond 16 ranks otherwise.
 static void launch_shrink(const AdapterArgs& a, hipStream_t stream) {
   const int rank = a.bank[0].rank;
   auto blocks = [&](int mt, int rt) {
     return dim3((unsigned)(((a.t.rows + 16 * mt - 1) / (16 * mt)) * ((rank + 16 * rt - 1) / (16 * rt))));
   };
-  if (rank <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<1, 1, 8>), blocks(1, 1), dim3(512), 0, stream, a);
+  if (a.t.rows <= 2048) {
+    if (rank <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<1, 1, 16>), blocks(1, 1), dim3(1024), 0, stream, a);
+    else hipLaunchKernelGGL((adapter_shrink_kernel<1, 2, 16>), blocks(1, 2), dim3(1024), 0, stream, a);
+  } else if (rank <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<1, 1, 8>), blocks(1, 1), dim3(512), 0, stream, a);
   else if (rank <= 32) hipLaunchKernelGGL((adapter_shrink_kernel<2, 2, 8>), blocks(2, 2), dim3(512), 0, stream, a);
   else hipLaunchKernelGGL((adapter_shrink_kernel<2, 4, 8>), blocks(2, 4), dim3(512), 0, stream, a);
 }
@@ -791,7 +851,7 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   const int rank0 = banks[0].slots ? banks[0].rank : 0, rank1 = banks[1].slots ? banks[1].rank : 0, n = n0 + n1;
   const AdapterPlan p = adapter_plan((int)rows, k, n, n0, rank0 > rank1 ? rank0 : rank1);
   const int64_t tiles = (int64_t)(n / p.tr) * ((rows + p.tm - 1) / p.tm) * p.splits;
-  const int64_t shrinks = (rows + 15) / 16 * p.chunks * ((rank0 + 15) / 16);
+  const int64_t shrinks = (rows + p.sub - 1) / p.sub * p.chunks * ((rank0 + 15) / 16 + (rank1 + 15) / 16);
   const int64_t reduces = (rows + 15) / 16 * ((n + 63) / 64);
   DSV41_REQUIRE(tiles < (1ll << 31) && shrinks < (1ll << 31) && reduces < (1ll << 31), DSV41_E_ARG, "%s: too many tiles",
                 what);
@@ -811,6 +871,7 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   a.k = k;
   a.chunk = p.chunk;
   a.chunks = p.chunks;
+  a.sub = p.sub;
   a.y = static_cast<bf16_t*>(y0);
   a.y1 = static_cast<bf16_t*>(y1);
   if (p.direct && rank0) launch_shrink(a, stream);

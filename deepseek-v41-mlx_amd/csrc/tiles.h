@@ -111,7 +111,8 @@ __device__ __forceinline__ void wait_copies(int pending) {
 
 // Sums of output tile (rt, mt) over contraction range or group grp, left in acc: lane (g, l16) of a wave holds
 // weight rows 16 i + 4 g .. + 3 and query row 16 j + l16 of the wave's block. lds: C::LDS bytes, 16-byte aligned.
-// beside() runs once the ring's first copies are on their way; what it leaves outstanding it waits for itself.
+// beside() runs once the ring's first copies are on their way, on sums of zero, which it may add to; what it leaves
+// outstanding it waits for itself.
 struct NothingBeside {
   __device__ __forceinline__ void operator()() const {}
 };
