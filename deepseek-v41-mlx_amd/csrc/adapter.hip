@@ -54,6 +54,102 @@ __global__ __launch_bounds__(256) void adapter_expand_plain_kernel(const T* y, c
   io<T>::st(out + i, fmaf(scale[t], s, io<T>::ld(y + i)));
 }
 
+// The projection and its adapters for any width and type on the float32 matrix cores (v_mfma_f32_16x16x4_f32: exact
+// float32 arithmetic in the order of the channels): a wave per 16 rows and 16 WR output columns. Rows are the MFMA's
+// columns; a lane supplies 4 channels of its row and of its weight row per load, the same 4 channels of both. The first
+// product's result - ranks 4 g .. 4 g + 3 of row l16 in lane (g, l16) - is the operand of the second as it lies. Every
+// adapter of the 16 rows multiplies all of them, a lane keeps its own row's. VEC: widths in whole steps of 16 channels
+// and ranks of 4, loaded 4 at a time; else one by one, with zeros past the ends.
+template <typename T, bool VEC>
+__device__ __forceinline__ f32x4 load4(const T* p, int at, int end) {
+  f32x4 v;
+  if constexpr (VEC && sizeof(T) == 4) {
+    v = *reinterpret_cast<const f32x4*>(p + at);
+  } else if constexpr (VEC) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p + at);
+    v = f32x4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16),
+              __uint_as_float(u.y & 0xFFFF0000u)};
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = at + e < end ? io<T>::ld(p + at + e) : 0.0f;
+  }
+  return v;
+}
+
+template <typename T, int WR, bool VEC>
+__global__ __launch_bounds__(256) void adapter_plain_kernel(const T* __restrict__ x, const T* __restrict__ w,
+                                                            const T* __restrict__ a, const T* __restrict__ b,
+                                                            const float* __restrict__ scale,
+                                                            const int32_t* __restrict__ ids, T* __restrict__ y, int rows,
+                                                            int tokens, int k, int n, int rank, int slots) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+  const int ctiles = (n + 16 * WR - 1) / (16 * WR);
+  const int64_t tile = (int64_t)blockIdx.x * 4 + wave;
+  if (tile >= (int64_t)ctiles * ((rows + 15) / 16)) return;
+  const int col = (int)(tile % ctiles) * 16 * WR, m = (int)(tile / ctiles) * 16 + l16;
+  const T* xp = x + (int64_t)min(m, rows - 1) * k;
+  const T* wp[WR];
+  f32x4 acc[WR];
+#pragma unroll
+  for (int i = 0; i < WR; ++i) {
+    wp[i] = w + (int64_t)min(col + 16 * i + l16, n - 1) * k;
+    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll 4
+  for (int c = 0; c < k; c += 16) {
+    const f32x4 xf = load4<T, VEC>(xp, c + 4 * g, k);
+#pragma unroll
+    for (int i = 0; i < WR; ++i) {
+      const f32x4 wf = load4<T, VEC>(wp[i], c + 4 * g, k);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[e], xf[e], acc[i], 0, 0, 0);
+    }
+  }
+  settle(acc);
+  const int t0 = m < rows ? ids[m / tokens] : -1, id = (uint32_t)t0 < (uint32_t)slots ? t0 : -1;
+  const float s = id < 0 ? 0.0f : scale[id];
+  uint32_t todo = (uint32_t)__ballot(id >= 0) & 0xFFFFu;
+  while (todo) {
+    const int t = __builtin_amdgcn_readlane(id, __builtin_ctz(todo));
+    todo &= ~(uint32_t)__ballot(id == t);
+    f32x4 sum[WR];
+#pragma unroll
+    for (int i = 0; i < WR; ++i) sum[i] = acc[i];
+    for (int q = 0; q < rank; q += 16) {
+      f32x4 h[1] = {{0.f, 0.f, 0.f, 0.f}};
+      const T* ap = a + ((int64_t)t * rank + min(q + l16, rank - 1)) * k;
+#pragma unroll 4
+      for (int c = 0; c < k; c += 16) {
+        const f32x4 xf = load4<T, VEC>(xp, c + 4 * g, k), af = load4<T, VEC>(ap, c + 4 * g, k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) h[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(af[e], xf[e], h[0], 0, 0, 0);
+      }
+      settle(h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[0][e] = q + 4 * g + e < rank ? h[0][e] * s : 0.0f;
+#pragma unroll
+      for (int i = 0; i < WR; ++i) {
+        const T* bp = b + ((int64_t)t * n + min(col + 16 * i + l16, n - 1)) * rank;
+        // a rank tile's last chunks may lie past the ranks, where B is not read
+        const f32x4 bf = VEC && q + 4 * g >= rank ? f32x4{0.f, 0.f, 0.f, 0.f} : load4<T, VEC>(bp, q + 4 * g, rank);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(bf[e], h[0][e], sum[i], 0, 0, 0);
+      }
+    }
+    settle(sum);
+#pragma unroll
+    for (int i = 0; i < WR; ++i) acc[i] = id == t ? sum[i] : acc[i];
+  }
+  if (m >= rows) return;
+#pragma unroll
+  for (int i = 0; i < WR; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = col + 16 * i + 4 * g + e;
+      if (c < n) io<T>::st(y + (int64_t)m * n + c, acc[i][e]);
+    }
+}
+
 // ------------------------------------------------------------------ matrix cores (bf16)
 
 // One projection's adapters as the kernels see them.
@@ -75,6 +171,7 @@ struct AdapterArgs {
   int tokens, k;
   int chunk, chunks;     // channels of one partial h, and how many
   int sub;               // rows of a share of it: 4 or 16
+  int apart;             // leading workgroups that compute shares of h and no tile (0: the tiles' workgroups do)
   bf16_t* y;             // [rows, t.r0]
   bf16_t* y1;            // [rows, t.r - t.r0]
 };
@@ -438,20 +535,22 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
 }
 
 // The projection's tiles. kExpand*: the adapters' part is added to the float32 sums in registers and the result stored,
-// rounded once (h complete before the launch). Else the sums of one contraction range go to t.out in float32, and the
-// workgroups also compute h, each its share while its first copies are on their way.
+// rounded once (h complete before the launch). Else the sums of one contraction range go to t.out in float32, and h is
+// computed beside them: by workgroups of their own where the launch leaves room for them, else by the tiles' own, each
+// its share while its first copies are on their way.
 enum AdapterPart { kSplitSums, kExpandOne, kExpandAny };
 
 template <int WR, int WM, int GR, int GM, int BK, int NS, AdapterPart PART>
-__global__ __launch_bounds__(64 * GR * GM, (TileCfg<WR, WM, GR, GM, BK, NS>::LDS <= 73 * 1024) ? 2 : 1) void
+__global__ __launch_bounds__(64 * GR * GM, (TileCfg<WR, WM, GR, GM, BK, NS>::LDS <= 72 * 1024) ? 2 : 1) void
 adapter_tiles_kernel(AdapterArgs a) {
   using C = TileCfg<WR, WM, GR, GM, BK, NS>;
   __shared__ __align__(16) uint8_t lds[C::LDS];
-  const int mtiles = (a.t.rows + C::TM - 1) / C::TM, rtiles = a.t.r / C::TR, total = (int)gridDim.x;
+  const int mtiles = (a.t.rows + C::TM - 1) / C::TM, rtiles = a.t.r / C::TR;
+  const int apart = PART == kSplitSums ? a.apart : 0, total = (int)gridDim.x - apart, block = (int)blockIdx.x - apart;
   int rt, mt, grp = 0;
   if constexpr (PART == kSplitSums) {
     // consecutive tiles on one XCD, the weight tile fastest, as the output projection's
-    const int tile = total % 8 ? (int)blockIdx.x : ((int)blockIdx.x % 8) * (total / 8) + (int)blockIdx.x / 8;
+    const int tile = total % 8 ? block : (block % 8) * (total / 8) + block / 8;
     rt = tile % rtiles;
     mt = (tile / rtiles) % mtiles;
     grp = tile / (rtiles * mtiles);
@@ -459,8 +558,8 @@ adapter_tiles_kernel(AdapterArgs a) {
     // consecutive tiles on one XCD, in bands of 4 query tiles: 32 CUs work on 4 x 8 tiles and share their 12 operand
     // panels in the XCD's L2, where 1 x 32 tiles read 33 (TIMING)
     constexpr int kBand = 4;
-    const int xcd = (int)blockIdx.x % 8, per = total / 8, more = total % 8;
-    const int tile = xcd * per + min(xcd, more) + (int)blockIdx.x / 8;
+    const int xcd = block % 8, per = total / 8, more = total % 8;
+    const int tile = xcd * per + min(xcd, more) + block / 8;
     const int band = tile / (kBand * rtiles), in = tile - band * kBand * rtiles, width = min(kBand, mtiles - band * kBand);
     rt = in / width;
     mt = band * kBand + in - rt * width;
@@ -492,13 +591,20 @@ adapter_tiles_kernel(AdapterArgs a) {
   } else {
     static_assert(GR * GM == 4, "a partial h is the work of four waves");
     __shared__ __align__(16) float red[4 * 256];
-    auto beside = [&]() {
+    auto shares = [&](int first, int step) {
       const int items0 = shrink_items(a, a.bank[0]), items = items0 + shrink_items(a, a.bank[1]);
-      for (int it = blockIdx.x; it < items; it += total)
+      for (int it = first; it < items; it += step)
         if (it < items0) shrink_item(a, a.bank[0], it, red);
         else shrink_item(a, a.bank[1], it - items0, red);
+      return first < items;
+    };
+    if (block < 0) {
+      shares(blockIdx.x, apart);
+      return;
+    }
+    auto beside = [&]() {
       // the ring's waits count its own copies only
-      if ((int)blockIdx.x < items) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (apart == 0 && shares(block, total)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
     if constexpr (BK == 64 && NS == 2) tile_sums_ahead<WR, WM, GR, GM>(a.t, lds, rt, mt, grp, acc, beside);
     else tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc, beside);
@@ -609,6 +715,7 @@ struct AdapterPlan {
   int splits;            // contraction ranges; 1 with direct
   bool direct;
   int chunk, chunks, sub;
+  bool two;              // two of the tile's workgroups fit a CU
 };
 
 // Ranges for decode row counts, by the rule of the decode-row projections: at 33-64 rows the ranges whose wide tiles
@@ -649,6 +756,7 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
       p.tr = 32;
       p.tm = 32 * q;
     }
+    p.two = p.tile == kRows32 || p.tile == kRows64;      // 68 and 76 KB of LDS
     // partial h: one share per CU, of 512 to 1024 channels (4 to 8 steps of each wave)
     p.sub = 4;
     const int64_t tiles = (int64_t)((rows + 3) / 4) * ((rank + 15) / 16);
@@ -693,6 +801,7 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
       }
     }
     p.direct = p.splits == 1;
+    p.two = p.tile != kTile256 && p.tile != kTile32;
     // beside split sums: enough shares of h to fill the chip, at most 8 of them for the next kernel to sum
     const int64_t items = (int64_t)((rows + 15) / 16) * ((rank + 15) / 16);
     const int parts = (int)(items >= 768 ? 1 : (768 + items - 1) / items > 8 ? 8 : (768 + items - 1) / items);
@@ -738,7 +847,7 @@ static void launch_direct_tiles(const AdapterArgs& a, int64_t tiles, hipStream_t
 }
 
 static void launch_projection(const AdapterArgs& a, const AdapterPlan& p, hipStream_t stream) {
-  const int64_t tiles = (int64_t)(a.t.r / p.tr) * ((a.t.rows + p.tm - 1) / p.tm) * p.splits;
+  const int64_t tiles = (int64_t)(a.t.r / p.tr) * ((a.t.rows + p.tm - 1) / p.tm) * p.splits + a.apart;
   switch (p.tile) {
     case kRows32: launch_adapter_tiles<1, 1, 2, 2, 64, 8, kSplitSums>(a, tiles, stream); break;
     case kRows64: launch_adapter_tiles<1, 2, 2, 2, 64, 6, kSplitSums>(a, tiles, stream); break;
@@ -872,6 +981,10 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   a.chunk = p.chunk;
   a.chunks = p.chunks;
   a.sub = p.sub;
+  // shares of h on workgroups of their own while all of them and all tiles run at once (a multiple of 8, so that the
+  // tiles keep their XCDs): one row 5120 -> 1280 + 512 at rank 16 TIMING3
+  const int64_t room = p.two ? 512 : 256, spare = (shrinks + 7) / 8 * 8;
+  a.apart = !p.direct && tiles + spare <= room ? (int)spare : 0;
   a.y = static_cast<bf16_t*>(y0);
   a.y1 = static_cast<bf16_t*>(y1);
   if (p.direct && rank0) launch_shrink(a, stream);
@@ -882,6 +995,47 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
       hipLaunchKernelGGL(adapter_reduce_kernel<4>, dim3((unsigned)((rows + 15) / 16 * ((n + 255) / 256))), dim3(256), 0,
                          stream, a);
     else hipLaunchKernelGGL(adapter_reduce_kernel<1>, dim3((unsigned)reduces), dim3(256), 0, stream, a);
+  }
+  return check_launch(what);
+}
+
+template <typename T, bool VEC>
+static void launch_plain(const void* x, const void* w, const void* a, const void* b, const float* scale,
+                         const int32_t* ids, void* y, int rows, int tokens, int k, int n, int rank, int slots,
+                         hipStream_t stream) {
+  // 64 columns per wave where that still gives every SIMD a wave
+  const int64_t mtiles = (rows + 15) / 16, wide = mtiles * ((n + 63) / 64), narrow = mtiles * ((n + 15) / 16);
+  auto go = [&](auto kernel, int64_t tiles) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((tiles + 3) / 4)), dim3(256), 0, stream, static_cast<const T*>(x),
+                       static_cast<const T*>(w), static_cast<const T*>(a), static_cast<const T*>(b), scale, ids,
+                       static_cast<T*>(y), rows, tokens, k, n, rank, slots);
+  };
+  if (wide >= 1024) go(adapter_plain_kernel<T, 4, VEC>, wide);
+  else go(adapter_plain_kernel<T, 1, VEC>, narrow);
+}
+
+extern "C" int dsv41_adapter_plain(const void* x, const void* w, const void* a, const void* b, const float* scale,
+                                   const int32_t* ids, void* y, int64_t rows, int32_t tokens, int32_t k, int32_t n,
+                                   int32_t rank, int32_t slots, int32_t dtype, hipStream_t stream) {
+  const char* what = "dsv41_adapter_plain";
+  DSV41_REQUIRE(rows >= 0 && tokens > 0 && k > 0 && n > 0 && rank > 0 && slots > 0 && rows % tokens == 0, DSV41_E_ARG,
+                "%s: rows %lld, tokens %d, k %d, n %d, rank %d, slots %d", what, (long long)rows, tokens, k, n, rank,
+                slots);
+  DSV41_REQUIRE(dtype == DSV41_BF16 || dtype == DSV41_F32, DSV41_E_DTYPE, "%s: dtype %d not supported (BF16 or F32)",
+                what, dtype);
+  DSV41_REQUIRE(rows < (1ll << 31) && k < (1 << 30) && n < (1 << 30) && rank < (1 << 30) &&
+                    (rows + 15) / 16 * ((n + 15) / 16) < (1ll << 31),
+                DSV41_E_ARG, "%s: too many outputs", what);
+  if (rows == 0) return 0;
+  DSV41_REQUIRE(x && w && a && b && scale && ids && y, DSV41_E_ARG, "%s: null tensor", what);
+  const int m = (int)rows;
+  const bool vec = k % 16 == 0 && rank % 4 == 0 && aligned16(x) && aligned16(w) && aligned16(a) && aligned16(b);
+  if (dtype == DSV41_BF16) {
+    if (vec) launch_plain<bf16_t, true>(x, w, a, b, scale, ids, y, m, tokens, k, n, rank, slots, stream);
+    else launch_plain<bf16_t, false>(x, w, a, b, scale, ids, y, m, tokens, k, n, rank, slots, stream);
+  } else {
+    if (vec) launch_plain<float, true>(x, w, a, b, scale, ids, y, m, tokens, k, n, rank, slots, stream);
+    else launch_plain<float, false>(x, w, a, b, scale, ids, y, m, tokens, k, n, rank, slots, stream);
   }
   return check_launch(what);
 }

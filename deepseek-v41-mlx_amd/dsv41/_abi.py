@@ -118,6 +118,7 @@ _SIGNATURES = {
     "dsv41_adapter_linear_workspace_bytes": [_i64, _i32, _i32, _i32, _i32, _i32],
     "dsv41_adapter_linear": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _sz, _i64, _i32, _i32, _i32, _i32, _i32,
                              _i32, _c_p],
+    "dsv41_adapter_plain": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_adapter_linear_pair": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _sz,
                                   _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_cache_move_workspace_bytes": [_i32, _i32],
@@ -1271,7 +1272,7 @@ def sparse_mla_fp8(q, win_kv, chunk_kv, comp8, comp_scale, scale_rb, n_comp, att
 
 def _call_on(device, name: str, *args) -> None:
     """_call with `device` as the current one: a kernel launches on the current device, whatever stream it is given."""
-    if device.type != "cuda" or torch.cuda.current_device() == device.index:
+    if device.type != "cuda" or torch._C._cuda_getDevice() == device.index:
         _call(name, *args)
     else:
         with torch.cuda.device(device):
@@ -1289,21 +1290,32 @@ def _one_device(name: str, *tensors) -> torch.device:
 def _adapter_args(name, x, a, b, scale, ids, n):
     """Checks one bank (a [slots, rank, k], b [slots, n, rank], scale [slots]) and the sequences' ids against x
     [sequences, (tokens,) k]; returns (rows, tokens, k, rank, slots)."""
+    sizes, dtype, at = x.shape, x.dtype, x.get_device()
+    slots, rank, k = a.shape if a.dim() == 3 else (0, 0, 0)
+    if not (x.is_contiguous() and a.is_contiguous() and b.is_contiguous() and scale.is_contiguous()
+            and ids.is_contiguous() and at == a.get_device() == b.get_device() == scale.get_device() == ids.get_device()
+            and x.is_cuda and len(sizes) > 1 and slots and k == sizes[-1] and b.shape == (slots, n, rank)
+            and dtype is a.dtype is b.dtype and scale.dtype is torch.float32 and scale.shape == (slots,)
+            and ids.dtype is torch.int32 and ids.shape == sizes[:1]):
+        _adapter_refusal(name, x, a, b, scale, ids, n)
+    rows = x.numel() // k
+    return rows, (rows // sizes[0] if rows else 1), k, rank, slots
+
+
+def _adapter_refusal(name, x, a, b, scale, ids, n):
+    """What _adapter_args found wrong."""
     _gpu(name, x, a, b, scale, ids)
     _contig(name, x, a, b, scale, ids)
     _one_device(name, x, a, b, scale, ids)
     if x.dim() < 2:
         raise ValueError(f"{name}: x must be [sequences, (tokens,) channels], got {tuple(x.shape)}")
-    k = x.shape[-1]
-    if a.dim() != 3 or b.dim() != 3 or a.shape[2] != k or b.shape != (a.shape[0], n, a.shape[1]):
-        raise ValueError(f"{name}: a {tuple(a.shape)} and b {tuple(b.shape)} are no adapters of [{n}, {k}]")
+    if a.dim() != 3 or b.dim() != 3 or 0 in a.shape or a.shape[2] != x.shape[-1] or b.shape != (a.shape[0], n, a.shape[1]):
+        raise ValueError(f"{name}: a {tuple(a.shape)} and b {tuple(b.shape)} are no adapters of [{n}, {x.shape[-1]}]")
     if a.dtype != x.dtype or b.dtype != x.dtype:
         raise ValueError(f"{name}: adapters of {a.dtype} and {b.dtype} on x of {x.dtype}")
     _vec(name, "scale", scale, a.shape[0])
     if ids.dtype != torch.int32 or ids.shape != (x.shape[0],):
         raise ValueError(f"{name}: ids must be int32 [{x.shape[0]}], got {ids.dtype} {list(ids.shape)}")
-    rows = x.numel() // k if k else 0
-    return rows, (rows // x.shape[0] if x.shape[0] else 1), k, a.shape[1], a.shape[0]
 
 
 def adapter_add(x, a, b, scale, ids, y, out=None, workspace=None):
@@ -1330,12 +1342,16 @@ def adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1) -> int:
 
 
 def _adapter_weight(name, x, w):
-    _gpu(name, w)
-    _contig(name, w)
-    if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
+    if not (x.dtype is w.dtype is torch.bfloat16):
         raise ValueError(f"{name}: x and w must be bfloat16")
-    if w.dim() != 2 or w.shape[1] != x.shape[-1] or w.device != x.device:
+    if w.dim() != 2 or w.shape[1] != x.shape[-1] or w.get_device() != x.get_device():
         raise ValueError(f"{name}: x {tuple(x.shape)} and w {tuple(w.shape)} do not contract")
+    if not w.is_contiguous():
+        _contig(name, w)
+
+
+def _adapter_out(name, out, x, n):
+    return x.new_empty((*x.shape[:-1], n)) if out is None else _out(name, out, (*x.shape[:-1], n), x.dtype, x.device)
 
 
 def adapter_linear(x, w, a, b, scale, ids, out=None, workspace=None):
@@ -1345,13 +1361,29 @@ def adapter_linear(x, w, a, b, scale, ids, out=None, workspace=None):
     rows, tokens, k, rank, slots = _adapter_args(name, x, a, b, scale, ids, w.shape[0])
     _adapter_weight(name, x, w)
     n = w.shape[0]
-    out = _out(name, out, (*x.shape[:-1], n), x.dtype, x.device)
+    out = _adapter_out(name, out, x, n)
     if rows == 0:
         return out
     need = adapter_linear_workspace_bytes(rows, k, n, 0, rank, 0)
     ws = _ws(name, workspace, need, x.device)
-    _call_on(x.device, name, _ptr(x), _ptr(w), _ptr(a), _ptr(b), _ptr(scale), _ptr(ids), _ptr(out), _ptr(ws), need, rows,
-             tokens, k, n, rank, slots, dtype_code(x, name), _stream(x))
+    _call_on(x.device, name, x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(), ids.data_ptr(),
+             out.data_ptr(), _ptr(ws), need, rows, tokens, k, n, rank, slots, BF16, _stream(x))
+    return out
+
+
+def adapter_plain(x, w, a, b, scale, ids, out=None):
+    """adapter_linear for any width, rank and type (float32 or bfloat16) on the float32 matrix cores:
+    dsv41_adapter_plain, for small products."""
+    name = "dsv41_adapter_plain"
+    rows, tokens, k, rank, slots = _adapter_args(name, x, a, b, scale, ids, w.shape[0])
+    if w.dim() != 2 or w.shape[1] != k or w.dtype is not x.dtype or w.get_device() != x.get_device():
+        raise ValueError(f"{name}: x {x.dtype} {tuple(x.shape)} and w {w.dtype} {tuple(w.shape)} do not contract")
+    _contig(name, w)
+    code = dtype_code(x, name)
+    out = _adapter_out(name, out, x, w.shape[0])
+    if rows:
+        _call_on(x.device, name, x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(),
+                 ids.data_ptr(), out.data_ptr(), rows, tokens, k, w.shape[0], rank, slots, code, _stream(x))
     return out
 
 
@@ -1370,16 +1402,15 @@ def adapter_linear_pair(x, w0, w1, bank0, bank1, ids, out0=None, out1=None, work
     (rank0, slots0) = sizes[0][3:] if bank0 is not None else (0, 0)
     (rank1, slots1) = sizes[-1][3:] if bank1 is not None else (0, 0)
     n0, n1 = w0.shape[0], w1.shape[0]
-    out0 = _out(name, out0, (*x.shape[:-1], n0), x.dtype, x.device)
-    out1 = _out(name, out1, (*x.shape[:-1], n1), x.dtype, x.device)
+    out0, out1 = _adapter_out(name, out0, x, n0), _adapter_out(name, out1, x, n1)
     if rows == 0:
         return out0, out1
     need = adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1)
     ws = _ws(name, workspace, need, x.device)
     p0 = [t.data_ptr() for t in bank0] if bank0 is not None else [None] * 3
     p1 = [t.data_ptr() for t in bank1] if bank1 is not None else [None] * 3
-    _call_on(x.device, name, _ptr(x), _ptr(w0), _ptr(w1), *p0, *p1, _ptr(ids), _ptr(out0), _ptr(out1), _ptr(ws), need,
-             rows, tokens, k, n0, n1, rank0, rank1, slots0, slots1, dtype_code(x, name), _stream(x))
+    _call_on(x.device, name, x.data_ptr(), w0.data_ptr(), w1.data_ptr(), *p0, *p1, ids.data_ptr(), out0.data_ptr(),
+             out1.data_ptr(), _ptr(ws), need, rows, tokens, k, n0, n1, rank0, rank1, slots0, slots1, BF16, _stream(x))
     return out0, out1
 
 

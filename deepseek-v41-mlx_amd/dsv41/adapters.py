@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _abi
-from .layers import DECODE_ROWS, _only_the_product, decode_linear, decode_linear_pair
+from .layers import DECODE_ROWS, decode_linear, decode_linear_pair
 
 
 class AdapterBank:
@@ -64,21 +64,36 @@ class AdapterBank:
         self.scale[slot] = 0.0
 
 
-def _check(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank, ids: torch.Tensor) -> None:
-    if (bank.out_features, bank.in_features) != tuple(lin.weight.shape):
-        raise ValueError(f"adapters of [{bank.out_features}, {bank.in_features}] on a projection of "
-                         f"{list(lin.weight.shape)}")
-    if torch.is_grad_enabled() and (x.requires_grad or lin.weight.requires_grad):
+def _no_gradient(x: torch.Tensor, w: torch.Tensor) -> None:
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         raise ValueError("adapter projections are not differentiable: call them under torch.no_grad()")
 
 
-def _fused_ok(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank | None) -> bool:
-    """Whether the projection runs with its adapters in dsv41_adapter_linear: bf16 in whole 64-channel steps and 32-row
-    weight tiles, ranks up to 128, and a module whose call is the product alone."""
-    w = lin.weight
-    return (x.dtype == torch.bfloat16 == w.dtype and x.is_cuda and lin.bias is None and w.is_contiguous()
-            and w.shape[1] % 64 == 0 and w.shape[0] % 32 == 0 and (bank is None or bank.a.shape[1] <= 128)
-            and _only_the_product(lin, x))
+_module = torch.nn.modules.module
+_FORWARD_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+# multiply-adds up to which a product off the bf16 tiles' shapes runs with its adapters in one launch
+# (dsv41_adapter_plain) instead of after torch's linear
+_PLAIN_MACS = 1 << 28
+
+
+def _product_weight(lin: torch.nn.Linear, x: torch.Tensor) -> torch.Tensor | None:
+    """The projection's weight where the module's call is the product alone (no hooks, bias or forward of its own), of
+    x's type and in one piece, so that a kernel may stand in for the module."""
+    own = lin.__dict__
+    if (type(lin) is not torch.nn.Linear or "forward" in own or any(own[h] for h in _FORWARD_HOOKS)
+            or _module._global_forward_hooks or _module._global_forward_pre_hooks
+            or own["_parameters"]["bias"] is not None):
+        return None
+    w = own["_parameters"]["weight"]
+    return w if w.dtype is x.dtype and w.is_contiguous() else None
+
+
+def _tiles_ok(w: torch.Tensor, x: torch.Tensor, rank: int) -> bool:
+    """What dsv41_adapter_linear takes: bf16 in whole 64-channel steps and 32-row weight tiles, 16-byte addresses."""
+    return (x.dtype is torch.bfloat16 and rank <= 128 and w.shape[1] % 64 == 0 and w.shape[0] % 32 == 0
+            and w.data_ptr() % 16 == 0 and x.data_ptr() % 16 == 0)
 
 
 def adapter_linear(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank | None, ids: torch.Tensor | None,
@@ -87,11 +102,19 @@ def adapter_linear(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank | No
     ids it is decode_linear(lin, x, wide_only)."""
     if bank is None or ids is None:
         return decode_linear(lin, x, wide_only)
-    _check(lin, x, bank, ids)
-    if _fused_ok(lin, x, bank):
-        return _abi.adapter_linear(x.contiguous(), lin.weight, bank.a, bank.b, bank.scale, ids)
-    y = lin(x)
-    return _abi.adapter_add(x.contiguous(), bank.a, bank.b, bank.scale, ids, y.contiguous())
+    x = x.contiguous()
+    w = _product_weight(lin, x)
+    if w is not None:
+        _no_gradient(x, w)
+        if _tiles_ok(w, x, bank.a.shape[1]):
+            return _abi.adapter_linear(x, w, bank.a, bank.b, bank.scale, ids)
+        if x.numel() * w.shape[0] <= _PLAIN_MACS:
+            return _abi.adapter_plain(x, w, bank.a, bank.b, bank.scale, ids)
+    _no_gradient(x, lin.weight)
+    if (bank.out_features, bank.in_features) != tuple(lin.weight.shape):
+        raise ValueError(f"adapters of [{bank.out_features}, {bank.in_features}] on a projection of "
+                         f"{list(lin.weight.shape)}")
+    return _abi.adapter_add(x, bank.a, bank.b, bank.scale, ids, lin(x).contiguous())
 
 
 def adapter_linear_pair(lin0: torch.nn.Linear, lin1: torch.nn.Linear, x: torch.Tensor, bank0: AdapterBank | None,
@@ -100,11 +123,14 @@ def adapter_linear_pair(lin0: torch.nn.Linear, lin1: torch.nn.Linear, x: torch.T
     without any bank or ids it is decode_linear_pair."""
     if ids is None or (bank0 is None and bank1 is None):
         return decode_linear_pair(lin0, lin1, x)
-    for lin, bank in ((lin0, bank0), (lin1, bank1)):
-        if bank is not None:
-            _check(lin, x, bank, ids)
-    if (x.numel() <= DECODE_ROWS * x.shape[-1] and lin0.weight.shape[1] == lin1.weight.shape[1]
-            and _fused_ok(lin0, x, bank0) and _fused_ok(lin1, x, bank1)):
-        pair = [None if bank is None else (bank.a, bank.b, bank.scale) for bank in (bank0, bank1)]
-        return _abi.adapter_linear_pair(x.contiguous(), lin0.weight, lin1.weight, *pair, ids)
+    if x.numel() <= DECODE_ROWS * x.shape[-1]:
+        x = x.contiguous()
+        w0, w1 = _product_weight(lin0, x), _product_weight(lin1, x)
+        if (w0 is not None and w1 is not None and w0.shape[1] == w1.shape[1]
+                and _tiles_ok(w0, x, 0 if bank0 is None else bank0.a.shape[1])
+                and _tiles_ok(w1, x, 0 if bank1 is None else bank1.a.shape[1])):
+            _no_gradient(x, w0)
+            _no_gradient(x, w1)
+            return _abi.adapter_linear_pair(x, w0, w1, None if bank0 is None else (bank0.a, bank0.b, bank0.scale),
+                                            None if bank1 is None else (bank1.a, bank1.b, bank1.scale), ids)
     return adapter_linear(lin0, x, bank0, ids), adapter_linear(lin1, x, bank1, ids)

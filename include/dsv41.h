@@ -587,6 +587,12 @@ int dsv41_adapter_linear(const void* x, const void* w, const void* a, const void
                          int32_t tokens, int32_t k, int32_t n, int32_t rank, int32_t slots, int32_t dtype,
                          hipStream_t stream);
 
+/* The same for any k, n and rank, F32 or BF16, in one launch on the fp32 matrix cores: exact fp32 arithmetic, meant for
+ * small products (float32 activations, widths that the other call does not take). */
+int dsv41_adapter_plain(const void* x, const void* w, const void* a, const void* b, const float* scale,
+                        const int32_t* ids, void* y, int64_t rows, int32_t tokens, int32_t k, int32_t n, int32_t rank,
+                        int32_t slots, int32_t dtype, hipStream_t stream);
+
 /* Two projections of the same rows (at most 128), each with adapters of its own under the same ids, in one call:
  * y0 [rows, n0] and y1 [rows, n1] as two dsv41_adapter_linear calls give them, up to the order of fp32 additions.
  * A bank of 0 slots (its pointers unused) has no adapters; one of the two must have some. The workspace of both calls

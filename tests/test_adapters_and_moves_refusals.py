@@ -99,6 +99,17 @@ def test_adapter_linear_checks_its_tensors(host_abi):
     _refused(call(out=torch.zeros(2, 5, 32)), "out must be")
     _refused(call(workspace=torch.zeros(64)), "workspace")
 
+    def plain(**kw):
+        args = dict(x=x, w=w, a=b.a, b=b.b, scale=b.scale, ids=ids)
+        args.update(kw)
+        return lambda: A.adapter_plain(**args)
+
+    _reaches(plain())
+    assert A.adapter_plain(x[:0], w, b.a, b.b, b.scale, ids[:0]).shape == (0, 5, 32)
+    _refused(plain(w=w.float()), "contract")
+    _refused(plain(w=w1), "no adapters")
+    _refused(plain(out=torch.zeros(2, 5, 32)), "out must be")
+
     def pair(**kw):
         args = dict(x=x, w0=w, w1=w1, bank0=(b.a, b.b, b.scale), bank1=(c.a, c.b, c.scale), ids=ids)
         args.update(kw)
@@ -140,6 +151,7 @@ def test_banks():
         _refused(lambda: AdapterBank(*bad, device="cpu"), "positive")
     _refused(lambda: AdapterBank(1, 64, 32, 8, torch.float16, "cpu"), "dtype")
     lin = torch.nn.Linear(64, 40, bias=False, dtype=BF)
+    lin.register_forward_hook(lambda *a: None)            # the module's own call, which the bank does not go with
     _refused(lambda: adapter_linear(lin, torch.zeros(2, 64, dtype=BF), b, torch.zeros(2, dtype=torch.int32)), "projection")
 
 
@@ -229,6 +241,19 @@ def test_c_entry_points_refuse_bad_sizes():
     need = lib.dsv41_adapter_linear_workspace_bytes(4, 64, 32, 0, 8, 0)
     assert need > 0 and linear(bytes=need - 1) == -4 and linear(ws=None) == -4
     assert lib.dsv41_adapter_linear_workspace_bytes(0, 64, 32, 0, 8, 0) == 0
+
+    def plain(**kw):
+        a = dict(x=p, w=p, a=p, b=p, scale=p, ids=p, y=p, rows=4, tokens=2, k=7, n=5, rank=3, slots=1, dtype=_abi.F32)
+        a.update(kw)
+        return lib.dsv41_adapter_plain(*a.values(), None)
+
+    assert plain(rows=0) == 0
+    for bad in (dict(rows=-1), dict(rows=5), dict(tokens=0), dict(k=0), dict(n=0), dict(rank=0), dict(slots=0),
+                dict(rows=1 << 31, tokens=1), dict(rows=1 << 30, tokens=1, n=1 << 20)):
+        assert plain(**bad) == -1, bad
+    for name in ("x", "w", "a", "b", "scale", "ids", "y"):
+        assert plain(**{name: None}) == -1, name
+    assert plain(dtype=_abi.FP8_E4M3) == -2
 
     def pair(**kw):
         a = dict(x=p, w0=p, w1=p, a0=p, b0=p, s0=p, a1=p, b1=p, s1=p, ids=p, y0=p, y1=p, ws=p, bytes=1 << 30, rows=4,
