@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256) void adapter_plain_split_kernel(const T* __res
           h[u] = f32x4{0.f, 0.f, 0.f, 0.f};
           ap[u] = a + ((int64_t)t[u] * rank + min(q + l16, rank - 1)) * k;
         }
-#pragma unroll 2
+#pragma unroll 4
         for (int c = 16 * wave; c < k; c += 64) {
           const f32x4 xf = load4<T, VEC>(xp, c + 4 * g, k);
 #pragma unroll
@@ -278,6 +278,7 @@ struct AdapterArgs {
   int tokens, k;
   int chunk, chunks;     // channels of one partial h, and how many
   int sub;               // rows of a share of it: 4 or 16
+  int done;              // h is finished before the tiles' launch
   int apart;             // leading workgroups that compute shares of h and no tile (0: the tiles' workgroups do)
   bf16_t* y;             // [rows, t.r0]
   bf16_t* y1;            // [rows, t.r - t.r0]
@@ -526,19 +527,15 @@ struct Expand {
         named(named_), todo(named_), q(0) {
     load();
   }
-  // hval(c, v) gives scale times ranks 8 c .. 8 c + 7 of the lane's row
+  // operand(at) gives the lane's part of scale h for a rank slot
   template <typename H>
-  __device__ __forceinline__ void add(f32x4 (&acc)[WR], H hval) {
+  __device__ __forceinline__ void add(f32x4 (&acc)[WR], H operand) {
     const int end = 2 * (rank >> 3);
     bf16x8 hf;
     bool fresh = true;
     for (;;) {
       const RankSlot at(q, rank >> 3);
-      if (fresh) {
-        float v[8];
-        hval(at.c, v);
-        hf = or_zero(half_of(v, at.low), at.live);
-      }
+      if (fresh) hf = or_zero(operand(at), at.live);
       int now[U];
       uint4 cur[U][WR];
 #pragma unroll
@@ -711,7 +708,7 @@ adapter_tiles_kernel(AdapterArgs a) {
     }
     auto beside = [&]() {
       // the ring's waits count its own copies only
-      if (apart == 0 && shares(block, total)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (!a.done && apart == 0 && shares(block, total)) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     };
     if constexpr (BK == 64 && NS == 2) tile_sums_ahead<WR, WM, GR, GM>(a.t, lds, rt, mt, grp, acc, beside);
     else tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc, beside);
@@ -732,11 +729,12 @@ adapter_tiles_kernel(AdapterArgs a) {
 
 // The contraction ranges' parts summed in order, plus the adapters' part, rounded once: a workgroup per 16 rows and
 // 64 WR columns, a wave per 16 WR of them (whole blocks of one projection: n0 and n are multiples of 16 WR). The parts
-// and the first adapters' B are on their way while h is summed over its chunks into LDS.
-template <int WR>
+// and the first adapters' B are on their way while h is summed over its chunks into LDS. DONE: h is the finished first
+// product, as it lies.
+template <int WR, bool DONE>
 __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
   constexpr int kStride = kMaxRank + 4;
-  __shared__ __align__(16) float hs[2][16 * kStride];
+  __shared__ __align__(16) float hs[DONE ? 1 : 2][DONE ? 4 : 16 * kStride];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int ctiles = (a.t.r + 64 * WR - 1) / (64 * WR);
   const int col0 = (int)(blockIdx.x % ctiles) * 64 * WR, m0 = (int)(blockIdx.x / ctiles) * 16;
@@ -760,8 +758,9 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
       }
   };
   auto sum_h = [&]() {
+    if constexpr (DONE) return;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 2 && !DONE; ++s) {
       const Bank& bs = a.bank[s];
       if (bs.slots == 0 || (s == 0 ? col0 >= a.t.r0 : col0 + 64 * WR <= a.t.r0)) continue;
       const int quads = bs.rank >> 2;
@@ -786,10 +785,17 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
     }
     __syncthreads();
   };
-  auto hval = [&](int c, float* v) {
-    const float* from = hs[sel] + l16 * kStride + 8 * c;
+  auto operand = [&](const RankSlot& slot) {
+    if constexpr (DONE) {
+      const uint16_t* from = reinterpret_cast<const uint16_t*>(bk.h) + (int64_t)min(m, a.t.rows - 1) * 2 * bk.rank;
+      return *reinterpret_cast<const uint4*>(from + 8 * slot.c + (slot.low ? bk.rank : 0));
+    } else {
+      float v[8];
+      const float* from = hs[sel] + l16 * kStride + 8 * slot.c;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = from[e];
+      for (int e = 0; e < 8; ++e) v[e] = from[e];
+      return half_of(v, slot.low);
+    }
   };
   const bool one = named == 0 || __ballot(id >= 0 && id != __builtin_amdgcn_readlane(id, __builtin_ctz(named | 0x10000u))) == 0;
   if (named == 0) {
@@ -799,12 +805,12 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
     Expand<WR, 1> ex(bk, n, at, id, named);
     sum_parts();
     sum_h();
-    ex.add(acc, hval);
+    ex.add(acc, operand);
   } else {
     Expand<WR, 4> ex(bk, n, at, id, named);
     sum_parts();
     sum_h();
-    ex.add(acc, hval);
+    ex.add(acc, operand);
   }
   if (m < a.t.rows)
 #pragma unroll
@@ -821,11 +827,12 @@ struct AdapterPlan {
   int tr, tm;            // the tile's weight rows and query rows
   int splits;            // contraction ranges; 1 with direct
   bool direct;
+  bool done;             // h finished by a launch of its own; else in shares beside the split sums
   int chunk, chunks, sub;
   bool two;              // two of the tile's workgroups fit a CU
 };
 
-// Ranges for decode row counts, by the rule of the decode-row projections: at 33-64 rows the ranges whose wide tiles
+// Ranges for decode row counts, near the rule of the decode-row projections: at 33-64 rows the ranges whose wide tiles
 // make the most workgroups when some do, otherwise the most that keep n / 32 x ranges workgroups within 256.
 static int decode_splits(int rows, int k, int n) {
   int best = 0;
@@ -842,6 +849,10 @@ static int decode_splits(int rows, int k, int n) {
   best = 1;
   for (int s = 1; s <= 64; ++s)
     if (k % (64 * s) == 0 && (int64_t)(n / 32) * s <= 256) best = s;
+  // up to 32 rows two workgroups share a CU: a few more ranges where a quarter of the CUs would have none (8192 -> 5120,
+  // 160 tiles, 2 rows: two ranges 28.8 us, one 38.4; but 5120 -> 1280 at 8 rows: five ranges 17.9, ten 20.2)
+  for (int s = best + 1; rows <= 32 && s <= 64 && (int64_t)(n / 32) * best < 192 && (int64_t)(n / 32) * s <= 512; ++s)
+    if (k % (64 * s) == 0) best = s;
   return best;
 }
 
@@ -849,8 +860,10 @@ static int decode_splits(int rows, int k, int n) {
 static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
   AdapterPlan p;
   p.splits = 1;
-  p.direct = false;
-  if (rows <= 128) {
+  p.direct = p.done = false;
+  // up to 64 rows, and up to 128 of narrow or paired projections, tiles of few weight rows that stream the weight; wide
+  // ones at 65 to 128 rows take the prompts' tiles (90 rows 1280 -> 32768: 29 against 51 us, 8192 -> 5120: 47 against 56)
+  if (rows <= 64 || (rows <= 128 && (n <= 4096 || n0 != n))) {
     p.splits = decode_splits(rows, k, n);
     const int wide = wide_split_tile(rows, k / p.splits, n, p.splits);
     if (wide && n0 % wide == 0) {
@@ -908,11 +921,14 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
       }
     }
     p.direct = p.splits == 1;
-    p.two = p.tile != kTile256 && p.tile != kTile32;
-    // beside split sums: enough shares of h to fill the chip, at most 8 of them for the next kernel to sum
+    // h in shares beside split sums while it is few tiles of 16 rows and 16 ranks, in a launch of its own beyond (200 rows
+    // 5120 -> 512 at rank 64, 52 tiles: 30 against 39 us; 4,144 rows, 1,036 tiles: 122 against 92)
     const int64_t items = (int64_t)((rows + 15) / 16) * ((rank + 15) / 16);
-    const int parts = (int)(items >= 768 ? 1 : (768 + items - 1) / items > 8 ? 8 : (768 + items - 1) / items);
-    p.chunk = p.direct ? k : ((k + parts - 1) / parts + 127) / 128 * 128;
+    p.done = p.direct || items > 128;
+    p.two = p.tile != kTile256 && p.tile != kTile32;
+    // enough shares to fill the chip, at most 8 for the next kernel to sum
+    const int parts = (int)((768 + items - 1) / items > 8 ? 8 : (768 + items - 1) / items);
+    p.chunk = p.done ? k : ((k + parts - 1) / parts + 127) / 128 * 128;
   }
   p.chunks = (k + p.chunk - 1) / p.chunk;
   return p;
@@ -1091,17 +1107,23 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   // shares of h on workgroups of their own while all of them and all tiles run at once (a multiple of 8, so that the
   // tiles keep their XCDs): one row 5120 -> 1280 + 512 at rank 16 TIMING3
   const int64_t room = p.two ? 512 : 256, spare = (shrinks + 7) / 8 * 8;
-  a.apart = !p.direct && tiles + spare <= room ? (int)spare : 0;
+  a.apart = !p.done && tiles + spare <= room ? (int)spare : 0;
+  a.done = p.done;
   a.y = static_cast<bf16_t*>(y0);
   a.y1 = static_cast<bf16_t*>(y1);
-  if (p.direct && rank0) launch_shrink(a, stream);
+  if (p.done && rank0) launch_shrink(a, stream);
   launch_projection(a, p, stream);
   if (!p.direct) {
     // 256 columns per workgroup where that still gives every CU two of them, 64 otherwise
-    if (n0 % 64 == 0 && n1 % 64 == 0 && (rows + 15) / 16 * ((n + 255) / 256) >= 512)
-      hipLaunchKernelGGL(adapter_reduce_kernel<4>, dim3((unsigned)((rows + 15) / 16 * ((n + 255) / 256))), dim3(256), 0,
-                         stream, a);
-    else hipLaunchKernelGGL(adapter_reduce_kernel<1>, dim3((unsigned)reduces), dim3(256), 0, stream, a);
+    const int64_t wide = (rows + 15) / 16 * ((n + 255) / 256);
+    auto reduce = [&](auto kernel, int64_t blocks) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
+    };
+    if (n0 % 64 == 0 && n1 % 64 == 0 && wide >= 512) {
+      if (p.done) reduce(adapter_reduce_kernel<4, true>, wide);
+      else reduce(adapter_reduce_kernel<4, false>, wide);
+    } else if (p.done) reduce(adapter_reduce_kernel<1, true>, reduces);
+    else reduce(adapter_reduce_kernel<1, false>, reduces);
   }
   return check_launch(what);
 }
