@@ -405,95 +405,93 @@ struct RankSlot {
   }
 };
 
-// The whole first product of 16 MT rows and 16 RT ranks: the channels in 64-wide steps in turn over NW waves, each
-// step's x rows read once for all ranks and each adapter row once for all x rows; the waves' sums meet in LDS. Writes
-// the second product's operand: per row the upper halves of scale h's ranks, then the lower ones ([rows, 2 rank] bf16).
-// A tile whose rows name several adapters repeats the channels for each and keeps every row's own.
-template <int MT, int RT, int NW>
-__global__ __launch_bounds__(64 * NW) void adapter_shrink_kernel(AdapterArgs a) {
-  __shared__ __align__(16) float red[NW][MT * RT * 256];
+// The whole first product of up to 16 MT rows of one sequence - so of one adapter - and 16 RT ranks. x and A come to LDS
+// 256 channels at a time (a copy instruction takes 512 bytes of each of two rows: fragments loaded from memory directly
+// touch 16 rows per instruction: 8,192 rows of 8192 channels at rank 64 took 63 us, 41 this way), NS - 1 steps ahead; MT RT waves a 16 x 16
+// tile each, times KS that share a step's channels. Writes the second product's operand: per row the upper halves of
+// scale h's ranks, then the lower ones ([rows, 2 rank] bf16). Rows without an adapter are left as they are.
+//
+// A step's tile row is 32 chunks of 16 bytes; chunk c of row r lies at c ^ (r & 15) (and within the 32), so that the 16
+// rows of a fragment read start in different banks.
+template <int MT, int RT, int KS>
+struct ShrinkCfg {
+  static constexpr int NW = MT * RT * KS, ROWS = 16 * (MT + RT), STAGE = ROWS * 512;
+  static constexpr int COPIES = ROWS / 2 / NW;                                     // per wave and step
+  static constexpr int NS = 156 * 1024 / STAGE > 6 ? 6 : 156 * 1024 / STAGE;
+  static_assert(COPIES * NW * 2 == ROWS, "whole copies per wave");
+  static_assert(KS * MT * RT * 1024 <= NS * STAGE, "the waves' sums fit the ring");
+};
+
+template <int MT, int RT, int KS>
+__global__ __launch_bounds__(64 * MT * RT * KS) void adapter_shrink_kernel(AdapterArgs a) {
+  using C = ShrinkCfg<MT, RT, KS>;
+  __shared__ __align__(16) uint8_t ring[C::NS * C::STAGE];
   const Bank& bk = a.bank[0];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int rtiles = (bk.rank + 16 * RT - 1) / (16 * RT);
-  const int r0 = (int)(blockIdx.x % rtiles) * 16 * RT, m0 = (int)(blockIdx.x / rtiles) * 16 * MT;
-  int id[MT];
-  const bf16_t* xp[MT];
-  uint32_t todo[MT];
+  const int rtiles = (bk.rank + 16 * RT - 1) / (16 * RT), mtiles = (a.tokens + 16 * MT - 1) / (16 * MT);
+  const int rt = (int)(blockIdx.x % rtiles), mt = (int)(blockIdx.x / rtiles % mtiles), seq = (int)(blockIdx.x / rtiles / mtiles);
+  const int t = a.ids[seq];
+  if ((uint32_t)t >= (uint32_t)bk.slots) return;
+  const int r0 = rt * 16 * RT, rows = min(16 * MT, a.tokens - mt * 16 * MT);
+  const int64_t m0 = (int64_t)seq * a.tokens + mt * 16 * MT;
+  // copy j of a wave: tile rows 2 (wave COPIES + j) and + 1, x's first; lane l takes position l % 32 of its row. Rows past
+  // the sequence or the ranks repeat the last one: not stored
+  uint64_t src[C::COPIES];
+  int chunk[C::COPIES];
 #pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int m = m0 + 16 * j + l16;
-    id[j] = row_adapter(a, bk, m);
-    xp[j] = a.t.o + (int64_t)min(m, a.t.rows - 1) * a.k + 8 * g;
-    todo[j] = (uint32_t)__ballot(id[j] >= 0) & 0xFFFFu;
+  for (int j = 0; j < C::COPIES; ++j) {
+    const int r = 2 * (wave * C::COPIES + j) + (lane >> 5);
+    chunk[j] = (lane & 31) ^ (r & 15);
+    src[j] = r < 16 * MT ? reinterpret_cast<uint64_t>(a.t.o + (m0 + min(r, rows - 1)) * a.k)
+                         : reinterpret_cast<uint64_t>(bk.a + ((int64_t)t * bk.rank + min(r0 + r - 16 * MT, bk.rank - 1)) * a.k);
   }
-  f32x4 res[MT][RT];
+  const uint32_t lds0 = lds_offset(ring);
+  const int chunks = a.k / 8, steps = (a.k + 255) / 256;
+  auto issue = [&](int buf, int step) {
+    const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + (uint32_t)(buf * C::STAGE + wave * C::COPIES * 1024)));
 #pragma unroll
-  for (int j = 0; j < MT; ++j)
+    for (int j = 0; j < C::COPIES; ++j)      // chunks past the last channel repeat the last: not multiplied
+      dma16_vaddr(src[j] + 16 * (uint64_t)min(32 * step + chunk[j], chunks - 1), at + j * 1024);
+  };
+  const int part = wave % KS, j0 = wave / KS % MT, i0 = wave / KS / MT;     // this wave's channels and tile
+  f32x4 acc[1] = {{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int i = 0; i < RT; ++i) res[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (;;) {
-    int t = -1;
+  for (int p = 0; p < C::NS - 1; ++p)
+    if (p < steps) issue(p, p);
+  for (int st = 0; st < steps; ++st) {
+    wait_copies_deep<C::COPIES, C::NS - 2>(min(C::NS - 2, steps - 1 - st));
+    __syncthreads();
+    if (st + C::NS - 1 < steps) issue((st + C::NS - 1) % C::NS, st + C::NS - 1);
+    const uint8_t* xt = ring + (st % C::NS) * C::STAGE + (16 * j0 + l16) * 512;
+    const uint8_t* at = ring + (st % C::NS) * C::STAGE + (16 * (MT + i0) + l16) * 512;
+    const int live = min(8, (a.k - 256 * st) / 32);
 #pragma unroll
-    for (int j = 0; j < MT; ++j)
-      if (t < 0 && todo[j]) t = __builtin_amdgcn_readlane(id[j], __builtin_ctz(todo[j]));
-    if (t < 0) break;
-#pragma unroll
-    for (int j = 0; j < MT; ++j) todo[j] &= ~(uint32_t)__ballot(id[j] == t);
-    const bf16_t* ap[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i)   // ranks past the end: not stored
-      ap[i] = bk.a + ((int64_t)t * bk.rank + min(r0 + 16 * i + l16, bk.rank - 1)) * a.k + 8 * g;
-    f32x4 acc[MT][RT];
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-#pragma unroll
-      for (int i = 0; i < RT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-    for (int k = 64 * wave; k < a.k; k += 64 * NW) {
-      bf16x8 xf[2][MT], af[2][RT];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int j = 0; j < MT; ++j) xf[h][j] = ld_bf16x8(xp[j] + k + 32 * h);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) af[h][i] = ld_bf16x8(ap[i] + k + 32 * h);
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-          for (int i = 0; i < RT; ++i) acc[j][i] = mfma16x16x32(af[h][i], xf[h][j], acc[j][i]);
-    }
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      settle(acc[j]);
-#pragma unroll
-      for (int i = 0; i < RT; ++i) res[j][i] = id[j] == t ? acc[j][i] : res[j][i];
+    for (int s = 0; s < 8; s += KS) {
+      if (s + part >= live) continue;
+      const int c = ((4 * (s + part) + g) ^ l16) << 4;
+      acc[0] = mfma16x16x32(ld_bf16x8(at + c), ld_bf16x8(xt + c), acc[0]);
     }
   }
-  // lane (g, l16) holds ranks 4 g .. 4 g + 3 of row l16 of every tile
-#pragma unroll
-  for (int j = 0; j < MT; ++j)
-#pragma unroll
-    for (int i = 0; i < RT; ++i)
-      *reinterpret_cast<f32x4*>(&red[wave][((j * 16 + l16) * RT + i) * 16 + 4 * g]) = res[j][i];
+  settle(acc);
+  // lane (g, l16) holds ranks 4 g .. 4 g + 3 of row l16 of its tile
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(ring);               // [KS][16 MT][16 RT]
+  *reinterpret_cast<f32x4*>(red + ((part * 16 * MT + 16 * j0 + l16) * RT + i0) * 16 + 4 * g) = acc[0];
   __syncthreads();
   uint16_t* hl = reinterpret_cast<uint16_t*>(bk.h);
-  for (int q = threadIdx.x; q < MT * RT * 32; q += 64 * NW) {          // 8 ranks of one row each
-    const int row = q / (2 * RT), c = q % (2 * RT), m = m0 + row, r = r0 + 8 * c;
-    if (m >= a.t.rows || r >= bk.rank) continue;
-    const int t = row_adapter(a, bk, m);
-    const float scale = t < 0 ? 0.0f : bk.scale[t];
+  const float scale = bk.scale[t];
+  for (int q = threadIdx.x; q < MT * RT * 32; q += 64 * C::NW) {           // 8 ranks of one row each
+    const int row = q / (2 * RT), r = r0 + 8 * (q % (2 * RT));
+    if (row >= rows || r >= bk.rank) continue;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      float sum = red[0][q * 8 + e];
+      float sum = red[q * 8 + e];
 #pragma unroll
-      for (int w = 1; w < NW; ++w) sum += red[w][q * 8 + e];
+      for (int w = 1; w < KS; ++w) sum += red[w * MT * RT * 256 + q * 8 + e];
       v[e] = sum * scale;
     }
-    uint16_t* to = hl + (int64_t)m * 2 * bk.rank + r;
+    uint16_t* to = hl + (m0 + row) * 2 * bk.rank + r;
     *reinterpret_cast<uint4*>(to) = half_of(v, false);
     *reinterpret_cast<uint4*>(to + bk.rank) = half_of(v, true);
   }
@@ -660,7 +658,7 @@ adapter_tiles_kernel(AdapterArgs a) {
     grp = tile / (rtiles * mtiles);
   } else {
     // consecutive tiles on one XCD, in bands of 4 query tiles: 32 CUs work on 4 x 8 tiles and share their 12 operand
-    // panels in the XCD's L2, where 1 x 32 tiles read 33 (TIMING)
+    // panels in the XCD's L2, where 1 x 32 tiles read 33 (no faster by itself; bands of 2, 8 and 16 measure alike)
     constexpr int kBand = 4;
     const int xcd = block % 8, per = total / 8, more = total % 8;
     const int tile = xcd * per + min(xcd, more) + block / 8;
@@ -948,19 +946,24 @@ static void launch_adapter_tiles(const AdapterArgs& a, int64_t tiles, hipStream_
                      stream, a);
 }
 
-// Rows and ranks per workgroup of the finished first product: 16 rows and 16 waves while the rows do not fill the chip
-// (latency: 999 rows of 1280 channels at rank 32 TIMING2), 32 rows beyond 16 ranks otherwise.
+// Rows and ranks per workgroup of the finished first product (one per CU): 32 rows where the fewer rounds are the less,
+// each about 1.35 of one of 16 rows (5120 channels at rank 64: 20.1 against 14.7 us, at rank 16 12.5 against 9.6).
+static int64_t shrink_blocks(int64_t rows, int tokens, int rank, int mt, int rt) {
+  return rows / tokens * ((tokens + 16 * mt - 1) / (16 * mt)) * ((rank + 16 * rt - 1) / (16 * rt));
+}
+
 static void launch_shrink(const AdapterArgs& a, hipStream_t stream) {
   const int rank = a.bank[0].rank;
-  auto blocks = [&](int mt, int rt) {
-    return dim3((unsigned)(((a.t.rows + 16 * mt - 1) / (16 * mt)) * ((rank + 16 * rt - 1) / (16 * rt))));
+  const int rt = rank <= 16 ? 1 : rank <= 32 ? 2 : 4;
+  auto rounds = [&](int mt) { return (double)((shrink_blocks(a.t.rows, a.tokens, rank, mt, rt) + 255) / 256); };
+  const bool two = 1.35 * rounds(2) < rounds(1);
+  auto go = [&](auto kernel, int mt, int waves) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)shrink_blocks(a.t.rows, a.tokens, rank, mt, rt)), dim3(64 * waves), 0, stream,
+                       a);
   };
-  if (a.t.rows <= 2048) {
-    if (rank <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<1, 1, 16>), blocks(1, 1), dim3(1024), 0, stream, a);
-    else hipLaunchKernelGGL((adapter_shrink_kernel<1, 2, 16>), blocks(1, 2), dim3(1024), 0, stream, a);
-  } else if (rank <= 16) hipLaunchKernelGGL((adapter_shrink_kernel<1, 1, 8>), blocks(1, 1), dim3(512), 0, stream, a);
-  else if (rank <= 32) hipLaunchKernelGGL((adapter_shrink_kernel<2, 2, 8>), blocks(2, 2), dim3(512), 0, stream, a);
-  else hipLaunchKernelGGL((adapter_shrink_kernel<2, 4, 8>), blocks(2, 4), dim3(512), 0, stream, a);
+  if (rt == 1) two ? go(adapter_shrink_kernel<2, 1, 2>, 2, 4) : go(adapter_shrink_kernel<1, 1, 4>, 1, 4);
+  else if (rt == 2) two ? go(adapter_shrink_kernel<2, 2, 1>, 2, 4) : go(adapter_shrink_kernel<1, 2, 2>, 1, 4);
+  else two ? go(adapter_shrink_kernel<2, 4, 1>, 2, 8) : go(adapter_shrink_kernel<1, 4, 2>, 1, 8);
 }
 
 template <int WR, int WM, int GR, int GM, int BK, int NS>
@@ -1083,7 +1086,8 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   const int rank0 = banks[0].slots ? banks[0].rank : 0, rank1 = banks[1].slots ? banks[1].rank : 0, n = n0 + n1;
   const AdapterPlan p = adapter_plan((int)rows, k, n, n0, rank0 > rank1 ? rank0 : rank1);
   const int64_t tiles = (int64_t)(n / p.tr) * ((rows + p.tm - 1) / p.tm) * p.splits;
-  const int64_t shrinks = (rows + p.sub - 1) / p.sub * p.chunks * ((rank0 + 15) / 16 + (rank1 + 15) / 16);
+  const int64_t shrinks = p.done ? shrink_blocks(rows, tokens, rank0, 1, 1)
+                                 : (rows + p.sub - 1) / p.sub * p.chunks * ((rank0 + 15) / 16 + (rank1 + 15) / 16);
   const int64_t reduces = (rows + 15) / 16 * ((n + 63) / 64);
   DSV41_REQUIRE(tiles < (1ll << 31) && shrinks < (1ll << 31) && reduces < (1ll << 31), DSV41_E_ARG, "%s: too many tiles",
                 what);
@@ -1105,7 +1109,7 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   a.chunks = p.chunks;
   a.sub = p.sub;
   // shares of h on workgroups of their own while all of them and all tiles run at once (a multiple of 8, so that the
-  // tiles keep their XCDs): one row 5120 -> 1280 + 512 at rank 16 TIMING3
+  // tiles keep their XCDs): one row 5120 -> 1280 + 512 at rank 16 7.2 against 9.8 us
   const int64_t room = p.two ? 512 : 256, spare = (shrinks + 7) / 8 * 8;
   a.apart = !p.done && tiles + spare <= room ? (int)spare : 0;
   a.done = p.done;
