@@ -426,13 +426,15 @@ template <int MT, int RT, int KS>
 __global__ __launch_bounds__(64 * MT * RT * KS) void adapter_shrink_kernel(AdapterArgs a) {
   using C = ShrinkCfg<MT, RT, KS>;
   __shared__ __align__(16) uint8_t ring[C::NS * C::STAGE];
-  const Bank& bk = a.bank[0];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int rtiles = (bk.rank + 16 * RT - 1) / (16 * RT), mtiles = (a.tokens + 16 * MT - 1) / (16 * MT);
+  // rank tiles of the first bank, then the second's
+  const int rtiles0 = (a.bank[0].rank + 16 * RT - 1) / (16 * RT), rtiles = rtiles0 + (a.bank[1].rank + 16 * RT - 1) / (16 * RT);
+  const int mtiles = (a.tokens + 16 * MT - 1) / (16 * MT);
   const int rt = (int)(blockIdx.x % rtiles), mt = (int)(blockIdx.x / rtiles % mtiles), seq = (int)(blockIdx.x / rtiles / mtiles);
+  const Bank& bk = a.bank[rt >= rtiles0];
   const int t = a.ids[seq];
   if ((uint32_t)t >= (uint32_t)bk.slots) return;
-  const int r0 = rt * 16 * RT, rows = min(16 * MT, a.tokens - mt * 16 * MT);
+  const int r0 = (rt >= rtiles0 ? rt - rtiles0 : rt) * 16 * RT, rows = min(16 * MT, a.tokens - mt * 16 * MT);
   const int64_t m0 = (int64_t)seq * a.tokens + mt * 16 * MT;
   // copy j of a wave: tile rows 2 (wave COPIES + j) and + 1, x's first; lane l takes position l % 32 of its row. Rows past
   // the sequence or the ranks repeat the last one: not stored
@@ -566,8 +568,8 @@ struct Expand {
 // each multiplies all rows and every lane keeps its own row's, one result beside the sums at a time (they fill the
 // registers). ONE: the sequences are whole blocks, so the second kind is never met.
 template <int WR, int WM, bool ONE>
-__device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const AdapterArgs& a, int m0, int col) {
-  const Bank& bk = a.bank[0];
+__device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const AdapterArgs& a, const Bank& bk, int n, int m0,
+                                             int col) {
   const int l16 = threadIdx.x & 15, r8 = bk.rank >> 3;
   int id[WM];
   uint32_t todo[WM];
@@ -586,7 +588,7 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
 #pragma unroll
   for (int j = 0; j < WM && !ONE; ++j) one = one && __ballot(id[j] != t && m0 + 16 * j + l16 < a.t.rows) == 0;
   const bf16_t* b0 = bk.b + (int64_t)(col + l16) * bk.rank;
-  const int64_t slot = (int64_t)a.t.r * bk.rank;
+  const int64_t slot = (int64_t)n * bk.rank;
   if (ONE || one) {
     for (int q = 0; q < 2 * r8; q += 4) {
       const RankSlot at(q, r8);
@@ -670,9 +672,12 @@ adapter_tiles_kernel(AdapterArgs a) {
   const int wr = (wave % GR) * 16 * WR, wm = (wave / GR) * 16 * WM;   // this wave's block
   f32x4 acc[WR][WM];
   if constexpr (PART != kSplitSums) {
-    const int col = rt * C::TR + wr;
+    // a tile lies within one of the two projections
+    const int sel = rt * C::TR >= a.t.r0, n = sel ? a.t.r - a.t.r0 : a.t.r0, col = rt * C::TR + wr - (sel ? a.t.r0 : 0);
+    const Bank& bk = a.bank[sel];
+    bf16_t* y = sel ? a.y1 : a.y;
     // the adapters' part first, while the ring's first copies are on their way
-    auto beside = [&]() { expand_block<WR, WM, PART == kExpandOne>(acc, a, mt * C::TM + wm, col); };
+    auto beside = [&]() { expand_block<WR, WM, PART == kExpandOne>(acc, a, bk, n, mt * C::TM + wm, col); };
     if constexpr (BK == 64 && NS == 2) tile_sums_ahead<WR, WM, GR, GM>(a.t, lds, rt, mt, grp, acc, beside);
     else tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc, beside);
 #pragma unroll
@@ -680,7 +685,7 @@ adapter_tiles_kernel(AdapterArgs a) {
 #pragma unroll
     for (int j = 0; j < WM; ++j) {
       const int m = mt * C::TM + wm + 16 * j + l16;
-      bf16_t* to = a.y + (int64_t)m * a.t.r + col;
+      bf16_t* to = y + (int64_t)m * n + col;
       // the swaps of a pair need every lane: a row past the end gives the store up after them
 #pragma unroll
       for (int i = 0; i + 1 < WR; i += 2) {
@@ -859,9 +864,9 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
   AdapterPlan p;
   p.splits = 1;
   p.direct = p.done = false;
-  // up to 64 rows, and up to 128 of narrow or paired projections, tiles of few weight rows that stream the weight; wide
-  // ones at 65 to 128 rows take the prompts' tiles (90 rows 1280 -> 32768: 29 against 51 us, 8192 -> 5120: 47 against 56)
-  if (rows <= 64 || (rows <= 128 && (n <= 4096 || n0 != n))) {
+  // up to 64 rows, and up to 128 of narrow projections, tiles of few weight rows that stream the weight; wide ones at 65
+  // to 128 rows take the prompts' tiles (90 rows 1280 -> 32768: 29 against 51 us, 8192 -> 5120: 47 against 56)
+  if (rows <= 64 || (rows <= 128 && n <= 4096)) {
     p.splits = decode_splits(rows, k, n);
     const int wide = wide_split_tile(rows, k / p.splits, n, p.splits);
     if (wide && n0 % wide == 0) {
@@ -898,7 +903,7 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
                                    {kTile32, 32, 128, 4.0, 0.45, 0.45, true}};
     double best = 1e30;
     for (const Shape& s : shapes) {
-      if (n % s.tr) continue;
+      if (n0 % s.tr || n % s.tr) continue;
       const int64_t tiles = (int64_t)(n / s.tr) * ((rows + s.tm - 1) / s.tm);
       for (int splits = 1; splits <= (s.split ? 16 : 1); ++splits) {
         if (k % (64 * splits) || (splits > 1 && tiles * splits > 512)) continue;
@@ -921,7 +926,7 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
     p.direct = p.splits == 1;
     // h in shares beside split sums while it is few tiles of 16 rows and 16 ranks, in a launch of its own beyond (200 rows
     // 5120 -> 512 at rank 64, 52 tiles: 30 against 39 us; 4,144 rows, 1,036 tiles: 122 against 92)
-    const int64_t items = (int64_t)((rows + 15) / 16) * ((rank + 15) / 16);
+    const int64_t items = (int64_t)((rows + 15) / 16) * ((rank + 15) / 16);   // rank: both banks'
     p.done = p.direct || items > 128;
     p.two = p.tile != kTile256 && p.tile != kTile32;
     // enough shares to fill the chip, at most 8 for the next kernel to sum
@@ -948,17 +953,18 @@ static void launch_adapter_tiles(const AdapterArgs& a, int64_t tiles, hipStream_
 
 // Rows and ranks per workgroup of the finished first product (one per CU): 32 rows where the fewer rounds are the less,
 // each about 1.35 of one of 16 rows (5120 channels at rank 64: 20.1 against 14.7 us, at rank 16 12.5 against 9.6).
-static int64_t shrink_blocks(int64_t rows, int tokens, int rank, int mt, int rt) {
-  return rows / tokens * ((tokens + 16 * mt - 1) / (16 * mt)) * ((rank + 16 * rt - 1) / (16 * rt));
+static int64_t shrink_blocks(int64_t rows, int tokens, int rank0, int rank1, int mt, int rt) {
+  return rows / tokens * ((tokens + 16 * mt - 1) / (16 * mt)) *
+         ((rank0 + 16 * rt - 1) / (16 * rt) + (rank1 + 16 * rt - 1) / (16 * rt));
 }
 
 static void launch_shrink(const AdapterArgs& a, hipStream_t stream) {
-  const int rank = a.bank[0].rank;
+  const int rank0 = a.bank[0].rank, rank1 = a.bank[1].rank, rank = rank0 > rank1 ? rank0 : rank1;
   const int rt = rank <= 16 ? 1 : rank <= 32 ? 2 : 4;
-  auto rounds = [&](int mt) { return (double)((shrink_blocks(a.t.rows, a.tokens, rank, mt, rt) + 255) / 256); };
+  auto rounds = [&](int mt) { return (double)((shrink_blocks(a.t.rows, a.tokens, rank0, rank1, mt, rt) + 255) / 256); };
   const bool two = 1.35 * rounds(2) < rounds(1);
   auto go = [&](auto kernel, int mt, int waves) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)shrink_blocks(a.t.rows, a.tokens, rank, mt, rt)), dim3(64 * waves), 0, stream,
+    hipLaunchKernelGGL(kernel, dim3((unsigned)shrink_blocks(a.t.rows, a.tokens, rank0, rank1, mt, rt)), dim3(64 * waves), 0, stream,
                        a);
   };
   if (rt == 1) two ? go(adapter_shrink_kernel<2, 1, 2>, 2, 4) : go(adapter_shrink_kernel<1, 1, 4>, 1, 4);
@@ -1048,14 +1054,13 @@ extern "C" int dsv41_adapter_add(const void* x, const void* a, const void* b, co
 static bool projection_sizes(int64_t rows, int32_t k, int32_t n0, int32_t n1, int32_t rank0, int32_t rank1) {
   return rows > 0 && rows < (1ll << 31) && k > 0 && k % 64 == 0 && n0 > 0 && n1 >= 0 && n0 % 32 == 0 && n1 % 32 == 0 &&
          (int64_t)n0 + n1 < (1ll << 30) && rank0 >= 0 && rank1 >= 0 && rank0 <= kMaxRank && rank1 <= kMaxRank &&
-         rank0 % 8 == 0 && rank1 % 8 == 0 && (n1 == 0 || rows <= 128);
+         rank0 % 8 == 0 && rank1 % 8 == 0;
 }
 
 extern "C" size_t dsv41_adapter_linear_workspace_bytes(int64_t rows, int32_t k, int32_t n0, int32_t n1, int32_t rank0,
                                                        int32_t rank1) {
   if (!projection_sizes(rows, k, n0, n1, rank0, rank1)) return 0;
-  const int most = rank0 > rank1 ? rank0 : rank1;
-  return plan_bytes(adapter_plan((int)rows, k, n0 + n1, n0, most), (int)rows, n0 + n1, rank0, rank1);
+  return plan_bytes(adapter_plan((int)rows, k, n0 + n1, n0, rank0 + rank1), (int)rows, n0 + n1, rank0, rank1);
 }
 
 static int run_adapter_linear(const char* what, const void* x, const void* w0, const void* w1, const Bank* banks,
@@ -1077,16 +1082,14 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   }
   DSV41_REQUIRE(k % 64 == 0 && n0 % 32 == 0 && n1 % 32 == 0, DSV41_E_SHAPE,
                 "%s: k = %d must be a multiple of 64, n = %d (+ %d) of 32", what, k, n0, n1);
-  DSV41_REQUIRE(n1 == 0 || rows <= 128, DSV41_E_SHAPE, "%s: two projections of %lld rows (at most 128)", what,
-                (long long)rows);
   if (rows == 0) return 0;
   DSV41_REQUIRE(x && w0 && y0 && ids && (n1 == 0 || (w1 && y1)), DSV41_E_ARG, "%s: null tensor", what);
   DSV41_REQUIRE(aligned16(x) && aligned16(w0) && aligned16(y0) && (n1 == 0 || (aligned16(w1) && aligned16(y1))),
                 DSV41_E_ARG, "%s: tensors must be 16-byte aligned", what);
   const int rank0 = banks[0].slots ? banks[0].rank : 0, rank1 = banks[1].slots ? banks[1].rank : 0, n = n0 + n1;
-  const AdapterPlan p = adapter_plan((int)rows, k, n, n0, rank0 > rank1 ? rank0 : rank1);
+  const AdapterPlan p = adapter_plan((int)rows, k, n, n0, rank0 + rank1);
   const int64_t tiles = (int64_t)(n / p.tr) * ((rows + p.tm - 1) / p.tm) * p.splits;
-  const int64_t shrinks = p.done ? shrink_blocks(rows, tokens, rank0, 1, 1)
+  const int64_t shrinks = p.done ? shrink_blocks(rows, tokens, rank0, rank1, 1, 1)
                                  : (rows + p.sub - 1) / p.sub * p.chunks * ((rank0 + 15) / 16 + (rank1 + 15) / 16);
   const int64_t reduces = (rows + 15) / 16 * ((n + 63) / 64);
   DSV41_REQUIRE(tiles < (1ll << 31) && shrinks < (1ll << 31) && reduces < (1ll << 31), DSV41_E_ARG, "%s: too many tiles",
@@ -1099,6 +1102,8 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
                 k / p.splits, n, 1, static_cast<const bf16_t*>(n1 ? w1 : nullptr), n0};
   a.bank[0] = banks[0];
   a.bank[1] = banks[1];
+  a.bank[0].rank = rank0;
+  a.bank[1].rank = rank1;
   uint8_t* at = static_cast<uint8_t*>(workspace) + (p.direct ? 0 : pad256((size_t)rows * p.splits * n * sizeof(float)));
   a.bank[0].h = reinterpret_cast<float*>(at);
   a.bank[1].h = reinterpret_cast<float*>(at + pad256((size_t)p.chunks * rows * rank0 * sizeof(float)));
@@ -1115,7 +1120,7 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   a.done = p.done;
   a.y = static_cast<bf16_t*>(y0);
   a.y1 = static_cast<bf16_t*>(y1);
-  if (p.done && rank0) launch_shrink(a, stream);
+  if (p.done && shrinks) launch_shrink(a, stream);
   launch_projection(a, p, stream);
   if (!p.direct) {
     // 256 columns per workgroup where that still gives every CU two of them, 64 otherwise

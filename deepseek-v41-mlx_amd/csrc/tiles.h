@@ -197,7 +197,7 @@ __device__ __forceinline__ void tile_sums(const WoaArgs& a, uint8_t* lds, int rt
   }
 }
 
-// tile_sums for large tiles of one projection (the split form, w1 null; two ring stages of 64 channels): the fragments of each
+// tile_sums for large tiles (the split form, r0 a multiple of the tile's weight rows; two ring stages of 64 channels): the fragments of each
 // 32-channel half step are read while the half before is multiplied, across the step's barrier too. Half way through a
 // step every wave has its second half in registers, so the barrier there frees the step's stage for the copies of the
 // step after next, which then have a whole step to land. Same order of additions as tile_sums.
@@ -223,7 +223,9 @@ __device__ __forceinline__ void tile_sums_ahead(const WoaArgs& a, uint8_t* lds, 
   }
   const int uwave = __builtin_amdgcn_readfirstlane(wave);
   const uint64_t range = (uint64_t)grp * a.d * 2;
-  const uint64_t wbase = reinterpret_cast<uint64_t>(a.w) + range + ((uint64_t)rt * C::TR + (uint64_t)uwave * kRowsW) * row_bytes;
+  const bool second = a.w1 != nullptr && rt * C::TR >= a.r0;
+  const uint64_t wbase = reinterpret_cast<uint64_t>(second ? a.w1 : a.w) + range +
+                         ((uint64_t)(rt * C::TR - (second ? a.r0 : 0)) + (uint64_t)uwave * kRowsW) * row_bytes;
   const uint64_t obase = reinterpret_cast<uint64_t>(a.o) + range + (uint64_t)mt * C::TM * row_bytes;
   const uint32_t lds0 = lds_offset(lds);
   auto issue = [&](int stage, int kt) {

@@ -17,7 +17,7 @@ from __future__ import annotations
 import torch
 
 from . import _abi
-from .layers import DECODE_ROWS, decode_linear, decode_linear_pair
+from .layers import decode_linear, decode_linear_pair
 
 
 class AdapterBank:
@@ -119,18 +119,17 @@ def adapter_linear(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank | No
 
 def adapter_linear_pair(lin0: torch.nn.Linear, lin1: torch.nn.Linear, x: torch.Tensor, bank0: AdapterBank | None,
                         bank1: AdapterBank | None, ids: torch.Tensor | None):
-    """(adapter_linear(lin0, x, bank0, ids), adapter_linear(lin1, x, bank1, ids)), at decode row counts in one call;
-    without any bank or ids it is decode_linear_pair."""
+    """(adapter_linear(lin0, x, bank0, ids), adapter_linear(lin1, x, bank1, ids)) in one call where both run on the bf16
+    tiles; without any bank or ids it is decode_linear_pair."""
     if ids is None or (bank0 is None and bank1 is None):
         return decode_linear_pair(lin0, lin1, x)
-    if x.numel() <= DECODE_ROWS * x.shape[-1]:
-        x = x.contiguous()
-        w0, w1 = _product_weight(lin0, x), _product_weight(lin1, x)
-        if (w0 is not None and w1 is not None and w0.shape[1] == w1.shape[1]
-                and _tiles_ok(w0, x, 0 if bank0 is None else bank0.a.shape[1])
-                and _tiles_ok(w1, x, 0 if bank1 is None else bank1.a.shape[1])):
-            _no_gradient(x, w0)
-            _no_gradient(x, w1)
-            return _abi.adapter_linear_pair(x, w0, w1, None if bank0 is None else (bank0.a, bank0.b, bank0.scale),
-                                            None if bank1 is None else (bank1.a, bank1.b, bank1.scale), ids)
+    x = x.contiguous()
+    w0, w1 = _product_weight(lin0, x), _product_weight(lin1, x)
+    if (w0 is not None and w1 is not None and w0.shape[1] == w1.shape[1]
+            and _tiles_ok(w0, x, 0 if bank0 is None else bank0.a.shape[1])
+            and _tiles_ok(w1, x, 0 if bank1 is None else bank1.a.shape[1])):
+        _no_gradient(x, w0)
+        _no_gradient(x, w1)
+        return _abi.adapter_linear_pair(x, w0, w1, None if bank0 is None else (bank0.a, bank0.b, bank0.scale),
+                                        None if bank1 is None else (bank1.a, bank1.b, bank1.scale), ids)
     return adapter_linear(lin0, x, bank0, ids), adapter_linear(lin1, x, bank1, ids)

@@ -593,7 +593,7 @@ int dsv41_adapter_plain(const void* x, const void* w, const void* a, const void*
                         const int32_t* ids, void* y, int64_t rows, int32_t tokens, int32_t k, int32_t n, int32_t rank,
                         int32_t slots, int32_t dtype, hipStream_t stream);
 
-/* Two projections of the same rows (at most 128), each with adapters of its own under the same ids, in one call:
+/* Two projections of the same rows, each with adapters of its own under the same ids, in one call:
  * y0 [rows, n0] and y1 [rows, n1] as two dsv41_adapter_linear calls give them, up to the order of fp32 additions.
  * A bank of 0 slots (its pointers unused) has no adapters; one of the two must have some. The workspace of both calls
  * is dsv41_adapter_linear_workspace_bytes (n1, rank1 0 for the single projection, rank 0 for no bank). */

@@ -263,7 +263,7 @@ def test_c_entry_points_refuse_bad_sizes():
 
     assert pair(rows=0) == 0
     assert pair(slots0=0, slots1=0) == -1 and pair(n1=0) == -1 and pair(w1=None) == -1 and pair(y1=None) == -1
-    assert pair(a1=None) == -1 and pair(rank1=0) == -1 and pair(rank1=4) == -3 and pair(rows=129) == -3
+    assert pair(a1=None) == -1 and pair(rank1=0) == -1 and pair(rank1=4) == -3
     assert pair(slots0=0, a0=None, b0=None, s0=None, rank0=0, rows=0) == 0
 
     ptrs = (ctypes.c_void_p * 1)(4096)

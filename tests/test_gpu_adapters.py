@@ -130,6 +130,9 @@ def test_infinite_intermediate_gives_the_formula(gpu):
 
 @pytest.mark.parametrize("b,n,k,n0,n1,r0,r1", [(1, 1, 1280, 256, 96, 16, 8), (17, 1, 5120, 1280, 512, 8, 8),
                                                (64, 1, 512, 128, 64, 16, 64), (3, 77, 512, 256, 128, 16, 16),
+                                               (100, 1, 512, 8192, 512, 16, 24), (1, 1100, 640, 1280, 512, 16, 64),
+                                               (7, 300, 1024, 1280, 512, 64, 64), (2, 300, 320, 256, 96, 8, 40),
+                                               (2, 2000, 512, 2560, 512, 32, 8),
                                                (2, 2, 72, 40, 24, 4, 4)])
 def test_pair_equals_two_projections(gpu, b, n, k, n0, n1, r0, r1):
     from dsv41.adapters import adapter_linear_pair
