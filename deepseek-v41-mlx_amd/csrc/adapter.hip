@@ -730,22 +730,23 @@ adapter_tiles_kernel(AdapterArgs a) {
   }
 }
 
-// The contraction ranges' parts summed in order, plus the adapters' part, rounded once: a workgroup per 16 rows and
+// The contraction ranges' parts summed in order, plus the adapters' part, rounded once: a workgroup per SUB rows (4, each
+// four times in the MFMA, where they may all name different adapters: one load of B behind another for each; else 16) and
 // 64 WR columns, a wave per 16 WR of them (whole blocks of one projection: n0 and n are multiples of 16 WR). The parts
 // and the first adapters' B are on their way while h is summed over its chunks into LDS. DONE: h is the finished first
 // product, as it lies.
-template <int WR, bool DONE>
+template <int WR, bool DONE, int SUB>
 __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
   constexpr int kStride = kMaxRank + 4;
-  __shared__ __align__(16) float hs[DONE ? 1 : 2][DONE ? 4 : 16 * kStride];
+  __shared__ __align__(16) float hs[DONE ? 1 : 2][DONE ? 4 : SUB * kStride];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int ctiles = (a.t.r + 64 * WR - 1) / (64 * WR);
-  const int col0 = (int)(blockIdx.x % ctiles) * 64 * WR, m0 = (int)(blockIdx.x / ctiles) * 16;
-  const int m = m0 + l16, col = min(col0 + wave * 16 * WR, a.t.r - 16 * WR);   // a wave past the end repeats the last
+  const int col0 = (int)(blockIdx.x % ctiles) * 64 * WR, m0 = (int)(blockIdx.x / ctiles) * SUB;
+  const int m = m0 + (l16 & (SUB - 1)), col = min(col0 + wave * 16 * WR, a.t.r - 16 * WR);   // a wave past the end repeats the last
   const int sel = col >= a.t.r0, n = sel ? a.t.r - a.t.r0 : a.t.r0, at = sel ? col - a.t.r0 : col;
   const Bank& bk = a.bank[sel];
   const int id = row_adapter(a, bk, m);
-  const uint32_t named = (uint32_t)__ballot(id >= 0) & 0xFFFFu;
+  const uint32_t named = (uint32_t)__ballot(id >= 0) & ((1u << SUB) - 1u);
   const float* part = reinterpret_cast<const float*>(a.t.out) + (int64_t)min(m, a.t.rows - 1) * a.t.groups * a.t.r + col + 4 * g;
   f32x4 acc[WR];
 
@@ -767,7 +768,7 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
       const Bank& bs = a.bank[s];
       if (bs.slots == 0 || (s == 0 ? col0 >= a.t.r0 : col0 + 64 * WR <= a.t.r0)) continue;
       const int quads = bs.rank >> 2;
-      for (int i = threadIdx.x; i < 16 * quads; i += 256) {
+      for (int i = threadIdx.x; i < SUB * quads; i += 256) {
         const int row = i / quads, r = (i - row * quads) * 4, t = row_adapter(a, bs, m0 + row);
         f32x4 v = {0.f, 0.f, 0.f, 0.f};
         if (t >= 0) {
@@ -794,7 +795,7 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
       return *reinterpret_cast<const uint4*>(from + 8 * slot.c + (slot.low ? bk.rank : 0));
     } else {
       float v[8];
-      const float* from = hs[sel] + l16 * kStride + 8 * slot.c;
+      const float* from = hs[sel] + (l16 & (SUB - 1)) * kStride + 8 * slot.c;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = from[e];
       return half_of(v, slot.low);
@@ -815,7 +816,7 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
     sum_h();
     ex.add(acc, operand);
   }
-  if (m < a.t.rows)
+  if (m < a.t.rows && l16 < SUB)
 #pragma unroll
     for (int i = 0; i < WR; ++i) store4<bf16_t>((sel ? a.y1 : a.y) + (int64_t)m * n + at + 16 * i + 4 * g, acc[i]);
 }
@@ -1091,7 +1092,7 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   const int64_t tiles = (int64_t)(n / p.tr) * ((rows + p.tm - 1) / p.tm) * p.splits;
   const int64_t shrinks = p.done ? shrink_blocks(rows, tokens, rank0, rank1, 1, 1)
                                  : (rows + p.sub - 1) / p.sub * p.chunks * ((rank0 + 15) / 16 + (rank1 + 15) / 16);
-  const int64_t reduces = (rows + 15) / 16 * ((n + 63) / 64);
+  const int64_t reduces = (rows + 3) / 4 * ((n + 63) / 64);
   DSV41_REQUIRE(tiles < (1ll << 31) && shrinks < (1ll << 31) && reduces < (1ll << 31), DSV41_E_ARG, "%s: too many tiles",
                 what);
   const size_t need = plan_bytes(p, (int)rows, n, rank0, rank1);
@@ -1123,16 +1124,18 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   if (p.done && shrinks) launch_shrink(a, stream);
   launch_projection(a, p, stream);
   if (!p.direct) {
-    // 256 columns per workgroup where that still gives every CU two of them, 64 otherwise
-    const int64_t wide = (rows + 15) / 16 * ((n + 255) / 256);
     auto reduce = [&](auto kernel, int64_t blocks) {
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
     };
+    // 256 columns per workgroup where that still gives every CU two of them, 64 otherwise; 4 rows where 16 leave CUs
+    // without two (28 rows of 512 outputs at rank 64: 12.6 against 21.5 us; 64 rows of 32768 at rank 16: 26.8 against 18.5)
+    const int64_t wide = (rows + 15) / 16 * ((n + 255) / 256), narrow = (rows + 15) / 16 * ((n + 63) / 64);
     if (n0 % 64 == 0 && n1 % 64 == 0 && wide >= 512) {
-      if (p.done) reduce(adapter_reduce_kernel<4, true>, wide);
-      else reduce(adapter_reduce_kernel<4, false>, wide);
-    } else if (p.done) reduce(adapter_reduce_kernel<1, true>, reduces);
-    else reduce(adapter_reduce_kernel<1, false>, reduces);
+      if (p.done) reduce(adapter_reduce_kernel<4, true, 16>, wide);
+      else reduce(adapter_reduce_kernel<4, false, 16>, wide);
+    } else if (p.done) reduce(adapter_reduce_kernel<1, true, 16>, narrow);
+    else if (p.sub == 16 || narrow >= 512) reduce(adapter_reduce_kernel<1, false, 16>, narrow);
+    else reduce(adapter_reduce_kernel<1, false, 4>, (rows + 3) / 4 * ((n + 63) / 64));
   }
   return check_launch(what);
 }
