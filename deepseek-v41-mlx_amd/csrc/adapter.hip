@@ -392,17 +392,20 @@ __device__ __forceinline__ uint4 half_of(const float* v, bool low) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The rank chunk of 8 that lane group g supplies to MFMA step q (the upper parts of the r8 chunks, then the lower ones;
-// past them nothing).
+// The rank chunk of 8 that lane group g supplies to step q of the second product. Up to 16 ranks are one step: the upper
+// parts of the chunks, then the lower ones, in one MFMA. More take 4 chunks a step and two MFMAs, upper and lower, on one
+// load of B (16 sequences' own B of rank 64 for 32768 outputs: 24.6 us, 43 when it was loaded for each).
 struct RankSlot {
   int c;
   bool low, live;
   __device__ __forceinline__ RankSlot(int q, int r8) {
-    const int s = q + ((threadIdx.x >> 4) & 3);
-    live = s < 2 * r8;
-    low = s >= r8;
-    c = live ? (low ? s - r8 : s) : 0;
+    const int g = (threadIdx.x >> 4) & 3;
+    low = r8 <= 2 && g >= r8;
+    c = r8 <= 2 ? (low ? g - r8 : g) : 4 * q + g;
+    live = r8 <= 2 ? g < 2 * r8 : c < r8;
+    if (!live) c = 0;
   }
+  __device__ __forceinline__ static int steps(int r8) { return r8 <= 2 ? 1 : (r8 + 3) / 4; }
 };
 
 // The whole first product of up to 16 MT rows of one sequence - so of one adapter - and 16 RT ranks. x and A come to LDS
@@ -508,7 +511,7 @@ struct Expand {
   int64_t slot;
   int rank, id;
   uint32_t named, todo;  // rows with an adapter; those whose adapter is still to come in this rank group
-  int q;                 // the rank group
+  int q;                 // the rank step
   int t[U];
   uint4 next[U][WR];
 
@@ -527,15 +530,18 @@ struct Expand {
         named(named_), todo(named_), q(0) {
     load();
   }
-  // operand(at) gives the lane's part of scale h for a rank slot
+  // operand(c, low) gives the upper or lower parts of scale h's ranks 8 c .. 8 c + 7 of the lane's row
   template <typename H>
   __device__ __forceinline__ void add(f32x4 (&acc)[WR], H operand) {
-    const int end = 2 * (rank >> 3);
-    bf16x8 hf;
+    const int r8 = rank >> 3, end = RankSlot::steps(r8);
+    bf16x8 hf, lf;
     bool fresh = true;
     for (;;) {
-      const RankSlot at(q, rank >> 3);
-      if (fresh) hf = or_zero(operand(at), at.live);
+      const RankSlot at(q, r8);
+      if (fresh) {
+        hf = or_zero(operand(at.c, at.low), at.live);
+        lf = or_zero(operand(at.c, true), at.live && r8 > 2);     // no branch between an MFMA and the choice of its result
+      }
       int now[U];
       uint4 cur[U][WR];
 #pragma unroll
@@ -546,7 +552,7 @@ struct Expand {
       }
       fresh = todo == 0;
       if (fresh) {
-        q += 4;
+        ++q;
         todo = named;
       }
       const bool more = q < end;
@@ -555,7 +561,9 @@ struct Expand {
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < WR; ++i) {
-          const f32x4 sum = mfma16x16x32(or_zero(cur[u][i], at.live), hf, acc[i]);
+          const bf16x8 bf = or_zero(cur[u][i], at.live);
+          f32x4 sum = mfma16x16x32(bf, hf, acc[i]);
+          sum = mfma16x16x32(bf, lf, sum);
           acc[i] = id == now[u] && (u == 0 || now[u] != now[0]) ? sum : acc[i];
         }
       if (!more) return;
@@ -590,19 +598,26 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
   const bf16_t* b0 = bk.b + (int64_t)(col + l16) * bk.rank;
   const int64_t slot = (int64_t)n * bk.rank;
   if (ONE || one) {
-    for (int q = 0; q < 2 * r8; q += 4) {
+    for (int q = 0; q < RankSlot::steps(r8); ++q) {
       const RankSlot at(q, r8);
-      const int from = 8 * at.c + (at.low ? bk.rank : 0);
       const bf16_t* bp = b0 + t * slot + 8 * at.c;
-      bf16x8 hf[WM], bf[WR];
+      bf16x8 hf[WM], lf[WM], bf[WR];
 #pragma unroll
       for (int i = 0; i < WR; ++i) bf[i] = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), at.live);
 #pragma unroll
-      for (int j = 0; j < WM; ++j) hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + from), at.live);
+      for (int j = 0; j < WM; ++j) {
+        hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * at.c + (at.low ? bk.rank : 0)), at.live);
+        if (r8 > 2) lf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * at.c + bk.rank), at.live);
+      }
 #pragma unroll
       for (int j = 0; j < WM; ++j)
 #pragma unroll
         for (int i = 0; i < WR; ++i) acc[i][j] = mfma16x16x32(bf[i], hf[j], acc[i][j]);
+      if (r8 > 2)
+#pragma unroll
+        for (int j = 0; j < WM; ++j)
+#pragma unroll
+          for (int i = 0; i < WR; ++i) acc[i][j] = mfma16x16x32(bf[i], lf[j], acc[i][j]);
     }
 #pragma unroll
     for (int i = 0; i < WR; ++i) settle(acc[i]);
@@ -611,15 +626,18 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
   while (t >= 0) {
 #pragma unroll
     for (int j = 0; j < WM; ++j) todo[j] &= ~(uint32_t)__ballot(id[j] == t);
+    // upper and lower parts of the rank chunks in one row of steps, B loaded for each: both at once, or in turn inside a
+    // step, and the sums leave the registers (3 x 333 rows 1280 -> 32768: 294 us against 100)
     for (int q = 0; q < 2 * r8; q += 4) {
-      const RankSlot at(q, r8);
-      const int from = 8 * at.c + (at.low ? bk.rank : 0);
-      const bf16_t* bp = b0 + t * slot + 8 * at.c;
+      const int s = q + ((threadIdx.x >> 4) & 3);
+      const bool live = s < 2 * r8, low = s >= r8;
+      const int c = live ? (low ? s - r8 : s) : 0;
+      const bf16_t* bp = b0 + t * slot + 8 * c;
       bf16x8 hf[WM], bf[WR];
 #pragma unroll
-      for (int i = 0; i < WR; ++i) bf[i] = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), at.live);
+      for (int i = 0; i < WR; ++i) bf[i] = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), live);
 #pragma unroll
-      for (int j = 0; j < WM; ++j) hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + from), at.live);
+      for (int j = 0; j < WM; ++j) hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * c + (low ? bk.rank : 0)), live);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < WR; ++i) {
@@ -789,16 +807,16 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
     }
     __syncthreads();
   };
-  auto operand = [&](const RankSlot& slot) {
+  auto operand = [&](int c, bool low) {
     if constexpr (DONE) {
       const uint16_t* from = reinterpret_cast<const uint16_t*>(bk.h) + (int64_t)min(m, a.t.rows - 1) * 2 * bk.rank;
-      return *reinterpret_cast<const uint4*>(from + 8 * slot.c + (slot.low ? bk.rank : 0));
+      return *reinterpret_cast<const uint4*>(from + 8 * c + (low ? bk.rank : 0));
     } else {
       float v[8];
-      const float* from = hs[sel] + (l16 & (SUB - 1)) * kStride + 8 * slot.c;
+      const float* from = hs[sel] + (l16 & (SUB - 1)) * kStride + 8 * c;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = from[e];
-      return half_of(v, slot.low);
+      return half_of(v, low);
     }
   };
   const bool one = named == 0 || __ballot(id >= 0 && id != __builtin_amdgcn_readlane(id, __builtin_ctz(named | 0x10000u))) == 0;
