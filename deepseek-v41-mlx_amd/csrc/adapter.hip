@@ -574,8 +574,8 @@ struct Expand {
 // acc[i][j] += scale (h B^T) for a wave's block of 16 WM rows from m0 on and 16 WR columns from col on, h from the
 // finished first product. One adapter for all rows that are stored: its products go straight into the sums. Several:
 // each multiplies all rows and every lane keeps its own row's, one result beside the sums at a time (they fill the
-// registers). ONE: the sequences are whole blocks, so the second kind is never met.
-template <int WR, int WM, bool ONE>
+// registers).
+template <int WR, int WM>
 __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const AdapterArgs& a, const Bank& bk, int n, int m0,
                                              int col) {
   const int l16 = threadIdx.x & 15, r8 = bk.rank >> 3;
@@ -594,10 +594,10 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
   if (t < 0) return;
   bool one = true;
 #pragma unroll
-  for (int j = 0; j < WM && !ONE; ++j) one = one && __ballot(id[j] != t && m0 + 16 * j + l16 < a.t.rows) == 0;
+  for (int j = 0; j < WM; ++j) one = one && __ballot(id[j] != t && m0 + 16 * j + l16 < a.t.rows) == 0;
   const bf16_t* b0 = bk.b + (int64_t)(col + l16) * bk.rank;
   const int64_t slot = (int64_t)n * bk.rank;
-  if (ONE || one) {
+  if (one) {
     for (int q = 0; q < RankSlot::steps(r8); ++q) {
       const RankSlot at(q, r8);
       const bf16_t* bp = b0 + t * slot + 8 * at.c;
@@ -656,21 +656,19 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
   }
 }
 
-// The projection's tiles. kExpand*: the adapters' part is added to the float32 sums in registers and the result stored,
+// The projection's tiles. DIRECT: the adapters' part is added to the float32 sums in registers and the result stored,
 // rounded once (h complete before the launch). Else the sums of one contraction range go to t.out in float32, and h is
 // computed beside them: by workgroups of their own where the launch leaves room for them, else by the tiles' own, each
 // its share while its first copies are on their way.
-enum AdapterPart { kSplitSums, kExpandOne, kExpandAny };
-
-template <int WR, int WM, int GR, int GM, int BK, int NS, AdapterPart PART>
+template <int WR, int WM, int GR, int GM, int BK, int NS, bool DIRECT>
 __global__ __launch_bounds__(64 * GR * GM, (TileCfg<WR, WM, GR, GM, BK, NS>::LDS <= 72 * 1024) ? 2 : 1) void
 adapter_tiles_kernel(AdapterArgs a) {
   using C = TileCfg<WR, WM, GR, GM, BK, NS>;
   __shared__ __align__(16) uint8_t lds[C::LDS];
   const int mtiles = (a.t.rows + C::TM - 1) / C::TM, rtiles = a.t.r / C::TR;
-  const int apart = PART == kSplitSums ? a.apart : 0, total = (int)gridDim.x - apart, block = (int)blockIdx.x - apart;
+  const int apart = DIRECT ? 0 : a.apart, total = (int)gridDim.x - apart, block = (int)blockIdx.x - apart;
   int rt, mt, grp = 0;
-  if constexpr (PART == kSplitSums) {
+  if constexpr (!DIRECT) {
     // consecutive tiles on one XCD, the weight tile fastest, as the output projection's
     const int tile = total % 8 ? block : (block % 8) * (total / 8) + block / 8;
     rt = tile % rtiles;
@@ -689,13 +687,13 @@ adapter_tiles_kernel(AdapterArgs a) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wr = (wave % GR) * 16 * WR, wm = (wave / GR) * 16 * WM;   // this wave's block
   f32x4 acc[WR][WM];
-  if constexpr (PART != kSplitSums) {
+  if constexpr (DIRECT) {
     // a tile lies within one of the two projections
     const int sel = rt * C::TR >= a.t.r0, n = sel ? a.t.r - a.t.r0 : a.t.r0, col = rt * C::TR + wr - (sel ? a.t.r0 : 0);
     const Bank& bk = a.bank[sel];
     bf16_t* y = sel ? a.y1 : a.y;
     // the adapters' part first, while the ring's first copies are on their way
-    auto beside = [&]() { expand_block<WR, WM, PART == kExpandOne>(acc, a, bk, n, mt * C::TM + wm, col); };
+    auto beside = [&]() { expand_block<WR, WM>(acc, a, bk, n, mt * C::TM + wm, col); };
     if constexpr (BK == 64 && NS == 2) tile_sums_ahead<WR, WM, GR, GM>(a.t, lds, rt, mt, grp, acc, beside);
     else tile_sums<WR, WM, GR, GM, BK, NS>(a.t, lds, rt, mt, grp, acc, beside);
 #pragma unroll
@@ -964,9 +962,9 @@ static size_t plan_bytes(const AdapterPlan& p, int rows, int n, int rank0, int r
          pad256((size_t)p.chunks * rows * rank1 * sizeof(float));
 }
 
-template <int WR, int WM, int GR, int GM, int BK, int NS, AdapterPart PART>
+template <int WR, int WM, int GR, int GM, int BK, int NS, bool DIRECT>
 static void launch_adapter_tiles(const AdapterArgs& a, int64_t tiles, hipStream_t stream) {
-  hipLaunchKernelGGL((adapter_tiles_kernel<WR, WM, GR, GM, BK, NS, PART>), dim3((unsigned)tiles), dim3(64 * GR * GM), 0,
+  hipLaunchKernelGGL((adapter_tiles_kernel<WR, WM, GR, GM, BK, NS, DIRECT>), dim3((unsigned)tiles), dim3(64 * GR * GM), 0,
                      stream, a);
 }
 
@@ -991,38 +989,32 @@ static void launch_shrink(const AdapterArgs& a, hipStream_t stream) {
   else two ? go(adapter_shrink_kernel<2, 4, 1>, 2, 8) : go(adapter_shrink_kernel<1, 4, 2>, 1, 8);
 }
 
-template <int WR, int WM, int GR, int GM, int BK, int NS>
-static void launch_direct_tiles(const AdapterArgs& a, int64_t tiles, hipStream_t stream) {
-  if (a.tokens % (16 * WM) == 0 || a.tokens == a.t.rows) launch_adapter_tiles<WR, WM, GR, GM, BK, NS, kExpandOne>(a, tiles, stream);
-  else launch_adapter_tiles<WR, WM, GR, GM, BK, NS, kExpandAny>(a, tiles, stream);
-}
-
 static void launch_projection(const AdapterArgs& a, const AdapterPlan& p, hipStream_t stream) {
   const int64_t tiles = (int64_t)(a.t.r / p.tr) * ((a.t.rows + p.tm - 1) / p.tm) * p.splits + a.apart;
   switch (p.tile) {
-    case kRows32: launch_adapter_tiles<1, 1, 2, 2, 64, 8, kSplitSums>(a, tiles, stream); break;
-    case kRows64: launch_adapter_tiles<1, 2, 2, 2, 64, 6, kSplitSums>(a, tiles, stream); break;
-    case kRows64Deep: launch_adapter_tiles<1, 2, 2, 2, 64, 8, kSplitSums>(a, tiles, stream); break;
-    case kRows96: launch_adapter_tiles<1, 3, 2, 2, 64, 8, kSplitSums>(a, tiles, stream); break;
-    case kRows128: launch_adapter_tiles<1, 4, 2, 2, 64, 4, kSplitSums>(a, tiles, stream); break;
-    case kWide128: launch_adapter_tiles<4, 2, 2, 2, 64, 4, kSplitSums>(a, tiles, stream); break;
-    case kWide160: launch_adapter_tiles<5, 2, 2, 2, 64, 4, kSplitSums>(a, tiles, stream); break;
-    case kTile256: launch_direct_tiles<8, 4, 2, 4, 64, 2>(a, tiles, stream); break;
+    case kRows32: launch_adapter_tiles<1, 1, 2, 2, 64, 8, false>(a, tiles, stream); break;
+    case kRows64: launch_adapter_tiles<1, 2, 2, 2, 64, 6, false>(a, tiles, stream); break;
+    case kRows64Deep: launch_adapter_tiles<1, 2, 2, 2, 64, 8, false>(a, tiles, stream); break;
+    case kRows96: launch_adapter_tiles<1, 3, 2, 2, 64, 8, false>(a, tiles, stream); break;
+    case kRows128: launch_adapter_tiles<1, 4, 2, 2, 64, 4, false>(a, tiles, stream); break;
+    case kWide128: launch_adapter_tiles<4, 2, 2, 2, 64, 4, false>(a, tiles, stream); break;
+    case kWide160: launch_adapter_tiles<5, 2, 2, 2, 64, 4, false>(a, tiles, stream); break;
+    case kTile256: launch_adapter_tiles<8, 4, 2, 4, 64, 2, true>(a, tiles, stream); break;
     case kTile160:
-      if (p.direct) launch_direct_tiles<5, 4, 2, 2, 64, 2>(a, tiles, stream);
-      else launch_adapter_tiles<5, 4, 2, 2, 64, 2, kSplitSums>(a, tiles, stream);
+      if (p.direct) launch_adapter_tiles<5, 4, 2, 2, 64, 2, true>(a, tiles, stream);
+      else launch_adapter_tiles<5, 4, 2, 2, 64, 2, false>(a, tiles, stream);
       break;
     case kTile128:
-      if (p.direct) launch_direct_tiles<4, 4, 2, 2, 64, 2>(a, tiles, stream);
-      else launch_adapter_tiles<4, 4, 2, 2, 64, 2, kSplitSums>(a, tiles, stream);
+      if (p.direct) launch_adapter_tiles<4, 4, 2, 2, 64, 2, true>(a, tiles, stream);
+      else launch_adapter_tiles<4, 4, 2, 2, 64, 2, false>(a, tiles, stream);
       break;
     case kTile64:
-      if (p.direct) launch_direct_tiles<2, 4, 2, 2, 64, 3>(a, tiles, stream);
-      else launch_adapter_tiles<2, 4, 2, 2, 64, 3, kSplitSums>(a, tiles, stream);
+      if (p.direct) launch_adapter_tiles<2, 4, 2, 2, 64, 3, true>(a, tiles, stream);
+      else launch_adapter_tiles<2, 4, 2, 2, 64, 3, false>(a, tiles, stream);
       break;
     case kTile32:
-      if (p.direct) launch_direct_tiles<1, 4, 2, 2, 64, 4>(a, tiles, stream);
-      else launch_adapter_tiles<1, 4, 2, 2, 64, 4, kSplitSums>(a, tiles, stream);
+      if (p.direct) launch_adapter_tiles<1, 4, 2, 2, 64, 4, true>(a, tiles, stream);
+      else launch_adapter_tiles<1, 4, 2, 2, 64, 4, false>(a, tiles, stream);
       break;
   }
 }
@@ -1071,7 +1063,7 @@ extern "C" int dsv41_adapter_add(const void* x, const void* a, const void* b, co
 // ------------------------------------------------------------------ the projection and its adapters
 
 static bool projection_sizes(int64_t rows, int32_t k, int32_t n0, int32_t n1, int32_t rank0, int32_t rank1) {
-  return rows > 0 && rows < (1ll << 31) && k > 0 && k % 64 == 0 && n0 > 0 && n1 >= 0 && n0 % 32 == 0 && n1 % 32 == 0 &&
+  return rows > 0 && rows < (1ll << 30) && k > 0 && k < (1 << 22) && k % 64 == 0 && n0 > 0 && n1 >= 0 && n0 % 32 == 0 && n1 % 32 == 0 &&
          (int64_t)n0 + n1 < (1ll << 30) && rank0 >= 0 && rank1 >= 0 && rank0 <= kMaxRank && rank1 <= kMaxRank &&
          rank0 % 8 == 0 && rank1 % 8 == 0;
 }
@@ -1087,8 +1079,8 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
                               int64_t rows, int32_t tokens, int32_t k, int32_t n0, int32_t n1, int32_t dtype,
                               hipStream_t stream) {
   DSV41_REQUIRE(dtype == DSV41_BF16, DSV41_E_DTYPE, "%s: bf16 only (dtype %d)", what, dtype);
-  DSV41_REQUIRE(rows >= 0 && rows < (1ll << 31) && tokens > 0 && rows % tokens == 0 && k > 0 && n0 > 0 && n1 >= 0 &&
-                    (int64_t)n0 + n1 < (1ll << 30),
+  DSV41_REQUIRE(rows >= 0 && rows < (1ll << 30) && tokens > 0 && rows % tokens == 0 && k > 0 && k < (1 << 22) && n0 > 0 &&
+                    n1 >= 0 && (int64_t)n0 + n1 < (1ll << 30),
                 DSV41_E_ARG, "%s: rows %lld of %d tokens, k %d, n %d + %d", what, (long long)rows, tokens, k, n0, n1);
   for (int s = 0; s < 2; ++s) {
     const Bank& b = banks[s];
@@ -1185,7 +1177,7 @@ extern "C" int dsv41_adapter_plain(const void* x, const void* w, const void* a, 
                 slots);
   DSV41_REQUIRE(dtype == DSV41_BF16 || dtype == DSV41_F32, DSV41_E_DTYPE, "%s: dtype %d not supported (BF16 or F32)",
                 what, dtype);
-  DSV41_REQUIRE(rows < (1ll << 31) && k < (1 << 30) && n < (1 << 30) && rank < (1 << 30) &&
+  DSV41_REQUIRE(rows < (1ll << 30) && k < (1 << 30) && n < (1 << 30) && rank < (1 << 30) &&
                     (rows + 15) / 16 * ((n + 15) / 16) < (1ll << 31),
                 DSV41_E_ARG, "%s: too many outputs", what);
   if (rows == 0) return 0;

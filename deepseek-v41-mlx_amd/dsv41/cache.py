@@ -43,6 +43,7 @@ reference does (attention.py:127, 163, 166); a cache in the activation dtype is 
 from __future__ import annotations
 
 import ctypes
+import weakref
 
 import numpy as np
 import torch
@@ -218,44 +219,54 @@ _MINUS_INF = 0xFF800000
 
 class _RowTable:
     """A cache's buffers as moves of sequences take them: one entry per buffer, in layer order. Kept on the ModelCache
-    and built again when one of the buffers is another tensor or lies elsewhere."""
+    (it holds no buffer alive, and copies and pickles of the cache leave it out) and built again when one of the buffers
+    is another tensor or lies elsewhere."""
 
     def __init__(self, cache: ModelCache):
-        self.at, self.tensors, self.layout, self.rows, self.width, fills = [], [], [], [], [], []
+        self.names, self.layout, self.rows, self.width, tensors, fills = [], [], [], [], [], []
         self.need = {}                     # (what the rows count, ratio, rows per scale) -> fewest rows of such a buffer
         for i, lc in enumerate(cache.layers):
-            for name in _BUFFERS + ("kv_state", "score_state"):
-                holder = lc.comp_state if name.endswith("_state") else lc
-                t = getattr(holder, name) if holder is not None else None
-                if t is None:
-                    continue
+            names = tuple(n for n in _BUFFERS if getattr(lc, n) is not None)
+            self.names.append((names, lc.comp_state is not None))
+            for name in names + (("kv_state", "score_state") if lc.comp_state is not None else ()):
+                t = getattr(lc.comp_state if name.endswith("_state") else lc, name)
                 if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
                     raise ValueError(f"layer {i}: {name} {tuple(t.shape)} must be [sequences, rows, channels] with dense rows")
                 kind = ("state", t.shape[1], 1) if name.endswith("_state") else ("ring", lc.window, 1) if name.startswith(
                     "win") else ("comp", lc.ratio, lc.fp8_rb if name in ("comp_ks", "index_k8s") else 1)
-                self.at.append((holder, name))
-                self.tensors.append(t)
+                tensors.append(t)
                 self.layout.append((i, name, t.dtype, t.shape[2], kind))
                 self.rows.append(kind)
                 self.width.append(t.shape[2] * t.element_size())
                 self.need[kind] = min(self.need.get(kind, t.shape[1]), t.shape[1])
                 fills.append(_MINUS_INF if name == "score_state" else 0)
-        if not self.tensors:
+        if not tensors:
             raise ValueError("a cache without buffers")
-        self.batch, self.device = self.tensors[0].shape[0], self.tensors[0].device
-        for (i, name, *_), t in zip(self.layout, self.tensors):
+        self.batch, self.device = tensors[0].shape[0], tensors[0].device
+        for (i, name, *_), t in zip(self.layout, tensors):
             if t.shape[0] != self.batch or t.device != self.device:
                 raise ValueError(f"layer {i}: {name} {tuple(t.shape)} on {t.device} in a cache of {self.batch} sequences on "
                                  f"{self.device}")
-        self.where = [(t.data_ptr(), t.numel()) for t in self.tensors]
-        n = len(self.tensors)
+        self.tensors = [weakref.ref(t) for t in tensors]
+        self.where = [(t.data_ptr(), t.numel()) for t in tensors]
+        n = len(tensors)
         self.pointers = (ctypes.c_int64 * n)(*(p for p, _ in self.where))
-        self.strides = (ctypes.c_int64 * n)(*(t.stride(0) * t.element_size() for t in self.tensors))
+        self.strides = (ctypes.c_int64 * n)(*(t.stride(0) * t.element_size() for t in tensors))
         self.fills = (ctypes.c_uint32 * n)(*fills)
 
-    def current(self) -> bool:
-        return (all(getattr(o, n) is t for (o, n), t in zip(self.at, self.tensors))
-                and [(t.data_ptr(), t.numel()) for t in self.tensors] == self.where)
+    def __reduce__(self):
+        return type(None), ()
+
+    def current(self, cache: ModelCache) -> bool:
+        if len(cache.layers) != len(self.names):
+            return False
+        now = []
+        for lc, (names, state) in zip(cache.layers, self.names):
+            now += [getattr(lc, n) for n in names]
+            if state and lc.comp_state is not None:
+                now += [lc.comp_state.kv_state, lc.comp_state.score_state]
+        return (len(now) == len(self.tensors) and all(t is r() for t, r in zip(now, self.tensors))
+                and [(t.data_ptr(), t.numel()) for t in now] == self.where)
 
     def check(self, offset: int) -> dict:
         """Rows that `offset` positions have written, by kind of buffer: ring slots, compressed rows (or their scale
@@ -277,7 +288,7 @@ class _RowTable:
 
 def _row_table(cache: ModelCache) -> _RowTable:
     table = cache.__dict__.get("_row_table")
-    if table is None or not table.current():
+    if table is None or not table.current(cache):
         table = cache._row_table = _RowTable(cache)
     return table
 
@@ -339,7 +350,8 @@ def reorder_sequences(cache: ModelCache, order, rows=None) -> None:
 
     order and rows are int32 device tensors, read by the kernel (a rows entry outside the batch then moves nothing), or
     host sequences, checked here. Of several moves to one row the last counts. Only what cache.offset positions have
-    written moves; the offset stays."""
+    written moves; the offset stays. A captured call (device tensors) reads order and rows when it is replayed and moves
+    what was visible when it was captured."""
     _move("reorder_sequences", cache, cache, order, rows)
 
 

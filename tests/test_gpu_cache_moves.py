@@ -180,6 +180,61 @@ def test_strided_buffers_and_many_layers(gpu):
     _same(cache, want)
 
 
+def test_replaced_buffers_are_seen(gpu):
+    """Every call looks at the buffers as they are: ones replaced whole, states replaced, layers replaced, contents moved
+    to other storage; copies and pickles of a cache that has moved sequences work."""
+    import copy
+    import pickle
+
+    from dsv41.cache import reorder_sequences
+    from dsv41.compressor import CompressorState
+    cache = _cache(RELEASE_TOY, 3, 30, 19, ("dense", "dense", 1), 8)
+    order = _dev([1, 2, 0])
+
+    def moves():
+        want = _expect(cache, cache, 19, [1, 2, 0], range(3))
+        reorder_sequences(cache, order)
+        _same(cache, want)
+
+    moves()
+    owner = next(lc for lc in cache.layers if lc.comp_state is not None)
+    owner.comp_kv = owner.comp_kv.clone().mul_(2)
+    moves()
+    owner.comp_state = CompressorState(3, owner.ratio, 64)
+    owner.comp_state.kv_state.normal_()
+    moves()
+    owner.win_kv.data = owner.win_kv.clone()
+    moves()
+    cache.layers[0] = _cache(RELEASE_TOY, 3, 30, 19, ("dense", "dense", 1), 9).layers[0]
+    moves()
+    other = copy.deepcopy(cache)
+    assert len(pickle.dumps(cache)) > 0
+    before = _bytes(cache)
+    reorder_sequences(other, order)
+    _same(cache, before)
+    _same(other, _expect(cache, cache, 19, [1, 2, 0], range(3)))
+    owner.win_kv = owner.win_kv[:2]
+    with pytest.raises(ValueError, match="win_kv"):
+        reorder_sequences(cache, order)
+
+
+def test_two_streams_at_once(gpu):
+    """Calls on two streams have workspaces of their own."""
+    from dsv41.cache import reorder_sequences
+    caches = [_cache(C4_TOY, 6, 60, 50, ("dense", "dense", 1), 10 + i) for i in range(2)]
+    orders = [[5, 4, 3, 2, 1, 0], [1, -1, 0, 5, 5, 2]]
+    wants = [_expect(c, c, 50, o, range(6)) for c, o in zip(caches, orders)]
+    devs = [_dev(o) for o in orders]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for s, c, o in zip(streams, caches, devs):
+        with torch.cuda.stream(s):
+            reorder_sequences(c, o)
+    torch.cuda.synchronize()
+    for c, w in zip(caches, wants):
+        _same(c, w)
+
+
 def test_captured_moves_follow_the_order(gpu):
     from dsv41.cache import reorder_sequences
     cache = _cache(RELEASE_TOY, 4, 40, 37, ("dense", "dense", 1), 5)
