@@ -6,6 +6,14 @@
 //
 // and y[m, :] = x[m, :] w^T for any other t, whatever the adapters hold. h and all sums are float32, y is rounded
 // once.
+//
+// bf16 launch shapes (the plan below picks by sizes; us of kernels on one MI355X):
+//   few rows   the projection's weight is streamed once in split sums; h is computed beside it, and a second launch sums
+//              the ranges and adds the adapters' part. Bound by the weight and, where every row names another adapter,
+//              by B: 64 rows 1280 -> 32768 under 64 adapters of rank 16 (158 MB) 41 us, 3.9 TB/s.
+//   prompts    h first, then the projection's tiles with the adapters' part in their sums when the products begin:
+//              8,192 rows 8192 -> 5120 at rank 64 42 + 580 us, 1.13 PFLOP/s; few tiles split the contraction and end
+//              in the same second launch.
 #include "tiles.h"
 
 namespace dsv41 {
@@ -410,9 +418,10 @@ struct RankSlot {
 
 // The whole first product of up to 16 MT rows of one sequence - so of one adapter - and 16 RT ranks. x and A come to LDS
 // 256 channels at a time (a copy instruction takes 512 bytes of each of two rows: fragments loaded from memory directly
-// touch 16 rows per instruction: 8,192 rows of 8192 channels at rank 64 took 63 us, 41 this way), NS - 1 steps ahead; MT RT waves a 16 x 16
-// tile each, times KS that share a step's channels. Writes the second product's operand: per row the upper halves of
-// scale h's ranks, then the lower ones ([rows, 2 rank] bf16). Rows without an adapter are left as they are.
+// touch 16 rows per instruction: 8,192 rows of 8192 channels at rank 64 took 63 us, 41 this way), NS - 1 steps ahead;
+// MT RT waves take a 16 x 16 tile each, times KS that share a step's channels. Writes the second product's operand: per
+// row the upper halves of scale h's ranks, then the lower ones ([rows, 2 rank] bf16). Rows without an adapter are left
+// as they are.
 //
 // A step's tile row is 32 chunks of 16 bytes; chunk c of row r lies at c ^ (r & 15) (and within the 32), so that the 16
 // rows of a fragment read start in different banks.
@@ -913,7 +922,7 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
       double fixed, alone, paired;     // paired 0: one per CU
       bool split;
     };
-    static const Shape shapes[] = {{kTile256, 256, 256, 15.0, 1.65, 0.0, false},
+    static const Shape shapes[] = {{kTile256, 256, 256, 20.0, 1.30, 0.0, false},
                                    {kTile160, 160, 128, 8.0, 0.80, 1.29, true},
                                    {kTile128, 128, 128, 7.6, 0.71, 1.04, true},
                                    {kTile64, 64, 128, 4.3, 0.51, 0.67, true},

@@ -68,7 +68,6 @@ struct TileCfg {
   static constexpr int STAGE = (TR + TM) * RB;
   static constexpr int LDS = NS * STAGE;
   static_assert(BK == 32 || BK == 64, "32- or 64-channel steps");
-  static_assert(NW * 1024 * NWV == TR * RB && NO * 1024 * NWV == TM * RB, "whole copy instructions per wave");
 };
 
 // The same for deep rings: at most `pending` (clamped to P) later steps of N copies each may
@@ -120,6 +119,8 @@ template <int WR, int WM, int GR, int GM, int BK, int NS, typename Beside = Noth
 __device__ __forceinline__ void tile_sums(const WoaArgs& a, uint8_t* lds, int rt, int mt, int grp,
                                           f32x4 (&acc)[WR][WM], Beside beside = Beside()) {
   using C = TileCfg<WR, WM, GR, GM, BK, NS>;
+  static_assert(C::NW * 1024 * C::NWV == C::TR * C::RB && C::NO * 1024 * C::NWV == C::TM * C::RB,
+                "whole copy instructions per wave");
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wr = (wave % GR) * 16 * WR, wm = (wave / GR) * 16 * WM;   // this wave's block
 
@@ -197,63 +198,65 @@ __device__ __forceinline__ void tile_sums(const WoaArgs& a, uint8_t* lds, int rt
   }
 }
 
-// tile_sums for large tiles (the split form, r0 a multiple of the tile's weight rows; two ring stages of 64 channels): the fragments of each
-// 32-channel half step are read while the half before is multiplied, across the step's barrier too. Half way through a
-// step every wave has its second half in registers, so the barrier there frees the step's stage for the copies of the
+// tile_sums for large tiles (the split form, r0 a multiple of the tile's weight rows; two ring stages of 64 channels):
+// the fragments of each 32-channel half step are read while the half before is multiplied, across the step's barrier
+// too. Half way through a step every wave has its second half in registers, so the barrier there frees the step's stage for the copies of the
 // step after next, which then have a whole step to land. Same order of additions as tile_sums.
 template <int WR, int WM, int GR, int GM, typename Beside = NothingBeside>
 __device__ __forceinline__ void tile_sums_ahead(const WoaArgs& a, uint8_t* lds, int rt, int mt, int grp,
                                                 f32x4 (&acc)[WR][WM], Beside beside = Beside()) {
   using C = TileCfg<WR, WM, GR, GM, 64, 2>;
-  constexpr int kRowsW = C::TR / C::NWV, kRowsO = C::TM / C::NWV;   // tile rows that a wave copies, 8 at a time
-  static_assert(kRowsW % 8 == 0 && kRowsO % 8 == 0, "whole copy instructions per wave");
+  static_assert(C::TR % (8 * C::NWV) == 0 && C::TM % (8 * C::NWV) == 0 && C::NWV % 2 == 0,
+                "copies of 8 tile rows, in turn over the waves");
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int wr = (wave % GR) * 16 * WR, wm = (wave / GR) * 16 * WM;
   const uint32_t row_bytes = (uint32_t)a.groups * (uint32_t)a.d * 2;
-  // copy sources: a wave-uniform base per copy, the lane's row and swizzled chunk (tile_swz of 8 rows from a multiple
-  // of 8: the row's low bits and the multiple's parity) as a 32-bit offset
-  uint32_t woff[2], ooff[C::NO];
+  // Copies of 8 tile rows in turn over the waves: copy j of a wave takes rows 8 (wave + NWV j) .. + 7. Sources: a
+  // wave-uniform base, the lane's row and swizzled chunk (tile_swz: the row's low bits and the parity of wave + NWV j,
+  // the wave's) as a 32-bit offset.
+  constexpr int kW = C::TR / 8 / C::NWV, kO = C::TM / 8 / C::NWV, kCopies = kW + kO, kFrags = WM + WR;
+  const uint32_t chunk = 16u * (uint32_t)((lane & 7) ^ (lane >> 3) ^ (wave & 1));
+  const uint32_t woff = (uint32_t)(lane >> 3) * row_bytes + chunk;
+  uint32_t ooff[kO];
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
-    woff[j] = (uint32_t)(lane >> 3) * row_bytes + 16u * (uint32_t)((lane & 7) ^ (lane >> 3) ^ ((wave * (kRowsW / 8) + j) & 1));
-#pragma unroll
-  for (int j = 0; j < C::NO; ++j) {
-    const int row = wave * kRowsO + 8 * j + (lane >> 3);
-    ooff[j] = (uint32_t)min(row, a.rows - 1 - mt * C::TM) * row_bytes + 16u * (uint32_t)((lane & 7) ^ tile_swz<64>(row));
-  }
+  for (int j = 0; j < kO; ++j)
+    ooff[j] = (uint32_t)min(8 * (wave + C::NWV * j) + (lane >> 3), a.rows - 1 - mt * C::TM) * row_bytes + chunk;
   const int uwave = __builtin_amdgcn_readfirstlane(wave);
   const uint64_t range = (uint64_t)grp * a.d * 2;
   const bool second = a.w1 != nullptr && rt * C::TR >= a.r0;
   const uint64_t wbase = reinterpret_cast<uint64_t>(second ? a.w1 : a.w) + range +
-                         ((uint64_t)(rt * C::TR - (second ? a.r0 : 0)) + (uint64_t)uwave * kRowsW) * row_bytes;
+                         ((uint64_t)(rt * C::TR - (second ? a.r0 : 0)) + (uint64_t)(8 * uwave)) * row_bytes;
   const uint64_t obase = reinterpret_cast<uint64_t>(a.o) + range + (uint64_t)mt * C::TM * row_bytes;
   const uint32_t lds0 = lds_offset(lds);
-  auto issue = [&](int stage, int kt) {
-    const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + (uint32_t)(stage * C::STAGE)));
+  // copies [first, last) of a step, the weight's first
+  auto issue = [&](int stage, int kt, int first, int last) {
+    const uint32_t at = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds0 + (uint32_t)(stage * C::STAGE + 8 * uwave * C::RB)));
     const uint64_t kb = (uint64_t)kt * C::RB;
 #pragma unroll
-    for (int j = 0; j < C::NW; ++j)
-      dma16_sgpr(wbase + kb + (uint64_t)(8 * j) * row_bytes, woff[j & 1], at + (uint32_t)((uwave * kRowsW + 8 * j) * C::RB));
-#pragma unroll
-    for (int j = 0; j < C::NO; ++j)
-      dma16_sgpr(obase + kb, ooff[j], at + (uint32_t)(C::TR * C::RB + (uwave * kRowsO + 8 * j) * C::RB));
+    for (int c = 0; c < kCopies; ++c) {
+      if (c < first || c >= last) continue;
+      if (c < kW)
+        dma16_sgpr(wbase + kb + (uint64_t)(8 * C::NWV * c) * row_bytes, woff, at + (uint32_t)(8 * C::NWV * c * C::RB));
+      else
+        dma16_sgpr(obase + kb, ooff[c - kW], at + (uint32_t)((C::TR + 8 * C::NWV * (c - kW)) * C::RB));
+    }
   };
   const int swz = (l16 & 7) ^ (l16 >> 3);
   const uint8_t* wl = lds + (wr + l16) * C::RB;
   const uint8_t* ol = lds + C::TR * C::RB + (wm + l16) * C::RB;
-  auto read = [&](int stage, int half, bf16x8 (&af)[WR], bf16x8 (&bf)[WM]) {
+  // fragments [first, last) of a half step: the query's, then the weight's in the order of their use
+  auto read = [&](int stage, int half, int first, int last, bf16x8 (&af)[WR], bf16x8 (&bf)[WM]) {
     const int at = stage * C::STAGE + (((4 * half + g) ^ swz) << 4);
 #pragma unroll
-    for (int i = 0; i < WR; ++i) af[i] = as_bf16x8(*reinterpret_cast<const uint4*>(wl + at + 16 * i * C::RB));
-#pragma unroll
-    for (int j = 0; j < WM; ++j) bf[j] = as_bf16x8(*reinterpret_cast<const uint4*>(ol + at + 16 * j * C::RB));
+    for (int f = 0; f < kFrags; ++f) {
+      if (f < first || f >= last) continue;
+      if (f < WM) bf[f] = as_bf16x8(*reinterpret_cast<const uint4*>(ol + at + 16 * f * C::RB));
+      else af[f - WM] = as_bf16x8(*reinterpret_cast<const uint4*>(wl + at + 16 * (f - WM) * C::RB));
+    }
   };
-  auto multiply = [&](const bf16x8 (&af)[WR], const bf16x8 (&bf)[WM]) {
-    __builtin_amdgcn_sched_barrier(0);
+  auto multiply = [&](int i, const bf16x8 (&af)[WR], const bf16x8 (&bf)[WM]) {
 #pragma unroll
-    for (int i = 0; i < WR; ++i)
-#pragma unroll
-      for (int j = 0; j < WM; ++j) acc[i][j] = mfma16x16x32(af[i], bf[j], acc[i][j]);
+    for (int j = 0; j < WM; ++j) acc[i][j] = mfma16x16x32(af[i], bf[j], acc[i][j]);
     __builtin_amdgcn_sched_barrier(0);
   };
 #pragma unroll
@@ -263,23 +266,49 @@ __device__ __forceinline__ void tile_sums_ahead(const WoaArgs& a, uint8_t* lds, 
 
   const int nk = a.d / 64;
   bf16x8 a0[WR], b0[WM], a1[WR], b1[WM];
-  issue(0, 0);
-  if (nk > 1) issue(1, 1);
+  // Eight waves, alone on their CU: reads and copies between the products, a few at a time. In a burst behind the barrier
+  // both waves of a SIMD issue them at once and its matrix core waits (8,192 rows 8192 -> 5120: 699 us, 620 between).
+  // Four waves with a second workgroup beside them fare better with the burst (4,096 rows: 340 us, 375 between).
+  constexpr bool kBetween = C::NWV == 8;
+  issue(0, 0, 0, kCopies);
+  if (nk > 1) issue(1, 1, 0, kCopies);
   beside();
-  if (nk > 1) wait_vmcnt<C::NW + C::NO>();
+  if (nk > 1) wait_vmcnt<kCopies>();
   else wait_vmcnt<0>();
   __syncthreads();
-  read(0, 0, a0, b0);
+  read(0, 0, 0, kFrags, a0, b0);
   for (int kt = 0; kt < nk; ++kt) {
     const int stage = kt & 1;
-    read(stage, 1, a1, b1);
-    multiply(a0, b0);
+    const bool copy = kt + 2 < nk, more = kt + 1 < nk;
+    if constexpr (kBetween) {
+#pragma unroll
+      for (int i = 0; i < WR; ++i) {
+        read(stage, 1, i * kFrags / WR, (i + 1) * kFrags / WR, a1, b1);
+        multiply(i, a0, b0);
+      }
+    } else {
+      read(stage, 1, 0, kFrags, a1, b1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < WR; ++i) multiply(i, a0, b0);
+    }
     // step kt + 1, issued a step ago, has landed, and this wave has read stage `stage`; then every wave's
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
-    if (kt + 2 < nk) issue(stage, kt + 2);
-    if (kt + 1 < nk) read(stage ^ 1, 0, a0, b0);
-    multiply(a1, b1);
+    if constexpr (kBetween) {
+#pragma unroll
+      for (int i = 0; i < WR; ++i) {
+        if (copy) issue(stage, kt + 2, i * kCopies / WR, (i + 1) * kCopies / WR);
+        if (more) read(stage ^ 1, 0, i * kFrags / WR, (i + 1) * kFrags / WR, a0, b0);
+        multiply(i, a1, b1);
+      }
+    } else {
+      if (copy) issue(stage, kt + 2, 0, kCopies);
+      if (more) read(stage ^ 1, 0, 0, kFrags, a0, b0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < WR; ++i) multiply(i, a1, b1);
+    }
   }
 }
 
