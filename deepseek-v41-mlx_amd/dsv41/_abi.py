@@ -1290,6 +1290,8 @@ def _one_device(name: str, *tensors) -> torch.device:
 def _adapter_args(name, x, a, b, scale, ids, n):
     """Checks one bank (a [slots, rank, k], b [slots, n, rank], scale [slots]) and the sequences' ids against x
     [sequences, (tokens,) k]; returns (rows, tokens, k, rank, slots)."""
+    if not all(isinstance(t, torch.Tensor) for t in (x, a, b, scale, ids)):
+        raise TypeError(f"{name}: x, the adapters and the sequences' ids must be tensors")
     sizes, dtype, at = x.shape, x.dtype, x.get_device()
     slots, rank, k = a.shape if a.dim() == 3 else (0, 0, 0)
     if not (x.is_contiguous() and a.is_contiguous() and b.is_contiguous() and scale.is_contiguous()
@@ -1351,7 +1353,11 @@ def _adapter_weight(name, x, w):
 
 
 def _adapter_out(name, out, x, n):
-    return x.new_empty((*x.shape[:-1], n)) if out is None else _out(name, out, (*x.shape[:-1], n), x.dtype, x.device)
+    if out is None:
+        return x.new_empty((*x.shape[:-1], n))
+    if isinstance(out, torch.Tensor) and out.numel() and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
+        raise ValueError(f"{name}: out shares x's memory")
+    return _out(name, out, (*x.shape[:-1], n), x.dtype, x.device)
 
 
 def adapter_linear(x, w, a, b, scale, ids, out=None, workspace=None):

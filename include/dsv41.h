@@ -567,11 +567,12 @@ int dsv41_linear_rows_pair(const void* x, const void* w0, const void* w1, void* 
  * device, rows / tokens of them). For t in [0, slots):
  *   y[m] = x[m] @ w^T + scale[t] * ((x[m] @ a[t]^T) @ b[t]^T),   a [slots, rank, k], b [slots, n, rank],
  * and y[m] = x[m] @ w^T for any other t (-1: no adapter), whatever the slots hold. Sums and the
- * rank-wide intermediate are fp32, in a fixed order: deterministic.
+ * rank-wide intermediate are fp32, in a fixed order: deterministic. No output may share x's memory.
  */
 
 /* The adapters' part on top of a projection already computed: out = y + scale (x a^T) b^T, y and out
- * [rows, n] in dtype (F32 or BF16; y == out allowed); any k, n and rank. */
+ * [rows, n] in dtype (F32 or BF16; y == out allowed); any k, n and rank. Two launches on fp32 arithmetic: the form
+ * for what the calls below do not take. */
 size_t dsv41_adapter_add_workspace_bytes(int64_t rows, int32_t rank);
 int dsv41_adapter_add(const void* x, const void* a, const void* b, const float* scale, const int32_t* ids,
                       const void* y, void* out, void* workspace, size_t workspace_bytes, int64_t rows,
@@ -612,7 +613,7 @@ int dsv41_adapter_linear_pair(const void* x, const void* w0, const void* w1, con
  * same buffers (same != 0 says so: a row onto itself is left alone). An order entry outside
  * [0, src_rows) empties the row: its bytes[b] bytes become the word fill[b] (low byte first). A rows
  * entry outside [0, dst_rows) moves nothing; of several moves to one row the last counts. order and
- * rows: int32 on the device. src, dst, the strides (bytes between sequences), bytes and fill: host
+ * rows: int32 on the device, read when the kernels run. src, dst, the strides (bytes between sequences), bytes and fill: host
  * arrays of `buffers` entries, read during the call. moves and dst_rows at most 4,096. The workspace holds
  * the call's table and list until its kernels have run. */
 size_t dsv41_cache_move_workspace_bytes(int32_t buffers, int32_t moves);

@@ -91,6 +91,10 @@ def test_adapter_linear_checks_its_tensors(host_abi):
     _reaches(call())
     _reaches(call(out=torch.zeros(2, 5, 32, dtype=BF), workspace=torch.zeros(1 << 20, dtype=torch.uint8)))
     assert A.adapter_linear(x[:0], w, b.a, b.b, b.scale, ids[:0]).shape == (0, 5, 32)
+    with pytest.raises(TypeError):
+        A.adapter_linear(x, w, b.a, b.b, b.scale, [0, 1])
+    square, c64 = torch.zeros(64, 64, dtype=BF), _bank(n=64)
+    _refused(lambda: A.adapter_linear(x, square, c64.a, c64.b, c64.scale, ids, out=x), "shares x's memory")
     _refused(call(w=w.float()), "bfloat16")
     _refused(call(w=w1), "no adapters")
     _refused(call(w=torch.zeros(32, 128, dtype=BF)), "contract")

@@ -70,8 +70,8 @@ SHAPES = [
     # prompts: one token past the decode rows, odd lengths, several sequences in a tile
     (1, 129, 512, 256, 16, 2), (3, 333, 320, 512, 32, 2), (7, 61, 256, 160, 8, 3), (2, 1000, 1024, 1280, 64, 2),
     (1, 4096, 256, 256, 16, 1), (200, 1, 256, 192, 16, 9), (300, 2, 64, 64, 8, 40),
-    # widths that no tile takes
-    (4, 1, 72, 40, 5, 3), (2, 150, 100, 33, 3, 2),
+    # widths and ranks that no tile takes
+    (4, 1, 72, 40, 5, 3), (2, 150, 100, 33, 3, 2), (3, 2, 128, 64, 200, 3), (3, 400, 512, 1024, 136, 2),
 ]
 
 
@@ -250,3 +250,29 @@ def test_stack_with_adapters_equals_merged_weights(gpu, monkeypatch):
         for row, of in ((0, 1), (1, 2), (2, 0)):
             assert (got[row] - want[of][row]).abs().max() <= 2e-5 * max(1.0, float(want[of][row].abs().max()))
         assert (want[0] - want[2]).abs().max() > 1e-3               # the adapters do something
+
+
+def test_outputs_past_32_bits(gpu):
+    """70,000 rows of 32,768 outputs: the last rows of 2.3 billion values, against the formula."""
+    from dsv41.adapters import adapter_linear
+    lin, x, bank, ids = _case(21, 2, 35000, 64, 32768, 8, 2, ids=[1, 0])
+    got = adapter_linear(lin, x, bank, ids)
+    assert got.numel() > 1 << 31
+    for rows in (slice(0, 3), slice(34990, 35000)):
+        _assert_close(got[:, rows].contiguous(), lin, x[:, rows].contiguous(), bank, ids)
+
+
+def test_an_output_of_the_callers(gpu):
+    from dsv41 import _abi
+    lin, x, bank, ids = _case(22, 5, 1, 256, 256, 16, 4)
+    want = _abi.adapter_linear(x, lin.weight, bank.a, bank.b, bank.scale, ids)
+    out = torch.full((6, 1, 256), 7.0, dtype=BF, device="cuda")
+    _abi.adapter_linear(x, lin.weight, bank.a, bank.b, bank.scale, ids, out=out[:5])
+    assert torch.equal(out[:5], want) and (out[5] == 7).all()       # the row behind the last sequence
+    plain = _abi.adapter_plain(x, lin.weight, bank.a, bank.b, bank.scale, ids, out=out[:5])
+    _assert_close(plain, lin, x, bank, ids)
+    assert (out[5] == 7).all()
+    with pytest.raises(ValueError, match="shares"):
+        _abi.adapter_linear(x, lin.weight, bank.a, bank.b, bank.scale, ids, out=x)
+    with pytest.raises(TypeError):
+        _abi.adapter_linear(x, lin.weight, bank.a, bank.b, bank.scale, [0, 1, 2, 3, 0])

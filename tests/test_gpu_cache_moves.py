@@ -251,6 +251,22 @@ def test_captured_moves_follow_the_order(gpu):
         _same(cache, want)
 
 
+def test_offsets_past_32_bits(gpu):
+    """Rows of 1.6 GB, the last one past 4 GB of its buffer: two swapped, one emptied."""
+    from dsv41.cache import reorder_sequences
+    cfg = dict(C1, n_layers=1, head_dim=512, compress_ratios=(1,), kv_source_layers=(0,), index_source_layers=())
+    cache = _cache(cfg, 4, 1600000, 1599999, ("dense", "dense", 1), 11)
+    kv = cache.layers[0].comp_kv
+    assert kv.stride(0) * 2 * 3 > 1 << 32
+    old = [kv[i].clone() for i in range(4)]
+    reorder_sequences(cache, _dev([3, -1, 2, 0]))
+    seen = 1599999
+    same = lambda a, b: torch.equal(a.view(torch.int16), b.view(torch.int16))     # noqa: E731
+    assert same(kv[0, :seen], old[3][:seen]) and same(kv[2], old[2]) and same(kv[3, :seen], old[0][:seen])
+    assert not kv[1, :seen].view(torch.int16).any()
+    assert all(same(kv[i, seen:], old[i][seen:]) for i in range(4))
+
+
 def test_engram_ids_move_too(gpu):
     from dsv41.cache import copy_sequences, reorder_sequences
     cfg = dict(RELEASE_TOY, engram_layer_ids=(1,))
