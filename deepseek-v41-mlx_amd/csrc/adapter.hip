@@ -20,23 +20,27 @@ namespace dsv41 {
 
 // ------------------------------------------------------------------ any shape
 
+// Most workgroups of a launch that takes its items in turn: a grid holds fewer than 2^32 threads.
+constexpr int64_t kMostBlocks = 1 << 23;
+
 // h[m, r] in float32 for any width, rank and type: a workgroup per row, a wave per rank, the channels over its lanes.
 template <typename T>
 __global__ __launch_bounds__(256) void adapter_shrink_plain_kernel(const T* __restrict__ x, const T* __restrict__ a,
                                                                    const int32_t* __restrict__ ids,
-                                                                   float* __restrict__ h, int tokens, int k, int rank,
-                                                                   int slots) {
-  const int64_t m = blockIdx.x;
-  const int t = ids[m / tokens];
-  if (t < 0 || t >= slots) return;
+                                                                   float* __restrict__ h, int64_t rows, int tokens,
+                                                                   int k, int rank, int slots) {
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const T* xp = x + m * k;
-  for (int r = wave; r < rank; r += 4) {
-    const T* ap = a + ((int64_t)t * rank + r) * k;
-    float s = 0.0f;
-    for (int c = lane; c < k; c += 64) s = fmaf(io<T>::ld(xp + c), io<T>::ld(ap + c), s);
-    s = group_sum(s, 64);
-    if (lane == 0) h[m * rank + r] = s;
+  for (int64_t m = blockIdx.x; m < rows; m += gridDim.x) {
+    const int t = ids[m / tokens];
+    if (t < 0 || t >= slots) continue;
+    const T* xp = x + m * k;
+    for (int r = wave; r < rank; r += 4) {
+      const T* ap = a + ((int64_t)t * rank + r) * k;
+      float s = 0.0f;
+      for (int c = lane; c < k; c += 64) s = fmaf(io<T>::ld(xp + c), io<T>::ld(ap + c), s);
+      s = group_sum(s, 64);
+      if (lane == 0) h[m * rank + r] = s;
+    }
   }
 }
 
@@ -47,19 +51,19 @@ __global__ __launch_bounds__(256) void adapter_expand_plain_kernel(const T* y, c
                                                                    const int32_t* __restrict__ ids,
                                                                    const float* __restrict__ h, T* out, int64_t rows,
                                                                    int tokens, int n, int rank, int slots) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * n) return;
-  const int64_t m = i / n;
-  const int j = (int)(i - m * n), t = ids[m / tokens];
-  if (t < 0 || t >= slots) {
-    out[i] = y[i];
-    return;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * n; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / n;
+    const int j = (int)(i - m * n), t = ids[m / tokens];
+    if (t < 0 || t >= slots) {
+      out[i] = y[i];
+      continue;
+    }
+    const T* bp = b + ((int64_t)t * n + j) * rank;
+    const float* hp = h + m * rank;
+    float s = 0.0f;
+    for (int r = 0; r < rank; ++r) s = fmaf(hp[r], io<T>::ld(bp + r), s);
+    io<T>::st(out + i, fmaf(scale[t], s, io<T>::ld(y + i)));
   }
-  const T* bp = b + ((int64_t)t * n + j) * rank;
-  const float* hp = h + m * rank;
-  float s = 0.0f;
-  for (int r = 0; r < rank; ++r) s = fmaf(hp[r], io<T>::ld(bp + r), s);
-  io<T>::st(out + i, fmaf(scale[t], s, io<T>::ld(y + i)));
 }
 
 // The projection and its adapters for any width and type on the float32 matrix cores (v_mfma_f32_16x16x4_f32: exact
@@ -1040,9 +1044,10 @@ template <typename T>
 static void launch_add(const void* x, const void* a, const void* b, const float* scale, const int32_t* ids,
                        const void* y, void* out, float* h, int64_t rows, int tokens, int k, int n, int rank, int slots,
                        hipStream_t stream) {
-  hipLaunchKernelGGL((adapter_shrink_plain_kernel<T>), dim3((unsigned)rows), dim3(256), 0, stream,
-                     static_cast<const T*>(x), static_cast<const T*>(a), ids, h, tokens, k, rank, slots);
-  hipLaunchKernelGGL((adapter_expand_plain_kernel<T>), dim3((unsigned)((rows * n + 255) / 256)), dim3(256), 0, stream,
+  auto grid = [](int64_t blocks) { return dim3((unsigned)(blocks < kMostBlocks ? blocks : kMostBlocks)); };
+  hipLaunchKernelGGL((adapter_shrink_plain_kernel<T>), grid(rows), dim3(256), 0, stream, static_cast<const T*>(x),
+                     static_cast<const T*>(a), ids, h, rows, tokens, k, rank, slots);
+  hipLaunchKernelGGL((adapter_expand_plain_kernel<T>), grid((rows * n + 255) / 256), dim3(256), 0, stream,
                      static_cast<const T*>(y), static_cast<const T*>(b), scale, ids, h, static_cast<T*>(out), rows,
                      tokens, n, rank, slots);
 }
@@ -1057,7 +1062,7 @@ extern "C" int dsv41_adapter_add(const void* x, const void* a, const void* b, co
                 slots);
   DSV41_REQUIRE(dtype == DSV41_BF16 || dtype == DSV41_F32, DSV41_E_DTYPE, "%s: dtype %d not supported (BF16 or F32)",
                 what, dtype);
-  DSV41_REQUIRE(rows < (1ll << 31) && (rows * n + 255) / 256 < (1ll << 31), DSV41_E_ARG, "%s: too many outputs", what);
+  DSV41_REQUIRE(rows < (1ll << 31) && rows * n < (1ll << 39), DSV41_E_ARG, "%s: too many outputs", what);
   if (rows == 0) return 0;
   DSV41_REQUIRE(x && a && b && scale && ids && y && out, DSV41_E_ARG, "%s: null tensor", what);
   const size_t need = dsv41_adapter_add_workspace_bytes(rows, rank);
@@ -1112,8 +1117,9 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   const int64_t shrinks = p.done ? shrink_blocks(rows, tokens, rank0, rank1, 1, 1)
                                  : (rows + p.sub - 1) / p.sub * p.chunks * ((rank0 + 15) / 16 + (rank1 + 15) / 16);
   const int64_t reduces = (rows + 3) / 4 * ((n + 63) / 64);
-  DSV41_REQUIRE(tiles < (1ll << 31) && shrinks < (1ll << 31) && reduces < (1ll << 31), DSV41_E_ARG, "%s: too many tiles",
-                what);
+  DSV41_REQUIRE(tiles < kMostBlocks && (p.done ? shrinks < kMostBlocks : shrinks < (1ll << 31)) &&
+                    (p.direct || reduces < kMostBlocks),
+                DSV41_E_ARG, "%s: too many tiles", what);
   const size_t need = plan_bytes(p, (int)rows, n, rank0, rank1);
   DSV41_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))), DSV41_E_WORKSPACE,
                 "%s: workspace of %zu bytes needed, %zu given", what, need, workspace_bytes);
@@ -1187,7 +1193,7 @@ extern "C" int dsv41_adapter_plain(const void* x, const void* w, const void* a, 
   DSV41_REQUIRE(dtype == DSV41_BF16 || dtype == DSV41_F32, DSV41_E_DTYPE, "%s: dtype %d not supported (BF16 or F32)",
                 what, dtype);
   DSV41_REQUIRE(rows < (1ll << 30) && k < (1 << 30) && n < (1 << 30) && rank < (1 << 30) &&
-                    (rows + 15) / 16 * ((n + 15) / 16) < (1ll << 31),
+                    (rows + 15) / 16 * ((n + 63) / 64) < 4 * kMostBlocks,
                 DSV41_E_ARG, "%s: too many outputs", what);
   if (rows == 0) return 0;
   DSV41_REQUIRE(x && w && a && b && scale && ids && y, DSV41_E_ARG, "%s: null tensor", what);

@@ -204,7 +204,7 @@ extern "C" int dsv41_cache_move(const void* const* src, void* const* dst, const 
     DSV41_REQUIRE(bytes[i] == 0 || (src[i] && dst[i]), DSV41_E_ARG, "%s: buffer %d is null", what, i);
     live += bytes[i] > 0;
     blocks += (bytes[i] + span - 1) / span;
-    DSV41_REQUIRE(blocks < (1ll << 31), DSV41_E_ARG, "%s: too many bytes", what);
+    DSV41_REQUIRE(blocks < (1 << 24), DSV41_E_ARG, "%s: too many bytes", what);   // a grid holds fewer than 2^32 threads
   }
   if (live == 0) return 0;
   const size_t need = dsv41_cache_move_workspace_bytes(buffers, moves);

@@ -1296,7 +1296,7 @@ def _adapter_args(name, x, a, b, scale, ids, n):
     slots, rank, k = a.shape if a.dim() == 3 else (0, 0, 0)
     if not (x.is_contiguous() and a.is_contiguous() and b.is_contiguous() and scale.is_contiguous()
             and ids.is_contiguous() and at == a.get_device() == b.get_device() == scale.get_device() == ids.get_device()
-            and x.is_cuda and len(sizes) > 1 and slots and k == sizes[-1] and b.shape == (slots, n, rank)
+            and x.is_cuda and len(sizes) > 1 and slots and rank and k and k == sizes[-1] and b.shape == (slots, n, rank)
             and dtype is a.dtype is b.dtype and scale.dtype is torch.float32 and scale.shape == (slots,)
             and ids.dtype is torch.int32 and ids.shape == sizes[:1]):
         _adapter_refusal(name, x, a, b, scale, ids, n)
@@ -1355,9 +1355,16 @@ def _adapter_weight(name, x, w):
 def _adapter_out(name, out, x, n):
     if out is None:
         return x.new_empty((*x.shape[:-1], n))
-    if isinstance(out, torch.Tensor) and out.numel() and out.untyped_storage().data_ptr() == x.untyped_storage().data_ptr():
-        raise ValueError(f"{name}: out shares x's memory")
-    return _out(name, out, (*x.shape[:-1], n), x.dtype, x.device)
+    _out(name, out, (*x.shape[:-1], n), x.dtype, x.device)
+    _apart(name, out, x)
+    return out
+
+
+def _apart(name, out, other):
+    """Two contiguous tensors that must not overlap."""
+    if (out.data_ptr() < other.data_ptr() + other.numel() * other.element_size()
+            and other.data_ptr() < out.data_ptr() + out.numel() * out.element_size()):
+        raise ValueError(f"{name}: out overlaps x or the other output")
 
 
 def adapter_linear(x, w, a, b, scale, ids, out=None, workspace=None):
@@ -1411,6 +1418,7 @@ def adapter_linear_pair(x, w0, w1, bank0, bank1, ids, out0=None, out1=None, work
     out0, out1 = _adapter_out(name, out0, x, n0), _adapter_out(name, out1, x, n1)
     if rows == 0:
         return out0, out1
+    _apart(name, out0, out1)
     need = adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1)
     ws = _ws(name, workspace, need, x.device)
     p0 = [t.data_ptr() for t in bank0] if bank0 is not None else [None] * 3

@@ -42,6 +42,7 @@ class AdapterBank:
             raise ValueError(f"AdapterBank: slot {slot} of {self.slots}")
         return slot
 
+    @torch.no_grad()
     def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
         """Puts the adapter a [r, in], b [out, r] (r at most the bank's rank) into a slot."""
         slot = self._slot(slot)
@@ -56,6 +57,7 @@ class AdapterBank:
         self.b[slot, :, r:].zero_()
         self.scale[slot] = scale
 
+    @torch.no_grad()
     def clear(self, slot: int) -> None:
         """Empties a slot: sequences under it get the plain projection."""
         slot = self._slot(slot)

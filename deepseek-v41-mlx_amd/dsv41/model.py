@@ -62,6 +62,8 @@ class AttentionStack(torch.nn.Module):
     def forward(self, h: torch.Tensor, cache: ModelCache, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
         """h [b, n, dim] continues the sequence at cache.offset; advances the cache. adapter_ids [b] int32: every
         sequence's slot in the layers' adapter banks (-1: none)."""
+        if adapter_ids is not None and not any(attn.adapters for attn in self.layers):
+            raise ValueError("adapter_ids without adapters (add_adapters)")
         start_pos = cache.offset
         shared = SharedState()
         shared.adapter_ids = adapter_ids

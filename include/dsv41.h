@@ -567,7 +567,8 @@ int dsv41_linear_rows_pair(const void* x, const void* w0, const void* w1, void* 
  * device, rows / tokens of them). For t in [0, slots):
  *   y[m] = x[m] @ w^T + scale[t] * ((x[m] @ a[t]^T) @ b[t]^T),   a [slots, rank, k], b [slots, n, rank],
  * and y[m] = x[m] @ w^T for any other t (-1: no adapter), whatever the slots hold. Sums and the
- * rank-wide intermediate are fp32, in a fixed order: deterministic. No output may share x's memory.
+ * rank-wide intermediate are fp32, in a fixed order: deterministic. No output may overlap
+ * x or the other output. An infinite value of b gives NaN where the intermediate is zero or, in bf16, short.
  */
 
 /* The adapters' part on top of a projection already computed: out = y + scale (x a^T) b^T, y and out

@@ -48,6 +48,17 @@ def _bank(slots=3, k=64, n=32, rank=8, dtype=BF):
     return AdapterBank(slots, k, n, rank, dtype, "cpu")
 
 
+def test_loading_leaves_no_graph():
+    """Weights that require gradients are copied into a bank, and the bank's tensors follow no graph."""
+    b = _bank()
+    a0, b0 = torch.randn(4, 64, dtype=BF).requires_grad_(), torch.randn(32, 4, dtype=BF).requires_grad_()
+    b.load(1, a0, b0, 0.5)
+    assert not (b.a.requires_grad or b.b.requires_grad or b.scale.requires_grad)
+    assert torch.equal(b.a[1, :4], a0) and torch.equal(b.b[1, :, :4], b0) and not b.a[1, 4:].any()
+    b.clear(1)
+    assert not b.a.any() and not b.b.any() and not b.scale.any()
+
+
 def test_adapter_add_checks_its_tensors(host_abi):
     A, b = host_abi, _bank()
     x, y, ids = torch.zeros(2, 5, 64, dtype=BF), torch.zeros(2, 5, 32, dtype=BF), torch.zeros(2, dtype=torch.int32)
@@ -94,7 +105,12 @@ def test_adapter_linear_checks_its_tensors(host_abi):
     with pytest.raises(TypeError):
         A.adapter_linear(x, w, b.a, b.b, b.scale, [0, 1])
     square, c64 = torch.zeros(64, 64, dtype=BF), _bank(n=64)
-    _refused(lambda: A.adapter_linear(x, square, c64.a, c64.b, c64.scale, ids, out=x), "shares x's memory")
+    _refused(lambda: A.adapter_linear(x, square, c64.a, c64.b, c64.scale, ids, out=x), "overlaps x")
+    arena = torch.zeros(40, 64, dtype=BF)                 # input and output side by side in one allocation, or not
+    _reaches(lambda: A.adapter_linear(arena[:10], square, c64.a, c64.b, c64.scale, ids.repeat(5), out=arena[10:20]))
+    _refused(lambda: A.adapter_linear(arena[:10], square, c64.a, c64.b, c64.scale, ids.repeat(5), out=arena[9:19]),
+             "overlaps x")
+    _refused(call(x=x[..., :0], a=b.a[..., :0], w=w[:, :0]), "no adapters")
     _refused(call(w=w.float()), "bfloat16")
     _refused(call(w=w1), "no adapters")
     _refused(call(w=torch.zeros(32, 128, dtype=BF)), "contract")
@@ -123,6 +139,8 @@ def test_adapter_linear_checks_its_tensors(host_abi):
     _reaches(pair(bank0=None))
     _reaches(pair(bank1=None))
     _refused(pair(bank0=None, bank1=None), "no adapters")
+    one = torch.zeros(2, 5, 32, dtype=BF)
+    _refused(pair(w1=w, bank1=None, out0=one, out1=one), "other output")
     _refused(pair(bank1=(b.a, b.b, b.scale)), "no adapters")
     _refused(pair(w1=w1.float()), "bfloat16")
     _refused(pair(out1=torch.zeros(2, 5, 32, dtype=BF)), "out must be")

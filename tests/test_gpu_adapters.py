@@ -240,6 +240,9 @@ def test_stack_with_adapters_equals_merged_weights(gpu, monkeypatch):
                 w = getattr(merged[t].layers[layer], name).weight
                 w.copy_((w.double() + (0.5 + t) * (b.double() @ a.double())).float())
     plain = stack()
+    with pytest.raises(ValueError, match="without adapters"):
+        plain(torch.zeros(1, 1, C1["dim"], device="cuda"), plain.make_cache(1, 64),
+              torch.zeros(1, dtype=torch.int32, device="cuda"))
     h = torch.randn(3, 40, C1["dim"], generator=g, device="cuda")
     caches = [st.make_cache(3, 64) for st in (many, *merged, plain)]
     ids = torch.tensor([1, -1, 0], dtype=torch.int32, device="cuda")
@@ -262,6 +265,23 @@ def test_outputs_past_32_bits(gpu):
         _assert_close(got[:, rows].contiguous(), lin, x[:, rows].contiguous(), bank, ids)
 
 
+def test_add_past_32_bits(gpu):
+    """2^20 + 3 rows of 4,096 outputs, more than one launch has threads: the sum taken in turn, in place."""
+    from dsv41 import _abi
+    rows = (1 << 20) + 3
+    g = torch.Generator(device="cuda").manual_seed(23)
+    x, a, b = (torch.randint(-3, 4, s, generator=g, device="cuda").to(BF) for s in ((rows, 8), (2, 1, 8), (2, 4096, 1)))
+    ids = torch.randint(-1, 2, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    y = torch.ones(rows, 4096, dtype=BF, device="cuda")
+    assert y.numel() > 1 << 32
+    _abi.adapter_add(x, a, b, torch.ones(2, device="cuda"), ids, y, out=y)
+    for part in (slice(0, 5), slice(rows - 5, rows)):
+        t = ids[part].long()
+        h = (x[part].double()[:, None] @ a.double()[t].transpose(1, 2).contiguous())[:, 0]        # small integers
+        want = 1 + torch.where(t[:, None] >= 0, h * b.double()[t, :, 0], 0.0)
+        assert torch.equal(y[part].double(), want.to(BF).double())
+
+
 def test_an_output_of_the_callers(gpu):
     from dsv41 import _abi
     lin, x, bank, ids = _case(22, 5, 1, 256, 256, 16, 4)
@@ -272,7 +292,7 @@ def test_an_output_of_the_callers(gpu):
     plain = _abi.adapter_plain(x, lin.weight, bank.a, bank.b, bank.scale, ids, out=out[:5])
     _assert_close(plain, lin, x, bank, ids)
     assert (out[5] == 7).all()
-    with pytest.raises(ValueError, match="shares"):
+    with pytest.raises(ValueError, match="overlaps"):
         _abi.adapter_linear(x, lin.weight, bank.a, bank.b, bank.scale, ids, out=x)
     with pytest.raises(TypeError):
         _abi.adapter_linear(x, lin.weight, bank.a, bank.b, bank.scale, [0, 1, 2, 3, 0])
