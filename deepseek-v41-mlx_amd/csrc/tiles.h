@@ -200,8 +200,8 @@ __device__ __forceinline__ void tile_sums(const WoaArgs& a, uint8_t* lds, int rt
 
 // tile_sums for large tiles (the split form, r0 a multiple of the tile's weight rows; two ring stages of 64 channels):
 // the fragments of each 32-channel half step are read while the half before is multiplied, across the step's barrier
-// too. Half way through a step every wave has its second half in registers, so the barrier there frees the step's stage for the copies of the
-// step after next, which then have a whole step to land. Same order of additions as tile_sums.
+// too. Half way through a step every wave has its second half in registers, so the barrier there frees the step's stage
+// for the copies of the step after next, which then have a whole step to land. Same order of additions as tile_sums.
 template <int WR, int WM, int GR, int GM, typename Beside = NothingBeside>
 __device__ __forceinline__ void tile_sums_ahead(const WoaArgs& a, uint8_t* lds, int rt, int mt, int grp,
                                                 f32x4 (&acc)[WR][WM], Beside beside = Beside()) {
