@@ -1437,6 +1437,11 @@ def _move_index(name, what, index, device, moves):
         raise ValueError(f"{name}: {what} must be a contiguous int32 vector of {moves} moves on {device}")
 
 
+@functools.lru_cache(maxsize=1024)
+def cache_move_workspace_bytes(buffers, moves) -> int:
+    return lib().dsv41_cache_move_workspace_bytes(buffers, moves)
+
+
 def cache_move(src, dst, src_strides, dst_strides, nbytes, fills, order, rows, src_rows, dst_rows, same, device):
     """dsv41_cache_move over host tables (ctypes arrays, one entry per buffer): pointers and bytes between sequences of
     both sides, bytes of a sequence that move, the word an emptied row holds. The caller has checked that the buffers
@@ -1448,7 +1453,7 @@ def cache_move(src, dst, src_strides, dst_strides, nbytes, fills, order, rows, s
         _move_index(name, "rows", rows, device, moves)
     _gpu(name, order, rows)
     n = len(nbytes)
-    need = lib().dsv41_cache_move_workspace_bytes(n, moves)
+    need = cache_move_workspace_bytes(n, moves)
     ws = _workspace(need, device)
     at = ctypes.addressof
     _call_on(device, name, at(src), at(dst), at(src_strides), at(dst_strides), at(nbytes), at(fills), n, _ptr(order),

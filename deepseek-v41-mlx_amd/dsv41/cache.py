@@ -43,6 +43,7 @@ reference does (attention.py:127, 163, 166); a cache in the activation dtype is 
 from __future__ import annotations
 
 import ctypes
+import operator
 import weakref
 
 import numpy as np
@@ -223,23 +224,31 @@ class _RowTable:
     is another tensor or lies elsewhere."""
 
     def __init__(self, cache: ModelCache):
-        self.names, self.layout, self.rows, self.width, tensors, fills = [], [], [], [], [], []
-        self.need = {}                     # (what the rows count, ratio, rows per scale) -> fewest rows of such a buffer
+        self.layout, self.width, tensors, fills = [], [], [], []
+        self.at = []                       # a layer's buffers in one call
+        self.kinds, self.need = {}, []     # (what the rows count, ratio, rows per scale), the fewest rows of such a buffer
+        self.kind = []                     # a buffer's entry of those
         for i, lc in enumerate(cache.layers):
-            names = tuple(n for n in _BUFFERS if getattr(lc, n) is not None)
-            self.names.append((names, lc.comp_state is not None))
-            for name in names + (("kv_state", "score_state") if lc.comp_state is not None else ()):
-                t = getattr(lc.comp_state if name.endswith("_state") else lc, name)
+            names = [n for n in _BUFFERS if getattr(lc, n) is not None]
+            if lc.comp_state is not None:
+                names += ["comp_state.kv_state", "comp_state.score_state"]
+            self.at.append((operator.attrgetter(*names), len(names)) if names else None)
+            for name in names:
+                t = operator.attrgetter(name)(lc)
                 if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
                     raise ValueError(f"layer {i}: {name} {tuple(t.shape)} must be [sequences, rows, channels] with dense rows")
                 kind = ("state", t.shape[1], 1) if name.endswith("_state") else ("ring", lc.window, 1) if name.startswith(
                     "win") else ("comp", lc.ratio, lc.fp8_rb if name in ("comp_ks", "index_k8s") else 1)
+                if kind not in self.kinds:
+                    self.kinds[kind] = len(self.need)
+                    self.need.append(t.shape[1])
+                k = self.kinds[kind]
                 tensors.append(t)
                 self.layout.append((i, name, t.dtype, t.shape[2], kind))
-                self.rows.append(kind)
+                self.kind.append(k)
                 self.width.append(t.shape[2] * t.element_size())
-                self.need[kind] = min(self.need.get(kind, t.shape[1]), t.shape[1])
-                fills.append(_MINUS_INF if name == "score_state" else 0)
+                self.need[k] = min(self.need[k], t.shape[1])
+                fills.append(_MINUS_INF if name.endswith("score_state") else 0)
         if not tensors:
             raise ValueError("a cache without buffers")
         self.batch, self.device = tensors[0].shape[0], tensors[0].device
@@ -248,9 +257,10 @@ class _RowTable:
                 raise ValueError(f"layer {i}: {name} {tuple(t.shape)} on {t.device} in a cache of {self.batch} sequences on "
                                  f"{self.device}")
         self.tensors = [weakref.ref(t) for t in tensors]
-        self.where = [(t.data_ptr(), t.numel()) for t in tensors]
+        self.none = [None] * len(tensors)
+        self.where, self.sizes = [t.data_ptr() for t in tensors], [t.numel() for t in tensors]
         n = len(tensors)
-        self.pointers = (ctypes.c_int64 * n)(*(p for p, _ in self.where))
+        self.pointers = (ctypes.c_int64 * n)(*self.where)
         self.strides = (ctypes.c_int64 * n)(*(t.stride(0) * t.element_size() for t in tensors))
         self.fills = (ctypes.c_uint32 * n)(*fills)
 
@@ -258,32 +268,36 @@ class _RowTable:
         return type(None), ()
 
     def current(self, cache: ModelCache) -> bool:
-        if len(cache.layers) != len(self.names):
+        if len(cache.layers) != len(self.at):
             return False
         now = []
-        for lc, (names, state) in zip(cache.layers, self.names):
-            now += [getattr(lc, n) for n in names]
-            if state and lc.comp_state is not None:
-                now += [lc.comp_state.kv_state, lc.comp_state.score_state]
-        return (len(now) == len(self.tensors) and all(t is r() for t, r in zip(now, self.tensors))
-                and [(t.data_ptr(), t.numel()) for t in now] == self.where)
+        try:
+            for lc, layer in zip(cache.layers, self.at):
+                if layer is not None:
+                    get, many = layer
+                    now += get(lc) if many > 1 else (get(lc),)
+        except AttributeError:             # a compressor's state has gone
+            return False
+        known = [r() for r in self.tensors]
+        return (all(map(operator.is_, now, known)) and all(map(operator.is_not, now, self.none))
+                and list(map(torch.Tensor.data_ptr, now)) == self.where
+                and list(map(torch.Tensor.numel, now)) == self.sizes)
 
-    def check(self, offset: int) -> dict:
+    def check(self, offset: int) -> list:
         """Rows that `offset` positions have written, by kind of buffer: ring slots, compressed rows (or their scale
         blocks), the open group's state."""
-        rows = {}
-        for kind, held in self.need.items():
-            what, per, block = kind
+        rows = []
+        for (what, per, block), held in zip(self.kinds, self.need):
             n = per if what == "state" else min(offset, per) if what == "ring" else -(-(offset // per) // block)
             if n > held:
                 raise ValueError(f"a buffer holds {held} of the {n} rows that {offset} positions take")
-            rows[kind] = n
+            rows.append(n)
         return rows
 
     def visible(self, offset: int):
         """Bytes of a sequence that move, buffer by buffer."""
         rows = self.check(offset)
-        return (ctypes.c_int64 * len(self.rows))(*[rows[k] * w for k, w in zip(self.rows, self.width)])
+        return (ctypes.c_int64 * len(self.kind))(*[rows[k] * w for k, w in zip(self.kind, self.width)])
 
 
 def _row_table(cache: ModelCache) -> _RowTable:
