@@ -1290,15 +1290,17 @@ def _one_device(name: str, *tensors) -> torch.device:
 def _adapter_args(name, x, a, b, scale, ids, n):
     """Checks one bank (a [slots, rank, k], b [slots, n, rank], scale [slots]) and the sequences' ids against x
     [sequences, (tokens,) k]; returns (rows, tokens, k, rank, slots)."""
-    if not all(isinstance(t, torch.Tensor) for t in (x, a, b, scale, ids)):
-        raise TypeError(f"{name}: x, the adapters and the sequences' ids must be tensors")
-    sizes, dtype, at = x.shape, x.dtype, x.get_device()
-    slots, rank, k = a.shape if a.dim() == 3 else (0, 0, 0)
-    if not (x.is_contiguous() and a.is_contiguous() and b.is_contiguous() and scale.is_contiguous()
-            and ids.is_contiguous() and at == a.get_device() == b.get_device() == scale.get_device() == ids.get_device()
-            and x.is_cuda and len(sizes) > 1 and slots and rank and k and k == sizes[-1] and b.shape == (slots, n, rank)
-            and dtype is a.dtype is b.dtype and scale.dtype is torch.float32 and scale.shape == (slots,)
-            and ids.dtype is torch.int32 and ids.shape == sizes[:1]):
+    try:
+        sizes, dtype, at = x.shape, x.dtype, x.get_device()
+        slots, rank, k = a.shape if a.dim() == 3 else (0, 0, 0)
+        good = (at == a.get_device() == b.get_device() == scale.get_device() == ids.get_device() and x.is_cuda
+                and x.is_contiguous() and a.is_contiguous() and b.is_contiguous() and scale.is_contiguous()
+                and ids.is_contiguous() and len(sizes) > 1 and slots and rank and k and k == sizes[-1]
+                and b.shape == (slots, n, rank) and dtype is a.dtype is b.dtype and scale.dtype is torch.float32
+                and scale.shape == (slots,) and ids.dtype is torch.int32 and ids.shape == (sizes[0],))
+    except AttributeError:
+        raise TypeError(f"{name}: x, the adapters and the sequences' ids must be tensors") from None
+    if not good:
         _adapter_refusal(name, x, a, b, scale, ids, n)
     rows = x.numel() // k
     return rows, (rows // sizes[0] if rows else 1), k, rank, slots
@@ -1346,8 +1348,9 @@ def adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1) -> int:
 def _adapter_weight(name, x, w):
     if not (x.dtype is w.dtype is torch.bfloat16):
         raise ValueError(f"{name}: x and w must be bfloat16")
-    if w.dim() != 2 or w.shape[1] != x.shape[-1] or w.get_device() != x.get_device():
-        raise ValueError(f"{name}: x {tuple(x.shape)} and w {tuple(w.shape)} do not contract")
+    sizes = w.shape
+    if len(sizes) != 2 or sizes[1] != x.shape[-1] or w.get_device() != x.get_device():
+        raise ValueError(f"{name}: x {tuple(x.shape)} and w {tuple(sizes)} do not contract")
     if not w.is_contiguous():
         _contig(name, w)
 
@@ -1406,25 +1409,28 @@ def adapter_linear_pair(x, w0, w1, bank0, bank1, ids, out0=None, out1=None, work
     name = "dsv41_adapter_linear_pair"
     if bank0 is None and bank1 is None:
         raise ValueError(f"{name}: no adapters")
-    sizes = []
-    for w, bank in ((w0, bank0), (w1, bank1)):
-        _adapter_weight(name, x, w)
-        if bank is not None:
-            sizes.append(_adapter_args(name, x, *bank, ids, w.shape[0]))
-    rows, tokens, k = sizes[0][:3]
-    (rank0, slots0) = sizes[0][3:] if bank0 is not None else (0, 0)
-    (rank1, slots1) = sizes[-1][3:] if bank1 is not None else (0, 0)
     n0, n1 = w0.shape[0], w1.shape[0]
+    _adapter_weight(name, x, w0)
+    _adapter_weight(name, x, w1)
+    rank0 = rank1 = slots0 = slots1 = 0
+    a0 = b0 = scale0 = a1 = b1 = scale1 = None
+    if bank0 is not None:
+        a0, b0, scale0 = bank0
+        rows, tokens, k, rank0, slots0 = _adapter_args(name, x, a0, b0, scale0, ids, n0)
+    if bank1 is not None:
+        a1, b1, scale1 = bank1
+        rows, tokens, k, rank1, slots1 = _adapter_args(name, x, a1, b1, scale1, ids, n1)
+    given = out0 is not None and out1 is not None
     out0, out1 = _adapter_out(name, out0, x, n0), _adapter_out(name, out1, x, n1)
     if rows == 0:
         return out0, out1
-    _apart(name, out0, out1)
+    if given:
+        _apart(name, out0, out1)
     need = adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1)
     ws = _ws(name, workspace, need, x.device)
-    p0 = [t.data_ptr() for t in bank0] if bank0 is not None else [None] * 3
-    p1 = [t.data_ptr() for t in bank1] if bank1 is not None else [None] * 3
-    _call_on(x.device, name, x.data_ptr(), w0.data_ptr(), w1.data_ptr(), *p0, *p1, ids.data_ptr(), out0.data_ptr(),
-             out1.data_ptr(), _ptr(ws), need, rows, tokens, k, n0, n1, rank0, rank1, slots0, slots1, BF16, _stream(x))
+    _call_on(x.device, name, x.data_ptr(), w0.data_ptr(), w1.data_ptr(), _ptr(a0), _ptr(b0), _ptr(scale0), _ptr(a1),
+             _ptr(b1), _ptr(scale1), ids.data_ptr(), out0.data_ptr(), out1.data_ptr(), _ptr(ws), need, rows, tokens, k, n0,
+             n1, rank0, rank1, slots0, slots1, BF16, _stream(x))
     return out0, out1
 
 

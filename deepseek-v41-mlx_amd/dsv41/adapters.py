@@ -67,7 +67,7 @@ class AdapterBank:
 
 
 def _no_gradient(x: torch.Tensor, w: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
+    if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
         raise ValueError("adapter projections are not differentiable: call them under torch.no_grad()")
 
 
@@ -94,8 +94,9 @@ def _product_weight(lin: torch.nn.Linear, x: torch.Tensor) -> torch.Tensor | Non
 
 def _tiles_ok(w: torch.Tensor, x: torch.Tensor, rank: int) -> bool:
     """What dsv41_adapter_linear takes: bf16 in whole 64-channel steps and 32-row weight tiles, 16-byte addresses."""
-    return (x.dtype is torch.bfloat16 and rank <= 128 and w.shape[1] % 64 == 0 and w.shape[0] % 32 == 0
-            and w.data_ptr() % 16 == 0 and x.data_ptr() % 16 == 0)
+    n, k = w.shape
+    return (x.dtype is torch.bfloat16 and rank <= 128 and k % 64 == 0 and n % 32 == 0 and w.data_ptr() % 16 == 0
+            and x.data_ptr() % 16 == 0)
 
 
 def adapter_linear(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank | None, ids: torch.Tensor | None,
