@@ -114,8 +114,9 @@ class Attention(torch.nn.Module):
         self._break_sink = False
 
     def add_adapters(self, slots: int, rank: int, names=ADAPTED) -> dict:
-        """Banks of `slots` empty adapters for the named projections, kept in self.adapters and returned; a forward
-        whose shared.adapter_ids names a slot per sequence applies them."""
+        """Banks of `slots` empty adapters for the named projections, of the weights' type and on their device as they
+        are now, kept in self.adapters and returned; a forward whose shared.adapter_ids names a slot per sequence applies
+        them."""
         for name in names:
             if name not in ADAPTED:
                 raise ValueError(f"adapters go on {ADAPTED}, not on {name!r}")
