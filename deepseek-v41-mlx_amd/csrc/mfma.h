@@ -24,8 +24,9 @@ __device__ __forceinline__ f32x4 mfma16x16x16(i16x4 a, i16x4 b, f32x4 c) {
 }
 
 // Between an MFMA loop of a run-time length and the first VALU use of its results: a v_mfma_f32_16x16x32 result may be
-// read 8 wait states after issue (a v_mfma_f32_16x16x4_f32 result 11), which the compiler keeps inside a block but has been seen to miss across a loop's
-// exit branch (a v_cndmask two states after the last MFMA read a stale upper half of the result).
+// read 8 wait states after issue (a v_mfma_f32_16x16x4_f32 result 11), which the compiler keeps inside a block but has
+// been seen to miss across a loop's exit branch (a v_cndmask two states after the last MFMA read a stale upper half of
+// the result).
 template <int N>
 __device__ __forceinline__ void settle(f32x4 (&v)[N]) {
 #pragma unroll

@@ -235,7 +235,8 @@ class _RowTable:
             self.at.append((operator.attrgetter(*names), len(names)) if names else None)
             for name in names:
                 t = operator.attrgetter(name)(lc)
-                if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+                if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2] or (
+                        t.shape[0] > 1 and t.stride(0) < t.shape[1] * t.shape[2]):
                     raise ValueError(f"layer {i}: {name} {tuple(t.shape)} must be [sequences, rows, channels] with dense rows")
                 kind = ("state", t.shape[1], 1) if name.endswith("_state") else ("ring", lc.window, 1) if name.startswith(
                     "win") else ("comp", lc.ratio, lc.fp8_rb if name in ("comp_ks", "index_k8s") else 1)
@@ -260,6 +261,9 @@ class _RowTable:
         self.none = [None] * len(tensors)
         self.where, self.sizes = [t.data_ptr() for t in tensors], [t.numel() for t in tensors]
         n = len(tensors)
+        held = [p for p, size in zip(self.where, self.sizes) if size]
+        if len(set(held)) != len(held):
+            raise ValueError("two buffers of the cache are the same memory")
         self.pointers = (ctypes.c_int64 * n)(*self.where)
         self.strides = (ctypes.c_int64 * n)(*(t.stride(0) * t.element_size() for t in tensors))
         self.fills = (ctypes.c_uint32 * n)(*fills)

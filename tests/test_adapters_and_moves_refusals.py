@@ -219,6 +219,10 @@ def test_moves_check_their_arguments(host_abi):
     _refused(lambda: copy_sequences(_cache(cache_format="fp8"), _cache(cache_format="fp8", fp8_block_rows=32), [0]), "differ")
     c.layers[1].win_kv = c.layers[1].win_kv[:3]
     _refused(lambda: reorder_sequences(c, [1]), "layer 1")
+    c.layers[1].win_kv = c.layers[0].win_kv               # two layers on one buffer, sequences on one row
+    _refused(lambda: reorder_sequences(c, [1]), "same memory")
+    c.layers[1].win_kv = c.layers[0].win_kv[:1].clone().expand(4, -1, -1)
+    _refused(lambda: reorder_sequences(c, [1]), "dense rows")
 
 
 def test_c_entry_points_refuse_bad_sizes():
