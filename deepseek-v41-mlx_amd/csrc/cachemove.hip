@@ -202,6 +202,8 @@ extern "C" int dsv41_cache_move(const void* const* src, void* const* dst, const 
   for (int i = 0; i < buffers; ++i) {
     DSV41_REQUIRE(bytes[i] >= 0, DSV41_E_ARG, "%s: buffer %d moves %lld bytes", what, i, (long long)bytes[i]);
     DSV41_REQUIRE(bytes[i] == 0 || (src[i] && dst[i]), DSV41_E_ARG, "%s: buffer %d is null", what, i);
+    DSV41_REQUIRE(dst_rows == 1 || dst_stride[i] >= bytes[i], DSV41_E_ARG, "%s: buffer %d: rows of %lld bytes, %lld apart",
+                  what, i, (long long)bytes[i], (long long)dst_stride[i]);
     live += bytes[i] > 0;
     blocks += (bytes[i] + span - 1) / span;
     DSV41_REQUIRE(blocks < (1 << 24), DSV41_E_ARG, "%s: too many bytes", what);   // a grid holds fewer than 2^32 threads

@@ -218,6 +218,43 @@ def restore(cache: ModelCache, snap) -> None:
 _MINUS_INF = 0xFF800000
 
 
+def _rows_overlap(*caches) -> bool:
+    """Whether two rows (start, bytes between rows, bytes of a row; rows of one cache or of two) have bytes in common.
+    Of two caches, buffer i of the one may be whole rows of buffer i of the other, row for row: a move reads all rows of a
+    buffer before it writes any, but different buffers, or different columns of one, at any time. Rows of one pool in
+    turn (views whose spans interlace) are apart."""
+    starts, ends, buffers = [], [], []
+    for extents, batch in caches:
+        at, stride, size = extents.T
+        starts.append(at)
+        ends.append(at + stride * (batch - 1) + size)
+    lo, hi = np.concatenate(starts), np.concatenate(ends)
+    order = np.argsort(lo)
+    if (lo[order][1:] >= np.maximum.accumulate(hi[order])[:-1]).all():
+        return False                       # not even the buffers' whole spans meet
+    starts, ends = [], []
+    n = len(caches[0][0])
+    aligned = np.ones(n, dtype=bool)
+    if len(caches) == 2:
+        (a, batch_a), (b, batch_b) = caches
+        step = a[:, 1] if batch_a > 1 else b[:, 1]
+        aligned = ((a[:, 0] - b[:, 0]) % np.maximum(step, 1) == 0) & (
+            (a[:, 1] == b[:, 1]) if batch_a > 1 and batch_b > 1 else True)
+    for i, (extents, batch) in enumerate(caches):
+        at, stride, size = extents.T
+        first = at[:, None] + stride[:, None] * np.arange(batch)
+        starts.append(first.ravel())
+        ends.append((first + size[:, None]).ravel())
+        buffers.append(np.repeat(np.where(aligned, np.arange(n), np.arange(n) + n * i), batch))
+    lo, hi, buffer = np.concatenate(starts), np.concatenate(ends), np.concatenate(buffers)
+    held = hi > lo
+    lo, hi, buffer = lo[held], hi[held], buffer[held]
+    order = np.lexsort((hi, buffer, lo))
+    lo, hi, buffer = lo[order], hi[order], buffer[order]
+    met = lo[1:] < np.maximum.accumulate(hi)[:-1]
+    return bool((met & ((lo[1:] != lo[:-1]) | (buffer[1:] != buffer[:-1]))).any())
+
+
 class _RowTable:
     """A cache's buffers as moves of sequences take them: one entry per buffer, in layer order. Kept on the ModelCache
     (it holds no buffer alive, and copies and pickles of the cache leave it out) and built again when one of the buffers
@@ -261,9 +298,12 @@ class _RowTable:
         self.none = [None] * len(tensors)
         self.where, self.sizes = [t.data_ptr() for t in tensors], [t.numel() for t in tensors]
         n = len(tensors)
-        held = [p for p, size in zip(self.where, self.sizes) if size]
-        if len(set(held)) != len(held):
-            raise ValueError("two buffers of the cache are the same memory")
+        # where the buffers' rows lie: first row, bytes between rows, bytes of a row
+        self.extents = np.array([(t.data_ptr(), t.stride(0) * t.element_size(), t.shape[1] * w)
+                                 for t, w in zip(tensors, self.width)], dtype=np.int64)
+        self.apart = weakref.WeakSet()     # other caches' tables whose buffers do not reach into these
+        if _rows_overlap((self.extents, self.batch)):
+            raise ValueError("two buffers of the cache lie in the same memory")
         self.pointers = (ctypes.c_int64 * n)(*self.where)
         self.strides = (ctypes.c_int64 * n)(*(t.stride(0) * t.element_size() for t in tensors))
         self.fills = (ctypes.c_uint32 * n)(*fills)
@@ -334,6 +374,10 @@ def _move(what: str, dst: ModelCache, src: ModelCache, order, rows) -> None:
         if (dst.engram_ids is None) != (src.engram_ids is None):
             raise ValueError(f"{what}: one of the caches keeps engram ids")
         ours.check(src.offset)
+        if theirs not in ours.apart:
+            if _rows_overlap((ours.extents, ours.batch), (theirs.extents, theirs.batch)):
+                raise ValueError(f"{what}: buffers of the caches lie in the same memory")
+            ours.apart.add(theirs)
     visible = theirs.visible(src.offset)
     order = _index(f"{what}: order", order, theirs.batch, -1, ours.device)
     if rows is not None:

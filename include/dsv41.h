@@ -610,8 +610,10 @@ int dsv41_adapter_linear_pair(const void* x, const void* w0, const void* w1, con
 
 /* Moves of sequences (batch rows) between the buffers of one cache or of two: for each move i < moves,
  * row rows[i] (rows NULL: row i) of every destination buffer takes the first bytes[b] bytes of row
- * order[i] of its source buffer. Every row is read before any is written, so src and dst may be the
- * same buffers (same != 0 says so: a row onto itself is left alone). An order entry outside
+ * order[i] of its source buffer. Every row of a buffer is read before any of its rows is written, so src and dst
+ * may be the same buffers (same != 0 says so: a row onto itself is left alone) or whole rows of them; beyond that
+ * no destination row may overlap another buffer's rows or columns, or the next row (a destination stride below
+ * bytes[b] is refused). An order entry outside
  * [0, src_rows) empties the row: its bytes[b] bytes become the word fill[b] (low byte first). A rows
  * entry outside [0, dst_rows) moves nothing; of several moves to one row the last counts. order and
  * rows: int32 on the device, read when the kernels run. src, dst, the strides (bytes between sequences), bytes and fill: host
