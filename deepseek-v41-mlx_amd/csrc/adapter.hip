@@ -830,19 +830,23 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
       return half_of(v, low);
     }
   };
+  // Where the workgroup's columns are of both projections its waves may go different ways below: h is summed, and the
+  // waves meet, before they part. Elsewhere all of them see the same bank and rows and meet inside one branch.
+  const bool border = col0 < a.t.r0 && col0 + 64 * WR > a.t.r0;
+  if (border) sum_h();
   const bool one = named == 0 || __ballot(id >= 0 && id != __builtin_amdgcn_readlane(id, __builtin_ctz(named | 0x10000u))) == 0;
   if (named == 0) {
     sum_parts();
-    sum_h();
+    if (!border) sum_h();
   } else if (one) {
     Expand<WR, 1> ex(bk, n, at, id, named);
     sum_parts();
-    sum_h();
+    if (!border) sum_h();
     ex.add(acc, operand);
   } else {
     Expand<WR, 4> ex(bk, n, at, id, named);
     sum_parts();
-    sum_h();
+    if (!border) sum_h();
     ex.add(acc, operand);
   }
   if (m < a.t.rows && l16 < SUB)
