@@ -140,7 +140,8 @@ __device__ __forceinline__ void move_span(const uint8_t* src, uint8_t* dst, int6
   // behind the last pass's barrier: a row that was read may be emptied
   P none;
   if constexpr (W == 16) none = u32x4{fill, fill, fill, fill};
-  else none = (P)fill;
+  else if constexpr (W == 4) none = fill;
+  else none = (P)(fill >> 8 * (threadIdx.x & 3));           // byte by byte: spans and steps are whole words
   for (int i = 0; i < m; ++i)
     for (int off = threadIdx.x * W; off < bytes; off += kMoveThreads * W)
       put(reinterpret_cast<P*>(dst + gone[i].y * ds + off), none);
