@@ -50,7 +50,7 @@ import numpy as np
 import torch
 
 from . import _abi
-from .compressor import CompressorState
+from .compressor import CompressorState, CountedAttributes
 from .config import ModelArgs
 
 
@@ -71,7 +71,7 @@ class PackedKeys:
         return self.codes.shape
 
 
-class LayerCache:
+class LayerCache(CountedAttributes):
     def __init__(self, bsz: int, args: ModelArgs, layer_id: int, max_seq_len: int,
                  dtype=torch.float32, device="cuda", index_format: str = "dense", cache_format: str = "dense",
                  fp8_block_rows: int = 1):
@@ -255,21 +255,25 @@ def _rows_overlap(*caches) -> bool:
     return bool((met & ((lo[1:] != lo[:-1]) | (buffer[1:] != buffer[:-1]))).any())
 
 
+_changes = operator.attrgetter("_changes")
+
+
 class _RowTable:
     """A cache's buffers as moves of sequences take them: one entry per buffer, in layer order. Kept on the ModelCache
-    (it holds no buffer alive, and copies and pickles of the cache leave it out) and built again when one of the buffers
-    is another tensor or lies elsewhere."""
+    (it holds no buffer alive, and copies and pickles of the cache leave it out) and built again when a layer or a state
+    is another one, when anything has been assigned to one of them (a buffer exchanged, added or taken away), and when a
+    buffer lies elsewhere or has another shape or other strides."""
 
     def __init__(self, cache: ModelCache):
         self.layout, self.width, tensors, fills = [], [], [], []
-        self.at = []                       # a layer's buffers in one call
+        counted = []                       # layers and states
         self.kinds, self.need = {}, []     # (what the rows count, ratio, rows per scale), the fewest rows of such a buffer
         self.kind = []                     # a buffer's entry of those
         for i, lc in enumerate(cache.layers):
             names = [n for n in _BUFFERS if getattr(lc, n) is not None]
             if lc.comp_state is not None:
                 names += ["comp_state.kv_state", "comp_state.score_state"]
-            self.at.append((operator.attrgetter(*names), len(names)) if names else None)
+                counted.append(lc.comp_state)
             for name in names:
                 t = operator.attrgetter(name)(lc)
                 if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2] or (
@@ -294,38 +298,45 @@ class _RowTable:
             if t.shape[0] != self.batch or t.device != self.device:
                 raise ValueError(f"layer {i}: {name} {tuple(t.shape)} on {t.device} in a cache of {self.batch} sequences on "
                                  f"{self.device}")
+        counted[:0] = cache.layers
+        # an object that does not count its changes is not trusted to have had none: the table serves one call
+        self.known = all(isinstance(c, CountedAttributes) for c in counted)
+        self.layers, self.counted = len(cache.layers), [weakref.ref(c) for c in counted] if self.known else []
+        self.changes = [c._changes for c in counted] if self.known else None
         self.tensors = [weakref.ref(t) for t in tensors]
-        self.none = [None] * len(tensors)
-        self.where, self.sizes = [t.data_ptr() for t in tensors], [t.numel() for t in tensors]
+        self.where = [t.data_ptr() for t in tensors]
+        self.shapes, self.steps = [t.size() for t in tensors], [t.stride() for t in tensors]
+        self.dense = all(t.is_contiguous() for t in tensors)
         n = len(tensors)
         # where the buffers' rows lie: first row, bytes between rows, bytes of a row
         self.extents = np.array([(t.data_ptr(), t.stride(0) * t.element_size(), t.shape[1] * w)
                                  for t, w in zip(tensors, self.width)], dtype=np.int64)
-        self.apart = weakref.WeakSet()     # other caches' tables whose buffers do not reach into these
+        self.partners = weakref.WeakSet()  # other caches' tables that go with this one (_pair)
         if _rows_overlap((self.extents, self.batch)):
             raise ValueError("two buffers of the cache lie in the same memory")
-        self.pointers = (ctypes.c_int64 * n)(*self.where)
-        self.strides = (ctypes.c_int64 * n)(*(t.stride(0) * t.element_size() for t in tensors))
+        self.kind, self.width = np.array(self.kind), np.array(self.width, dtype=np.int64)
+        self.words = ctypes.c_int64 * n
+        self.pointers = self.words(*self.where)
+        self.strides = self.words(*(t.stride(0) * t.element_size() for t in tensors))
         self.fills = (ctypes.c_uint32 * n)(*fills)
 
     def __reduce__(self):
         return type(None), ()
 
     def current(self, cache: ModelCache) -> bool:
-        if len(cache.layers) != len(self.at):
+        if not self.known:
             return False
-        now = []
+        counted, now = [r() for r in self.counted], [r() for r in self.tensors]
         try:
-            for lc, layer in zip(cache.layers, self.at):
-                if layer is not None:
-                    get, many = layer
-                    now += get(lc) if many > 1 else (get(lc),)
-        except AttributeError:             # a compressor's state has gone
+            return (counted[:self.layers] == list(cache.layers)
+                    and list(map(_changes, counted)) == self.changes
+                    and list(map(torch.Tensor.data_ptr, now)) == self.where
+                    and list(map(torch.Tensor.size, now)) == self.shapes
+                    # a shape without gaps has one set of strides (2.0 us for 56 buffers, their strides 3.3)
+                    and (self.dense and all(map(torch.Tensor.is_contiguous, now))
+                         or list(map(torch.Tensor.stride, now)) == self.steps))
+        except (AttributeError, TypeError):    # a state or a buffer has gone
             return False
-        known = [r() for r in self.tensors]
-        return (all(map(operator.is_, now, known)) and all(map(operator.is_not, now, self.none))
-                and list(map(torch.Tensor.data_ptr, now)) == self.where
-                and list(map(torch.Tensor.numel, now)) == self.sizes)
 
     def check(self, offset: int) -> list:
         """Rows that `offset` positions have written, by kind of buffer: ring slots, compressed rows (or their scale
@@ -341,7 +352,7 @@ class _RowTable:
     def visible(self, offset: int):
         """Bytes of a sequence that move, buffer by buffer."""
         rows = self.check(offset)
-        return (ctypes.c_int64 * len(self.kind))(*[rows[k] * w for k, w in zip(self.kind, self.width)])
+        return self.words.from_buffer(np.array(rows, dtype=np.int64)[self.kind] * self.width)
 
 
 def _row_table(cache: ModelCache) -> _RowTable:
@@ -349,6 +360,17 @@ def _row_table(cache: ModelCache) -> _RowTable:
     if table is None or not table.current(cache):
         table = cache._row_table = _RowTable(cache)
     return table
+
+
+def _pair(what: str, ours: _RowTable, theirs: _RowTable) -> None:
+    """What two caches' buffers must have in common, and apart, for sequences to move between them: once per pair."""
+    if ours.layout != theirs.layout:
+        raise ValueError(f"{what}: the caches differ in layers, formats, widths or ratios")
+    if ours.device != theirs.device:
+        raise ValueError(f"{what}: caches on {ours.device} and {theirs.device}")
+    if _rows_overlap((ours.extents, ours.batch), (theirs.extents, theirs.batch)):
+        raise ValueError(f"{what}: buffers of the caches lie in the same memory")
+    ours.partners.add(theirs)
 
 
 def _index(what: str, values, rows: int, low: int, device) -> torch.Tensor:
@@ -367,17 +389,11 @@ def _move(what: str, dst: ModelCache, src: ModelCache, order, rows) -> None:
     theirs = _row_table(src)
     ours = theirs if same else _row_table(dst)
     if not same:
-        if ours.layout != theirs.layout:
-            raise ValueError(f"{what}: the caches differ in layers, formats, widths or ratios")
-        if ours.device != theirs.device:
-            raise ValueError(f"{what}: caches on {ours.device} and {theirs.device}")
+        if theirs not in ours.partners:
+            _pair(what, ours, theirs)
         if (dst.engram_ids is None) != (src.engram_ids is None):
             raise ValueError(f"{what}: one of the caches keeps engram ids")
         ours.check(src.offset)
-        if theirs not in ours.apart:
-            if _rows_overlap((ours.extents, ours.batch), (theirs.extents, theirs.batch)):
-                raise ValueError(f"{what}: buffers of the caches lie in the same memory")
-            ours.apart.add(theirs)
     visible = theirs.visible(src.offset)
     order = _index(f"{what}: order", order, theirs.batch, -1, ours.device)
     if rows is not None:

@@ -63,7 +63,22 @@ class Compressor(torch.nn.Module):
                                   self.norm.weight, self.ratio, start_pos, self.norm.eps, x.dtype)
 
 
-class CompressorState:
+class CountedAttributes:
+    """Counts what is assigned to it and deleted from it, so that a table of its tensors can tell whether it still lists
+    all of them."""
+
+    _changes = 0
+
+    def __setattr__(self, name, value):
+        super().__setattr__("_changes", self._changes + 1)
+        super().__setattr__(name, value)
+
+    def __delattr__(self, name):
+        super().__setattr__("_changes", self._changes + 1)
+        super().__delattr__(name)
+
+
+class CompressorState(CountedAttributes):
     """The open group's per-token kv/score rows, fp32 (compressor.py:82-88)."""
 
     def __init__(self, bsz: int, ratio: int, head_dim: int, device="cuda"):
