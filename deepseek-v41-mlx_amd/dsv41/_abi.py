@@ -1330,7 +1330,13 @@ def adapter_add(x, a, b, scale, ids, y, out=None, workspace=None):
     rows, tokens, k, rank, slots = _adapter_args(name, x, a, b, scale, ids, y.shape[-1])
     if y.dtype != x.dtype or y.shape[:-1] != x.shape[:-1] or y.device != x.device:
         raise ValueError(f"{name}: y {y.dtype} {tuple(y.shape)} does not go with x {x.dtype} {tuple(x.shape)}")
-    out = _out(name, out, y.shape, y.dtype, y.device)
+    if out is not None:
+        _out(name, out, y.shape, y.dtype, y.device)
+        if out.data_ptr() != y.data_ptr():         # an element is read and written by one thread: in place it may be
+            _apart(name, out, "y (in another place)", y)
+        _apart(name, out, "the adapters", b, scale, ids)
+    else:
+        out = torch.empty_like(y)
     if rows == 0:
         return out
     need = lib().dsv41_adapter_add_workspace_bytes(rows, rank)
@@ -1355,19 +1361,23 @@ def _adapter_weight(name, x, w):
         _contig(name, w)
 
 
-def _adapter_out(name, out, x, n):
+def _adapter_out(name, out, x, n, *operands):
+    """An output of n channels for x's rows; a caller's must lie apart from x and the operands (weights, adapters, ids;
+    None for one that is not there), which other workgroups still read when it is written."""
     if out is None:
         return x.new_empty((*x.shape[:-1], n))
     _out(name, out, (*x.shape[:-1], n), x.dtype, x.device)
-    _apart(name, out, x)
+    _apart(name, out, "x or the other output", x)
+    _apart(name, out, "a weight or the adapters", *operands)
     return out
 
 
-def _apart(name, out, other):
-    """Two contiguous tensors that must not overlap."""
-    if (out.data_ptr() < other.data_ptr() + other.numel() * other.element_size()
-            and other.data_ptr() < out.data_ptr() + out.numel() * out.element_size()):
-        raise ValueError(f"{name}: out overlaps x or the other output")
+def _apart(name, out, what, *others):
+    """A contiguous output that must not overlap the contiguous tensors it depends on."""
+    for other in others:
+        if (other is not None and out.data_ptr() < other.data_ptr() + other.numel() * other.element_size()
+                and other.data_ptr() < out.data_ptr() + out.numel() * out.element_size()):
+            raise ValueError(f"{name}: out overlaps {what}")
 
 
 def adapter_linear(x, w, a, b, scale, ids, out=None, workspace=None):
@@ -1377,7 +1387,7 @@ def adapter_linear(x, w, a, b, scale, ids, out=None, workspace=None):
     rows, tokens, k, rank, slots = _adapter_args(name, x, a, b, scale, ids, w.shape[0])
     _adapter_weight(name, x, w)
     n = w.shape[0]
-    out = _adapter_out(name, out, x, n)
+    out = _adapter_out(name, out, x, n, w, a, b, scale, ids)
     if rows == 0:
         return out
     need = adapter_linear_workspace_bytes(rows, k, n, 0, rank, 0)
@@ -1396,7 +1406,7 @@ def adapter_plain(x, w, a, b, scale, ids, out=None):
         raise ValueError(f"{name}: x {x.dtype} {tuple(x.shape)} and w {w.dtype} {tuple(w.shape)} do not contract")
     _contig(name, w)
     code = dtype_code(x, name)
-    out = _adapter_out(name, out, x, w.shape[0])
+    out = _adapter_out(name, out, x, w.shape[0], w, a, b, scale, ids)
     if rows:
         _call_on(x.device, name, x.data_ptr(), w.data_ptr(), a.data_ptr(), b.data_ptr(), scale.data_ptr(),
                  ids.data_ptr(), out.data_ptr(), rows, tokens, k, w.shape[0], rank, slots, code, _stream(x))
@@ -1421,11 +1431,12 @@ def adapter_linear_pair(x, w0, w1, bank0, bank1, ids, out0=None, out1=None, work
         a1, b1, scale1 = bank1
         rows, tokens, k, rank1, slots1 = _adapter_args(name, x, a1, b1, scale1, ids, n1)
     given = out0 is not None and out1 is not None
-    out0, out1 = _adapter_out(name, out0, x, n0), _adapter_out(name, out1, x, n1)
+    out0 = _adapter_out(name, out0, x, n0, w0, w1, a0, b0, scale0, a1, b1, scale1, ids)
+    out1 = _adapter_out(name, out1, x, n1, w0, w1, a0, b0, scale0, a1, b1, scale1, ids)
     if rows == 0:
         return out0, out1
     if given:
-        _apart(name, out0, out1)
+        _apart(name, out0, "x or the other output", out1)
     need = adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1)
     ws = _ws(name, workspace, need, x.device)
     _call_on(x.device, name, x.data_ptr(), w0.data_ptr(), w1.data_ptr(), _ptr(a0), _ptr(b0), _ptr(scale0), _ptr(a1),

@@ -568,12 +568,13 @@ int dsv41_linear_rows_pair(const void* x, const void* w0, const void* w1, void* 
  *   y[m] = x[m] @ w^T + scale[t] * ((x[m] @ a[t]^T) @ b[t]^T),   a [slots, rank, k], b [slots, n, rank],
  * and y[m] = x[m] @ w^T for any other t (-1: no adapter), whatever the slots hold. Sums and the
  * rank-wide intermediate are fp32, in a fixed order: deterministic. No output may overlap
- * x or the other output. An infinite value of b gives NaN where the intermediate is zero or, in bf16, short.
+ * an input or the other output, but for what dsv41_adapter_add allows. An infinite value of b gives NaN where the
+ * intermediate is zero or, in bf16, short.
  */
 
 /* The adapters' part on top of a projection already computed: out = y + scale (x a^T) b^T, y and out
- * [rows, n] in dtype (F32 or BF16; y == out allowed); any k, n and rank. Two launches on fp32 arithmetic: the form
- * for what the calls below do not take. */
+ * [rows, n] in dtype (F32 or BF16; out may be y itself, and lie over x or a, which an earlier launch has read);
+ * any k, n and rank. Two launches on fp32 arithmetic: the form for what the calls below do not take. */
 size_t dsv41_adapter_add_workspace_bytes(int64_t rows, int32_t rank);
 int dsv41_adapter_add(const void* x, const void* a, const void* b, const float* scale, const int32_t* ids,
                       const void* y, void* out, void* workspace, size_t workspace_bytes, int64_t rows,
