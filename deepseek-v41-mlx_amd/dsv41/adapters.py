@@ -9,7 +9,8 @@ none:
 ``ids`` is an int32 device tensor, read by the kernels, so a captured HIP graph replays with whatever it then holds.
 The rank-wide product and all sums are float32; the result is rounded once where the projection itself runs here, and
 once more where it is torch's (float32 activations, widths the matrix-core kernels do not take, a module with hooks).
-Inference only: a call that autograd would have to follow is refused.
+Inference only: a call that autograd would have to follow - x, the projection or a bank requires gradients or holds a
+tangent - is refused.
 """
 
 from __future__ import annotations
@@ -66,9 +67,21 @@ class AdapterBank:
         self.scale[slot] = 0.0
 
 
-def _no_gradient(x: torch.Tensor, w: torch.Tensor) -> None:
-    if (x.requires_grad or w.requires_grad) and torch.is_grad_enabled():
+_forward_ad = torch.autograd.forward_ad
+
+
+def _no_gradient(x: torch.Tensor, w: torch.Tensor, *banks: AdapterBank | None) -> None:
+    """Refuses operands of a call that autograd would have to follow, backward or forward."""
+    wanted = x.requires_grad or w.requires_grad
+    for k in banks:
+        if k is not None:
+            wanted = wanted or k.a.requires_grad or k.b.requires_grad or k.scale.requires_grad
+    if wanted and torch.is_grad_enabled():
         raise ValueError("adapter projections are not differentiable: call them under torch.no_grad()")
+    if _forward_ad._current_level >= 0:
+        held = [t for k in banks if k is not None for t in (k.a, k.b, k.scale)]
+        if any(_forward_ad.unpack_dual(t).tangent is not None for t in (x, w, *held)):
+            raise ValueError("adapter projections are not differentiable: their operands may hold no tangent")
 
 
 _module = torch.nn.modules.module
@@ -108,16 +121,18 @@ def adapter_linear(lin: torch.nn.Linear, x: torch.Tensor, bank: AdapterBank | No
     x = x.contiguous()
     w = _product_weight(lin, x)
     if w is not None:
-        _no_gradient(x, w)
+        _no_gradient(x, w, bank)
         if _tiles_ok(w, x, bank.a.shape[1]):
             return _abi.adapter_linear(x, w, bank.a, bank.b, bank.scale, ids)
         if x.numel() * w.shape[0] <= _PLAIN_MACS:
             return _abi.adapter_plain(x, w, bank.a, bank.b, bank.scale, ids)
-    _no_gradient(x, lin.weight)
+    _no_gradient(x, lin.weight, bank)
     if (bank.out_features, bank.in_features) != tuple(lin.weight.shape):
         raise ValueError(f"adapters of [{bank.out_features}, {bank.in_features}] on a projection of "
                          f"{list(lin.weight.shape)}")
-    return _abi.adapter_add(x, bank.a, bank.b, bank.scale, ids, lin(x).contiguous())
+    y = lin(x).contiguous()
+    _no_gradient(y, lin.weight)                # a bias, or what a module of its own multiplies with
+    return _abi.adapter_add(x, bank.a, bank.b, bank.scale, ids, y)
 
 
 def adapter_linear_pair(lin0: torch.nn.Linear, lin1: torch.nn.Linear, x: torch.Tensor, bank0: AdapterBank | None,
@@ -131,7 +146,7 @@ def adapter_linear_pair(lin0: torch.nn.Linear, lin1: torch.nn.Linear, x: torch.T
     if (w0 is not None and w1 is not None and w0.shape[1] == w1.shape[1]
             and _tiles_ok(w0, x, 0 if bank0 is None else bank0.a.shape[1])
             and _tiles_ok(w1, x, 0 if bank1 is None else bank1.a.shape[1])):
-        _no_gradient(x, w0)
+        _no_gradient(x, w0, bank0, bank1)
         _no_gradient(x, w1)
         return _abi.adapter_linear_pair(x, w0, w1, None if bank0 is None else (bank0.a, bank0.b, bank0.scale),
                                         None if bank1 is None else (bank1.a, bank1.b, bank1.scale), ids)
