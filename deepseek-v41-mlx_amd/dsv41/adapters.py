@@ -70,17 +70,14 @@ class AdapterBank:
 _forward_ad = torch.autograd.forward_ad
 
 
-def _no_gradient(x: torch.Tensor, w: torch.Tensor, *banks: AdapterBank | None) -> None:
+def _no_gradient(x: torch.Tensor, w: torch.Tensor, bank: AdapterBank | None = None) -> None:
     """Refuses operands of a call that autograd would have to follow, backward or forward."""
-    wanted = x.requires_grad or w.requires_grad
-    for k in banks:
-        if k is not None:
-            wanted = wanted or k.a.requires_grad or k.b.requires_grad or k.scale.requires_grad
-    if wanted and torch.is_grad_enabled():
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or bank is not None and (
+            bank.a.requires_grad or bank.b.requires_grad or bank.scale.requires_grad)):
         raise ValueError("adapter projections are not differentiable: call them under torch.no_grad()")
     if _forward_ad._current_level >= 0:
-        held = [t for k in banks if k is not None for t in (k.a, k.b, k.scale)]
-        if any(_forward_ad.unpack_dual(t).tangent is not None for t in (x, w, *held)):
+        held = (x, w) if bank is None else (x, w, bank.a, bank.b, bank.scale)
+        if any(_forward_ad.unpack_dual(t).tangent is not None for t in held):
             raise ValueError("adapter projections are not differentiable: their operands may hold no tangent")
 
 
@@ -146,8 +143,8 @@ def adapter_linear_pair(lin0: torch.nn.Linear, lin1: torch.nn.Linear, x: torch.T
     if (w0 is not None and w1 is not None and w0.shape[1] == w1.shape[1]
             and _tiles_ok(w0, x, 0 if bank0 is None else bank0.a.shape[1])
             and _tiles_ok(w1, x, 0 if bank1 is None else bank1.a.shape[1])):
-        _no_gradient(x, w0, bank0, bank1)
-        _no_gradient(x, w1)
+        _no_gradient(x, w0, bank0)
+        _no_gradient(x, w1, bank1)
         return _abi.adapter_linear_pair(x, w0, w1, None if bank0 is None else (bank0.a, bank0.b, bank0.scale),
                                         None if bank1 is None else (bank1.a, bank1.b, bank1.scale), ids)
     return adapter_linear(lin0, x, bank0, ids), adapter_linear(lin1, x, bank1, ids)
