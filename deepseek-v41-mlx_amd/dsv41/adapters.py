@@ -94,12 +94,12 @@ def _product_weight(lin: torch.nn.Linear, x: torch.Tensor) -> torch.Tensor | Non
     """The projection's weight where the module's call is the product alone (no hooks, bias or forward of its own), of
     x's type and in one piece, so that a kernel may stand in for the module."""
     own = lin.__dict__
+    params = own["_parameters"]            # a weight or bias that is no parameter (a plain tensor in its place) is not there
+    w = params.get("weight")
     if (type(lin) is not torch.nn.Linear or "forward" in own or any(own[h] for h in _FORWARD_HOOKS)
-            or _module._global_forward_hooks or _module._global_forward_pre_hooks
-            or own["_parameters"]["bias"] is not None):
+            or _module._global_forward_hooks or _module._global_forward_pre_hooks or params.get("bias", own) is not None):
         return None
-    w = own["_parameters"]["weight"]
-    return w if w.dtype is x.dtype and w.is_contiguous() else None
+    return w if w is not None and w.dtype is x.dtype and w.is_contiguous() else None
 
 
 def _tiles_ok(w: torch.Tensor, x: torch.Tensor, rank: int) -> bool:
