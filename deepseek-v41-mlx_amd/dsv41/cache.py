@@ -378,7 +378,7 @@ def _index(what: str, values, rows: int, low: int, device) -> torch.Tensor:
     by the kernel."""
     if isinstance(values, torch.Tensor) and values.is_cuda:
         return values
-    values = [int(v) for v in values]
+    values = [operator.index(v) for v in values]           # whole numbers: 1.5 is no sequence
     if any(not low <= v < rows for v in values):
         raise ValueError(f"{what} must lie in [{low}, {rows}), got {values}")
     return torch.tensor(values, dtype=torch.int32, device=device)

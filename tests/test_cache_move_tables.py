@@ -136,3 +136,17 @@ def test_two_caches_are_compared_again(moved):
         copy_sequences(b, a, [0, 1])
     with pytest.raises(ValueError, match="differ"):
         copy_sequences(_cache(cache_format="fp8"), a, [0] * 4)
+
+
+def test_sequences_are_whole_numbers(moved):
+    import numpy as np
+    from dsv41.cache import reorder_sequences
+    c = _cache()
+    for order in ([1, 0], (1, 0), range(2), np.array([1, 0], np.int16), torch.tensor([1, 0]), [np.int64(1), torch.tensor(0)]):
+        reorder_sequences(c, order)
+        reorder_sequences(c, order, order)
+    for order in ([0.9, 0], [1.0, 0], np.array([1.0, 0.0]), torch.tensor([0.5, 1]), ["1", "0"], [None, 0]):
+        with pytest.raises(TypeError):
+            reorder_sequences(c, order)
+        with pytest.raises(TypeError):
+            reorder_sequences(c, [1, 0], order)
