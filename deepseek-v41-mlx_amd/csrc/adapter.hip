@@ -574,9 +574,9 @@ struct Expand {
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < WR; ++i) {
-          const bf16x8 bf = or_zero(cur[u][i], at.live);
-          f32x4 sum = mfma16x16x32(bf, hf, acc[i]);
-          sum = mfma16x16x32(bf, lf, sum);
+          // an operand that is not there multiplies no B either: 0 times infinity would stay
+          f32x4 sum = mfma16x16x32(or_zero(cur[u][i], at.live), hf, acc[i]);
+          sum = mfma16x16x32(or_zero(cur[u][i], at.live && r8 > 2), lf, sum);
           acc[i] = id == now[u] && (u == 0 || now[u] != now[0]) ? sum : acc[i];
         }
       if (!more) return;
