@@ -14,6 +14,8 @@
 //   prompts    h first, then the projection's tiles with the adapters' part in their sums when the products begin:
 //              8,192 rows 8192 -> 5120 at rank 64 42 + 580 us, 1.13 PFLOP/s; few tiles split the contraction and end
 //              in the same second launch.
+#include <type_traits>
+
 #include "tiles.h"
 
 namespace dsv41 {
@@ -389,32 +391,37 @@ __device__ __forceinline__ void shrink_item(const AdapterArgs& a, const Bank& bk
   __syncthreads();
 }
 
-// Ranks 8 c .. 8 c + 7 of scale h as an operand of the second product: it takes the sum of two bf16 values - the upper
-// 8 bits, cut off, and the next 8, rounded - so that 16 bits of the intermediate count (2^-17 of it is lost, far below
-// the result's own rounding); each is multiplied with the same bf16 B, exactly. An infinite value has no lower part.
-__device__ __forceinline__ uint4 half_of(const float* v, bool low) {
-  uint32_t w[4];
+// Ranks 8 c .. 8 c + 7 of scale h as an operand of the second product: it takes the sum of three bf16 values - the upper
+// 8 bits, cut off, the next 8, cut off, and what is left, 8 bits again - so that all 24 bits count; each is multiplied
+// with the same bf16 B, exactly. An infinite value has no lower parts.
+__device__ __forceinline__ uint4 part_of(const float* v, int part) {
+  uint32_t w[8];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t h0 = __float_as_uint(v[2 * e]) & 0xFFFF0000u, h1 = __float_as_uint(v[2 * e + 1]) & 0xFFFF0000u;
-    const float l0 = h0 << 1 == 0xFF000000u ? 0.0f : v[2 * e] - __uint_as_float(h0);
-    const float l1 = h1 << 1 == 0xFF000000u ? 0.0f : v[2 * e + 1] - __uint_as_float(h1);
-    w[e] = low ? pack2_bf16(l0, l1) : (h0 >> 16) | h1;
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t upper = __float_as_uint(v[e]) & 0xFFFF0000u;
+    const float rest = upper << 1 == 0xFF000000u ? 0.0f : v[e] - __uint_as_float(upper);
+    const uint32_t next = __float_as_uint(rest) & 0xFFFF0000u;
+    const uint32_t last = __float_as_uint(rest - __uint_as_float(next));
+    w[e] = part == 0 ? upper : part == 1 ? next : last;
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  auto pair = [&](int e) { return (w[e] >> 16) | (w[e + 1] & 0xFFFF0000u); };
+  return make_uint4(pair(0), pair(2), pair(4), pair(6));
 }
 
-// The rank chunk of 8 that lane group g supplies to step q of the second product. Up to 16 ranks are one step: the upper
-// parts of the chunks, then the lower ones, in one MFMA. More take 4 chunks a step and two MFMAs, upper and lower, on one
-// load of B (16 sequences' own B of rank 64 for 32768 outputs: 24.6 us, 43 when it was loaded for each).
+// The operands that lane group g supplies to step q of the second product: parts of one rank chunk of 8. Up to 16 ranks
+// are one step of one MFMA for the chunks' upper, next and last parts in turn, and a second one for the last parts that
+// it has no room for (two chunks' six parts). More take 4 chunks a step and an MFMA per part, on one load of B (16
+// sequences' own B of rank 64 for 32768 outputs: 24.6 us, 43 when it was loaded for each of two parts).
 struct RankSlot {
-  int c;
-  bool low, live;
+  int c, part;                                             // the chunk, and its part in the first MFMA
+  bool live, last;                                         // in the first MFMA (and the next part's), in the last part's
   __device__ __forceinline__ RankSlot(int q, int r8) {
     const int g = (threadIdx.x >> 4) & 3;
-    low = r8 <= 2 && g >= r8;
-    c = r8 <= 2 ? (low ? g - r8 : g) : 4 * q + g;
-    live = r8 <= 2 ? g < 2 * r8 : c < r8;
+    const bool few = r8 <= 2;
+    part = few ? min(g / r8, 2) : 0;
+    c = few ? g % r8 : 4 * q + g;
+    live = few ? g < 3 * r8 : c < r8;
+    last = few ? g < 3 * r8 - 4 : live;
     if (!live) c = 0;
   }
   __device__ __forceinline__ static int steps(int r8) { return r8 <= 2 ? 1 : (r8 + 3) / 4; }
@@ -424,8 +431,8 @@ struct RankSlot {
 // 256 channels at a time (a copy instruction takes 512 bytes of each of two rows: fragments loaded from memory directly
 // touch 16 rows per instruction: 8,192 rows of 8192 channels at rank 64 took 63 us, 41 this way), NS - 1 steps ahead;
 // MT RT waves take a 16 x 16 tile each, times KS that share a step's channels. Writes the second product's operand: per
-// row the upper halves of scale h's ranks, then the lower ones ([rows, 2 rank] bf16). Rows without an adapter are left
-// as they are.
+// row the upper parts of scale h's ranks, then the next ones, then the last ([rows, 3 rank] bf16). Rows without an
+// adapter are left as they are.
 //
 // A step's tile row is 32 chunks of 16 bytes; chunk c of row r lies at c ^ (r & 15) (and within the 32), so that the 16
 // rows of a fragment read start in different banks.
@@ -509,16 +516,17 @@ __global__ __launch_bounds__(64 * MT * RT * KS) void adapter_shrink_kernel(Adapt
       for (int w = 1; w < KS; ++w) sum += red[w * MT * RT * 256 + q * 8 + e];
       v[e] = sum * scale;
     }
-    uint16_t* to = hl + (m0 + row) * 2 * bk.rank + r;
-    *reinterpret_cast<uint4*>(to) = half_of(v, false);
-    *reinterpret_cast<uint4*>(to + bk.rank) = half_of(v, true);
+    uint16_t* to = hl + (m0 + row) * 3 * bk.rank + r;
+#pragma unroll
+    for (int part = 0; part < 3; ++part) *reinterpret_cast<uint4*>(to + part * bk.rank) = part_of(v, part);
   }
 }
 
 // The second product for 16 rows (lane l16's, adapter id) and WR tiles of 16 output columns, in steps of one rank group
-// (32 of the 2 rank operands) and up to U adapters, each step's B loaded a step ahead; the first one's before the
+// (32 of the rank operands) and up to U adapters, each step's B loaded a step ahead; the first one's before the
 // caller has h at all. Rows are the MFMA's columns: each adapter multiplies all of them, a lane keeps its own row's.
-template <int WR, int U>
+// FEW: up to 16 ranks.
+template <int WR, int U, bool FEW>
 struct Expand {
   const bf16_t* b;       // slot 0, the lane's first output column
   int64_t slot;
@@ -543,17 +551,18 @@ struct Expand {
         named(named_), todo(named_), q(0) {
     load();
   }
-  // operand(c, low) gives the upper or lower parts of scale h's ranks 8 c .. 8 c + 7 of the lane's row
+  // operand(c, part) gives a part of scale h's ranks 8 c .. 8 c + 7 of the lane's row
   template <typename H>
   __device__ __forceinline__ void add(f32x4 (&acc)[WR], H operand) {
     const int r8 = rank >> 3, end = RankSlot::steps(r8);
-    bf16x8 hf, lf;
+    bf16x8 upper, next_part, last;
     bool fresh = true;
     for (;;) {
       const RankSlot at(q, r8);
       if (fresh) {
-        hf = or_zero(operand(at.c, at.low), at.live);
-        lf = or_zero(operand(at.c, true), at.live && r8 > 2);     // no branch between an MFMA and the choice of its result
+        upper = or_zero(operand(at.c, at.part), at.live);
+        if constexpr (!FEW) next_part = or_zero(operand(at.c, 1), at.live);
+        last = or_zero(operand(at.c, 2), at.last);
       }
       int now[U];
       uint4 cur[U][WR];
@@ -570,13 +579,15 @@ struct Expand {
       }
       const bool more = q < end;
       if (more) load();
+      // no branch between an MFMA and the choice of its result
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < WR; ++i) {
           // an operand that is not there multiplies no B either: 0 times infinity would stay
-          f32x4 sum = mfma16x16x32(or_zero(cur[u][i], at.live), hf, acc[i]);
-          sum = mfma16x16x32(or_zero(cur[u][i], at.live && r8 > 2), lf, sum);
+          f32x4 sum = mfma16x16x32(or_zero(cur[u][i], at.live), upper, acc[i]);
+          if constexpr (!FEW) sum = mfma16x16x32(or_zero(cur[u][i], at.live), next_part, sum);
+          sum = mfma16x16x32(or_zero(cur[u][i], at.last), last, sum);
           acc[i] = id == now[u] && (u == 0 || now[u] != now[0]) ? sum : acc[i];
         }
       if (!more) return;
@@ -602,7 +613,7 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
     id[j] = row_adapter(a, bk, m);
     todo[j] = (uint32_t)__ballot(id[j] >= 0) & 0xFFFFu;
     if (t < 0 && todo[j]) t = __builtin_amdgcn_readlane(id[j], __builtin_ctz(todo[j]));
-    hp[j] = reinterpret_cast<const uint16_t*>(bk.h) + (int64_t)min(m, a.t.rows - 1) * 2 * bk.rank;
+    hp[j] = reinterpret_cast<const uint16_t*>(bk.h) + (int64_t)min(m, a.t.rows - 1) * 3 * bk.rank;
   }
   if (t < 0) return;
   bool one = true;
@@ -614,23 +625,25 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
     for (int q = 0; q < RankSlot::steps(r8); ++q) {
       const RankSlot at(q, r8);
       const bf16_t* bp = b0 + t * slot + 8 * at.c;
-      bf16x8 hf[WM], lf[WM], bf[WR];
+      bf16x8 hf[WM], bf[WR];
 #pragma unroll
       for (int i = 0; i < WR; ++i) bf[i] = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), at.live);
+      // one part's operands at a time: more leave no registers (256 x 256 tiles spill 127 of them)
+#pragma unroll 1
+      for (int p = 0; p < (r8 < 3 ? r8 : 3); ++p) {
+        const bool live = p == 0 || r8 > 2 ? at.live : at.last;
+        const int part = r8 > 2 ? p : p == 0 ? at.part : 2;
 #pragma unroll
-      for (int j = 0; j < WM; ++j) {
-        hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * at.c + (at.low ? bk.rank : 0)), at.live);
-        if (r8 > 2) lf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * at.c + bk.rank), at.live);
-      }
+        for (int j = 0; j < WM; ++j)
+          hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * at.c + part * bk.rank), live);
+        // an operand that is not there multiplies no B either: 0 times infinity would stay
 #pragma unroll
-      for (int j = 0; j < WM; ++j)
-#pragma unroll
-        for (int i = 0; i < WR; ++i) acc[i][j] = mfma16x16x32(bf[i], hf[j], acc[i][j]);
-      if (r8 > 2)
+        for (int i = 0; i < WR; ++i) bf[i] = or_zero(__builtin_bit_cast(uint4, bf[i]), live);
 #pragma unroll
         for (int j = 0; j < WM; ++j)
 #pragma unroll
-          for (int i = 0; i < WR; ++i) acc[i][j] = mfma16x16x32(bf[i], lf[j], acc[i][j]);
+          for (int i = 0; i < WR; ++i) acc[i][j] = mfma16x16x32(bf[i], hf[j], acc[i][j]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < WR; ++i) settle(acc[i]);
@@ -639,18 +652,18 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
   while (t >= 0) {
 #pragma unroll
     for (int j = 0; j < WM; ++j) todo[j] &= ~(uint32_t)__ballot(id[j] == t);
-    // upper and lower parts of the rank chunks in one row of steps, B loaded for each: both at once, or in turn inside a
+    // the parts of the rank chunks in one row of steps, B loaded for each: several at once, or in turn inside a
     // step, and the sums leave the registers (3 x 333 rows 1280 -> 32768: 294 us against 100)
-    for (int q = 0; q < 2 * r8; q += 4) {
+    for (int q = 0; q < 3 * r8; q += 4) {
       const int s = q + ((threadIdx.x >> 4) & 3);
-      const bool live = s < 2 * r8, low = s >= r8;
-      const int c = live ? (low ? s - r8 : s) : 0;
+      const bool live = s < 3 * r8;
+      const int part = live ? (s >= r8) + (s >= 2 * r8) : 0, c = live ? s - part * r8 : 0;
       const bf16_t* bp = b0 + t * slot + 8 * c;
       bf16x8 hf[WM], bf[WR];
 #pragma unroll
       for (int i = 0; i < WR; ++i) bf[i] = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), live);
 #pragma unroll
-      for (int j = 0; j < WM; ++j) hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * c + (low ? bk.rank : 0)), live);
+      for (int j = 0; j < WM; ++j) hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * c + part * bk.rank), live);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < WR; ++i) {
@@ -818,16 +831,16 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
     }
     __syncthreads();
   };
-  auto operand = [&](int c, bool low) {
+  auto operand = [&](int c, int which) {
     if constexpr (DONE) {
-      const uint16_t* from = reinterpret_cast<const uint16_t*>(bk.h) + (int64_t)min(m, a.t.rows - 1) * 2 * bk.rank;
-      return *reinterpret_cast<const uint4*>(from + 8 * c + (low ? bk.rank : 0));
+      const uint16_t* from = reinterpret_cast<const uint16_t*>(bk.h) + (int64_t)min(m, a.t.rows - 1) * 3 * bk.rank;
+      return *reinterpret_cast<const uint4*>(from + 8 * c + which * bk.rank);
     } else {
       float v[8];
       const float* from = hs[sel] + (l16 & (SUB - 1)) * kStride + 8 * c;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = from[e];
-      return half_of(v, low);
+      return part_of(v, which);
     }
   };
   // Where the workgroup's columns are of both projections its waves may go different ways below: h is summed, and the
@@ -835,19 +848,23 @@ __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
   const bool border = col0 < a.t.r0 && col0 + 64 * WR > a.t.r0;
   if (border) sum_h();
   const bool one = named == 0 || __ballot(id >= 0 && id != __builtin_amdgcn_readlane(id, __builtin_ctz(named | 0x10000u))) == 0;
+  auto both = [&](auto adapters, auto few) {
+    Expand<WR, decltype(adapters)::value, decltype(few)::value> ex(bk, n, at, id, named);
+    sum_parts();
+    if (!border) sum_h();
+    ex.add(acc, operand);
+  };
+  const std::integral_constant<int, 1> single;
+  const std::integral_constant<int, 4> several;
   if (named == 0) {
     sum_parts();
     if (!border) sum_h();
-  } else if (one) {
-    Expand<WR, 1> ex(bk, n, at, id, named);
-    sum_parts();
-    if (!border) sum_h();
-    ex.add(acc, operand);
+  } else if (bk.rank <= 16) {
+    if (one) both(single, std::true_type());
+    else both(several, std::true_type());
   } else {
-    Expand<WR, 4> ex(bk, n, at, id, named);
-    sum_parts();
-    if (!border) sum_h();
-    ex.add(acc, operand);
+    if (one) both(single, std::false_type());
+    else both(several, std::false_type());
   }
   if (m < a.t.rows && l16 < SUB)
 #pragma unroll
@@ -975,10 +992,14 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
 
 static size_t pad256(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
+// h of one bank: three bf16 parts of the finished product, else float32 per chunk of channels
+static size_t h_bytes(const AdapterPlan& p, int rows, int rank) {
+  return pad256((size_t)rows * rank * (p.done ? 3 * sizeof(bf16_t) : p.chunks * sizeof(float)));
+}
+
 static size_t plan_bytes(const AdapterPlan& p, int rows, int n, int rank0, int rank1) {
   const size_t parts = p.direct ? 0 : (size_t)rows * p.splits * n * sizeof(float);
-  return pad256(parts) + pad256((size_t)p.chunks * rows * rank0 * sizeof(float)) +
-         pad256((size_t)p.chunks * rows * rank1 * sizeof(float));
+  return pad256(parts) + h_bytes(p, rows, rank0) + h_bytes(p, rows, rank1);
 }
 
 template <int WR, int WM, int GR, int GM, int BK, int NS, bool DIRECT>
@@ -1138,7 +1159,7 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   a.bank[1].rank = rank1;
   uint8_t* at = static_cast<uint8_t*>(workspace) + (p.direct ? 0 : pad256((size_t)rows * p.splits * n * sizeof(float)));
   a.bank[0].h = reinterpret_cast<float*>(at);
-  a.bank[1].h = reinterpret_cast<float*>(at + pad256((size_t)p.chunks * rows * rank0 * sizeof(float)));
+  a.bank[1].h = reinterpret_cast<float*>(at + h_bytes(p, (int)rows, rank0));
   a.ids = ids;
   a.tokens = tokens;
   a.k = k;

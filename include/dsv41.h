@@ -567,9 +567,10 @@ int dsv41_linear_rows_pair(const void* x, const void* w0, const void* w1, void* 
  * device, rows / tokens of them). For t in [0, slots):
  *   y[m] = x[m] @ w^T + scale[t] * ((x[m] @ a[t]^T) @ b[t]^T),   a [slots, rank, k], b [slots, n, rank],
  * and y[m] = x[m] @ w^T for any other t (-1: no adapter), whatever the slots hold. Sums and the
- * rank-wide intermediate are fp32, in a fixed order: deterministic. No output may overlap
- * an input or the other output, but for what dsv41_adapter_add allows. An infinite value of b gives NaN where the
- * intermediate is zero or, in bf16, short.
+ * rank-wide intermediate are fp32, in a fixed order: deterministic. No output may overlap an input or the
+ * other output, but for what dsv41_adapter_add allows. An infinite value of b gives NaN where scale times
+ * the intermediate is zero or, in dsv41_adapter_linear and _pair, the sum of two bf16 values (it is
+ * multiplied there in three parts of 8 bits, exactly).
  */
 
 /* The adapters' part on top of a projection already computed: out = y + scale (x a^T) b^T, y and out
