@@ -884,6 +884,7 @@ struct AdapterPlan {
   bool done;             // h finished by a launch of its own; else in shares beside the split sums
   int chunk, chunks, sub;
   bool two;              // two of the tile's workgroups fit a CU
+  int rcols, rrows;      // columns and rows per workgroup of the second launch (0 with direct)
 };
 
 // Ranges for decode row counts, near the rule of the decode-row projections: at 33-64 rows the ranges whose wide tiles
@@ -987,6 +988,11 @@ static AdapterPlan adapter_plan(int rows, int k, int n, int n0, int rank) {
     p.chunk = p.done ? k : ((k + parts - 1) / parts + 127) / 128 * 128;
   }
   p.chunks = (k + p.chunk - 1) / p.chunk;
+  // 256 columns per workgroup where that still gives every CU two of them, 64 otherwise; 4 rows where 16 leave CUs
+  // without two (28 rows of 512 outputs at rank 64: 12.6 against 21.5 us; 64 rows of 32768 at rank 16: 26.8 against 18.5)
+  const int64_t mtiles = (rows + 15) / 16, wide = mtiles * ((n + 255) / 256), narrow = mtiles * ((n + 63) / 64);
+  p.rcols = p.direct ? 0 : n0 % 64 == 0 && n % 64 == 0 && wide >= 512 ? 256 : 64;
+  p.rrows = p.direct ? 0 : p.rcols == 256 || p.done || p.sub == 16 || narrow >= 512 ? 16 : 4;
   return p;
 }
 
@@ -1115,6 +1121,17 @@ extern "C" size_t dsv41_adapter_linear_workspace_bytes(int64_t rows, int32_t k, 
   return plan_bytes(adapter_plan((int)rows, k, n0 + n1, n0, rank0 + rank1), (int)rows, n0 + n1, rank0, rank1);
 }
 
+extern "C" int dsv41_adapter_linear_plan(int64_t rows, int32_t k, int32_t n0, int32_t n1, int32_t rank0, int32_t rank1,
+                                         int32_t* plan) {
+  const char* what = "dsv41_adapter_linear_plan";
+  DSV41_REQUIRE(projection_sizes(rows, k, n0, n1, rank0, rank1) && plan, DSV41_E_ARG,
+                "%s: rows %lld, k %d, n %d + %d, rank %d and %d", what, (long long)rows, k, n0, n1, rank0, rank1);
+  const AdapterPlan p = adapter_plan((int)rows, k, n0 + n1, n0, rank0 + rank1);
+  const int32_t v[] = {p.tr, p.tm, p.splits, p.done, p.two ? 2 : 1, p.rcols, p.rrows};
+  for (size_t i = 0; i < sizeof(v) / sizeof(v[0]); ++i) plan[i] = v[i];
+  return 0;
+}
+
 static int run_adapter_linear(const char* what, const void* x, const void* w0, const void* w1, const Bank* banks,
                               const int32_t* ids, void* y0, void* y1, void* workspace, size_t workspace_bytes,
                               int64_t rows, int32_t tokens, int32_t k, int32_t n0, int32_t n1, int32_t dtype,
@@ -1176,18 +1193,14 @@ static int run_adapter_linear(const char* what, const void* x, const void* w0, c
   if (p.done && shrinks) launch_shrink(a, stream);
   launch_projection(a, p, stream);
   if (!p.direct) {
-    auto reduce = [&](auto kernel, int64_t blocks) {
+    auto reduce = [&](auto kernel) {
+      const int64_t blocks = (rows + p.rrows - 1) / p.rrows * ((n + p.rcols - 1) / p.rcols);
       hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, stream, a);
     };
-    // 256 columns per workgroup where that still gives every CU two of them, 64 otherwise; 4 rows where 16 leave CUs
-    // without two (28 rows of 512 outputs at rank 64: 12.6 against 21.5 us; 64 rows of 32768 at rank 16: 26.8 against 18.5)
-    const int64_t wide = (rows + 15) / 16 * ((n + 255) / 256), narrow = (rows + 15) / 16 * ((n + 63) / 64);
-    if (n0 % 64 == 0 && n1 % 64 == 0 && wide >= 512) {
-      if (p.done) reduce(adapter_reduce_kernel<4, true, 16>, wide);
-      else reduce(adapter_reduce_kernel<4, false, 16>, wide);
-    } else if (p.done) reduce(adapter_reduce_kernel<1, true, 16>, narrow);
-    else if (p.sub == 16 || narrow >= 512) reduce(adapter_reduce_kernel<1, false, 16>, narrow);
-    else reduce(adapter_reduce_kernel<1, false, 4>, (rows + 3) / 4 * ((n + 63) / 64));
+    if (p.rcols == 256) p.done ? reduce(adapter_reduce_kernel<4, true, 16>) : reduce(adapter_reduce_kernel<4, false, 16>);
+    else if (p.done) reduce(adapter_reduce_kernel<1, true, 16>);
+    else if (p.rrows == 16) reduce(adapter_reduce_kernel<1, false, 16>);
+    else reduce(adapter_reduce_kernel<1, false, 4>);
   }
   return check_launch(what);
 }

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
+import typing
 
 import torch
 
@@ -121,6 +122,7 @@ _SIGNATURES = {
     "dsv41_adapter_plain": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_adapter_linear_pair": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _sz,
                                   _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _c_p],
+    "dsv41_adapter_linear_plan": [_i64, _i32, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_cache_move_workspace_bytes": [_i32, _i32],
     "dsv41_cache_move": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _c_p, _c_p, _i32, _i32, _i32, _i32, _c_p, _sz, _c_p],
     "dsv41_version": [],
@@ -1349,6 +1351,24 @@ def adapter_add(x, a, b, scale, ids, y, out=None, workspace=None):
 @functools.lru_cache(maxsize=4096)
 def adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1) -> int:
     return lib().dsv41_adapter_linear_workspace_bytes(rows, k, n0, n1, rank0, rank1)
+
+
+class AdapterPlan(typing.NamedTuple):
+    """How an adapter_linear or adapter_linear_pair call of some sizes splits its work: dsv41_adapter_linear_plan."""
+
+    tile_weight_rows: int
+    tile_rows: int
+    ranges: int
+    first_apart: bool
+    per_cu: int
+    sum_columns: int
+    sum_rows: int
+
+
+def adapter_linear_plan(rows, k, n0, n1, rank0, rank1) -> AdapterPlan:
+    plan = (ctypes.c_int32 * 7)()
+    _call("dsv41_adapter_linear_plan", rows, k, n0, n1, rank0, rank1, ctypes.addressof(plan))
+    return AdapterPlan(*plan)._replace(first_apart=bool(plan[3]))
 
 
 def _adapter_weight(name, x, w):

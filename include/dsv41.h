@@ -607,6 +607,12 @@ int dsv41_adapter_linear_pair(const void* x, const void* w0, const void* w1, con
                               int64_t rows, int32_t tokens, int32_t k, int32_t n0, int32_t n1, int32_t rank0,
                               int32_t rank1, int32_t slots0, int32_t slots1, int32_t dtype, hipStream_t stream);
 
+/* How those two calls split their work, for tests and profiles: weight rows and activation rows of a tile, ranges of
+ * the contraction, whether x a^T comes from a launch of its own, workgroups per CU that the tiles leave room for, and
+ * columns and rows per workgroup of the launch that sums the ranges (0 and 0 where the tiles store the result). */
+int dsv41_adapter_linear_plan(int64_t rows, int32_t k, int32_t n0, int32_t n1, int32_t rank0, int32_t rank1,
+                              int32_t plan[7]);
+
 /* ---------------------------------------------------------------- cached sequences --
  */
 
