@@ -597,8 +597,9 @@ struct Expand {
 
 // acc[i][j] += scale (h B^T) for a wave's block of 16 WM rows from m0 on and 16 WR columns from col on, h from the
 // finished first product. One adapter for all rows that are stored: its products go straight into the sums. Several:
-// each multiplies all rows and every lane keeps its own row's, one result beside the sums at a time (they fill the
-// registers).
+// each multiplies the groups of 16 rows that name it and every lane keeps its own row's, one result beside the sums at a
+// time where they fill the registers (110 rows of 32768 outputs under 64 adapters of rank 64: 169 us, 299 when each
+// adapter met all rows, whose operands come through the L2 for every adapter).
 template <int WR, int WM>
 __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const AdapterArgs& a, const Bank& bk, int n, int m0,
                                              int col) {
@@ -616,63 +617,115 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
     hp[j] = reinterpret_cast<const uint16_t*>(bk.h) + (int64_t)min(m, a.t.rows - 1) * 3 * bk.rank;
   }
   if (t < 0) return;
+  // A load behind a branch, which the compiler takes to be on its way still, would have it wait in the tile's loop, for
+  // the copies there too (4,096 rows 5120 -> 1280: 98 us against 82). The copies issued so far have come before the loads.
+  auto drained = [&]() { __builtin_amdgcn_s_waitcnt(0x0F70); };        // vmcnt(0)
   bool one = true;
 #pragma unroll
   for (int j = 0; j < WM; ++j) one = one && __ballot(id[j] != t && m0 + 16 * j + l16 < a.t.rows) == 0;
   const bf16_t* b0 = bk.b + (int64_t)(col + l16) * bk.rank;
   const int64_t slot = (int64_t)n * bk.rank;
+  // an operand that is not there multiplies no B either: 0 times infinity would stay
   if (one) {
     for (int q = 0; q < RankSlot::steps(r8); ++q) {
       const RankSlot at(q, r8);
       const bf16_t* bp = b0 + t * slot + 8 * at.c;
-      bf16x8 hf[WM], bf[WR];
+      bf16x8 bf[WR];
 #pragma unroll
       for (int i = 0; i < WR; ++i) bf[i] = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), at.live);
-      // one part's operands at a time: more leave no registers (256 x 256 tiles spill 127 of them)
+      auto load = [&](bf16x8 (&h)[WM], int part, bool live) {
+#pragma unroll
+        for (int j = 0; j < WM; ++j) h[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * at.c + part * bk.rank), live);
+      };
+      auto multiply = [&](const bf16x8 (&h)[WM]) {
+#pragma unroll
+        for (int j = 0; j < WM; ++j)
+#pragma unroll
+          for (int i = 0; i < WR; ++i) acc[i][j] = mfma16x16x32(bf[i], h[j], acc[i][j]);
+      };
+      auto mask = [&]() {
+#pragma unroll
+        for (int i = 0; i < WR; ++i) bf[i] = or_zero(__builtin_bit_cast(uint4, bf[i]), at.last);
+      };
+      if constexpr (WR * WM <= 20) {
+        bf16x8 h0[WM], h1[WM], h2[WM];
+        load(h0, at.part, at.live);
+        if (r8 > 2) load(h1, 1, at.live);
+        if (r8 > 1) load(h2, 2, at.last);
+        multiply(h0);
+        if (r8 > 2) multiply(h1);
+        if (r8 > 1) {
+          mask();
+          multiply(h2);
+        }
+      } else {
+        bf16x8 h[WM];                                      // one part at a time: all of them spill 127 registers
 #pragma unroll 1
-      for (int p = 0; p < (r8 < 3 ? r8 : 3); ++p) {
-        const bool live = p == 0 || r8 > 2 ? at.live : at.last;
-        const int part = r8 > 2 ? p : p == 0 ? at.part : 2;
-#pragma unroll
-        for (int j = 0; j < WM; ++j)
-          hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * at.c + part * bk.rank), live);
-        // an operand that is not there multiplies no B either: 0 times infinity would stay
-#pragma unroll
-        for (int i = 0; i < WR; ++i) bf[i] = or_zero(__builtin_bit_cast(uint4, bf[i]), live);
-#pragma unroll
-        for (int j = 0; j < WM; ++j)
-#pragma unroll
-          for (int i = 0; i < WR; ++i) acc[i][j] = mfma16x16x32(bf[i], hf[j], acc[i][j]);
+        for (int p = 0; p < (r8 < 3 ? r8 : 3); ++p) {
+          load(h, p == 0 ? at.part : r8 > 2 ? p : 2, p == 0 || r8 > 2 ? at.live : at.last);
+          if (p > 0) mask();                               // the same lanes again beyond 16 ranks
+          multiply(h);
+        }
       }
     }
+    drained();
 #pragma unroll
     for (int i = 0; i < WR; ++i) settle(acc[i]);
     return;
   }
   while (t >= 0) {
+    uint32_t hit[WM];
 #pragma unroll
-    for (int j = 0; j < WM; ++j) todo[j] &= ~(uint32_t)__ballot(id[j] == t);
-    // the parts of the rank chunks in one row of steps, B loaded for each: several at once, or in turn inside a
-    // step, and the sums leave the registers (3 x 333 rows 1280 -> 32768: 294 us against 100)
-    for (int q = 0; q < 3 * r8; q += 4) {
-      const int s = q + ((threadIdx.x >> 4) & 3);
-      const bool live = s < 3 * r8;
-      const int part = live ? (s >= r8) + (s >= 2 * r8) : 0, c = live ? s - part * r8 : 0;
-      const bf16_t* bp = b0 + t * slot + 8 * c;
-      bf16x8 hf[WM], bf[WR];
+    for (int j = 0; j < WM; ++j) {
+      hit[j] = (uint32_t)__ballot(id[j] == t) & 0xFFFFu;
+      todo[j] &= ~hit[j];
+    }
+    // B is loaded once for its parts; 16 rows without this adapter are passed over
+    for (int q = 0; q < RankSlot::steps(r8); ++q) {
+      const RankSlot at(q, r8);
+      const bf16_t* bp = b0 + t * slot + 8 * at.c;
+      bf16x8 bf[WR];
 #pragma unroll
-      for (int i = 0; i < WR; ++i) bf[i] = or_zero(*reinterpret_cast<const uint4*>(bp + (int64_t)16 * i * bk.rank), live);
+      for (int i = 0; i < WR; ++i) bf[i] = ld_bf16x8(bp + (int64_t)16 * i * bk.rank);
+      auto load = [&](uint4 (&h)[WM], int part) {
 #pragma unroll
-      for (int j = 0; j < WM; ++j) hf[j] = or_zero(*reinterpret_cast<const uint4*>(hp[j] + 8 * c + part * bk.rank), live);
-      __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < WM; ++j)
+          if (hit[j]) h[j] = *reinterpret_cast<const uint4*>(hp[j] + 8 * at.c + part * bk.rank);
+      };
+      auto multiply = [&](const uint4 (&h)[WM], bool live) {
 #pragma unroll
-      for (int i = 0; i < WR; ++i) {
+        for (int i = 0; i < WR; ++i) bf[i] = or_zero(__builtin_bit_cast(uint4, bf[i]), live);
 #pragma unroll
         for (int j = 0; j < WM; ++j) {
-          const f32x4 sum = mfma16x16x32(bf[i], hf[j], acc[i][j]);
-          acc[i][j] = id[j] == t ? sum : acc[i][j];
+          if (hit[j] == 0) continue;
+          const bf16x8 hf = or_zero(h[j], live);
+#pragma unroll
+          for (int i = 0; i < WR; ++i) {
+            const f32x4 sum = mfma16x16x32(bf[i], hf, acc[i][j]);
+            acc[i][j] = id[j] == t ? sum : acc[i][j];
+            if constexpr (WR * WM > 8) __builtin_amdgcn_sched_barrier(0);
+          }
         }
-        __builtin_amdgcn_sched_barrier(0);
+      };
+      if constexpr (WR * WM <= 8) {
+        uint4 h0[WM], h1[WM], h2[WM];
+        load(h0, at.part);
+        if (r8 > 2) load(h1, 1);
+        if (r8 > 1) load(h2, 2);
+        multiply(h0, at.live);
+        if (r8 > 2) multiply(h1, at.live);
+        if (r8 > 1) multiply(h2, at.last);
+      } else {
+        uint4 now[WM], next[WM];                           // one part ahead: more leave no registers
+        load(next, at.part);
+#pragma unroll 1
+        for (int p = 0, parts = r8 < 3 ? r8 : 3; p < parts; ++p) {
+#pragma unroll
+          for (int j = 0; j < WM; ++j) now[j] = next[j];
+          if (p + 1 < parts) load(next, r8 > 2 ? p + 1 : 2);
+          __builtin_amdgcn_sched_barrier(0);
+          multiply(now, p == 0 || r8 > 2 ? at.live : at.last);
+        }
       }
     }
     t = -1;
@@ -680,6 +733,7 @@ __device__ __forceinline__ void expand_block(f32x4 (&acc)[WR][WM], const Adapter
     for (int j = 0; j < WM; ++j)
       if (t < 0 && todo[j]) t = __builtin_amdgcn_readlane(id[j], __builtin_ctz(todo[j]));
   }
+  drained();
 }
 
 // The projection's tiles. DIRECT: the adapters' part is added to the float32 sums in registers and the result stored,
