@@ -12,7 +12,7 @@
 //              the ranges and adds the adapters' part. Bound by the weight and, where every row names another adapter,
 //              by B: 64 rows 1280 -> 32768 under 64 adapters of rank 16 (158 MB) 41 us, 3.9 TB/s.
 //   prompts    h first, then the projection's tiles with the adapters' part in their sums when the products begin:
-//              8,192 rows 8192 -> 5120 at rank 64 42 + 580 us, 1.13 PFLOP/s; few tiles split the contraction and end
+//              8,192 rows 8192 -> 5120 at rank 64 594 us, 1.18 PFLOP/s; few tiles split the contraction and end
 //              in the same second launch.
 #include <type_traits>
 
@@ -828,8 +828,9 @@ adapter_tiles_kernel(AdapterArgs a) {
 
 // The contraction ranges' parts summed in order, plus the adapters' part, rounded once: a workgroup per SUB rows (4, each
 // four times in the MFMA, where they may all name different adapters: one load of B behind another for each; else 16) and
-// 64 WR columns, a wave per 16 WR of them (whole blocks of one projection: n0 and n are multiples of 16 WR). The parts
-// and the first adapters' B are on their way while h is summed over its chunks into LDS. DONE: h is the finished first
+// 64 WR columns, a wave per 16 WR of them (whole blocks of one projection: n0 and n are multiples of 16 WR). The first
+// adapters' B and the first range's parts are on their way while h is summed over its chunks into LDS; the other ranges'
+// parts come one behind another. DONE: h is the finished first
 // product, as it lies.
 template <int WR, bool DONE, int SUB>
 __global__ __launch_bounds__(256) void adapter_reduce_kernel(AdapterArgs a) {
