@@ -1,0 +1,70 @@
+// Rows and weights in 8 bits: e4m3fn codes with one power-of-two scale byte (ue8m0, 2^(byte - 127)) per block of 32 channels
+// of a row, or per 32 x 32 block of a weight -- the form the release stores its projections in and quantizes their inputs
+// to (docs/reference/kernel.py:40-124 with round_scale; deepseek_v41_mlx/fakequant.py:83-93).
+#pragma once
+
+#include "mfma.h"
+
+namespace dsv41 {
+
+// |v| as bits: ordered as the magnitudes are, infinity above every number and NaN above infinity, so that a block's
+// maximum also says whether all of it is finite.
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+
+constexpr uint32_t kNotFinite = 0x7F800000u;
+
+// The scale of a block whose largest magnitude has these bits: the smallest power of two s with max(amax, 1e-4) <= 448 s
+// (act_quant's formula; its product with 1/448, rounded to float32, is above a power of two exactly where the quotient
+// is). The byte, and 1 / s. A block that holds an infinity or NaN has the byte 255 (NaN).
+__device__ __forceinline__ uint32_t mx8_scale(uint32_t amax_bits, float& inv) {
+  const float s = pow2_ceil_log2(fmaxf(__uint_as_float(amax_bits), 1e-4f) * (float)(1.0 / 448.0));
+  inv = pow2_inverse(s);
+  return amax_bits >= kNotFinite ? 255u : __float_as_uint(s) >> 23;
+}
+
+// Four values of a block as codes, ties to even (v_cvt_pk_fp8_f32: nothing exceeds 448, so nothing is cut off). v / s is
+// exact as v * (1 / s). Codes under the byte 255 are NaN too.
+__device__ __forceinline__ uint32_t mx8_codes(const float* v, float inv, uint32_t byte) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, w, true);
+  return byte == 255u ? 0x7F7F7F7Fu : (uint32_t)w;
+}
+
+// Largest of a value over an aligned group of `width` lanes.
+__device__ __forceinline__ uint32_t group_max_u(uint32_t v, int width) {
+  for (int o = width >> 1; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  return v;
+}
+
+// Eight consecutive values of a row.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* v) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = a[i];
+      v[4 + i] = b[i];
+    }
+  } else {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float* v) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]),
+                                              pack2_bf16(v[6], v[7]));
+  }
+}
+
+}  // namespace dsv41

@@ -125,6 +125,12 @@ _SIGNATURES = {
     "dsv41_adapter_linear_plan": [_i64, _i32, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_cache_move_workspace_bytes": [_i32, _i32],
     "dsv41_cache_move": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _c_p, _c_p, _i32, _i32, _i32, _i32, _c_p, _sz, _c_p],
+    "dsv41_quant_mx8": [_c_p, _c_p, _c_p, _i64, _i32, _i32, _c_p],
+    "dsv41_quant_mx8_blocks": [_c_p, _c_p, _c_p, _i64, _i32, _i32, _c_p],
+    "dsv41_dequant_mx8": [_c_p, _c_p, _c_p, _i64, _i32, _i32, _i32, _c_p],
+    "dsv41_rmsnorm_mx8": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _i32, _f32, _i32, _c_p],
+    "dsv41_linear_mx8": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i32, _i32, _i32, _i32, _c_p],
+    "dsv41_linear_mx8_pair": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_version": [],
     "dsv41_last_error_string": [],
 }
@@ -1462,6 +1468,197 @@ def adapter_linear_pair(x, w0, w1, bank0, bank1, ids, out0=None, out1=None, work
     _call_on(x.device, name, x.data_ptr(), w0.data_ptr(), w1.data_ptr(), _ptr(a0), _ptr(b0), _ptr(scale0), _ptr(a1),
              _ptr(b1), _ptr(scale1), ids.data_ptr(), out0.data_ptr(), out1.data_ptr(), _ptr(ws), need, rows, tokens, k, n0,
              n1, rank0, rank1, slots0, slots1, BF16, _stream(x))
+    return out0, out1
+
+
+# ---------------------------------------------------------------------------- 8-bit projections
+
+ACTIVATIONS = {"none": 0, None: 0, "relu": 1, "silu": 2, "gelu": 3}
+
+
+def _mx8_rows(name, x):
+    """(rows, channels, dtype code) of a float tensor of whole 32-channel blocks, contiguous and 16-byte aligned."""
+    _gpu(name, x)
+    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
+        raise ValueError(f"{name}: x {tuple(x.shape)} must have whole blocks of 32 channels")
+    _contig(name, x)
+    k = x.shape[-1]
+    return x.numel() // k, k, dtype_code(x, name)
+
+
+def _mx8_out(name, x, codes, scales, shape):
+    """Codes of x's shape and scales of `shape`, a caller's checked and apart from each other and from x."""
+    codes = _out(name, codes, x.shape, torch.uint8, x.device)
+    scales = _out(name, scales, shape, torch.uint8, x.device)
+    _apart(name, codes, "x or the scales", x, scales)
+    _apart(name, scales, "x", x)
+    return codes, scales
+
+
+def quant_mx8(x, codes=None, scales=None):
+    """Rows x [..., k] as e4m3 codes [..., k] and ue8m0 scales [..., k/32], both uint8: dsv41_quant_mx8."""
+    name = "dsv41_quant_mx8"
+    rows, k, code = _mx8_rows(name, x)
+    codes, scales = _mx8_out(name, x, codes, scales, (*x.shape[:-1], k // 32))
+    if rows:
+        _call_on(x.device, name, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, k, code, _stream(x))
+    return codes, scales
+
+
+def quant_mx8_blocks(w, codes=None, scales=None):
+    """A weight w [n, k] as e4m3 codes and ue8m0 scales [ceil(n/32), k/32] of its 32 x 32 blocks: dsv41_quant_mx8_blocks."""
+    name = "dsv41_quant_mx8_blocks"
+    n, k, code = _mx8_rows(name, w)
+    if w.dim() != 2:
+        raise ValueError(f"{name}: w must be [n, k], got {tuple(w.shape)}")
+    codes, scales = _mx8_out(name, w, codes, scales, (-(-n // 32), k // 32))
+    if n:
+        _call_on(w.device, name, w.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, k, code, _stream(w))
+    return codes, scales
+
+
+def mx8_scale_rows(name, codes, scales) -> int:
+    """Rows that one scale of codes [..., k] covers: 1 for scales [..., k/32], 32 for [ceil(n/32), k/32] of codes [n, k]."""
+    shape = tuple(codes.shape)
+    if scales.shape == (*shape[:-1], shape[-1] // 32):
+        return 1
+    if len(shape) == 2 and scales.shape == (-(-shape[0] // 32), shape[1] // 32):
+        return 32
+    raise ValueError(f"{name}: scales {tuple(scales.shape)} do not go with codes {shape}")
+
+
+def _mx8_pair(name, codes, scales):
+    _gpu(name, codes, scales)
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError(f"{name}: codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
+    if codes.dim() < 1 or codes.shape[-1] == 0 or codes.shape[-1] % 32:
+        raise ValueError(f"{name}: codes {tuple(codes.shape)} must have whole blocks of 32 channels")
+    _contig(name, codes, scales)
+    _one_device(name, codes, scales)
+
+
+def dequant_mx8(codes, scales, dtype=torch.bfloat16, out=None):
+    """The values of codes and scales, of rows or of a weight's blocks: dsv41_dequant_mx8."""
+    name = "dsv41_dequant_mx8"
+    _mx8_pair(name, codes, scales)
+    per = mx8_scale_rows(name, codes, scales)
+    if dtype not in _DTYPES:
+        raise ValueError(f"{name}: dtype {dtype} not supported (float32 or bfloat16)")
+    out = _out(name, out, codes.shape, dtype, codes.device)
+    _apart(name, out, "the codes or scales", codes, scales)
+    k = codes.shape[-1]
+    if codes.numel():
+        _call_on(codes.device, name, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.numel() // k, k, per,
+                 _DTYPES[dtype], _stream(codes))
+    return out
+
+
+def rmsnorm_mx8(x, weight, eps, delta=None, rows=True, out=None, codes=None, scales=None):
+    """(y, codes, scales): rmsnorm(x), or with delta add_rmsnorm(x, delta) (x updated in place), and quant_mx8 of it;
+    y is None with rows=False: dsv41_rmsnorm_mx8."""
+    name = "dsv41_rmsnorm_mx8"
+    count, k, code = _mx8_rows(name, x)
+    _gpu(name, weight, delta)
+    _vec(name, "weight", weight, k)
+    _one_device(name, x, weight, delta)
+    if delta is not None:
+        if delta.shape != x.shape or delta.dtype != x.dtype:
+            raise ValueError(f"{name}: delta {tuple(delta.shape)} {delta.dtype} must match x {tuple(x.shape)} {x.dtype}")
+        _contig(name, delta)
+        _apart(name, x, "delta", delta)
+    if out is not None and not rows:
+        raise ValueError(f"{name}: out given, and rows not asked for")
+    given = out is not None or codes is not None or scales is not None
+    codes, scales = _mx8_out(name, x, codes, scales, (*x.shape[:-1], k // 32))
+    if rows:
+        out = _out(name, out, x.shape, x.dtype, x.device)
+    if given:
+        for what, t in (("out", out), ("codes", codes), ("scales", scales)):
+            if t is not None:
+                _apart(f"{name} ({what})", t, "x, delta, the weight or another output", x, delta, weight,
+                       *(o for o in (out, codes, scales) if o is not t))
+    if count:
+        _call_on(x.device, name, x.data_ptr(), _ptr(delta), weight.data_ptr(), _ptr(out), codes.data_ptr(),
+                 scales.data_ptr(), count, k, float(eps), code, _stream(x))
+    return out, codes, scales
+
+
+def _linear_mx8_args(name, x, x_scales, w, w_scales):
+    """(rows, k, n, rows per weight scale) of a product's operands, checked."""
+    try:
+        sizes, (n, k), at = x.shape, w.shape, x.get_device()
+        good = (at == x_scales.get_device() == w.get_device() == w_scales.get_device() and x.is_cuda
+                and x.dtype is x_scales.dtype is w.dtype is w_scales.dtype is torch.uint8
+                and x.is_contiguous() and x_scales.is_contiguous() and w.is_contiguous() and w_scales.is_contiguous()
+                and k and n and k % 32 == 0 and sizes[-1] == k and x_scales.shape == (*sizes[:-1], k // 32))
+    except AttributeError:
+        raise TypeError(f"{name}: codes and scales must be tensors") from None
+    except ValueError:
+        raise ValueError(f"{name}: w must be [n, k], got {tuple(w.shape)}") from None
+    if not good:                               # say what is wrong
+        _mx8_pair(name, x, x_scales)
+        _mx8_pair(name, w, w_scales)
+        _one_device(name, x, w)
+        if sizes[-1] != k or not n:
+            raise ValueError(f"{name}: x {tuple(sizes)} and w {tuple(w.shape)} do not contract")
+        if x_scales.shape != (*sizes[:-1], k // 32):
+            raise ValueError(f"{name}: scales {tuple(x_scales.shape)} do not go with rows {tuple(sizes)}")
+    if w_scales.shape == (n, k // 32):
+        per = 1
+    elif w_scales.shape == (-(-n // 32), k // 32):
+        per = 32
+    else:
+        raise ValueError(f"{name}: scales {tuple(w_scales.shape)} do not go with a weight {tuple(w.shape)}")
+    return x.numel() // k, k, n, per
+
+
+def _linear_mx8_out(name, out, x, n, *operands):
+    """An output of n bf16 channels for x's rows; a caller's must lie apart from the operands."""
+    if out is None:
+        return x.new_empty((*x.shape[:-1], n), dtype=torch.bfloat16)
+    _out(name, out, (*x.shape[:-1], n), torch.bfloat16, x.device)
+    _apart(name, out, "an operand", x, *operands)
+    return out
+
+
+def linear_mx8(x, x_scales, w, w_scales, bias=None, activation=None, residual=None, out=None):
+    """act(x w^T + bias) + residual in bf16 from 8-bit rows and an 8-bit weight (uint8 codes and scales); residual may be
+    out itself: dsv41_linear_mx8."""
+    name = "dsv41_linear_mx8"
+    rows, k, n, per = _linear_mx8_args(name, x, x_scales, w, w_scales)
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{name}: activation {activation!r} is none of {[a for a in ACTIVATIONS if a]}")
+    out = _linear_mx8_out(name, out, x, n, x_scales, w, w_scales, bias)
+    if bias is not None:
+        _vec(name, "bias", bias, n)
+        _one_device(name, x, bias)
+    if residual is not None:
+        if (residual.dtype is not torch.bfloat16 or residual.shape != out.shape or residual.get_device() != x.get_device()
+                or not residual.is_contiguous()):
+            raise ValueError(f"{name}: residual must be contiguous bfloat16 {list(out.shape)} on {x.device}")
+        if residual.data_ptr() != out.data_ptr():      # an element is read and written by one thread: in place it may be
+            _apart(name, out, "the residual (in another place)", residual)
+    if rows:
+        _call_on(x.device, name, x.data_ptr(), x_scales.data_ptr(), w.data_ptr(), w_scales.data_ptr(), _ptr(bias),
+                 _ptr(residual), out.data_ptr(), rows, k, n, per, ACTIVATIONS[activation], _stream(x))
+    return out
+
+
+def linear_mx8_pair(x, x_scales, w0, w0_scales, w1, w1_scales, out0=None, out1=None):
+    """(x w0^T, x w1^T) in one launch: dsv41_linear_mx8_pair."""
+    name = "dsv41_linear_mx8_pair"
+    rows, k, n0, per = _linear_mx8_args(name, x, x_scales, w0, w0_scales)
+    _, _, n1, per1 = _linear_mx8_args(name, x, x_scales, w1, w1_scales)
+    if per != per1 and n0 > 1 and n1 > 1:
+        raise ValueError(f"{name}: scales over {per} rows of one weight and {per1} of the other")
+    given = out0 is not None or out1 is not None
+    out0 = _linear_mx8_out(name, out0, x, n0, x_scales, w0, w0_scales, w1, w1_scales)
+    out1 = _linear_mx8_out(name, out1, x, n1, x_scales, w0, w0_scales, w1, w1_scales)
+    if given:
+        _apart(name, out0, "the other output", out1)
+    if rows:
+        _call_on(x.device, name, x.data_ptr(), x_scales.data_ptr(), w0.data_ptr(), w0_scales.data_ptr(), w1.data_ptr(),
+                 w1_scales.data_ptr(), out0.data_ptr(), out1.data_ptr(), rows, k, n0, n1, max(per, per1), _stream(x))
     return out0, out1
 
 

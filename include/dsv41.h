@@ -613,6 +613,49 @@ int dsv41_adapter_linear_pair(const void* x, const void* w0, const void* w1, con
 int dsv41_adapter_linear_plan(int64_t rows, int32_t k, int32_t n0, int32_t n1, int32_t rank0, int32_t rank1,
                               int32_t plan[7]);
 
+/* ---------------------------------------------------------------- 8-bit projections --
+ *
+ * Rows and weights as e4m3fn codes with ue8m0 scale bytes (value = code * 2^(byte - 127)): codes [rows, k] and scales
+ * [rows, k/32], one per 32 channels of a row, or [ceil(rows/32), k/32], one per 32 x 32 block. A block's scale is the smallest
+ * power of two s with max(|block|, 1e-4) <= 448 s (act_quant with round_scale, docs/reference/kernel.py:40-124); a block
+ * that holds an infinity or NaN gets the byte 255 and NaN codes. k is a multiple of 32, tensors are 16-byte aligned
+ * (scales need no alignment), at most 2^34 values each.
+ */
+
+/* Rows of x [rows, k] (dtype) to codes and scales [rows, k/32] (act_quant without inplace, kernel.py:98-124). */
+int dsv41_quant_mx8(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int32_t k, int32_t dtype,
+                    hipStream_t stream);
+
+/* A weight w [n, k] in 32 x 32 blocks: scales [ceil(n/32), k/32]; the last rows may be a part of a block. */
+int dsv41_quant_mx8_blocks(const void* w, uint8_t* codes, uint8_t* scales, int64_t n, int32_t k, int32_t dtype,
+                           hipStream_t stream);
+
+/* The values of codes as x [rows, k] (dtype); a scale covers scale_rows rows (1 or 32). Exact, but that bf16 rounds
+ * magnitudes under 2^-126. */
+int dsv41_dequant_mx8(const uint8_t* codes, const uint8_t* scales, void* x, int64_t rows, int32_t k,
+                      int32_t scale_rows, int32_t dtype, hipStream_t stream);
+
+/* dsv41_rmsnorm of x [rows, dim], or with delta dsv41_add_rmsnorm (x <- cast(x + delta) first), with the normed rows
+ * in 8 bits: codes [rows, dim] and scales [rows, dim/32] are dsv41_quant_mx8's of the rows rounded to dtype, which also
+ * go to y unless it is NULL. dim at most 16,384, fewer than 2^24 rows. y, codes and scales must not overlap x, delta or
+ * each other. */
+int dsv41_rmsnorm_mx8(void* x, const void* delta, const float* weight, void* y, uint8_t* codes, uint8_t* scales,
+                      int64_t rows, int32_t dim, float eps, int32_t dtype, hipStream_t stream);
+
+/* y [rows, n] (bf16) = act(x w^T + bias) + residual on the block-scaled matrix instructions (fp8_gemm, kernel.py:207-307, with
+ * an epilogue): x codes [rows, k] with scales [rows, k/32], w codes [n, k] with scales [n, k/32] (scale_rows 1) or
+ * [ceil(n/32), k/32] (32); bias [n] float32 or NULL; act 0 none, 1 relu, 2 silu, 3 gelu (by erf); residual [rows, n] bf16 or
+ * NULL, which may be y itself. Float32 accumulation over the instruction's sums of 128 channels (or 64), one rounding. Any n;
+ * rows and k at most 2^20. */
+int dsv41_linear_mx8(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w, const uint8_t* w_scales,
+                     const float* bias, const void* residual, void* y, int32_t rows, int32_t k, int32_t n,
+                     int32_t scale_rows, int32_t act, hipStream_t stream);
+
+/* Two plain products of the same rows in one launch: y0 [rows, n0] and y1 [rows, n1]. */
+int dsv41_linear_mx8_pair(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w0, const uint8_t* w0_scales,
+                          const uint8_t* w1, const uint8_t* w1_scales, void* y0, void* y1, int32_t rows, int32_t k,
+                          int32_t n0, int32_t n1, int32_t scale_rows, hipStream_t stream);
+
 /* ---------------------------------------------------------------- cached sequences --
  */
 
