@@ -6,6 +6,9 @@
 // are exact; the instruction sums its 128 channels with less than float32's 24 bits (within 2^-14 of sum |x w| on values of
 // very unlike size, 1e-5 on normal ones: it drops what lies far below its largest product), and adds that to a float32
 // accumulator. Against the result's one rounding to bf16 (2^-9) that is small, so results are bf16 only.
+#include <type_traits>
+#include <utility>
+
 #include "mx8.h"
 
 namespace dsv41 {
@@ -53,36 +56,64 @@ __device__ __forceinline__ float activated(float v, int act) {
   }
 }
 
-// The epilogue of four consecutive outputs j .. j + 3 of row m (j a multiple of 4), in float32 and rounded once. Rows of a
-// width that is no multiple of 4 are not aligned to four outputs and go one by one.
-__device__ __forceinline__ void finish4(const Mx8Args& a, const Mx8Side& s, int64_t m, int j, f32x4 v) {
+// The epilogue of output j of row m, in float32 and rounded once.
+__device__ __forceinline__ void finish1(const Mx8Args& a, const Mx8Side& s, int64_t m, int j, float v) {
   const int64_t at = m * s.n + j;
-  const bool whole = (s.n & 3) == 0;
-  float r[4] = {0.f, 0.f, 0.f, 0.f};
-  if (a.residual) {
-    if (whole) {
-      const uint2 u = *reinterpret_cast<const uint2*>(a.residual + at);
-      r[0] = bf2f((bf16_t)(u.x & 0xFFFFu)), r[1] = bf2f((bf16_t)(u.x >> 16));
-      r[2] = bf2f((bf16_t)(u.y & 0xFFFFu)), r[3] = bf2f((bf16_t)(u.y >> 16));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (j + e < s.n) r[e] = bf2f(a.residual[at + e]);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    float t = v[e];
-    if (a.bias && j + e < s.n) t += a.bias[j + e];
-    v[e] = activated(t, a.act) + r[e];
-  }
-  if (whole) {
-    *reinterpret_cast<uint2*>(s.y + at) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
-  } else {
+  v = activated(a.bias ? v + a.bias[j] : v, a.act);
+  s.y[at] = f2bf(a.residual ? v + bf2f(a.residual[at]) : v);
+}
+
+// Four consecutive outputs j .. j + 3, j a multiple of 4, some of them perhaps past the row's end. Rows of a width that is
+// no multiple of 4 are not aligned to four outputs and go one by one.
+__device__ __forceinline__ void finish4(const Mx8Args& a, const Mx8Side& s, int64_t m, int j, f32x4 v) {
+  if ((s.n & 3) != 0) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (j + e < s.n) s.y[at + e] = f2bf(v[e]);
+      if (j + e < s.n) finish1(a, s, m, j + e, v[e]);
+    return;
   }
+  const int64_t at = m * s.n + j;
+  if (a.bias) v += *reinterpret_cast<const f32x4*>(a.bias + j);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = activated(v[e], a.act);
+  if (a.residual) {
+    const uint2 u = *reinterpret_cast<const uint2*>(a.residual + at);
+    v[0] += bf2f((bf16_t)(u.x & 0xFFFFu)), v[1] += bf2f((bf16_t)(u.x >> 16));
+    v[2] += bf2f((bf16_t)(u.y & 0xFFFFu)), v[3] += bf2f((bf16_t)(u.y >> 16));
+  }
+  *reinterpret_cast<uint2*>(s.y + at) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+}
+
+// The same for eight outputs inside the row, of which the first `skip` are another's: j a multiple of 8 where the width is.
+__device__ __forceinline__ void finish8(const Mx8Args& a, const Mx8Side& s, int64_t m, int j, int skip, float (&v)[8]) {
+  if ((s.n & 7) != 0 || skip) {
+#pragma unroll 1
+    for (int e = skip; e < 8; ++e) {
+      float t = v[0];
+#pragma unroll
+      for (int q = 1; q < 8; ++q) t = q == e ? v[q] : t;
+      finish1(a, s, m, j + e, t);
+    }
+    return;
+  }
+  const int64_t at = m * s.n + j;
+  if (a.bias) {
+    float b[8];
+    load8(a.bias + j, b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += b[e];
+  }
+  if (a.act != ACT_NONE) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = activated(v[e], a.act);
+  }
+  if (a.residual) {
+    float r[8];
+    load8(a.residual + at, r);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += r[e];
+  }
+  store8(s.y + at, v);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -180,6 +211,285 @@ static bool launch_rows(const Mx8Args& a, hipStream_t stream) {
   return launch_tiles(mx8_rows_kernel<RT, WM, NW>, a, 16 * RT, 16 * WM, 64 * NW, stream);
 }
 
+// ------------------------------------------------------------------ many rows
+
+
+// A tile of 32 WR GR weight rows x 32 WM GM rows of x on GR x GM waves, 128 channels a step, two steps in LDS.
+template <int WR, int WM, int GR, int GM>
+struct Mx8Tile {
+  static constexpr int NWV = GR * GM, NT = 64 * NWV;
+  static constexpr int TR = 32 * WR * GR, TM = 32 * WM * GM, ROWS = TR + TM;
+  static constexpr int STAGE = ROWS * 128;              // both operands' codes of a step
+  static constexpr int SCALES = ROWS * 16;              // their scales of four steps
+  static constexpr int LDS = 2 * (STAGE + SCALES);
+  static constexpr int kW = TR / 8 / NWV, kX = TM / 8 / NWV, kCopies = kW + kX;   // copies of 8 rows per wave and step
+  static_assert(TR % (8 * NWV) == 0 && TM % (8 * NWV) == 0 && NWV % 2 == 0, "whole copies, in turn over the waves");
+};
+
+// dma16_sgpr with a constant added to the LDS offset on the way into M0: one scalar register for all copies of a step.
+template <int OFF>
+__device__ __forceinline__ void dma16_at(uint64_t base, uint32_t voff, uint32_t lds) {
+  asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds), "n"(OFF)
+               : "memory", "m0", "scc");
+}
+
+// f(0), f(1) .. f(N - 1) with compile-time indexes.
+template <typename F, int... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
+// Eight bytes at any address: the scales of a pair of steps.
+typedef __attribute__((ext_vector_type(2), aligned(1))) uint32_t u32x2_any;
+
+// acc += wf xf^T over 64 channels, scale byte OP of both words.
+template <int OP>
+__device__ __forceinline__ f32x16 mfma_mx8(i32x8 wf, i32x8 xf, f32x16 acc, uint32_t ws, uint32_t xs) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf, xf, acc, 0, 0, OP, (int)ws, OP, (int)xs);
+}
+
+template <int WR, int WM, int GR, int GM>
+__global__ __launch_bounds__(64 * GR * GM, (Mx8Tile<WR, WM, GR, GM>::LDS <= 80 * 1024) ? 2 : 1) void mx8_tiles_kernel(
+    Mx8Args a) {
+  using C = Mx8Tile<WR, WM, GR, GM>;
+  __shared__ __align__(16) uint8_t lds[C::LDS];
+  const int total = (int)gridDim.x;
+  // consecutive tiles on one XCD, the weight tile fastest
+  const int unit = total % 8 ? (int)blockIdx.x : ((int)blockIdx.x % 8) * (total / 8) + (int)blockIdx.x / 8;
+  const Mx8Side s = side_of(a, unit % a.tiles);
+  const int mt = unit / a.tiles;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  const int wr = (wave % GR) * 32 * WR, wm = (wave / GR) * 32 * WM;
+  const int kb = a.k / 32, pairs = a.k / 256;           // pairs of steps; the rest of a row is multiplied after them
+
+  // The last tile of a side lies back from its end, whole: rows that the tile before owns are multiplied and not stored.
+  const int own_r = s.tile * C::TR, r0 = min(own_r, s.n - C::TR);
+  const int own_m = mt * C::TM, m0 = min(own_m, a.rows - C::TM);
+
+  // copies of 8 tile rows, in turn over the waves: lane l brings chunk (l % 8) ^ swizzle of row l / 8
+  const uint32_t off = (uint32_t)(lane >> 3) * (uint32_t)a.k + 16u * (uint32_t)((lane & 7) ^ (lane >> 3) ^ (wave & 1));
+  const int uwave = __builtin_amdgcn_readfirstlane(wave);
+  uint64_t wnext = reinterpret_cast<uint64_t>(s.w) + (uint64_t)(r0 + 8 * uwave) * (uint64_t)a.k;   // the next step's channels
+  uint64_t xnext = reinterpret_cast<uint64_t>(a.x) + (uint64_t)(m0 + 8 * uwave) * (uint64_t)a.k;
+  const uint32_t pitch = (uint32_t)(8 * C::NWV) * (uint32_t)a.k;
+  const uint32_t lds0 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(lds_offset(lds) + (uint32_t)(8 * uwave * 128)));
+  int ahead = 2 * pairs - 1;                            // steps left after the next copied one
+  // copies [first, last) of a step into a stage (both stages of the weight's, then both of x's). Past the last step they
+  // bring it once more, which nobody reads: no branch stands between the products.
+  auto issue = [&](auto stage, int first, int last) {
+    constexpr int S = decltype(stage)::value;
+    each([&](auto copy) {
+      constexpr int c = decltype(copy)::value;
+      constexpr int at = c < C::kW ? S * C::TR + 8 * C::NWV * c : 2 * C::TR + S * C::TM + 8 * C::NWV * (c - C::kW);
+      if (c >= first && c < last)
+        dma16_at<at * 128>((c < C::kW ? wnext : xnext) + (uint64_t)(c < C::kW ? c : c - C::kW) * pitch, off, lds0);
+    }, std::make_integer_sequence<int, C::kCopies>{});
+    if (last == C::kCopies) {
+      const uint64_t by = ahead > 0 ? 128 : 0;
+      wnext += by, xnext += by, --ahead;
+    }
+  };
+  // scales: thread t brings rows t, t + NT .. of the tile, four steps at a time
+  constexpr int kS = (C::ROWS + C::NT - 1) / C::NT;
+  const uint8_t* srow[kS];
+#pragma unroll
+  for (int i = 0; i < kS; ++i) {
+    const int r = (int)threadIdx.x + C::NT * i;
+    srow[i] = r < C::TR ? s.ws + (int64_t)((r0 + r) >> a.shift) * kb : a.xs + (int64_t)(m0 + min(r, C::ROWS - 1) - C::TR) * kb;
+  }
+  uint8_t* const sc = lds + 2 * C::STAGE;
+  u32x2_any held[kS][2];
+  // the scales of four steps from step 4 f on; past the last pair they repeat its
+  auto load_scales = [&](int f) {
+#pragma unroll
+    for (int i = 0; i < kS; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) held[i][e] = *reinterpret_cast<const u32x2_any*>(srow[i] + 8 * min(2 * f + e, pairs - 1));
+  };
+  // into LDS as lanes take them: of lane group g and a pair, blocks g, 2 + g, 4 + g, 6 + g (its four half steps) in a word
+  auto store_scales = [&](int f) {
+#pragma unroll
+    for (int i = 0; i < kS; ++i) {
+      const int r = (int)threadIdx.x + C::NT * i;
+      if (C::ROWS % C::NT == 0 || r < C::ROWS)
+        *reinterpret_cast<uint4*>(sc + (f & 1) * C::SCALES + 16 * r) =
+            make_uint4(__builtin_amdgcn_perm(held[i][0][1], held[i][0][0], 0x06040200u),
+                       __builtin_amdgcn_perm(held[i][1][1], held[i][1][0], 0x06040200u),
+                       __builtin_amdgcn_perm(held[i][0][1], held[i][0][0], 0x07050301u),
+                       __builtin_amdgcn_perm(held[i][1][1], held[i][1][0], 0x07050301u));
+    }
+  };
+
+  // LDS addresses of this lane's row in both operands, for each half step and each half of a fragment's 32 bytes, and of its
+  // scale words; everything else is a constant offset. (The empty asm keeps the compiler from making one register per read.)
+  const int swz = (l32 & 7) ^ ((l32 >> 3) & 1);
+  uint32_t wadr[2][2], xadr[2][2];
+  uint32_t wsadr = lds_offset(sc) + (uint32_t)(16 * (wr + l32) + 8 * g), xsadr = lds_offset(sc) + (uint32_t)(16 * (C::TR + wm + l32) + 8 * g);
+  asm volatile("" : "+v"(wsadr), "+v"(xsadr));
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      wadr[h][e] = lds_offset(lds) + (uint32_t)((wr + l32) * 128 + (((4 * h + 2 * e + g) ^ swz) << 4));
+      xadr[h][e] = lds_offset(lds) + (uint32_t)((2 * C::TR + wm + l32) * 128 + (((4 * h + 2 * e + g) ^ swz) << 4));
+      asm volatile("" : "+v"(wadr[h][e]), "+v"(xadr[h][e]));
+    }
+  constexpr int kFrags = WR + WM;
+  auto frag = [&](const uint32_t (&adr)[2], int at) {
+    typedef const __attribute__((address_space(3))) i32x4* lds_i32x4;
+    return join(*(lds_i32x4)(uintptr_t)(adr[0] + (uint32_t)at), *(lds_i32x4)(uintptr_t)(adr[1] + (uint32_t)at));
+  };
+  // fragments [first, last) of a half step: x's, then the weight's in the order of their use
+  auto read = [&](int stage, int half, int first, int last, i32x8 (&wf)[WR], i32x8 (&xf)[WM]) {
+#pragma unroll
+    for (int f = 0; f < kFrags; ++f) {
+      if (f < first || f >= last) continue;
+      if (f < WM) xf[f] = frag(xadr[half], (stage * C::TM + 32 * f) * 128);
+      else wf[f - WM] = frag(wadr[half], (stage * C::TR + 32 * (f - WM)) * 128);
+    }
+  };
+  // the scale words of a pair of steps (bytes: half steps)
+  auto read_scales = [&](int q, uint32_t (&wsc)[WR], uint32_t (&xsc)[WM]) {
+    typedef const __attribute__((address_space(3))) uint32_t* lds_u32;
+    const uint32_t at = (uint32_t)(((q >> 1) & 1) * C::SCALES + 4 * (q & 1));
+#pragma unroll
+    for (int j = 0; j < WM; ++j) xsc[j] = *(lds_u32)(uintptr_t)(xsadr + at + (uint32_t)(16 * 32 * j));
+#pragma unroll
+    for (int i = 0; i < WR; ++i) wsc[i] = *(lds_u32)(uintptr_t)(wsadr + at + (uint32_t)(16 * 32 * i));
+  };
+
+  f32x16 acc[WR][WM];
+#pragma unroll
+  for (int i = 0; i < WR; ++i)
+#pragma unroll
+    for (int j = 0; j < WM; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+  i32x8 w0[WR], x0[WM], w1[WR], x1[WM];
+  uint32_t wsc[WR], xsc[WM], wsn[WR], xsn[WM];
+  // One step at stage P and scale bytes 2 P, 2 P + 1: the second half's fragments are read while the first is multiplied;
+  // at the barrier every wave has read the stage and the next step has landed; then the step after next is copied into
+  // the stage and the next step's first half read while the second half is multiplied.
+  auto step = [&](int q, auto parity) {
+    constexpr int P = decltype(parity)::value;
+#pragma unroll
+    for (int i = 0; i < WR; ++i) {
+      read(P, 1, i * kFrags / WR, (i + 1) * kFrags / WR, w1, x1);
+#pragma unroll
+      for (int j = 0; j < WM; ++j) {
+        acc[i][j] = mfma_mx8<2 * P>(w0[i], x0[j], acc[i][j], wsc[i], xsc[j]);
+        asm volatile("" : "+v"(acc[i][j]));        // in this order: the compiler gathers products of one sum otherwise
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    if (P == 1 && (q & 1) == 0) store_scales((q >> 1) + 1);      // that buffer was last read in an earlier step
+    __syncthreads();
+    if (P == 1 && (q & 1) == 0) load_scales((q >> 1) + 2);
+#pragma unroll
+    for (int i = 0; i < WR; ++i) {
+      issue(parity, i * C::kCopies / WR, (i + 1) * C::kCopies / WR);
+      read(P ^ 1, 0, i * kFrags / WR, (i + 1) * kFrags / WR, w0, x0);
+      if (P == 1 && i == 0) read_scales(q + 1, wsn, xsn);
+#pragma unroll
+      for (int j = 0; j < WM; ++j) {
+        acc[i][j] = mfma_mx8<2 * P + 1>(w1[i], x1[j], acc[i][j], wsc[i], xsc[j]);
+        asm volatile("" : "+v"(acc[i][j]));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (P == 1) {
+#pragma unroll
+      for (int i = 0; i < WR; ++i) wsc[i] = wsn[i];
+#pragma unroll
+      for (int j = 0; j < WM; ++j) xsc[j] = xsn[j];
+    }
+  };
+  if (pairs > 0) {
+    load_scales(0);
+    issue(std::integral_constant<int, 0>{}, 0, C::kCopies);
+    issue(std::integral_constant<int, 1>{}, 0, C::kCopies);
+    store_scales(0);
+    load_scales(1);
+    wait_vmcnt<0>();
+    __syncthreads();
+    read(0, 0, 0, kFrags, w0, x0);
+    read_scales(0, wsc, xsc);
+    for (int q = 0; q < pairs; ++q) {
+      step(q, std::integral_constant<int, 0>{});
+      step(q, std::integral_constant<int, 1>{});
+    }
+    wait_vmcnt<0>();                       // no copy may land in LDS any more
+  }
+
+  // the last channels (fewer than 256), straight from memory
+  for (int at = pairs * 256; at < a.k; at += 64) {
+    const i32x4 zero = {0, 0, 0, 0};
+    const bool lo = at + 16 * g < a.k, hi = at + 32 + 16 * g < a.k, in = at + 32 * g < a.k;
+    i32x8 wf[WR];
+#pragma unroll
+    for (int i = 0; i < WR; ++i) {
+      const int64_t row = r0 + wr + 32 * i + l32;
+      const uint8_t* p = s.w + row * a.k + at + 16 * g;
+      wf[i] = join(lo ? *reinterpret_cast<const i32x4*>(p) : zero, hi ? *reinterpret_cast<const i32x4*>(p + 32) : zero);
+      wsc[i] = in ? s.ws[(row >> a.shift) * kb + at / 32 + g] : 127u;
+    }
+#pragma unroll
+    for (int j = 0; j < WM; ++j) {
+      const int64_t row = m0 + wm + 32 * j + l32;
+      const uint8_t* p = a.x + row * a.k + at + 16 * g;
+      const i32x8 xf = join(lo ? *reinterpret_cast<const i32x4*>(p) : zero,
+                            hi ? *reinterpret_cast<const i32x4*>(p + 32) : zero);
+      const uint32_t xc = in ? a.xs[row * kb + at / 32 + g] : 127u;
+#pragma unroll
+      for (int i = 0; i < WR; ++i) acc[i][j] = mfma_mx8<0>(wf[i], xf, acc[i][j], wsc[i], xc);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < WR; ++i) settle(acc[i]);
+
+  // Lane (g, l32) holds outputs 8 q + 4 g .. + 3 of row l32, q = 0 .. 3. Through LDS (the wave's own part, 32 rows of x at a
+  // time; rows padded by 16 bytes for the banks) a row's outputs come to lie side by side in the wave's lanes: stores of
+  // whole lines, and an epilogue that is written once.
+  constexpr int PITCH = 32 * WR * 4 + 16, LPR = 4 * WR, RPT = 64 / LPR;
+  static_assert(C::NWV * 32 * PITCH <= C::LDS, "the results of 32 rows per wave");
+  uint8_t* const mine = lds + wave * 32 * PITCH;
+#pragma unroll
+  for (int j = 0; j < WM; ++j) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WR; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(mine + l32 * PITCH + (32 * i + 8 * q + 4 * g) * 4) =
+            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __syncthreads();
+    const int n = r0 + wr + 8 * (lane % LPR);
+#pragma unroll 1
+    for (int r = lane / LPR; r < 32; r += RPT) {
+      const int m = m0 + wm + 32 * j + r;
+      if (m < own_m || n + 8 <= own_r) continue;
+      float v[8];
+      load8(reinterpret_cast<const float*>(mine + r * PITCH) + 8 * (lane % LPR), v);
+      finish8(a, s, m, n, max(own_r - n, 0), v);
+    }
+  }
+}
+
+// Whole tiles of this shape are in the call.
+template <int WR, int WM, int GR, int GM>
+static bool holds(const Mx8Args& a) {
+  using C = Mx8Tile<WR, WM, GR, GM>;
+  return a.rows >= C::TM && a.n[0] >= C::TR && (a.n[1] == 0 || a.n[1] >= C::TR);
+}
+
+template <int WR, int WM, int GR, int GM>
+static bool launch_many(const Mx8Args& a, hipStream_t stream) {
+  using C = Mx8Tile<WR, WM, GR, GM>;
+  return launch_tiles(mx8_tiles_kernel<WR, WM, GR, GM>, a, C::TR, C::TM, C::NT, stream);
+}
+
 }  // namespace dsv41
 
 using namespace dsv41;
@@ -200,7 +510,10 @@ static int run_linear_mx8(const char* what, const Mx8Args& a, hipStream_t stream
   bool ok;
   if (a.rows <= 16) ok = launch_rows<2, 1, 8>(a, stream);
   else if (a.rows <= 32) ok = launch_rows<2, 2, 8>(a, stream);
-  else ok = launch_rows<2, 4, 8>(a, stream);
+  else if (a.rows <= 128 || !holds<2, 2, 2, 2>(a)) ok = launch_rows<2, 4, 8>(a, stream);
+  else if (holds<4, 2, 2, 4>(a) && (int64_t)((a.n[0] + 255) / 256 + (a.n[1] + 255) / 256) * ((a.rows + 255) / 256) >= 192)
+    ok = launch_many<4, 2, 2, 4>(a, stream);
+  else ok = launch_many<2, 2, 2, 2>(a, stream);
   DSV41_REQUIRE(ok, DSV41_E_SHAPE, "%s: rows %d, n %d + %d make too many tiles for one launch", what, a.rows, a.n[0], a.n[1]);
   return check_launch(what);
 }

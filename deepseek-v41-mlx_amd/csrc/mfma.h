@@ -36,6 +36,17 @@ __device__ __forceinline__ void settle(f32x4 (&v)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
 }
 
+// settle for 32 x 32 results: a v_mfma_scale_f32_32x32x64_f8f6f4 result takes 16 passes, so twice the states.
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+template <int N>
+__device__ __forceinline__ void settle(f32x16 (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
+  asm volatile("s_nop 15\n\ts_nop 15");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(v[i]));
+}
+
 typedef __attribute__((address_space(3))) void lds_void;
 typedef const __attribute__((address_space(1))) void gbl_void;
 
