@@ -10,6 +10,7 @@
 #include <utility>
 
 #include "mx8.h"
+#include "tiles.h"
 
 namespace dsv41 {
 
@@ -28,8 +29,23 @@ struct Mx8Args {
   const bf16_t* residual;  // [rows, n[0]], or null
   int n[2];              // a second product of the same rows, or 0
   int tiles0, tiles;     // weight tiles of the first product and of both
+  int mtiles, panel;     // tiles of x's rows, and how many of them one weight tile meets before the next
   int rows, k, shift, act;
 };
+
+// This workgroup's weight tile and tile of x's rows. Workgroups go round the eight XCDs; each XCD takes a run of the tiles,
+// in panels of a few tiles of x under all weight tiles, so that what its CUs multiply at a time is a block of both and its
+// L2 brings every line once for several of them.
+struct TileAt {
+  int w, m;
+};
+__device__ __forceinline__ TileAt tile_at(const Mx8Args& a) {
+  const int total = (int)gridDim.x, b = (int)blockIdx.x, xcd = b % 8;
+  const int unit = xcd * (total / 8) + min(xcd, total % 8) + b / 8;
+  const int panel = unit / (a.panel * a.tiles), at = unit - panel * a.panel * a.tiles;
+  const int high = min(a.panel, a.mtiles - panel * a.panel);
+  return TileAt{at / high, panel * a.panel + at % high};
+}
 
 // The part of a call that one workgroup's weight tile belongs to.
 struct Mx8Side {
@@ -119,76 +135,132 @@ __device__ __forceinline__ void finish8(const Mx8Args& a, const Mx8Side& s, int6
 // ------------------------------------------------------------------ few rows
 
 // A workgroup owns 16 RT weight rows and 16 WM rows of x; its NW waves share the channels out, 128 at a time and each a run of
-// its own, and load both operands straight into the instruction's registers: lane (g, l16) holds channels 16 g .. + 15
-// and 64 + 16 g .. + 15 of row l16, and the scale of channels 32 g .. + 31. Their sums meet in LDS, in the waves' order.
-template <int RT, int WM, int NW>
+// its own. Every wave copies both operands into a ring of its own in LDS, D steps deep, and waits for nothing but its copies
+// until the sums meet in LDS, in the waves' order. Copies take whole 128-byte lines, 8 rows per instruction: fragments
+// loaded straight into the instruction's registers touch a row per lane and cost 64 cycles a load (64 rows 5120 -> 1792:
+// 18.3 us).
+template <int RT, int WM, int NW, int D>
+struct Mx8Rows {
+  static constexpr int ROWS = 16 * (RT + WM), COPIES = 2 * (RT + WM);        // of a step, and copies of 8 rows each
+  static constexpr int SEG = 8;                                              // steps whose scales are in LDS at once
+  static constexpr int RING = D * ROWS * 128, WAVE = RING + ROWS * 4 * SEG;
+  static constexpr int SUMS = RT * WM * 1024;                                // a wave's sums
+  static constexpr int LDS = NW * (WAVE > SUMS ? WAVE : SUMS);
+  static_assert(COPIES * D <= 63, "vmcnt holds 6 bits");
+};
+typedef __attribute__((aligned(1))) uint32_t u32_any;
+
+template <int RT, int WM, int NW, int D>
 __global__ __launch_bounds__(64 * NW) void mx8_rows_kernel(Mx8Args a) {
-  __shared__ f32x4 part[NW][RT * WM][64];
-  const Mx8Side s = side_of(a, blockIdx.x % a.tiles);
+  using C = Mx8Rows<RT, WM, NW, D>;
+  __shared__ __align__(16) uint8_t lds[C::LDS];
+  const TileAt at = tile_at(a);
+  const Mx8Side s = side_of(a, at.w);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
-  const int j0 = s.tile * 16 * RT;
-  const int64_t m0 = (int64_t)(blockIdx.x / a.tiles) * 16 * WM;
-  const int kb = a.k / 32, steps = (a.k + 127) / 128, share = (steps + NW - 1) / NW;
+  const int j0 = s.tile * 16 * RT, m0 = at.m * 16 * WM;
+  const int kb = a.k / 32, steps = a.k / 128, share = (steps + NW - 1) / NW;
   const int first = min(wave * share, steps), last = min(first + share, steps);
-  const uint8_t *wp[RT], *wsp[RT], *xp[WM], *xsp[WM];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {           // rows past the end read the last one again and are not stored
-    const int64_t row = min(j0 + 16 * i + l16, s.n - 1);
-    wp[i] = s.w + row * a.k + 16 * g;
-    wsp[i] = s.ws + (row >> a.shift) * kb + g;
-  }
-#pragma unroll
-  for (int j = 0; j < WM; ++j) {
-    const int64_t row = min(m0 + 16 * j + l16, (int64_t)a.rows - 1);
-    xp[j] = a.x + row * a.k + 16 * g;
-    xsp[j] = a.xs + row * kb + g;
-  }
+  const uint8_t* const wt = s.w + (int64_t)j0 * a.k;
+  const uint8_t* const xt = a.x + (int64_t)m0 * a.k;
+  // rows of the tile, the weight's then x's, as rows of their tensors from the tile's first on; rows past the end repeat
+  // the last one and are not stored
+  auto tile_row = [&](int r) { return r < 16 * RT ? min(r, s.n - 1 - j0) : min(r - 16 * RT, a.rows - 1 - m0); };
+  auto scales_of = [&](int r) {
+    return r < 16 * RT ? s.ws + (int64_t)((j0 + tile_row(r)) >> a.shift) * kb : a.xs + (int64_t)(m0 + tile_row(r)) * kb;
+  };
   f32x4 acc[RT][WM];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int j = 0; j < WM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const i32x4 zero = {0, 0, 0, 0};
-  for (int t = first; t < last; ++t) {
-    const int left = a.k - 128 * t;        // channels from here on: the row's last step may have 32, 64 or 96
-    const bool lo = 16 * g < left, hi = 64 + 16 * g < left, sc = 32 * g < left;
-    i32x8 wf[RT], xf[WM];
-    int wsc[RT], xsc[WM];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      wf[i] = join(lo ? *reinterpret_cast<const i32x4*>(wp[i] + 128 * t) : zero,
-                   hi ? *reinterpret_cast<const i32x4*>(wp[i] + 128 * t + 64) : zero);
-      wsc[i] = sc ? wsp[i][4 * t] : 127;
-    }
-#pragma unroll
-    for (int j = 0; j < WM; ++j) {
-      xf[j] = join(lo ? *reinterpret_cast<const i32x4*>(xp[j] + 128 * t) : zero,
-                   hi ? *reinterpret_cast<const i32x4*>(xp[j] + 128 * t + 64) : zero);
-      xsc[j] = sc ? xsp[j][4 * t] : 127;
-    }
+  auto multiply = [&](const i32x8 (&wf)[RT], const i32x8 (&xf)[WM], const uint32_t (&wsc)[RT], const uint32_t (&xsc)[WM]) {
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
       for (int j = 0; j < WM; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[i], xf[j], acc[i][j], 0, 0, 0, wsc[i], 0, xsc[j]);
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[i], xf[j], acc[i][j], 0, 0, 0, (int)wsc[i], 0, (int)xsc[j]);
+  };
+
+  // copies: lane l of copy c brings chunk (l % 8) ^ swizzle of row 8 c + l / 8 (tile_swz<64>: fragment reads without conflicts)
+  uint32_t off[C::COPIES];
+#pragma unroll
+  for (int c = 0; c < C::COPIES; ++c)
+    off[c] = (uint32_t)tile_row(8 * c + (lane >> 3)) * (uint32_t)a.k + 16u * (uint32_t)((lane & 7) ^ (lane >> 3) ^ (c & 1));
+  uint8_t* const mine = lds + wave * C::WAVE;
+  const uint32_t ring = (uint32_t)__builtin_amdgcn_readfirstlane((int)lds_offset(mine));
+  auto issue = [&](int stage, int t) {
+    const uint32_t at = ring + (uint32_t)(stage * C::ROWS * 128);
+#pragma unroll
+    for (int c = 0; c < C::COPIES; ++c)
+      dma16_sgpr(reinterpret_cast<uint64_t>(c < 2 * RT ? wt : xt) + (uint64_t)t * 128, off[c], at + 1024u * c);
+  };
+  const int swz = (l16 & 7) ^ (l16 >> 3);
+  auto frag = [&](int stage, int row) {
+    const uint8_t* p = mine + (stage * C::ROWS + row + l16) * 128;
+    return join(*reinterpret_cast<const i32x4*>(p + ((g ^ swz) << 4)), *reinterpret_cast<const i32x4*>(p + (((4 + g) ^ swz) << 4)));
+  };
+  uint8_t* const sc = mine + C::RING;
+  const int ufirst = __builtin_amdgcn_readfirstlane(first), ulast = __builtin_amdgcn_readfirstlane(last);
+#pragma unroll
+  for (int d = 0; d < D; ++d)
+    if (ufirst + d < ulast) issue(d, ufirst + d);
+  int stage = 0;
+  for (int seg = ufirst; seg < ulast; seg += C::SEG) {
+    // the segment's scales, four of a row and step in a word, the row's words side by side
+#pragma unroll
+    for (int e = 0; e < C::ROWS * C::SEG / 64; ++e) {
+      const int r = (64 * e + lane) / C::SEG, t = min(seg + lane % C::SEG, ulast - 1);
+      reinterpret_cast<uint32_t*>(sc)[64 * e + lane] = *reinterpret_cast<const u32_any*>(scales_of(r) + 4 * t);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const int end = min(seg + C::SEG, ulast);
+    for (int t = seg; t < end; ++t) {
+      wait_copies_deep<C::COPIES, D - 1>(ulast - 1 - t);
+      i32x8 wf[RT], xf[WM];
+      uint32_t wsc[RT], xsc[WM];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) wf[i] = frag(stage, 16 * i), wsc[i] = sc[((16 * i + l16) * C::SEG + t - seg) * 4 + g];
+#pragma unroll
+      for (int j = 0; j < WM; ++j)
+        xf[j] = frag(stage, 16 * (RT + j)), xsc[j] = sc[((16 * (RT + j) + l16) * C::SEG + t - seg) * 4 + g];
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // the stage is in registers
+      if (t + D < ulast) issue(stage, t + D);
+      multiply(wf, xf, wsc, xsc);
+      stage = stage + 1 < D ? stage + 1 : 0;
+    }
+  }
+  const int left = a.k - 128 * steps;      // the last 32, 64 or 96 channels, straight from memory
+  if (left && wave == NW - 1) {
+    const i32x4 zero = {0, 0, 0, 0};
+    const bool lo = 16 * g < left, hi = 64 + 16 * g < left, in = 32 * g < left;
+    i32x8 wf[RT], xf[WM];
+    uint32_t wsc[RT], xsc[WM];
+    auto part = [&](const uint8_t* tensor, int r, i32x8& f, uint32_t& fs) {
+      const uint8_t* p = tensor + (int64_t)tile_row(r) * a.k + 128 * (int64_t)steps + 16 * g;
+      f = join(lo ? *reinterpret_cast<const i32x4*>(p) : zero, hi ? *reinterpret_cast<const i32x4*>(p + 64) : zero);
+      fs = in ? scales_of(r)[4 * steps + g] : 127u;
+    };
+#pragma unroll
+    for (int i = 0; i < RT; ++i) part(wt, 16 * i + l16, wf[i], wsc[i]);
+#pragma unroll
+    for (int j = 0; j < WM; ++j) part(xt, 16 * (RT + j) + l16, xf[j], xsc[j]);
+    multiply(wf, xf, wsc, xsc);
   }
 #pragma unroll
   for (int i = 0; i < RT; ++i) settle(acc[i]);
+  __syncthreads();                         // every wave's ring is done with
+  f32x4* const sums = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int j = 0; j < WM; ++j) part[wave][i * WM + j][lane] = acc[i][j];
+    for (int j = 0; j < WM; ++j) sums[(wave * RT * WM + i * WM + j) * 64 + lane] = acc[i][j];
   __syncthreads();
   for (int q = threadIdx.x; q < RT * WM * 64; q += 64 * NW) {
     const int tile = q >> 6, l = q & 63;
-    f32x4 v = part[0][tile][l];
+    f32x4 v = sums[q];
 #pragma unroll
-    for (int z = 1; z < NW; ++z) {
-      const f32x4 u = part[z][tile][l];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = v[e] + u[e];
-    }
-    const int64_t m = m0 + 16 * (tile % WM) + (l & 15);
+    for (int z = 1; z < NW; ++z) v += sums[z * RT * WM * 64 + q];
+    const int m = m0 + 16 * (tile % WM) + (l & 15);
     const int j = j0 + 16 * (tile / WM) + 4 * (l >> 4);
     if (m < a.rows && j < s.n) finish4(a, s, m, j, v);
   }
@@ -200,15 +272,17 @@ template <typename K>
 static bool launch_tiles(K kernel, Mx8Args a, int tr, int tm, int threads, hipStream_t stream) {
   a.tiles0 = (a.n[0] + tr - 1) / tr;
   a.tiles = a.tiles0 + (a.n[1] + tr - 1) / tr;
-  const int64_t groups = (int64_t)a.tiles * ((a.rows + tm - 1) / tm);
+  a.mtiles = (a.rows + tm - 1) / tm;
+  a.panel = a.mtiles < 8 ? a.mtiles : 8;
+  const int64_t groups = (int64_t)a.tiles * a.mtiles;
   if (groups * threads >= (1ll << 32)) return false;
   hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3((unsigned)threads), 0, stream, a);
   return true;
 }
 
-template <int RT, int WM, int NW>
+template <int RT, int WM, int NW, int D>
 static bool launch_rows(const Mx8Args& a, hipStream_t stream) {
-  return launch_tiles(mx8_rows_kernel<RT, WM, NW>, a, 16 * RT, 16 * WM, 64 * NW, stream);
+  return launch_tiles(mx8_rows_kernel<RT, WM, NW, D>, a, 16 * RT, 16 * WM, 64 * NW, stream);
 }
 
 // ------------------------------------------------------------------ many rows
@@ -221,7 +295,9 @@ struct Mx8Tile {
   static constexpr int TR = 32 * WR * GR, TM = 32 * WM * GM, ROWS = TR + TM;
   static constexpr int STAGE = ROWS * 128;              // both operands' codes of a step
   static constexpr int SCALES = ROWS * 16;              // their scales of four steps
-  static constexpr int LDS = 2 * (STAGE + SCALES);
+  static constexpr int PITCH = 32 * WR * 4 + 16;        // bytes of a row of results on their way out, padded for the banks
+  static constexpr int RING = 2 * (STAGE + SCALES), OUT = NWV * 32 * PITCH;
+  static constexpr int LDS = RING > OUT ? RING : OUT;
   static constexpr int kW = TR / 8 / NWV, kX = TM / 8 / NWV, kCopies = kW + kX;   // copies of 8 rows per wave and step
   static_assert(TR % (8 * NWV) == 0 && TM % (8 * NWV) == 0 && NWV % 2 == 0, "whole copies, in turn over the waves");
 };
@@ -248,23 +324,52 @@ __device__ __forceinline__ f32x16 mfma_mx8(i32x8 wf, i32x8 xf, f32x16 acc, uint3
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf, xf, acc, 0, 0, OP, (int)ws, OP, (int)xs);
 }
 
+// A wave's sums to y. Lane (g, l32) holds outputs 8 q + 4 g .. + 3 of row l32, q = 0 .. 3. Through LDS (the wave's own part,
+// 32 rows of x at a time; rows padded by 16 bytes for the banks) a row's outputs come to lie side by side in the wave's
+// lanes: stores of whole lines, and an epilogue that is written once. n0, m0: the wave's first output and row; outputs
+// before own_r and rows before own_m are another tile's.
+template <typename C, int WR, int WM>
+__device__ __forceinline__ void store_tile(const Mx8Args& a, const Mx8Side& s, uint8_t* lds, const f32x16 (&acc)[WR][WM], int own_r,
+                                           int n0, int own_m, int m0) {
+  constexpr int LPR = 4 * WR, RPT = 64 / LPR;           // lanes per row, rows at a time
+  const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+  uint8_t* const mine = lds + (threadIdx.x >> 6) * 32 * C::PITCH;
+#pragma unroll
+  for (int j = 0; j < WM; ++j) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WR; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f32x4*>(mine + l32 * C::PITCH + (32 * i + 8 * q + 4 * g) * 4) =
+            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __syncthreads();
+    const int n = n0 + 8 * (lane % LPR);
+#pragma unroll 1
+    for (int r = lane / LPR; r < 32; r += RPT) {
+      const int m = m0 + 32 * j + r;
+      if (lane >= LPR * RPT || m < own_m || n + 8 <= own_r) continue;
+      float v[8];
+      load8(reinterpret_cast<const float*>(mine + r * C::PITCH) + 8 * (lane % LPR), v);
+      finish8(a, s, m, n, max(own_r - n, 0), v);
+    }
+  }
+}
+
 template <int WR, int WM, int GR, int GM>
 __global__ __launch_bounds__(64 * GR * GM, (Mx8Tile<WR, WM, GR, GM>::LDS <= 80 * 1024) ? 2 : 1) void mx8_tiles_kernel(
     Mx8Args a) {
   using C = Mx8Tile<WR, WM, GR, GM>;
   __shared__ __align__(16) uint8_t lds[C::LDS];
-  const int total = (int)gridDim.x;
-  // consecutive tiles on one XCD, the weight tile fastest
-  const int unit = total % 8 ? (int)blockIdx.x : ((int)blockIdx.x % 8) * (total / 8) + (int)blockIdx.x / 8;
-  const Mx8Side s = side_of(a, unit % a.tiles);
-  const int mt = unit / a.tiles;
+  const TileAt tile = tile_at(a);
+  const Mx8Side s = side_of(a, tile.w);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wr = (wave % GR) * 32 * WR, wm = (wave / GR) * 32 * WM;
   const int kb = a.k / 32, pairs = a.k / 256;           // pairs of steps; the rest of a row is multiplied after them
 
   // The last tile of a side lies back from its end, whole: rows that the tile before owns are multiplied and not stored.
   const int own_r = s.tile * C::TR, r0 = min(own_r, s.n - C::TR);
-  const int own_m = mt * C::TM, m0 = min(own_m, a.rows - C::TM);
+  const int own_m = tile.m * C::TM, m0 = min(own_m, a.rows - C::TM);
 
   // copies of 8 tile rows, in turn over the waves: lane l brings chunk (l % 8) ^ swizzle of row l / 8
   const uint32_t off = (uint32_t)(lane >> 3) * (uint32_t)a.k + 16u * (uint32_t)((lane & 7) ^ (lane >> 3) ^ (wave & 1));
@@ -449,32 +554,7 @@ __global__ __launch_bounds__(64 * GR * GM, (Mx8Tile<WR, WM, GR, GM>::LDS <= 80 *
 #pragma unroll
   for (int i = 0; i < WR; ++i) settle(acc[i]);
 
-  // Lane (g, l32) holds outputs 8 q + 4 g .. + 3 of row l32, q = 0 .. 3. Through LDS (the wave's own part, 32 rows of x at a
-  // time; rows padded by 16 bytes for the banks) a row's outputs come to lie side by side in the wave's lanes: stores of
-  // whole lines, and an epilogue that is written once.
-  constexpr int PITCH = 32 * WR * 4 + 16, LPR = 4 * WR, RPT = 64 / LPR;
-  static_assert(C::NWV * 32 * PITCH <= C::LDS, "the results of 32 rows per wave");
-  uint8_t* const mine = lds + wave * 32 * PITCH;
-#pragma unroll
-  for (int j = 0; j < WM; ++j) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < WR; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f32x4*>(mine + l32 * PITCH + (32 * i + 8 * q + 4 * g) * 4) =
-            f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-    __syncthreads();
-    const int n = r0 + wr + 8 * (lane % LPR);
-#pragma unroll 1
-    for (int r = lane / LPR; r < 32; r += RPT) {
-      const int m = m0 + wm + 32 * j + r;
-      if (m < own_m || n + 8 <= own_r) continue;
-      float v[8];
-      load8(reinterpret_cast<const float*>(mine + r * PITCH) + 8 * (lane % LPR), v);
-      finish8(a, s, m, n, max(own_r - n, 0), v);
-    }
-  }
+  store_tile<C, WR, WM>(a, s, lds, acc, own_r, r0 + wr, own_m, m0 + wm);
 }
 
 // Whole tiles of this shape are in the call.
@@ -507,13 +587,15 @@ static int run_linear_mx8(const char* what, const Mx8Args& a, hipStream_t stream
                     && (!a.bias || aligned16(a.bias)) && (!a.residual || aligned16(a.residual)),
                 DSV41_E_ARG, "%s: tensors must be 16-byte aligned", what);
   if (a.rows == 0) return 0;
+  const int64_t n = (int64_t)a.n[0] + a.n[1];
+  const bool wide = n >= 4096;
   bool ok;
-  if (a.rows <= 16) ok = launch_rows<2, 1, 8>(a, stream);
-  else if (a.rows <= 32) ok = launch_rows<2, 2, 8>(a, stream);
-  else if (a.rows <= 128 || !holds<2, 2, 2, 2>(a)) ok = launch_rows<2, 4, 8>(a, stream);
-  else if (holds<4, 2, 2, 4>(a) && (int64_t)((a.n[0] + 255) / 256 + (a.n[1] + 255) / 256) * ((a.rows + 255) / 256) >= 192)
-    ok = launch_many<4, 2, 2, 4>(a, stream);
-  else ok = launch_many<2, 2, 2, 2>(a, stream);
+  if (a.rows <= 16) ok = wide ? launch_rows<2, 1, 4, 3>(a, stream) : launch_rows<1, 1, 8, 2>(a, stream);
+  else if (a.rows <= 32) ok = wide ? launch_rows<2, 2, 4, 3>(a, stream) : launch_rows<1, 2, 8, 2>(a, stream);
+  else if (a.rows <= 64) ok = wide ? launch_rows<2, 4, 4, 2>(a, stream) : launch_rows<1, 4, 8, 1>(a, stream);
+  else if (holds<4, 2, 2, 4>(a) && ((n + 255) / 256) * ((a.rows + 255) / 256) >= 192) ok = launch_many<4, 2, 2, 4>(a, stream);
+  else if (holds<2, 2, 2, 2>(a) && ((n + 127) / 128) * ((a.rows + 127) / 128) >= 256) ok = launch_many<2, 2, 2, 2>(a, stream);
+  else ok = launch_rows<4, 4, 8, 1>(a, stream);
   DSV41_REQUIRE(ok, DSV41_E_SHAPE, "%s: rows %d, n %d + %d make too many tiles for one launch", what, a.rows, a.n[0], a.n[1]);
   return check_launch(what);
 }

@@ -1476,20 +1476,31 @@ def adapter_linear_pair(x, w0, w1, bank0, bank1, ids, out0=None, out1=None, work
 ACTIVATIONS = {"none": 0, None: 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
+_U8 = torch.uint8
+
+
 def _mx8_rows(name, x):
-    """(rows, channels, dtype code) of a float tensor of whole 32-channel blocks, contiguous and 16-byte aligned."""
-    _gpu(name, x)
+    """(rows, channels, dtype code, device) of a float tensor of whole 32-channel blocks, contiguous, on the GPU."""
+    try:
+        k = x.shape[-1]
+        if x.is_cuda and k and k % 32 == 0 and x.is_contiguous():
+            return x.numel() // k, k, _DTYPES[x.dtype], x.device
+    except (AttributeError, IndexError, KeyError):
+        pass
+    _gpu(name, x)                              # say what is wrong
     if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
         raise ValueError(f"{name}: x {tuple(x.shape)} must have whole blocks of 32 channels")
     _contig(name, x)
     k = x.shape[-1]
-    return x.numel() // k, k, dtype_code(x, name)
+    return x.numel() // k, k, dtype_code(x, name), x.device
 
 
 def _mx8_out(name, x, codes, scales, shape):
     """Codes of x's shape and scales of `shape`, a caller's checked and apart from each other and from x."""
-    codes = _out(name, codes, x.shape, torch.uint8, x.device)
-    scales = _out(name, scales, shape, torch.uint8, x.device)
+    if codes is None and scales is None:
+        return torch.empty_like(x, dtype=_U8), x.new_empty(shape, dtype=_U8)
+    codes = _out(name, codes, x.shape, _U8, x.device)
+    scales = _out(name, scales, shape, _U8, x.device)
     _apart(name, codes, "x or the scales", x, scales)
     _apart(name, scales, "x", x)
     return codes, scales
@@ -1498,38 +1509,45 @@ def _mx8_out(name, x, codes, scales, shape):
 def quant_mx8(x, codes=None, scales=None):
     """Rows x [..., k] as e4m3 codes [..., k] and ue8m0 scales [..., k/32], both uint8: dsv41_quant_mx8."""
     name = "dsv41_quant_mx8"
-    rows, k, code = _mx8_rows(name, x)
+    rows, k, code, device = _mx8_rows(name, x)
     codes, scales = _mx8_out(name, x, codes, scales, (*x.shape[:-1], k // 32))
     if rows:
-        _call_on(x.device, name, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, k, code, _stream(x))
+        _call_on(device, name, x.data_ptr(), codes.data_ptr(), scales.data_ptr(), rows, k, code, _stream(x))
     return codes, scales
 
 
 def quant_mx8_blocks(w, codes=None, scales=None):
     """A weight w [n, k] as e4m3 codes and ue8m0 scales [ceil(n/32), k/32] of its 32 x 32 blocks: dsv41_quant_mx8_blocks."""
     name = "dsv41_quant_mx8_blocks"
-    n, k, code = _mx8_rows(name, w)
+    n, k, code, device = _mx8_rows(name, w)
     if w.dim() != 2:
         raise ValueError(f"{name}: w must be [n, k], got {tuple(w.shape)}")
     codes, scales = _mx8_out(name, w, codes, scales, (-(-n // 32), k // 32))
     if n:
-        _call_on(w.device, name, w.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, k, code, _stream(w))
+        _call_on(device, name, w.data_ptr(), codes.data_ptr(), scales.data_ptr(), n, k, code, _stream(w))
     return codes, scales
 
 
 def mx8_scale_rows(name, codes, scales) -> int:
     """Rows that one scale of codes [..., k] covers: 1 for scales [..., k/32], 32 for [ceil(n/32), k/32] of codes [n, k]."""
-    shape = tuple(codes.shape)
+    shape = codes.shape
     if scales.shape == (*shape[:-1], shape[-1] // 32):
         return 1
     if len(shape) == 2 and scales.shape == (-(-shape[0] // 32), shape[1] // 32):
         return 32
-    raise ValueError(f"{name}: scales {tuple(scales.shape)} do not go with codes {shape}")
+    raise ValueError(f"{name}: scales {tuple(scales.shape)} do not go with codes {tuple(shape)}")
 
 
 def _mx8_pair(name, codes, scales):
-    _gpu(name, codes, scales)
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+    """Checks that codes and scales are uint8 tensors in one piece on one GPU, of whole blocks."""
+    try:
+        if (codes.dtype is scales.dtype is _U8 and codes.is_cuda and codes.get_device() == scales.get_device()
+                and codes.is_contiguous() and scales.is_contiguous() and codes.shape[-1] and codes.shape[-1] % 32 == 0):
+            return
+    except (AttributeError, IndexError):
+        pass
+    _gpu(name, codes, scales)                  # say what is wrong
+    if codes.dtype != _U8 or scales.dtype != _U8:
         raise ValueError(f"{name}: codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
     if codes.dim() < 1 or codes.shape[-1] == 0 or codes.shape[-1] % 32:
         raise ValueError(f"{name}: codes {tuple(codes.shape)} must have whole blocks of 32 channels")
@@ -1544,12 +1562,16 @@ def dequant_mx8(codes, scales, dtype=torch.bfloat16, out=None):
     per = mx8_scale_rows(name, codes, scales)
     if dtype not in _DTYPES:
         raise ValueError(f"{name}: dtype {dtype} not supported (float32 or bfloat16)")
-    out = _out(name, out, codes.shape, dtype, codes.device)
-    _apart(name, out, "the codes or scales", codes, scales)
+    if out is None:
+        out = torch.empty_like(codes, dtype=dtype)
+    else:
+        _out(name, out, codes.shape, dtype, codes.device)
+        _apart(name, out, "the codes or scales", codes, scales)
     k = codes.shape[-1]
-    if codes.numel():
-        _call_on(codes.device, name, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), codes.numel() // k, k, per,
-                 _DTYPES[dtype], _stream(codes))
+    rows = codes.numel() // k
+    if rows:
+        _call_on(codes.device, name, codes.data_ptr(), scales.data_ptr(), out.data_ptr(), rows, k, per, _DTYPES[dtype],
+                 _stream(codes))
     return out
 
 
@@ -1557,28 +1579,37 @@ def rmsnorm_mx8(x, weight, eps, delta=None, rows=True, out=None, codes=None, sca
     """(y, codes, scales): rmsnorm(x), or with delta add_rmsnorm(x, delta) (x updated in place), and quant_mx8 of it;
     y is None with rows=False: dsv41_rmsnorm_mx8."""
     name = "dsv41_rmsnorm_mx8"
-    count, k, code = _mx8_rows(name, x)
-    _gpu(name, weight, delta)
-    _vec(name, "weight", weight, k)
-    _one_device(name, x, weight, delta)
+    count, k, code, device = _mx8_rows(name, x)
+    if (not isinstance(weight, torch.Tensor) or weight.dtype is not torch.float32 or weight.numel() != k
+            or not weight.is_contiguous() or weight.device != device):
+        _gpu(name, weight)
+        _vec(name, "weight", weight, k)
+        _one_device(name, x, weight)
     if delta is not None:
-        if delta.shape != x.shape or delta.dtype != x.dtype:
-            raise ValueError(f"{name}: delta {tuple(delta.shape)} {delta.dtype} must match x {tuple(x.shape)} {x.dtype}")
-        _contig(name, delta)
+        if (not isinstance(delta, torch.Tensor) or delta.shape != x.shape or delta.dtype != x.dtype
+                or delta.device != device or not delta.is_contiguous()):
+            _gpu(name, delta)
+            _one_device(name, x, delta)
+            if delta.shape != x.shape or delta.dtype != x.dtype:
+                raise ValueError(f"{name}: delta {tuple(delta.shape)} {delta.dtype} must match x {tuple(x.shape)} {x.dtype}")
+            _contig(name, delta)
         _apart(name, x, "delta", delta)
     if out is not None and not rows:
         raise ValueError(f"{name}: out given, and rows not asked for")
-    given = out is not None or codes is not None or scales is not None
-    codes, scales = _mx8_out(name, x, codes, scales, (*x.shape[:-1], k // 32))
-    if rows:
-        out = _out(name, out, x.shape, x.dtype, x.device)
-    if given:
+    if out is codes is scales is None:
+        codes, scales = torch.empty_like(x, dtype=_U8), x.new_empty((*x.shape[:-1], k // 32), dtype=_U8)
+        if rows:
+            out = torch.empty_like(x)
+    else:
+        codes, scales = _mx8_out(name, x, codes, scales, (*x.shape[:-1], k // 32))
+        if rows:
+            out = _out(name, out, x.shape, x.dtype, device)
         for what, t in (("out", out), ("codes", codes), ("scales", scales)):
             if t is not None:
                 _apart(f"{name} ({what})", t, "x, delta, the weight or another output", x, delta, weight,
                        *(o for o in (out, codes, scales) if o is not t))
     if count:
-        _call_on(x.device, name, x.data_ptr(), _ptr(delta), weight.data_ptr(), _ptr(out), codes.data_ptr(),
+        _call_on(device, name, x.data_ptr(), _ptr(delta), weight.data_ptr(), _ptr(out), codes.data_ptr(),
                  scales.data_ptr(), count, k, float(eps), code, _stream(x))
     return out, codes, scales
 

@@ -38,8 +38,9 @@ class Quantized(typing.NamedTuple):
 
 def _no_gradient(*tensors) -> None:
     """Refuses operands of a call that autograd would have to follow, backward or forward."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("8-bit projections are not differentiable: call them under torch.no_grad()")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("8-bit projections are not differentiable: call them under torch.no_grad()")
     if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None
                                                for t in tensors):
         raise ValueError("8-bit projections are not differentiable: their operands may hold no tangent")
@@ -113,15 +114,34 @@ class MX8Linear(torch.nn.Module):
         if isinstance(x, torch.Tensor):
             x = quantize(x)
         _no_gradient(residual, out)
-        return _abi.linear_mx8(x[0], x[1], self.codes, self.scales, self.bias, activation, residual, out)
+        held = self._buffers
+        return _abi.linear_mx8(x[0], x[1], held["codes"], held["scales"], held["bias"], activation, residual, out)
+
+
+_module = torch.nn.modules.module
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+def _only_the_product(lin) -> bool:
+    """Whether calling lin is the product alone: no bias, hooks or forward of its own."""
+    own = lin.__dict__
+    return (type(lin) is MX8Linear and "forward" not in own and own["_buffers"]["bias"] is None
+            and not any(own[h] for h in _HOOKS) and not _module._global_forward_hooks
+            and not _module._global_forward_pre_hooks)
+
+
+def _one_launch(w0, s0, w1, s1) -> bool:
+    """Whether both weights' scales cover as many rows (a weight of one row goes with any)."""
+    n0, n1 = w0.shape[0], w1.shape[0]
+    return n0 == 1 or n1 == 1 or (s0.shape[0] == n0) == (s1.shape[0] == n1)
 
 
 def linear_pair(lin0: MX8Linear, lin1: MX8Linear, x):
-    """(lin0(x), lin1(x)) in one launch where neither has a bias and both have scales of one kind; x as MX8Linear takes it,
-    quantized once."""
+    """(lin0(x), lin1(x)) in one launch where both are plain products (no bias, no hooks) with scales of one kind; x as
+    MX8Linear takes it, quantized once."""
     if isinstance(x, torch.Tensor):
         x = quantize(x)
-    if lin0.bias is None and lin1.bias is None and (
-            (lin0.scales.shape[0] == lin0.out_features) == (lin1.scales.shape[0] == lin1.out_features)):
-        return _abi.linear_mx8_pair(x[0], x[1], lin0.codes, lin0.scales, lin1.codes, lin1.scales)
+    a, b = lin0._buffers, lin1._buffers
+    if _only_the_product(lin0) and _only_the_product(lin1) and _one_launch(a["codes"], a["scales"], b["codes"], b["scales"]):
+        return _abi.linear_mx8_pair(x[0], x[1], a["codes"], a["scales"], b["codes"], b["scales"])
     return lin0(x), lin1(x)
