@@ -37,7 +37,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _abi, fakequant
+from . import _abi, fakequant, mx8
 from .adapters import AdapterBank, adapter_linear, adapter_linear_pair
 from .compressor import Compressor
 from .config import ModelArgs
@@ -46,6 +46,8 @@ from .layers import RMSNorm, yarn_inv_freqs
 
 # the projections that take low-rank adapters (Attention.add_adapters)
 ADAPTED = ("wq_a", "wkv", "wq_b", "wo_b")
+# the projections that can be held in 8 bits (Attention.quantize_projections)
+QUANTIZED = ("wq_a", "wkv", "wq_b", "wo_b")
 
 
 # multiply-adds from which fp32 activations take the batched GEMM for wo_a (the release shape
@@ -121,9 +123,44 @@ class Attention(torch.nn.Module):
             if name not in ADAPTED:
                 raise ValueError(f"adapters go on {ADAPTED}, not on {name!r}")
         for name in names:
+            if isinstance(getattr(self, name), mx8.MX8Linear):
+                raise ValueError(f"{name} is held in 8 bits: adapters go on projections of the activations' type")
+        for name in names:
             w = getattr(self, name).weight
             self.adapters[name] = AdapterBank(slots, w.shape[1], w.shape[0], rank, w.dtype, w.device)
         return self.adapters
+
+    def quantize_projections(self, names=QUANTIZED) -> dict:
+        """Holds the named projections in 8 bits from now on (mx8.MX8Linear.from_linear; one that is stays as it is) and
+        returns them. A checkpoint's own codes and scales go in as attributes: attn.wq_b = MX8Linear(codes, scales)."""
+        for name in names:
+            if name not in QUANTIZED:
+                raise ValueError(f"8 bits are for {QUANTIZED}, not for {name!r}")
+            if name in self.adapters:
+                raise ValueError(f"{name} has adapters: they go on projections of the activations' type")
+            if self.dtype != torch.bfloat16:
+                raise ValueError(f"8-bit projections give bfloat16; this layer's activations are {self.dtype}")
+        for name in names:
+            lin = getattr(self, name)
+            if not isinstance(lin, mx8.MX8Linear):
+                setattr(self, name, mx8.MX8Linear.from_linear(lin))
+        return {name: getattr(self, name) for name in names}
+
+    @property
+    def takes_quantized(self) -> bool:
+        """Whether both projections of the layer's input are in 8 bits: the rows in 8 bits (forward's x8) are used."""
+        return isinstance(self.wq_a, mx8.MX8Linear) and isinstance(self.wkv, mx8.MX8Linear)
+
+    def _input_projections(self, x, x8, banks, ids):
+        """wq_a and wkv of the layer's input, in one launch where they are of one kind."""
+        if self.takes_quantized:
+            return mx8.linear_pair(self.wq_a, self.wkv, mx8.quantize(x) if x8 is None else x8)
+        if isinstance(self.wq_a, mx8.MX8Linear):
+            return self.wq_a(x), adapter_linear(self.wkv, x, banks.get("wkv"), ids)
+        if isinstance(self.wkv, mx8.MX8Linear):
+            return adapter_linear(self.wq_a, x, banks.get("wq_a"), ids), self.wkv(x)
+        # wq_a and wkv read the same rows: one launch at decode row counts
+        return adapter_linear_pair(self.wq_a, self.wkv, x, banks.get("wq_a"), banks.get("wkv"), ids)
 
     def _freqs(self, upto: int):
         """Device (cos, sin) tables covering positions < upto; grown geometrically."""
@@ -166,8 +203,11 @@ class Attention(torch.nn.Module):
         _abi.comp_write(lat, staged, 0, self.ratio, cos[p0:], sin[p0:], rd)
         lc.comp_kv[:lat.shape[0], g0:g0 + lat.shape[1]] = staged
 
-    def forward(self, x: torch.Tensor, start_pos: int, cache, shared) -> torch.Tensor:
-        """x [b, n, dim] (post attn_norm), absolute positions [start_pos, start_pos + n)."""
+    def forward(self, x: torch.Tensor, start_pos: int, cache, shared, x8=None,
+                residual: torch.Tensor | None = None) -> torch.Tensor:
+        """x [b, n, dim] (post attn_norm), absolute positions [start_pos, start_pos + n). x8: x in 8 bits, where the caller
+        has it (mx8.norm_quantize) and takes_quantized. residual: the stream that the output goes on; it is added in wo_b's
+        own launch where wo_b is in 8 bits, in place, and returned."""
         bsz, n, _ = x.shape
         rd = self.rope_head_dim
         end_pos = start_pos + n
@@ -178,11 +218,15 @@ class Attention(torch.nn.Module):
         ids = getattr(shared, "adapter_ids", None)
         banks = self.adapters if ids is not None else {}
 
-        # wq_a and wkv read the same rows: one launch at decode row counts
-        qa, kv_raw = adapter_linear_pair(self.wq_a, self.wkv, x, banks.get("wq_a"), banks.get("wkv"), ids)
+        qa, kv_raw = self._input_projections(x, x8, banks, ids)
         # queries: q's rope tail (attention.py:117) is applied by the attention launch as it loads q
-        qr = self.q_norm(qa)
-        q = adapter_linear(self.wq_b, qr, banks.get("wq_b"), ids, wide_only=True)
+        if isinstance(self.wq_b, mx8.MX8Linear):       # the normed rows themselves are for the indexer alone
+            qr, q8 = mx8.norm_quantize(qa.contiguous(), self.q_norm.weight, self.q_norm.eps,
+                                       rows=bool(self.ratio) and self.is_index_source)
+            q = self.wq_b(q8)
+        else:
+            qr = self.q_norm(qa)
+            q = adapter_linear(self.wq_b, qr, banks.get("wq_b"), ids, wide_only=True)
         q = q.view(bsz, n, self.n_heads, self.head_dim).contiguous()
 
         # this chunk's window KV
@@ -252,7 +296,11 @@ class Attention(torch.nn.Module):
         # grouped block-diagonal wo_a, fp32 sums cast to x's dtype, then wo_b (attention.py:176-179)
         # wo_b at 33-64 rows: 128-row tiles over 4 contraction ranges and their reduce (24.4 + 4.5
         # us at 64 rows against 28.9 us for the library; the 40-layer token 5.748 against 5.78 ms)
-        return adapter_linear(self.wo_b, self._wo_a(o.view(bsz, n, -1), x.dtype), banks.get("wo_b"), ids, wide_only=True)
+        o = self._wo_a(o.view(bsz, n, -1), x.dtype)
+        if isinstance(self.wo_b, mx8.MX8Linear):
+            return self.wo_b(o, residual=residual, out=residual)
+        y = adapter_linear(self.wo_b, o, banks.get("wo_b"), ids, wide_only=True)
+        return y if residual is None else residual.add_(y)
 
     def _wo_a(self, o, out_dtype):
         g, r = self.n_groups, self.o_lora_rank

@@ -8,9 +8,10 @@ The reference's own tests replace that module by ``sys.modules["kernel"] = kerne
     sys.modules["kernel"] = dsv41.kernel
 
 Covered (the attention path): the in-place QAT round trips of ``act_quant`` /
-``fp4_act_quant`` and ``sparse_attn``. The weight GEMMs (``fp8_gemm``, ``fp4_gemm``) and the
-hyper-connection Sinkhorn are outside the attention path and raise, like the reference's
-test stub (tests/kernel_stub.py:127-134).
+``fp4_act_quant``, ``sparse_attn``, and the 8-bit projections: ``act_quant`` to codes and scales and
+``fp8_gemm``, in the release's form (blocks of 32 channels, weight blocks of 32 x 32, ue8m0 scales).
+``fp4_gemm`` (the experts') and the hyper-connection Sinkhorn are outside the attention path and
+raise, like the reference's test stub (tests/kernel_stub.py:127-134).
 """
 
 from __future__ import annotations
@@ -22,12 +23,30 @@ from . import _abi
 
 def act_quant(x: torch.Tensor, block_size: int = 128, scale_fmt=None, scale_dtype=None,
               inplace: bool = False):
-    """kernel.py:98-124. Only the fused quant->dequant form with power-of-two scales
-    (``scale_fmt="ue8m0"``, ``inplace=True``) is on the attention path."""
-    if not inplace or scale_fmt is None:
-        raise NotImplementedError("dsv41.kernel.act_quant implements the inplace ue8m0 round trip only")
-    _abi.fq_fp8_ue8m0(x, block_size, out=x)
-    return x
+    """kernel.py:98-124 with power-of-two scales (``scale_fmt="ue8m0"``): the fused quant->dequant form
+    (``inplace=True``), or the e4m3 codes of x and their e8m0 scales, one per 32 channels, as fp8_gemm takes them."""
+    if scale_fmt is None:
+        raise NotImplementedError("dsv41.kernel.act_quant implements power-of-two (ue8m0) scales only")
+    if inplace:
+        _abi.fq_fp8_ue8m0(x, block_size, out=x)
+        return x
+    if block_size != 32 or scale_dtype not in (None, torch.float8_e8m0fnu):
+        raise NotImplementedError("dsv41.kernel.act_quant gives codes in blocks of 32 with e8m0 scales only")
+    codes, scales = _abi.quant_mx8(x)
+    return codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu)
+
+
+def fp8_gemm(a: torch.Tensor = None, a_s: torch.Tensor = None, b: torch.Tensor = None, b_s: torch.Tensor = None,
+             scale_dtype=torch.float8_e8m0fnu) -> torch.Tensor:
+    """kernel.py:277-307: a [..., k] b [n, k]^T in bf16 from e4m3 codes and e8m0 scales, a_s [..., k/32] and
+    b_s [ceil(n/32), k/32] (act_quant's and the release's blocks)."""
+    if a is None or a_s is None or b is None or b_s is None:
+        raise RuntimeError("fp8_gemm: codes and scales of both operands are needed")
+    if scale_dtype is not torch.float8_e8m0fnu or not a_s.dtype == b_s.dtype == torch.float8_e8m0fnu:
+        raise NotImplementedError("dsv41.kernel.fp8_gemm implements e8m0 scales only")
+    if not a.dtype == b.dtype == torch.float8_e4m3fn:
+        raise ValueError(f"fp8_gemm: operands must be float8_e4m3fn, got {a.dtype} and {b.dtype}")
+    return _abi.linear_mx8(*(t.view(torch.uint8) for t in (a, a_s, b, b_s)))
 
 
 def fp4_act_quant(x: torch.Tensor, block_size: int = 32, inplace: bool = False,
@@ -55,6 +74,5 @@ def _outside_path(name):
     return f
 
 
-fp8_gemm = _outside_path("fp8_gemm")
 fp4_gemm = _outside_path("fp4_gemm")
 hc_split_sinkhorn = _outside_path("hc_split_sinkhorn")

@@ -11,8 +11,8 @@ from __future__ import annotations
 
 import torch
 
-from . import _abi
-from .attention import ADAPTED, Attention
+from . import _abi, mx8
+from .attention import ADAPTED, QUANTIZED, Attention
 from .cache import ModelCache
 from .config import ModelArgs
 from .layers import RMSNorm
@@ -22,6 +22,11 @@ def _fused_norm_ok(h: torch.Tensor) -> bool:
     """dsv41_add_rmsnorm's row shapes: whole 16-byte chunks, at most 1,024 of them per row."""
     per = 16 // h.element_size()
     return h.shape[-1] % per == 0 and h.shape[-1] // per <= 1024 and h.data_ptr() % 16 == 0
+
+
+def _mx8_norm_ok(h: torch.Tensor) -> bool:
+    """dsv41_rmsnorm_mx8's rows: whole blocks of 32 channels, at most 16,384."""
+    return h.shape[-1] % 32 == 0 and h.shape[-1] <= 16384 and h.data_ptr() % 16 == 0
 
 
 class SharedState:
@@ -59,6 +64,10 @@ class AttentionStack(torch.nn.Module):
         """Attention.add_adapters on every layer; the layers' banks."""
         return [attn.add_adapters(slots, rank, names) for attn in self.layers]
 
+    def quantize_projections(self, names=QUANTIZED) -> list:
+        """Attention.quantize_projections on every layer; the layers' 8-bit projections."""
+        return [attn.quantize_projections(names) for attn in self.layers]
+
     def forward(self, h: torch.Tensor, cache: ModelCache, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
         """h [b, n, dim] continues the sequence at cache.offset; advances the cache. adapter_ids [b] int32: every
         sequence's slot in the layers' adapter banks (-1: none)."""
@@ -81,14 +90,22 @@ class AttentionStack(torch.nn.Module):
                 use.index_src_cache = shared.index_src_cache
                 use.topk_idxs = (torch.full_like(shared.topk_idxs, -1)
                                  if shared.topk_idxs is not None else None)
-            if delta is None:
+            x8 = None
+            if getattr(attn, "takes_quantized", False) and _mx8_norm_ok(h):
+                # 8-bit projections: the same norm also gives the rows in 8 bits
+                x, x8 = mx8.norm_quantize(h, norm.weight, norm.eps, None if delta is None else delta.contiguous())
+            elif delta is None:
                 x = norm(h)
             elif _fused_norm_ok(h):
                 x = _abi.add_rmsnorm(h, delta.contiguous(), norm.weight, norm.eps)
             else:
                 h.add_(delta)
                 x = norm(h)
-            delta = attn(x, start_pos, cache, use)
+            given = () if x8 is None else (x8,)
+            if isinstance(getattr(attn, "wo_b", None), mx8.MX8Linear):
+                h, delta = attn(x, start_pos, cache, use, *given, residual=h), None    # added in wo_b's launch, in place
+            else:
+                delta = attn(x, start_pos, cache, use, *given)
         if delta is not None:
             h = h + delta
         cache.offset = start_pos + h.shape[1]

@@ -39,7 +39,11 @@ class Quantized(typing.NamedTuple):
 def _no_gradient(*tensors) -> None:
     """Refuses operands of a call that autograd would have to follow, backward or forward."""
     for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"8-bit projections take tensors, got {type(t).__name__}")
+        if t.requires_grad and torch.is_grad_enabled():
             raise ValueError("8-bit projections are not differentiable: call them under torch.no_grad()")
     if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None
                                                for t in tensors):
