@@ -131,6 +131,7 @@ _SIGNATURES = {
     "dsv41_rmsnorm_mx8": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _i32, _f32, _i32, _c_p],
     "dsv41_linear_mx8": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i32, _i32, _i32, _i32, _c_p],
     "dsv41_linear_mx8_pair": [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i32, _i32, _i32, _i32, _c_p],
+    "dsv41_linear_mx8_plan": [_i32, _i32, _i32, _i32, _c_p],
     "dsv41_version": [],
     "dsv41_last_error_string": [],
 }
@@ -1641,6 +1642,21 @@ def _linear_mx8_args(name, x, x_scales, w, w_scales):
     else:
         raise ValueError(f"{name}: scales {tuple(w_scales.shape)} do not go with a weight {tuple(w.shape)}")
     return x.numel() // k, k, n, per
+
+
+class MX8Plan(typing.NamedTuple):
+    """How a linear_mx8 or linear_mx8_pair call of some sizes splits its work: dsv41_linear_mx8_plan."""
+
+    kernel: int
+    tile_weight_rows: int
+    tile_rows: int
+    ranges: int
+
+
+def linear_mx8_plan(rows, k, n0, n1=0) -> MX8Plan:
+    plan = (ctypes.c_int32 * 4)()
+    _call("dsv41_linear_mx8_plan", rows, k, n0, n1, ctypes.addressof(plan))
+    return MX8Plan(*plan)
 
 
 def _linear_mx8_out(name, out, x, n, *operands):

@@ -1,8 +1,10 @@
 """Rows and weights in 8 bits, the norm that ends in them and their products, against plain implementations in 64 bits.
 
 Codes, scales and read-back values are exact. The products' bound: half a bf16 step of the result (2^-8 of it), and what the
-block-scaled instruction leaves out of a sum of 128 products. That was measured on a lone wave before these tests were
-written: at most 2^-14 of sum |x w| on values spread over 2^+-8, less on others; the bound takes twice that."""
+block-scaled instruction cuts off. It sums eight neighbouring channels at a time: products are lined up at the largest of
+the eight, and of each what lies under 2^-13 of that one's power of two is cut off (one product at 2^0 and another at 2^-13
+in its eight give both, at 2^-14 the first alone; in other eights products count down to float32's last bit). So each of the
+seven others loses less than 2^-13 of the largest, which is at most the eight's sum |x w|: 7 * 2^-13 of it in all."""
 
 from __future__ import annotations
 
@@ -11,12 +13,14 @@ import math
 import pytest
 import torch
 
+from mx8_sizes import SIZES
+
 pytestmark = pytest.mark.gpu
 
 BF, F32 = torch.bfloat16, torch.float32
 E4M3 = torch.float8_e4m3fn
 HALF = {BF: 2.0 ** -8, F32: 2.0 ** -24}      # half a step, relative
-SUMS = 2.0 ** -13                            # the instruction's sums, of sum |x w|
+SUMS = 7 * 2.0 ** -13                        # the instruction's sums, of sum |x w|
 
 
 # ---------------------------------------------------------------------------- the plain forms
@@ -264,6 +268,37 @@ def test_epilogues(gpu, rows, k, n, act, per, bias, residual):
     check(got, *product(x, w), b, act, r)
     if residual:                             # the residual stream in place
         assert lin(x, activation=act, residual=r, out=r) is r and torch.equal(r, got)
+
+
+@pytest.mark.parametrize("rows,k,n", SIZES)
+def test_every_tile_shape(gpu, rows, k, n):
+    """Each shape's products, its last tiles where nothing divides, and its epilogue with the residual stream in place; the
+    same bits on every call."""
+    from dsv41 import mx8
+    x, w = operands(rows, k, n, 28)
+    y, size = product(x, w)
+    lin = mx8.MX8Linear(*w, torch.randn(n, device=gpu))
+    r = spread((rows, n), 29).to(gpu)
+    want = lin(x, activation="silu", residual=r)
+    check(want, y, size, lin.bias, "silu", r)
+    assert lin(x, activation="silu", residual=r, out=r) is r and torch.equal(r, want)
+    got = mx8.MX8Linear(*w)(x)
+    check(got, y, size)
+    assert torch.equal(got, mx8.MX8Linear(*w)(x))
+
+
+def test_scales_off_words(gpu):
+    """Scales that begin anywhere in memory: the kernels that copy them by words are not for those."""
+    from dsv41 import _abi
+    x, w = operands(444, 640, 4912, 27)
+    assert _abi.linear_mx8_plan(444, 640, 4912).kernel == 2
+    want = product(x, w)
+    for off in (1, 2, 3):
+        held = [torch.zeros(t.numel() + 8, dtype=torch.uint8, device=gpu) for t in (x.scales, w.scales)]
+        for i, (h, t) in enumerate(zip(held, (x.scales, w.scales))):
+            h[off * (i + 1):off * (i + 1) + t.numel()] = t.flatten()
+        xs, ws = (h[off * (i + 1):off * (i + 1) + t.numel()].view(t.shape) for i, (h, t) in enumerate(zip(held, (x.scales, w.scales))))
+        check(_abi.linear_mx8(x.codes, xs, w.codes, ws), *want)
 
 
 @pytest.mark.parametrize("rows", [1, 16, 40, 200, 1024])
