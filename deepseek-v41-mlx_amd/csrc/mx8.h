@@ -36,18 +36,14 @@ __device__ __forceinline__ uint32_t group_max_u(uint32_t v, int width) {
   return v;
 }
 
-// Eight consecutive values of a row.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* v) {
-  if constexpr (sizeof(T) == 4) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = a[i];
-      v[4 + i] = b[i];
-    }
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+// Eight consecutive values of a row as they lie in memory. Rounding, maxima and widening work on pairs of bf16 as they are
+// (one instruction for two values instead of six for each: norm over 8,192 rows of 5,120 34.5 -> 29.9 us).
+template <typename T> struct Eight;
+template <> struct Eight<bf16_t> {
+  uint4 u;
+  __device__ __forceinline__ void load(const bf16_t* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(bf16_t* p) const { *reinterpret_cast<uint4*>(p) = u; }
+  __device__ __forceinline__ void get(float* v) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -55,16 +51,55 @@ __device__ __forceinline__ void load8(const T* p, float* v) {
       v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
   }
+  __device__ __forceinline__ void round(const float* v) {
+    u = make_uint4(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7]));
+  }
+  // the largest magnitude, as abs_bits of the float
+  __device__ __forceinline__ uint32_t top() const {
+    typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+    auto mag = [](uint32_t w) { return __builtin_bit_cast(u16x2, w & 0x7FFF7FFFu); };
+    const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(mag(u.x), mag(u.y)),
+                                              __builtin_elementwise_max(mag(u.z), mag(u.w)));
+    return (uint32_t)max(m[0], m[1]) << 16;
+  }
+};
+template <> struct Eight<float> {
+  f32x4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    *reinterpret_cast<f32x4*>(p) = a, *reinterpret_cast<f32x4*>(p + 4) = b;
+  }
+  __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+  }
+  __device__ __forceinline__ void round(const float* v) { a = f32x4{v[0], v[1], v[2], v[3]}, b = f32x4{v[4], v[5], v[6], v[7]}; }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, max(abs_bits(a[i]), abs_bits(b[i])));
+    return m;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* v) {
+  Eight<T> e;
+  e.load(p);
+  e.get(v);
 }
 template <typename T>
 __device__ __forceinline__ void store8(T* p, const float* v) {
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<f32x4*>(p) = f32x4{v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]), pack2_bf16(v[4], v[5]),
-                                              pack2_bf16(v[6], v[7]));
-  }
+  Eight<T> e;
+  e.round(v);
+  e.store(p);
+}
+
+// Eight values of a block as codes.
+__device__ __forceinline__ uint2 mx8_codes8(const float* v, float inv, uint32_t byte) {
+  return make_uint2(mx8_codes(v, inv, byte), mx8_codes(v + 4, inv, byte));
 }
 
 }  // namespace dsv41

@@ -11,14 +11,12 @@ template <typename T>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* x, uint8_t* codes, uint8_t* scales, int64_t blocks) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;      // over the eights of all blocks
   if (i >= blocks * 4) return;                                    // whole groups of four leave together
-  float v[8];
-  load8(x + 8 * i, v);
-  uint32_t m = 0u;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m = max(m, abs_bits(v[e]));
-  float inv;
-  const uint32_t byte = mx8_scale(group_max_u(m, 4), inv);
-  *reinterpret_cast<uint2*>(codes + 8 * i) = make_uint2(mx8_codes(v, inv, byte), mx8_codes(v + 4, inv, byte));
+  Eight<T> e;
+  e.load(x + 8 * i);
+  float v[8], inv;
+  e.get(v);
+  const uint32_t byte = mx8_scale(group_max_u(e.top(), 4), inv);
+  *reinterpret_cast<uint2*>(codes + 8 * i) = mx8_codes8(v, inv, byte);
   if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)byte;
 }
 
@@ -35,24 +33,25 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const T* w, uint8_t* 
   const int c = (int)(unit % strips) * 256 + (lane & 31) * 8;
   if (unit / strips * 32 >= n) return;                            // whole waves
   const bool in = c < k;                                          // whole blocks: k is a multiple of 32
-  float v[16][8];
+  // rows past the end (and lanes past the row) read the last of theirs again: no load waits behind a branch
+  const int64_t last = n - 1;
+  const T* const from = w + (in ? c : k - 8);
+  Eight<T> v[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) v[j].load(from + min(r0 + 2 * j, last) * k);
   uint32_t m = 0u;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    if (in && r0 + 2 * j < n) {
-      load8(w + (r0 + 2 * j) * k + c, v[j]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m = max(m, abs_bits(v[j][e]));
-    }
-  }
-  m = max(group_max_u(m, 4), (uint32_t)__shfl_xor((int)group_max_u(m, 4), 32, 64));
+  for (int j = 0; j < 16; ++j) m = max(m, v[j].top());
+  m = group_max_u(m, 4);
+  m = max(m, (uint32_t)__shfl_xor((int)m, 32, 64));
   float inv;
   const uint32_t byte = mx8_scale(m, inv);
 #pragma unroll
-  for (int j = 0; j < 16; ++j)
-    if (in && r0 + 2 * j < n)
-      *reinterpret_cast<uint2*>(codes + (r0 + 2 * j) * k + c) =
-          make_uint2(mx8_codes(v[j], inv, byte), mx8_codes(v[j] + 4, inv, byte));
+  for (int j = 0; j < 16; ++j) {
+    float f[8];
+    v[j].get(f);
+    if (in && r0 + 2 * j < n) *reinterpret_cast<uint2*>(codes + (r0 + 2 * j) * k + c) = mx8_codes8(f, inv, byte);
+  }
   if (in && (lane & 35) == 0) scales[r0 / 32 * (k / 32) + c / 32] = (uint8_t)byte;
 }
 
@@ -81,56 +80,73 @@ __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* codes, cons
 
 // ------------------------------------------------------------------ norm
 
-// One workgroup per row, C eights of it in each thread's registers: the residual addition first (x <- cast(x + delta),
-// stored back), the norm of the rounded sum with float32 statistics, the normed row rounded to its type -- what the
-// separate operators store between them and what every other reader of the row gets -- and that row's blocks in 8 bits.
-// Bound by memory: every tensor crosses the bus once.
-template <typename T, int C, bool ADD, bool KEEP>
+// The residual addition first (x <- cast(x + delta), stored back), the norm of the rounded sum with float32 statistics, the
+// normed row rounded to its type -- what the separate operators store between them and what every other reader of the row
+// gets -- and that row's blocks in 8 bits. Everything between stays in registers, so every tensor crosses the bus once.
+// Thread t holds eights t, t + 256 .. of a row, C of them. WAVE: one wave takes the row (dim at most 2,048), its lanes four
+// times 64 eights, without a barrier; the sums are added in the order that 256 threads add them in, which is
+// rmsnorm_rows_kernel's, so that bf16 rows come out the same to the last bit.
+template <typename T, int C, bool ADD, bool KEEP, bool WAVE>
 __global__ __launch_bounds__(256) void rmsnorm_mx8_kernel(T* x, const T* delta, const float* w, T* y, uint8_t* codes,
-                                                          uint8_t* scales, int dim, float eps) {
+                                                          uint8_t* scales, int64_t rows, int dim, float eps) {
+  constexpr int SPAN = WAVE ? 64 : 256;
   __shared__ float red[4];
-  const int64_t row = blockIdx.x;
-  const int eights = dim / 8;
-  float v[C][8];
+  const int64_t row = WAVE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+  if (WAVE && row >= rows) return;         // whole waves, which wait for nobody
+  const int t = WAVE ? threadIdx.x & 63 : threadIdx.x, eights = dim / 8;
+  Eight<T> e[C];
+  float part[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+    if (t + SPAN * c < eights) e[c].load(x + row * dim + 8 * (t + SPAN * c));
   float ss = 0.0f;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int ch = threadIdx.x + 256 * c;
-    if (ch < eights) {
-      load8(x + row * dim + 8 * ch, v[c]);
+    if (WAVE) ss = 0.0f;
+    if (t + SPAN * c < eights) {
+      float v[8];
+      e[c].get(v);
       if constexpr (ADD) {
         float d[8];
-        load8(delta + row * dim + 8 * ch, d);
+        load8(delta + row * dim + 8 * (t + SPAN * c), d);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[c][i] = io<T>::rnd(v[c][i] + d[i]);
-        store8(x + row * dim + 8 * ch, v[c]);
+        for (int i = 0; i < 8; ++i) v[i] = v[i] + d[i];
+        e[c].round(v);
+        e[c].get(v);
+        e[c].store(x + row * dim + 8 * (t + SPAN * c));
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += v[c][i] * v[c][i];
+      for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
     }
+    part[c] = ss;
   }
-  ss = group_sum(ss, 64);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
-  __syncthreads();
-  const float tot = (red[0] + red[1]) + (red[2] + red[3]);
+  float tot;
+  if constexpr (WAVE) {
+    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int c = 0; c < C; ++c) r[c] = group_sum(part[c], 64);
+    tot = (r[0] + r[1]) + (r[2] + r[3]);
+  } else {
+    ss = group_sum(ss, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
+    __syncthreads();
+    tot = (red[0] + red[1]) + (red[2] + red[3]);
+  }
   const float inv = 1.0f / sqrtf(tot / (float)dim + eps);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int ch = threadIdx.x + 256 * c;
+    const int ch = t + SPAN * c;
     if (ch < eights) {                     // dim is a multiple of 32: a block's four lanes are here or not
-      float g[8];
+      float g[8], v[8], s;
       load8(w + 8 * ch, g);
-      uint32_t m = 0u;
+      e[c].get(v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[c][i] = io<T>::rnd(g[i] * (v[c][i] * inv));
-        m = max(m, abs_bits(v[c][i]));
-      }
-      if constexpr (KEEP) store8(y + row * dim + 8 * ch, v[c]);
-      float s;
-      const uint32_t byte = mx8_scale(group_max_u(m, 4), s);
-      *reinterpret_cast<uint2*>(codes + row * dim + 8 * ch) =
-          make_uint2(mx8_codes(v[c], s, byte), mx8_codes(v[c] + 4, s, byte));
+      for (int i = 0; i < 8; ++i) v[i] = g[i] * (v[i] * inv);
+      e[c].round(v);
+      e[c].get(v);
+      if constexpr (KEEP) e[c].store(y + row * dim + 8 * ch);
+      const uint32_t byte = mx8_scale(group_max_u(e[c].top(), 4), s);
+      *reinterpret_cast<uint2*>(codes + row * dim + 8 * ch) = mx8_codes8(v, s, byte);
       if ((ch & 3) == 0) scales[row * (dim / 32) + (ch >> 2)] = (uint8_t)byte;
     }
   }
@@ -138,21 +154,29 @@ __global__ __launch_bounds__(256) void rmsnorm_mx8_kernel(T* x, const T* delta, 
 
 constexpr int kNormDim = 16384;            // the widest row: eight eights per thread
 
+// A wave per row where the row fits and rows are many; for a few the row's eights side by side in four waves are quicker.
+constexpr int64_t kWaveRows = 1024;
+
 template <typename T, bool ADD, bool KEEP>
 static void launch_norm(void* x, const void* delta, const float* w, void* y, uint8_t* codes, uint8_t* scales,
                         int64_t rows, int dim, float eps, hipStream_t stream) {
-  const dim3 grid((unsigned)rows), block(256);
   T* xt = static_cast<T*>(x);
   const T* dt = static_cast<const T*>(delta);
   T* yt = static_cast<T*>(y);
-#define DSV41_NORM(C) \
-  hipLaunchKernelGGL((rmsnorm_mx8_kernel<T, C, ADD, KEEP>), grid, block, 0, stream, xt, dt, w, yt, codes, scales, dim, eps)
-  const int per = (dim / 8 + 255) / 256;
-  if (per == 1) DSV41_NORM(1);
-  else if (per == 2) DSV41_NORM(2);
-  else if (per == 3) DSV41_NORM(3);
-  else if (per == 4) DSV41_NORM(4);
-  else DSV41_NORM(8);
+#define DSV41_NORM(C, WAVE)                                                                                             \
+  hipLaunchKernelGGL((rmsnorm_mx8_kernel<T, C, ADD, KEEP, WAVE>), dim3((unsigned)(WAVE ? (rows + 3) / 4 : rows)), dim3(256), 0, \
+                     stream, xt, dt, w, yt, codes, scales, rows, dim, eps)
+  const int eights = dim / 8, per = (eights + 255) / 256;
+  if (per == 1 && rows >= kWaveRows) {
+    if (eights <= 64) DSV41_NORM(1, true);
+    else if (eights <= 128) DSV41_NORM(2, true);
+    else if (eights <= 192) DSV41_NORM(3, true);
+    else DSV41_NORM(4, true);
+  } else if (per == 1) DSV41_NORM(1, false);
+  else if (per == 2) DSV41_NORM(2, false);
+  else if (per == 3) DSV41_NORM(3, false);
+  else if (per == 4) DSV41_NORM(4, false);
+  else DSV41_NORM(8, false);
 #undef DSV41_NORM
 }
 

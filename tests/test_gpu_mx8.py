@@ -200,6 +200,22 @@ def test_norm_gives_the_rows_of_the_separate_norms(gpu):
     assert torch.equal(mx8.norm_quantize(x, w, 1e-6)[0], _abi.rmsnorm(x, w, 1e-6))
 
 
+@pytest.mark.parametrize("rows", [1023, 1024, 2051])
+@pytest.mark.parametrize("dim", [32, 512, 544, 1024, 1280, 1536, 2048, 2080])
+def test_norm_of_many_narrow_rows(gpu, rows, dim):
+    """A wave per row and four waves per row give the rows of the separate norms to the last bit."""
+    from dsv41 import _abi, mx8
+    x, d = spread((rows, dim), 11).to(gpu), spread((rows, dim), 12).to(gpu)
+    w = torch.rand(dim, device=gpu) + 0.5
+    want = _abi.rmsnorm(x, w, 1e-6)
+    y, q = mx8.norm_quantize(x, w, 1e-6)
+    assert torch.equal(y, want) and all(torch.equal(a, b) for a, b in zip(q, mx8.quantize(want)))
+    h = x.clone()
+    want = _abi.add_rmsnorm(h, d, w, 1e-6)
+    y, q = mx8.norm_quantize(x, w, 1e-6, d)
+    assert torch.equal(x, h) and torch.equal(y, want) and all(torch.equal(a, b) for a, b in zip(q, mx8.quantize(want)))
+
+
 def test_norm_of_a_row_that_is_not_finite(gpu):
     from dsv41 import mx8
     x = spread((3, 128), 10).to(gpu)
