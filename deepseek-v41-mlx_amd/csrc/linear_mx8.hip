@@ -126,12 +126,18 @@ __device__ __forceinline__ void finish8(const Mx8Args& a, const Mx8Side& s, int6
     for (int e = 0; e < 8; ++e) v[e] = activated(v[e], a.act);
   }
   if (a.residual) {
+    Eight<bf16_t> held;
+    held.load_past(a.residual + at);
     float r[8];
-    load8(a.residual + at, r);
+    held.get(r);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += r[e];
   }
-  store8(s.y + at, v);
+  // past the L2, which keeps the operands that the other tiles read (999 rows 1280 -> 32768: 59 -> 52 us, 8,192 rows 1280 ->
+  // 8192: 110 -> 93)
+  Eight<bf16_t> out;
+  out.round(v);
+  out.store_past(s.y + at);
 }
 
 // ------------------------------------------------------------------ few rows

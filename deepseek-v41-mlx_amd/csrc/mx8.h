@@ -36,6 +36,19 @@ __device__ __forceinline__ uint32_t group_max_u(uint32_t v, int width) {
   return v;
 }
 
+// Loads and stores of data that this launch does not meet again, which the L2 need not keep. What large calls write then leaves
+// the L2 to what they read: 8,192 rows of 5,120 quantized 24.0 -> 20.6 us, read back 24.8 -> 19.8.
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_once;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_once;
+template <typename V>
+__device__ __forceinline__ V past_l2(const void* p) {
+  return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+}
+template <typename V>
+__device__ __forceinline__ void past_l2(void* p, V v) {
+  __builtin_nontemporal_store(v, reinterpret_cast<V*>(p));
+}
+
 // Eight consecutive values of a row as they lie in memory. Rounding, maxima and widening work on pairs of bf16 as they are
 // (one instruction for two values instead of six for each: norm over 8,192 rows of 5,120 34.5 -> 29.9 us).
 template <typename T> struct Eight;
@@ -43,6 +56,8 @@ template <> struct Eight<bf16_t> {
   uint4 u;
   __device__ __forceinline__ void load(const bf16_t* p) { u = *reinterpret_cast<const uint4*>(p); }
   __device__ __forceinline__ void store(bf16_t* p) const { *reinterpret_cast<uint4*>(p) = u; }
+  __device__ __forceinline__ void load_past(const bf16_t* p) { u = __builtin_bit_cast(uint4, past_l2<u32x4_once>(p)); }
+  __device__ __forceinline__ void store_past(bf16_t* p) const { past_l2(p, __builtin_bit_cast(u32x4_once, u)); }
   __device__ __forceinline__ void get(float* v) const {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -71,6 +86,8 @@ template <> struct Eight<float> {
   __device__ __forceinline__ void store(float* p) const {
     *reinterpret_cast<f32x4*>(p) = a, *reinterpret_cast<f32x4*>(p + 4) = b;
   }
+  __device__ __forceinline__ void load_past(const float* p) { a = past_l2<f32x4>(p), b = past_l2<f32x4>(p + 4); }
+  __device__ __forceinline__ void store_past(float* p) const { past_l2(p, a), past_l2(p + 4, b); }
   __device__ __forceinline__ void get(float* v) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
@@ -90,16 +107,9 @@ __device__ __forceinline__ void load8(const T* p, float* v) {
   e.load(p);
   e.get(v);
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* v) {
-  Eight<T> e;
-  e.round(v);
-  e.store(p);
-}
-
-// Eight values of a block as codes.
-__device__ __forceinline__ uint2 mx8_codes8(const float* v, float inv, uint32_t byte) {
-  return make_uint2(mx8_codes(v, inv, byte), mx8_codes(v + 4, inv, byte));
+// Eight values of a block as codes, to p.
+__device__ __forceinline__ void put_codes8(uint8_t* p, const float* v, float inv, uint32_t byte) {
+  past_l2(p, u32x2_once{mx8_codes(v, inv, byte), mx8_codes(v + 4, inv, byte)});
 }
 
 }  // namespace dsv41

@@ -16,7 +16,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* x, uint8_t* co
   float v[8], inv;
   e.get(v);
   const uint32_t byte = mx8_scale(group_max_u(e.top(), 4), inv);
-  *reinterpret_cast<uint2*>(codes + 8 * i) = mx8_codes8(v, inv, byte);
+  put_codes8(codes + 8 * i, v, inv, byte);
   if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)byte;
 }
 
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(256) void quant_blocks_kernel(const T* w, uint8_t* 
   for (int j = 0; j < 16; ++j) {
     float f[8];
     v[j].get(f);
-    if (in && r0 + 2 * j < n) *reinterpret_cast<uint2*>(codes + (r0 + 2 * j) * k + c) = mx8_codes8(f, inv, byte);
+    if (in && r0 + 2 * j < n) put_codes8(codes + (r0 + 2 * j) * k + c, f, inv, byte);
   }
   if (in && (lane & 35) == 0) scales[r0 / 32 * (k / 32) + c / 32] = (uint8_t)byte;
 }
@@ -75,7 +75,9 @@ __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* codes, cons
   const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8(c.x, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(c.x, true);
   const f2 d = __builtin_amdgcn_cvt_pk_f32_fp8(c.y, false), e = __builtin_amdgcn_cvt_pk_f32_fp8(c.y, true);
   const float v[8] = {a[0] * s, a[1] * s, b[0] * s, b[1] * s, d[0] * s, d[1] * s, e[0] * s, e[1] * s};
-  store8(x + 8 * i, v);
+  Eight<T> out;
+  out.round(v);
+  out.store_past(x + 8 * i);
 }
 
 // ------------------------------------------------------------------ norm
@@ -113,7 +115,7 @@ __global__ __launch_bounds__(256) void rmsnorm_mx8_kernel(T* x, const T* delta, 
         for (int i = 0; i < 8; ++i) v[i] = v[i] + d[i];
         e[c].round(v);
         e[c].get(v);
-        e[c].store(x + row * dim + 8 * (t + SPAN * c));
+        e[c].store_past(x + row * dim + 8 * (t + SPAN * c));
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
@@ -144,9 +146,9 @@ __global__ __launch_bounds__(256) void rmsnorm_mx8_kernel(T* x, const T* delta, 
       for (int i = 0; i < 8; ++i) v[i] = g[i] * (v[i] * inv);
       e[c].round(v);
       e[c].get(v);
-      if constexpr (KEEP) e[c].store(y + row * dim + 8 * ch);
+      if constexpr (KEEP) e[c].store_past(y + row * dim + 8 * ch);
       const uint32_t byte = mx8_scale(group_max_u(e[c].top(), 4), s);
-      *reinterpret_cast<uint2*>(codes + row * dim + 8 * ch) = mx8_codes8(v, s, byte);
+      put_codes8(codes + row * dim + 8 * ch, v, s, byte);
       if ((ch & 3) == 0) scales[row * (dim / 32) + (ch >> 2)] = (uint8_t)byte;
     }
   }
