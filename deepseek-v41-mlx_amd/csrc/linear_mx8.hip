@@ -804,8 +804,9 @@ static bool any(const Mx8Args&) { return true; }
 
 // A tile shape, the ranges of k that one workgroup's waves share out, workgroups that a CU holds, and what a call's time
 // was measured to consist of, in us: 1 + per round of all CUs + per round and step + per tile of a CU + per tile and step +
-// per GB that tiles read + per 10 MB of results. Fitted to 270 to 330 sizes for each (1 to 8,192 rows, k 256 to 8,192, n 512
-// to 32,768): 9 of 10 estimates are within 10 to 15 % of the time.
+// per GB that tiles read + per 10 MB of results. Fitted to 230 to 330 sizes for each (1 to 8,192 rows, k 256 to 8,192, n 512
+// to 32,768): 9 of 10 estimates are within 10 to 15 % of the time (rows of odd widths, stored by the value, take up to a third
+// longer than estimated, whatever the shape).
 struct Mx8Shape {
   int kind, tr, tm, ranges, held;      // kind 0: few rows, 1: tiles, 2: tiles over a ring
   float us[7];
@@ -813,26 +814,26 @@ struct Mx8Shape {
   bool (*takes)(const Mx8Args&);
 };
 static const Mx8Shape kShapes[] = {
-    {0, 16, 16, 8, 2, {2.49f, 0.f, 0.215f, 0.649f, 0.0465f, 20.6f, 0.f}, launch_rows<1, 1, 8, 2>, any},
-    {0, 32, 16, 8, 1, {1.74f, 1.47f, 0.f, 0.f, 0.414f, 16.4f, 0.f}, launch_rows<2, 1, 8, 2>, any},
-    {0, 32, 16, 2, 5, {2.62f, 0.f, 0.228f, 0.251f, 0.0039f, 22.9f, 0.f}, launch_rows<2, 1, 2, 2>, any},
-    {0, 32, 32, 4, 1, {1.67f, 1.56f, 0.359f, 0.f, 0.f, 6.84f, 6.17f}, launch_rows<2, 2, 4, 3>, any},
-    {0, 32, 48, 8, 1, {1.99f, 1.32f, 0.773f, 0.f, 0.f, 10.f, 5.74f}, launch_rows<2, 3, 8, 1>, any},
-    {0, 64, 32, 8, 1, {2.02f, 1.45f, 0.98f, 0.f, 0.f, 10.7f, 3.86f}, launch_rows<4, 2, 8, 1>, any},
-    {0, 64, 64, 8, 1, {2.24f, 2.02f, 1.4f, 0.f, 0.f, 7.99f, 3.58f}, launch_rows<4, 4, 8, 1>, any},
-    {0, 64, 96, 4, 1, {2.21f, 3.71f, 0.f, 0.f, 0.975f, 0.143f, 4.09f}, launch_rows<4, 6, 4, 1>, any},
-    {1, 64, 64, 1, 4, {2.45f, 0.f, 0.361f, 0.688f, 0.0474f, 19.1f, 0.702f}, launch_many<1, 1, 2, 2>, holds<1, 1, 2, 2>},
-    {1, 128, 128, 1, 2, {3.43f, 0.63f, 0.403f, 0.721f, 0.269f, 2.14f, 2.07f}, launch_many<2, 2, 2, 2>, holds<2, 2, 2, 2>},
-    {1, 192, 256, 1, 1, {2.02f, 5.88f, 0.f, 0.f, 1.07f, 8.53f, 1.32f}, launch_many<3, 2, 2, 4>, holds<3, 2, 2, 4>},
-    {1, 256, 256, 1, 1, {0.967f, 0.f, 1.18f, 8.13f, 0.f, 16.8f, 1.09f}, launch_many<4, 2, 2, 4>, holds<4, 2, 2, 4>},
-    {2, 64, 64, 1, 2, {2.78f, 0.f, 0.091f, 0.812f, 0.124f, 9.14f, 0.878f}, launch_ring<1, 1, 2, 2, 4>, holds_ring<1, 1, 2, 2>},
-    {2, 128, 64, 1, 1, {2.1f, 1.7f, 0.321f, 0.f, 0.f, 7.29f, 2.12f}, launch_ring<1, 1, 4, 2, 4>, holds_ring<1, 1, 4, 2>},
-    {2, 128, 128, 1, 1, {2.01f, 2.85f, 0.414f, 0.f, 0.f, 16.8f, 1.29f}, launch_ring<2, 1, 2, 4, 4>, holds_ring<2, 1, 2, 4>},
-    {2, 256, 128, 1, 1, {1.52f, 0.f, 0.634f, 5.08f, 0.f, 18.2f, 1.26f}, launch_ring<2, 2, 4, 2, 3>, holds_ring<2, 2, 4, 2>},
+    {0, 16, 16, 8, 2, {2.51f, 0.f, 0.207f, 0.65f, 0.0511f, 20.3f, 0.f}, launch_rows<1, 1, 8, 2>, any},
+    {0, 32, 16, 8, 1, {1.75f, 1.48f, 0.f, 0.f, 0.406f, 17.2f, 0.f}, launch_rows<2, 1, 8, 2>, any},
+    {0, 32, 16, 2, 5, {2.62f, 0.f, 0.231f, 0.262f, 0.f, 23.6f, 0.f}, launch_rows<2, 1, 2, 2>, any},
+    {0, 32, 32, 4, 1, {1.69f, 1.52f, 0.359f, 0.f, 0.f, 6.63f, 6.97f}, launch_rows<2, 2, 4, 3>, any},
+    {0, 32, 48, 8, 1, {2.01f, 1.27f, 0.f, 0.f, 0.78f, 9.31f, 6.4f}, launch_rows<2, 3, 8, 1>, any},
+    {0, 64, 32, 8, 1, {2.05f, 1.39f, 0.985f, 0.f, 0.f, 10.3f, 4.56f}, launch_rows<4, 2, 8, 1>, any},
+    {0, 64, 64, 8, 1, {2.2f, 2.04f, 0.f, 0.f, 1.41f, 6.97f, 3.67f}, launch_rows<4, 4, 8, 1>, any},
+    {0, 64, 96, 4, 1, {2.2f, 3.75f, 0.f, 0.f, 0.967f, 0.f, 3.94f}, launch_rows<4, 6, 4, 1>, any},
+    {1, 64, 64, 1, 4, {2.78f, 0.f, 0.354f, 0.652f, 0.0508f, 17.1f, 0.f}, launch_many<1, 1, 2, 2>, holds<1, 1, 2, 2>},
+    {1, 128, 128, 1, 2, {4.15f, 0.2f, 0.408f, 0.7f, 0.256f, 1.24f, 1.31f}, launch_many<2, 2, 2, 2>, holds<2, 2, 2, 2>},
+    {1, 192, 256, 1, 1, {2.28f, 5.7f, 1.07f, 0.f, 0.f, 2.13f, 0.695f}, launch_many<3, 2, 2, 4>, holds<3, 2, 2, 4>},
+    {1, 256, 256, 1, 1, {1.47f, 0.f, 1.19f, 7.72f, 0.f, 9.86f, 0.456f}, launch_many<4, 2, 2, 4>, holds<4, 2, 2, 4>},
+    {2, 64, 64, 1, 2, {3.19f, 0.f, 0.095f, 0.493f, 0.123f, 7.7f, 1.25f}, launch_ring<1, 1, 2, 2, 4>, holds_ring<1, 1, 2, 2>},
+    {2, 128, 64, 1, 1, {2.91f, 0.925f, 0.324f, 0.f, 0.f, 5.31f, 2.57f}, launch_ring<1, 1, 4, 2, 4>, holds_ring<1, 1, 4, 2>},
+    {2, 128, 128, 1, 1, {2.99f, 1.93f, 0.f, 0.f, 0.424f, 11.f, 1.02f}, launch_ring<2, 1, 2, 4, 4>, holds_ring<2, 1, 2, 4>},
+    {2, 256, 128, 1, 1, {2.55f, 4.2f, 0.f, 0.f, 0.642f, 13.f, 0.269f}, launch_ring<2, 2, 4, 2, 3>, holds_ring<2, 2, 4, 2>},
 };
 
-// The shape whose estimate is the least: over those sizes 0.5 % slower than the best of them in the mean, 3 % at most for 19
-// of 20, 18 % at worst.
+// The shape whose estimate is the least: over those sizes 0.3 % slower than the best of them in the mean, 1 % at most for 19
+// of 20, 17 % at worst.
 static const Mx8Shape& shape_of(const Mx8Args& a) {
   const Mx8Shape* best = kShapes;
   float least = 0.0f;
