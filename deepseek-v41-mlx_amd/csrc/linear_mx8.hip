@@ -65,35 +65,62 @@ __device__ __forceinline__ i32x8 join(i32x4 lo, i32x4 hi) {
   return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
-__device__ __forceinline__ float activated(float v, int act) {
-  switch (act) {
-    case ACT_RELU: return v > 0.0f || v != v ? v : 0.0f;
-    case ACT_SILU: return v / (1.0f + expf(-v));
-    case ACT_GELU: return 0.5f * v * (1.0f + erff(v * 0.70710678f));
-    default: return v;
+// v[e] = act(v[e]), the choice outside of the values. SiLU takes the hardware's exponential and reciprocal: their errors, some
+// |v| 2^-24 of the result and 0 for v under -87 (exp(87) and more has no normal reciprocal), lie far under its rounding to bf16.
+// 8,192 rows 2304 -> 1112 with SiLU: 44.2 -> 33.4 us (none: 32.0).
+template <int N, typename V>
+__device__ __forceinline__ void activate(V& v, int act) {
+  if (act == ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = v[e] > 0.0f || v[e] != v[e] ? v[e] : 0.0f;
+  } else if (act == ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = v[e] * __builtin_amdgcn_rcpf(1.0f + __expf(-v[e]));
+  } else if (act == ACT_GELU) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] = 0.5f * v[e] * (1.0f + erff(v[e] * 0.70710678f));
   }
 }
 
-// The epilogue of output j of row m, in float32 and rounded once.
-__device__ __forceinline__ void finish1(const Mx8Args& a, const Mx8Side& s, int64_t m, int j, float v) {
-  const int64_t at = m * s.n + j;
-  v = activated(a.bias ? v + a.bias[j] : v, a.act);
-  s.y[at] = f2bf(a.residual ? v + bf2f(a.residual[at]) : v);
+// The epilogue of N outputs at row[e], j[e], in float32 and rounded once, for rows of a width that does not align them: all
+// are read (they lie in the tensor), and those with mine[e] are written. The loads stand together, in front of what waits for
+// them, and a wave's lanes take outputs side by side: 8,192 rows 2304 -> 1111 with bias, SiLU and a residual 109 -> 53 us (1112:
+// 43), 777 rows 16.4 -> 9.6.
+template <int N>
+__device__ __forceinline__ void finish_each(const Mx8Args& a, const Mx8Side& s, const int (&row)[N], const int (&j)[N],
+                                            const bool (&mine)[N], float (&v)[N]) {
+  if (a.bias) {
+    float b[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) b[e] = a.bias[j[e]];
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] += b[e];
+  }
+  activate<N>(v, a.act);
+  if (a.residual) {
+    bf16_t r[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) r[e] = a.residual[(int64_t)row[e] * s.n + j[e]];
+#pragma unroll
+    for (int e = 0; e < N; ++e) v[e] += bf2f(r[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+    if (mine[e]) s.y[(int64_t)row[e] * s.n + j[e]] = f2bf(v[e]);
 }
 
-// Four consecutive outputs j .. j + 3, j a multiple of 4, some of them perhaps past the row's end. Rows of a width that is
-// no multiple of 4 are not aligned to four outputs and go one by one.
-__device__ __forceinline__ void finish4(const Mx8Args& a, const Mx8Side& s, int64_t m, int j, f32x4 v) {
+// Four consecutive outputs j .. j + 3, j a multiple of 4, some of them perhaps past the row's end.
+__device__ __forceinline__ void finish4(const Mx8Args& a, const Mx8Side& s, int m, int j, f32x4 v) {
   if ((s.n & 3) != 0) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (j + e < s.n) finish1(a, s, m, j + e, v[e]);
+    const int rows[4] = {m, m, m, m}, at[4] = {j, min(j + 1, s.n - 1), min(j + 2, s.n - 1), min(j + 3, s.n - 1)};
+    const bool mine[4] = {true, j + 1 < s.n, j + 2 < s.n, j + 3 < s.n};
+    float f[4] = {v[0], v[1], v[2], v[3]};
+    finish_each(a, s, rows, at, mine, f);
     return;
   }
-  const int64_t at = m * s.n + j;
+  const int64_t at = (int64_t)m * s.n + j;
   if (a.bias) v += *reinterpret_cast<const f32x4*>(a.bias + j);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = activated(v[e], a.act);
+  activate<4>(v, a.act);
   if (a.residual) {
     const uint2 u = *reinterpret_cast<const uint2*>(a.residual + at);
     v[0] += bf2f((bf16_t)(u.x & 0xFFFFu)), v[1] += bf2f((bf16_t)(u.x >> 16));
@@ -102,18 +129,8 @@ __device__ __forceinline__ void finish4(const Mx8Args& a, const Mx8Side& s, int6
   *reinterpret_cast<uint2*>(s.y + at) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
 }
 
-// The same for eight outputs inside the row, of which the first `skip` are another's: j a multiple of 8 where the width is.
-__device__ __forceinline__ void finish8(const Mx8Args& a, const Mx8Side& s, int64_t m, int j, int skip, float (&v)[8]) {
-  if ((s.n & 7) != 0 || skip) {
-#pragma unroll 1
-    for (int e = skip; e < 8; ++e) {
-      float t = v[0];
-#pragma unroll
-      for (int q = 1; q < 8; ++q) t = q == e ? v[q] : t;
-      finish1(a, s, m, j + e, t);
-    }
-    return;
-  }
+// The same for eight outputs j .. j + 7 of a row, j and the width multiples of 8.
+__device__ __forceinline__ void finish8(const Mx8Args& a, const Mx8Side& s, int64_t m, int j, float (&v)[8]) {
   const int64_t at = m * s.n + j;
   if (a.bias) {
     float b[8];
@@ -121,10 +138,7 @@ __device__ __forceinline__ void finish8(const Mx8Args& a, const Mx8Side& s, int6
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += b[e];
   }
-  if (a.act != ACT_NONE) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = activated(v[e], a.act);
-  }
+  activate<8>(v, a.act);
   if (a.residual) {
     Eight<bf16_t> held;
     held.load_past(a.residual + at);
@@ -351,7 +365,7 @@ __device__ __forceinline__ f32x16 mfma_mx8(i32x8 wf, i32x8 xf, f32x16 acc, uint3
 template <typename C, int WR, int WM>
 __device__ __forceinline__ void store_tile(const Mx8Args& a, const Mx8Side& s, uint8_t* lds, const f32x16 (&acc)[WR][WM], int own_r,
                                            int n0, int own_m, int m0) {
-  constexpr int LPR = 4 * WR, RPT = 64 / LPR;           // lanes per row, rows at a time
+  constexpr int COLS = 32 * WR, LPR = 4 * WR, RPT = 64 / LPR;     // outputs of a wave's row, lanes per row, rows at a time
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   uint8_t* const mine = lds + (threadIdx.x >> 6) * 32 * C::PITCH;
 #pragma unroll
@@ -364,14 +378,30 @@ __device__ __forceinline__ void store_tile(const Mx8Args& a, const Mx8Side& s, u
         *reinterpret_cast<f32x4*>(mine + l32 * C::PITCH + (32 * i + 8 * q + 4 * g) * 4) =
             f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
     __syncthreads();
+    if ((s.n & 7) != 0) {                  // rows that are not aligned to eight outputs: a value per lane, in the row's order
+#pragma unroll 1
+      for (int q = lane; q < 32 * COLS; q += 64 * 8) {
+        int row[8], col[8];
+        bool own[8];
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int r = (q + 64 * e) / COLS, c = (q + 64 * e) % COLS;
+          row[e] = m0 + 32 * j + r, col[e] = n0 + c, own[e] = row[e] >= own_m && col[e] >= own_r;
+          v[e] = reinterpret_cast<const float*>(mine + r * C::PITCH)[c];
+        }
+        finish_each(a, s, row, col, own, v);
+      }
+      continue;
+    }
     const int n = n0 + 8 * (lane % LPR);
 #pragma unroll 1
     for (int r = lane / LPR; r < 32; r += RPT) {
       const int m = m0 + 32 * j + r;
-      if (lane >= LPR * RPT || m < own_m || n + 8 <= own_r) continue;
+      if (lane >= LPR * RPT || m < own_m || n < own_r) continue;      // own_r is a multiple of 8 here, or n0 on
       float v[8];
       load8(reinterpret_cast<const float*>(mine + r * C::PITCH) + 8 * (lane % LPR), v);
-      finish8(a, s, m, n, max(own_r - n, 0), v);
+      finish8(a, s, m, n, v);
     }
   }
 }
