@@ -32,6 +32,7 @@ struct Mx8Args {
   int n[2];              // a second product of the same rows, or 0
   int tiles0, tiles;     // weight tiles of the first product and of both
   int mtiles, panel;     // tiles of x's rows, and how many of them one weight tile meets before the next
+  int whole;             // tiles that are multiplied whole, where others are in halves
   int rows, k, shift, act;
 };
 
@@ -41,12 +42,15 @@ struct Mx8Args {
 struct TileAt {
   int w, m;
 };
-__device__ __forceinline__ TileAt tile_at(const Mx8Args& a) {
-  const int total = (int)gridDim.x, b = (int)blockIdx.x, xcd = b % 8;
-  const int unit = xcd * (total / 8) + min(xcd, total % 8) + b / 8;
+__device__ __forceinline__ TileAt tile_of(const Mx8Args& a, int unit) {
   const int panel = unit / (a.panel * a.tiles), at = unit - panel * a.panel * a.tiles;
   const int high = min(a.panel, a.mtiles - panel * a.panel);
   return TileAt{at / high, panel * a.panel + at % high};
+}
+
+__device__ __forceinline__ TileAt tile_at(const Mx8Args& a, int total) {
+  const int b = (int)blockIdx.x, xcd = b % 8;
+  return tile_of(a, xcd * (total / 8) + min(xcd, total % 8) + b / 8);
 }
 
 // The part of a call that one workgroup's weight tile belongs to.
@@ -176,7 +180,7 @@ template <int RT, int WM, int NW, int D>
 __global__ __launch_bounds__(64 * NW) void mx8_rows_kernel(Mx8Args a) {
   using C = Mx8Rows<RT, WM, NW, D>;
   __shared__ __align__(16) uint8_t lds[C::LDS];
-  const TileAt at = tile_at(a);
+  const TileAt at = tile_at(a, (int)gridDim.x);
   const Mx8Side s = side_of(a, at.w);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
   const int j0 = s.tile * 16 * RT, m0 = at.m * 16 * WM;
@@ -407,11 +411,8 @@ __device__ __forceinline__ void store_tile(const Mx8Args& a, const Mx8Side& s, u
 }
 
 template <int WR, int WM, int GR, int GM>
-__global__ __launch_bounds__(64 * GR * GM, (Mx8Tile<WR, WM, GR, GM>::LDS <= 80 * 1024) ? 2 : 1) void mx8_tiles_kernel(
-    Mx8Args a) {
+__device__ __forceinline__ void multiply_tile(const Mx8Args& a, TileAt tile, uint8_t* lds) {
   using C = Mx8Tile<WR, WM, GR, GM>;
-  __shared__ __align__(16) uint8_t lds[C::LDS];
-  const TileAt tile = tile_at(a);
   const Mx8Side s = side_of(a, tile.w);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wr = (wave % GR) * 32 * WR, wm = (wave / GR) * 32 * WM;
@@ -624,6 +625,13 @@ __global__ __launch_bounds__(64 * GR * GM, (Mx8Tile<WR, WM, GR, GM>::LDS <= 80 *
   store_tile<C, WR, WM>(a, s, lds, acc, own_r, r0 + wr, own_m, m0 + wm);
 }
 
+template <int WR, int WM, int GR, int GM>
+__global__ __launch_bounds__(64 * GR * GM, (Mx8Tile<WR, WM, GR, GM>::LDS <= 80 * 1024) ? 2 : 1) void mx8_tiles_kernel(
+    Mx8Args a) {
+  __shared__ __align__(16) uint8_t lds[Mx8Tile<WR, WM, GR, GM>::LDS];
+  multiply_tile<WR, WM, GR, GM>(a, tile_at(a, (int)gridDim.x), lds);
+}
+
 // ------------------------------------------------------------------ tiles on few workgroups
 
 // The same tile over a ring of NS steps: a workgroup that has its CU to itself waits for the memory's answer every step
@@ -644,10 +652,8 @@ struct Mx8Ring {
 };
 
 template <int WR, int WM, int GR, int GM, int NS>
-__global__ __launch_bounds__(64 * GR * GM, 1) void mx8_ring_kernel(Mx8Args a) {
+__device__ __forceinline__ void multiply_ring_tile(const Mx8Args& a, TileAt tile, uint8_t* lds) {
   using C = Mx8Ring<WR, WM, GR, GM, NS>;
-  __shared__ __align__(16) uint8_t lds[C::LDS];
-  const TileAt tile = tile_at(a);
   const Mx8Side s = side_of(a, tile.w);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wr = (wave % GR) * 32 * WR, wm = (wave / GR) * 32 * WM;
@@ -803,6 +809,31 @@ __global__ __launch_bounds__(64 * GR * GM, 1) void mx8_ring_kernel(Mx8Args a) {
   store_tile<C, WR, WM>(a, s, lds, acc, own_r, r0 + wr, own_m, m0 + wm);
 }
 
+template <int WR, int WM, int GR, int GM, int NS>
+__global__ __launch_bounds__(64 * GR * GM, 1) void mx8_ring_kernel(Mx8Args a) {
+  __shared__ __align__(16) uint8_t lds[Mx8Ring<WR, WM, GR, GM, NS>::LDS];
+  multiply_ring_tile<WR, WM, GR, GM, NS>(a, tile_at(a, (int)gridDim.x), lds);
+}
+
+// Tiles of 256 x 256 in whole rounds of the 256 CUs, and what is left (`rest` tiles, half a round at most) as two tiles of
+// 256 x 128 each over a ring: the last round takes little more than half of a whole one's time. 8,192 rows 8192 -> 5120 (2 1/2
+// rounds): 297 -> 283 us; 4,096 rows (1 1/4): 185 -> 152, by tiles of 192 x 256 170.
+__global__ __launch_bounds__(512, 1) void mx8_halves_kernel(Mx8Args a) {
+  using Whole = Mx8Tile<4, 2, 2, 4>;
+  using Half = Mx8Ring<2, 2, 4, 2, 3>;
+  static_assert(Whole::NT == Half::NT && Whole::TR == Half::TR && Whole::TM == 2 * Half::TM, "two halves make a tile");
+  __shared__ __align__(16) uint8_t lds[Whole::LDS > Half::LDS ? Whole::LDS : Half::LDS];
+  if ((int)blockIdx.x < a.whole) {
+    multiply_tile<4, 2, 2, 4>(a, tile_at(a, a.whole), lds);
+  } else {
+    const int b = (int)blockIdx.x - a.whole, unit = a.whole + b / 16 * 8 + b % 8;      // both halves on one XCD
+    if (unit >= a.tiles * a.mtiles) return;
+    TileAt tile = tile_of(a, unit);
+    tile.m = 2 * tile.m + b / 8 % 2;
+    if (tile.m * Half::TM < a.rows) multiply_ring_tile<2, 2, 4, 2, 3>(a, tile, lds);
+  }
+}
+
 // Whole tiles of this shape are in the call.
 template <int WR, int WM, int GR, int GM>
 static bool holds(const Mx8Args& a) {
@@ -828,54 +859,81 @@ static bool launch_many(const Mx8Args& a, hipStream_t stream) {
   return launch_tiles(mx8_tiles_kernel<WR, WM, GR, GM>, a, C::TR, C::TM, C::NT, stream);
 }
 
+static int64_t tiles_of(const Mx8Args& a, int tr, int tm) {
+  return (int64_t)((a.n[0] + tr - 1) / tr + (a.n[1] + tr - 1) / tr) * ((a.rows + tm - 1) / tm);
+}
+
+// Whole rounds of 256 x 256 tiles, and half a round or less.
+static bool holds_halves(const Mx8Args& a) {
+  const int64_t tiles = tiles_of(a, 256, 256);
+  return holds_ring<4, 2, 2, 4>(a) && tiles > 256 && tiles % 256 > 0 && tiles % 256 <= 128;
+}
+static bool launch_halves(const Mx8Args& args, hipStream_t stream) {
+  Mx8Args a = args;
+  a.tiles0 = (a.n[0] + 255) / 256;
+  a.tiles = a.tiles0 + (a.n[1] + 255) / 256;
+  a.mtiles = (a.rows + 255) / 256;
+  a.panel = a.mtiles < 8 ? a.mtiles : 8;
+  const int64_t tiles = (int64_t)a.tiles * a.mtiles, rest = tiles % 256;
+  if (tiles * 512 >= (1ll << 32) - (1 << 20)) return false;
+  a.whole = (int)(tiles - rest);
+  hipLaunchKernelGGL(mx8_halves_kernel, dim3((unsigned)(a.whole + (rest + 7) / 8 * 16)), dim3(512), 0, stream, a);
+  return true;
+}
+
 // ------------------------------------------------------------------ which tile
 
 static bool any(const Mx8Args&) { return true; }
 
 // A tile shape, the ranges of k that one workgroup's waves share out, workgroups that a CU holds, and what a call's time
 // was measured to consist of, in us: 1 + per round of all CUs + per round and step + per tile of a CU + per tile and step +
-// per GB that tiles read + per 10 MB of results. Fitted to 230 to 330 sizes for each (1 to 8,192 rows, k 256 to 8,192, n 512
+// per GB that tiles read + per 10 MB of results. Fitted to 290 to 420 sizes for each (1 to 8,192 rows, k 256 to 8,192, n 512
 // to 32,768): 9 of 10 estimates are within 10 to 15 % of the time (rows of odd widths, stored by the value, take up to a third
 // longer than estimated, whatever the shape).
 struct Mx8Shape {
-  int kind, tr, tm, ranges, held;      // kind 0: few rows, 1: tiles, 2: tiles over a ring
+  int kind, tr, tm, ranges, held;      // kind 0: few rows, 1: tiles, 2: tiles over a ring, 3: tiles, the last in halves
   float us[7];
   bool (*launch)(const Mx8Args&, hipStream_t);
   bool (*takes)(const Mx8Args&);
 };
 static const Mx8Shape kShapes[] = {
-    {0, 16, 16, 8, 2, {2.51f, 0.f, 0.207f, 0.65f, 0.0511f, 20.3f, 0.f}, launch_rows<1, 1, 8, 2>, any},
-    {0, 32, 16, 8, 1, {1.75f, 1.48f, 0.f, 0.f, 0.406f, 17.2f, 0.f}, launch_rows<2, 1, 8, 2>, any},
-    {0, 32, 16, 2, 5, {2.62f, 0.f, 0.231f, 0.262f, 0.f, 23.6f, 0.f}, launch_rows<2, 1, 2, 2>, any},
-    {0, 32, 32, 4, 1, {1.69f, 1.52f, 0.359f, 0.f, 0.f, 6.63f, 6.97f}, launch_rows<2, 2, 4, 3>, any},
-    {0, 32, 48, 8, 1, {2.01f, 1.27f, 0.f, 0.f, 0.78f, 9.31f, 6.4f}, launch_rows<2, 3, 8, 1>, any},
-    {0, 64, 32, 8, 1, {2.05f, 1.39f, 0.985f, 0.f, 0.f, 10.3f, 4.56f}, launch_rows<4, 2, 8, 1>, any},
-    {0, 64, 64, 8, 1, {2.2f, 2.04f, 0.f, 0.f, 1.41f, 6.97f, 3.67f}, launch_rows<4, 4, 8, 1>, any},
-    {0, 64, 96, 4, 1, {2.2f, 3.75f, 0.f, 0.f, 0.967f, 0.f, 3.94f}, launch_rows<4, 6, 4, 1>, any},
-    {1, 64, 64, 1, 4, {2.78f, 0.f, 0.354f, 0.652f, 0.0508f, 17.1f, 0.f}, launch_many<1, 1, 2, 2>, holds<1, 1, 2, 2>},
-    {1, 128, 128, 1, 2, {4.15f, 0.2f, 0.408f, 0.7f, 0.256f, 1.24f, 1.31f}, launch_many<2, 2, 2, 2>, holds<2, 2, 2, 2>},
-    {1, 192, 256, 1, 1, {2.28f, 5.7f, 1.07f, 0.f, 0.f, 2.13f, 0.695f}, launch_many<3, 2, 2, 4>, holds<3, 2, 2, 4>},
-    {1, 256, 256, 1, 1, {1.47f, 0.f, 1.19f, 7.72f, 0.f, 9.86f, 0.456f}, launch_many<4, 2, 2, 4>, holds<4, 2, 2, 4>},
-    {2, 64, 64, 1, 2, {3.19f, 0.f, 0.095f, 0.493f, 0.123f, 7.7f, 1.25f}, launch_ring<1, 1, 2, 2, 4>, holds_ring<1, 1, 2, 2>},
-    {2, 128, 64, 1, 1, {2.91f, 0.925f, 0.324f, 0.f, 0.f, 5.31f, 2.57f}, launch_ring<1, 1, 4, 2, 4>, holds_ring<1, 1, 4, 2>},
-    {2, 128, 128, 1, 1, {2.99f, 1.93f, 0.f, 0.f, 0.424f, 11.f, 1.02f}, launch_ring<2, 1, 2, 4, 4>, holds_ring<2, 1, 2, 4>},
-    {2, 256, 128, 1, 1, {2.55f, 4.2f, 0.f, 0.f, 0.642f, 13.f, 0.269f}, launch_ring<2, 2, 4, 2, 3>, holds_ring<2, 2, 4, 2>},
+    {0, 16, 16, 8, 2, {2.52f, 0.f, 0.203f, 0.644f, 0.0547f, 19.9f, 0.f}, launch_rows<1, 1, 8, 2>, any},
+    {0, 32, 16, 8, 1, {1.78f, 1.45f, 0.f, 0.f, 0.405f, 17.2f, 0.f}, launch_rows<2, 1, 8, 2>, any},
+    {0, 32, 16, 2, 5, {2.64f, 0.f, 0.229f, 0.244f, 0.0015f, 24.2f, 0.f}, launch_rows<2, 1, 2, 2>, any},
+    {0, 32, 32, 4, 1, {1.81f, 1.43f, 0.f, 0.f, 0.35f, 9.63f, 6.44f}, launch_rows<2, 2, 4, 3>, any},
+    {0, 32, 48, 8, 1, {2.f, 1.32f, 0.f, 0.f, 0.759f, 12.2f, 5.09f}, launch_rows<2, 3, 8, 1>, any},
+    {0, 64, 32, 8, 1, {2.06f, 1.38f, 0.981f, 0.f, 0.f, 11.f, 4.42f}, launch_rows<4, 2, 8, 1>, any},
+    {0, 64, 64, 8, 1, {2.19f, 2.1f, 0.f, 0.f, 1.4f, 8.71f, 2.88f}, launch_rows<4, 4, 8, 1>, any},
+    {0, 64, 96, 4, 1, {2.96f, 2.97f, 0.f, 0.f, 0.957f, 3.52f, 4.05f}, launch_rows<4, 6, 4, 1>, any},
+    {1, 64, 64, 1, 4, {2.61f, 0.f, 0.344f, 0.774f, 0.0668f, 14.3f, 0.f}, launch_many<1, 1, 2, 2>, holds<1, 1, 2, 2>},
+    {1, 128, 128, 1, 2, {2.79f, 0.979f, 0.429f, 1.35f, 0.236f, 1.67f, 0.906f}, launch_many<2, 2, 2, 2>, holds<2, 2, 2, 2>},
+    {1, 192, 256, 1, 1, {0.895f, 0.f, 1.06f, 7.03f, 0.f, 3.36f, 0.757f}, launch_many<3, 2, 2, 4>, holds<3, 2, 2, 4>},
+    {1, 256, 256, 1, 1, {0.f, 0.f, 0.f, 9.14f, 1.19f, 9.09f, 0.658f}, launch_many<4, 2, 2, 4>, holds<4, 2, 2, 4>},
+    {2, 64, 64, 1, 2, {2.97f, 0.f, 0.0924f, 0.815f, 0.125f, 8.08f, 0.f}, launch_ring<1, 1, 2, 2, 4>, holds_ring<1, 1, 2, 2>},
+    {2, 128, 64, 1, 1, {2.53f, 1.46f, 0.32f, 0.f, 0.f, 6.83f, 1.64f}, launch_ring<1, 1, 4, 2, 4>, holds_ring<1, 1, 4, 2>},
+    {2, 128, 128, 1, 1, {2.33f, 2.59f, 0.426f, 0.f, 0.f, 10.9f, 0.786f}, launch_ring<2, 1, 2, 4, 4>, holds_ring<2, 1, 2, 4>},
+    {2, 256, 128, 1, 1, {1.43f, 0.f, 0.646f, 5.26f, 0.f, 12.9f, 0.237f}, launch_ring<2, 2, 4, 2, 3>, holds_ring<2, 2, 4, 2>},
+    {3, 256, 256, 1, 1, {0.f, 0.f, 0.f, 9.14f, 1.19f, 9.09f, 0.658f}, launch_halves, holds_halves},
 };
+static const Mx8Shape& kHalf = kShapes[15];      // what the last shape's halves are
 
-// The shape whose estimate is the least: over those sizes 0.3 % slower than the best of them in the mean, 1 % at most for 19
-// of 20, 17 % at worst.
+
+// The shape whose estimate is the least: over those sizes 0.4 % slower than the best of them in the mean, 2.3 % at most for 19
+// of 20, 18 % at worst.
 static const Mx8Shape& shape_of(const Mx8Args& a) {
+  const float out = 2.0f * (float)a.rows * (float)(a.n[0] + a.n[1]) * 1e-7f;
+  auto rounds_of = [&](const Mx8Shape& s, int64_t tiles) {
+    const int64_t cu = (tiles + 255) / 256, rounds = (cu + s.held - 1) / s.held;
+    const float steps = (float)((a.k / 128 + s.ranges - 1) / s.ranges);
+    const float gb = (float)tiles * (float)(s.tr + s.tm) * (float)a.k * 1e-9f;
+    return (float)rounds * (s.us[1] + steps * s.us[2]) + (float)cu * (s.us[3] + steps * s.us[4]) + gb * s.us[5];
+  };
   const Mx8Shape* best = kShapes;
   float least = 0.0f;
   for (const Mx8Shape& s : kShapes) {
     if (!s.takes(a)) continue;
-    const int64_t wt = (a.n[0] + s.tr - 1) / s.tr + (a.n[1] + s.tr - 1) / s.tr, mt = (a.rows + s.tm - 1) / s.tm;
-    const float tiles = (float)(wt * mt), cu = (float)((wt * mt + 255) / 256);
-    const float rounds = (float)((int64_t)(cu + (float)s.held - 1.0f) / s.held);
-    const float steps = (float)((a.k / 128 + s.ranges - 1) / s.ranges);
-    const float gb = tiles * (float)(s.tr + s.tm) * (float)a.k * 1e-9f;
-    const float out = 2.0f * (float)a.rows * (float)(a.n[0] + a.n[1]) * 1e-7f;
-    const float us = s.us[0] + rounds * (s.us[1] + steps * s.us[2]) + cu * (s.us[3] + steps * s.us[4]) + gb * s.us[5] + out * s.us[6];
+    const int64_t tiles = tiles_of(a, s.tr, s.tm), rest = s.kind == 3 ? tiles % 256 : 0;
+    const float us = s.us[0] + out * s.us[6] + rounds_of(s, tiles - rest) + (rest ? rounds_of(kHalf, 2 * rest) : 0.0f);
     if (&s == kShapes || us < least) best = &s, least = us;
   }
   return *best;
