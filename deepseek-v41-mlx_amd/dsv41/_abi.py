@@ -1622,7 +1622,7 @@ def _linear_mx8_args(name, x, x_scales, w, w_scales):
         good = (at == x_scales.get_device() == w.get_device() == w_scales.get_device() and x.is_cuda
                 and x.dtype is x_scales.dtype is w.dtype is w_scales.dtype is torch.uint8
                 and x.is_contiguous() and x_scales.is_contiguous() and w.is_contiguous() and w_scales.is_contiguous()
-                and k and n and k % 32 == 0 and sizes[-1] == k and x_scales.shape == (*sizes[:-1], k // 32))
+                and k and n and k % 32 == 0 and sizes and sizes[-1] == k and x_scales.shape == (*sizes[:-1], k // 32))
     except AttributeError:
         raise TypeError(f"{name}: codes and scales must be tensors") from None
     except ValueError:

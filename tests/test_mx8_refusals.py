@@ -139,6 +139,7 @@ def test_products_check_their_operands(host_abi):
     _refused(call(x=x[:, :32].contiguous(), x_scales=xs[:, :1].contiguous()), "contract")
     _refused(call(x_scales=xs[:2].contiguous()), "do not go with rows")
     _refused(call(w_scales=ws[:1].contiguous()), "do not go with a weight")
+    _refused(call(x=x[0, 0], x_scales=xs[0, 0]), "whole blocks")
     _refused(call(w=w[None]), "must be")
     _refused(call(w=w[:0], w_scales=ws[:0]), "contract")
     _refused(call(bias=torch.zeros(39)), "bias")
