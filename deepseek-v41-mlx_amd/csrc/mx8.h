@@ -55,7 +55,6 @@ template <typename T> struct Eight;
 template <> struct Eight<bf16_t> {
   uint4 u;
   __device__ __forceinline__ void load(const bf16_t* p) { u = *reinterpret_cast<const uint4*>(p); }
-  __device__ __forceinline__ void store(bf16_t* p) const { *reinterpret_cast<uint4*>(p) = u; }
   __device__ __forceinline__ void load_past(const bf16_t* p) { u = __builtin_bit_cast(uint4, past_l2<u32x4_once>(p)); }
   __device__ __forceinline__ void store_past(bf16_t* p) const { past_l2(p, __builtin_bit_cast(u32x4_once, u)); }
   __device__ __forceinline__ void get(float* v) const {
@@ -82,9 +81,6 @@ template <> struct Eight<float> {
   f32x4 a, b;
   __device__ __forceinline__ void load(const float* p) {
     a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-  }
-  __device__ __forceinline__ void store(float* p) const {
-    *reinterpret_cast<f32x4*>(p) = a, *reinterpret_cast<f32x4*>(p + 4) = b;
   }
   __device__ __forceinline__ void load_past(const float* p) { a = past_l2<f32x4>(p), b = past_l2<f32x4>(p + 4); }
   __device__ __forceinline__ void store_past(float* p) const { past_l2(p, a), past_l2(p + 4, b); }

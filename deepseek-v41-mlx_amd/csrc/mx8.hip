@@ -82,29 +82,76 @@ __global__ __launch_bounds__(256) void dequant_kernel(const uint8_t* codes, cons
 
 // ------------------------------------------------------------------ norm
 
-// The residual addition first (x <- cast(x + delta), stored back), the norm of the rounded sum with float32 statistics, the
-// normed row rounded to its type -- what the separate operators store between them and what every other reader of the row
-// gets -- and that row's blocks in 8 bits. Everything between stays in registers, so every tensor crosses the bus once.
+// The sum over a wave's lanes.
+__device__ __forceinline__ double wave_total(double v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// 1 / sqrt(m): the hardware's estimate and one Newton step, which leaves some 2^-50. m = 0 and infinity keep the estimate.
+__device__ __forceinline__ double inverse_root(double m) {
+  const double r = __builtin_amdgcn_rsq(m);
+  return r > 0.0 && r < (double)INFINITY ? r * (1.5 - 0.5 * m * r * r) : r;
+}
+
+// v[i] = g[i] v[i] inv to within 1/2 + 2^-20 of float32's step, where inv = hi + lo: the products with their rounding errors, whose
+// own roundings come to some 2^-44. Errors that are no numbers, or zero, are not added: infinities and a zero's sign stay.
+__device__ __forceinline__ void scale_exactly(float* v, const float* g, float hi, float lo) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float p = v[i] * hi, pe = __builtin_fmaf(v[i], hi, -p) + v[i] * lo;
+    const float q = g[i] * p, qe = __builtin_fmaf(g[i], p, -q) + g[i] * pe;
+    v[i] = __builtin_amdgcn_classf(qe, 0x198) ? q + qe : q;        // normal or subnormal
+  }
+}
+
+// The same as far as T tells: for bf16 the plain products, unless one of the eight lies within 4 float32 steps of the middle
+// between two bf16 values (they are 3 off at most). About one wave in ten takes the long way.
+template <typename T>
+__device__ __forceinline__ void scale_rows(float* v, const float* g, float hi, float lo) {
+  if constexpr (sizeof(T) == 2) {
+    float q[8];
+    uint32_t near = 0xFFFFu;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      q[i] = g[i] * (v[i] * hi);
+      near = min(near, (__float_as_uint(q[i]) - 0x7FFCu) & 0xFFFFu);
+    }
+    if (near > 8u) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = q[i];
+      return;
+    }
+  }
+  scale_exactly(v, g, hi, lo);
+}
+
+// The residual addition first (x <- cast(x + delta), stored back), the norm of the rounded sum, the normed row rounded to its
+// type -- what every other reader of the row gets -- and that row's blocks in 8 bits. Everything between stays in registers, so
+// every tensor crosses the bus once. A value in 8 bits has steps of an eighth: a normed value that is rounded to the other side
+// of a border is a whole step off. So the squares are summed in float64 and the products carried past float32 where it
+// matters: bf16 rows are the formula's values rounded (through float32), whatever the order of the sum. In float32 a value in
+// some 500,000 came out a step of 8 bits off. It costs 32,768 rows of 1,280 alone 26.6 -> 30.0 us, 8,192 rows of 8,192 with the
+// addition and the row kept 115.6 -> 116.9, one row of 5,120 3.4 -> 3.6.
 // Thread t holds eights t, t + 256 .. of a row, C of them. WAVE: one wave takes the row (dim at most 2,048), its lanes four
-// times 64 eights, without a barrier; the sums are added in the order that 256 threads add them in, which is
-// rmsnorm_rows_kernel's, so that bf16 rows come out the same to the last bit.
+// times 64 eights, without a barrier.
 template <typename T, int C, bool ADD, bool KEEP, bool WAVE>
 __global__ __launch_bounds__(256) void rmsnorm_mx8_kernel(T* x, const T* delta, const float* w, T* y, uint8_t* codes,
                                                           uint8_t* scales, int64_t rows, int dim, float eps) {
   constexpr int SPAN = WAVE ? 64 : 256;
-  __shared__ float red[4];
+  __shared__ double red[4];
   const int64_t row = WAVE ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
   if (WAVE && row >= rows) return;         // whole waves, which wait for nobody
   const int t = WAVE ? threadIdx.x & 63 : threadIdx.x, eights = dim / 8;
   Eight<T> e[C];
-  float part[C];
 #pragma unroll
   for (int c = 0; c < C; ++c)
     if (t + SPAN * c < eights) e[c].load(x + row * dim + 8 * (t + SPAN * c));
-  float ss = 0.0f;
+  double ss = 0.0;
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    if (WAVE) ss = 0.0f;
     if (t + SPAN * c < eights) {
       float v[8];
       e[c].get(v);
@@ -118,23 +165,17 @@ __global__ __launch_bounds__(256) void rmsnorm_mx8_kernel(T* x, const T* delta, 
         e[c].store_past(x + row * dim + 8 * (t + SPAN * c));
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss += v[i] * v[i];
+      for (int i = 0; i < 8; ++i) ss = __builtin_fma((double)v[i], (double)v[i], ss);
     }
-    part[c] = ss;
   }
-  float tot;
-  if constexpr (WAVE) {
-    float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int c = 0; c < C; ++c) r[c] = group_sum(part[c], 64);
-    tot = (r[0] + r[1]) + (r[2] + r[3]);
-  } else {
-    ss = group_sum(ss, 64);
+  ss = wave_total(ss);
+  if constexpr (!WAVE) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
     __syncthreads();
-    tot = (red[0] + red[1]) + (red[2] + red[3]);
+    ss = (red[0] + red[1]) + (red[2] + red[3]);
   }
-  const float inv = 1.0f / sqrtf(tot / (float)dim + eps);
+  const double inv = inverse_root(ss / dim + (double)eps);
+  const float hi = (float)inv, lo = (float)(inv - (double)hi);
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int ch = t + SPAN * c;
@@ -142,8 +183,7 @@ __global__ __launch_bounds__(256) void rmsnorm_mx8_kernel(T* x, const T* delta, 
       float g[8], v[8], s;
       load8(w + 8 * ch, g);
       e[c].get(v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = g[i] * (v[i] * inv);
+      scale_rows<T>(v, g, hi, lo);
       e[c].round(v);
       e[c].get(v);
       if constexpr (KEEP) e[c].store_past(y + row * dim + 8 * ch);

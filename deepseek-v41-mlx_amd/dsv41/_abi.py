@@ -1577,8 +1577,8 @@ def dequant_mx8(codes, scales, dtype=torch.bfloat16, out=None):
 
 
 def rmsnorm_mx8(x, weight, eps, delta=None, rows=True, out=None, codes=None, scales=None):
-    """(y, codes, scales): rmsnorm(x), or with delta add_rmsnorm(x, delta) (x updated in place), and quant_mx8 of it;
-    y is None with rows=False: dsv41_rmsnorm_mx8."""
+    """(y, codes, scales): the RMS norm of x, or with delta of x <- x + delta, and quant_mx8 of it; y is None with
+    rows=False: dsv41_rmsnorm_mx8."""
     name = "dsv41_rmsnorm_mx8"
     count, k, code, device = _mx8_rows(name, x)
     if (not isinstance(weight, torch.Tensor) or weight.dtype is not torch.float32 or weight.numel() != k

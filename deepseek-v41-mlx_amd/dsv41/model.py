@@ -92,7 +92,7 @@ class AttentionStack(torch.nn.Module):
                                  if shared.topk_idxs is not None else None)
             x8 = None
             if getattr(attn, "takes_quantized", False) and _mx8_norm_ok(h):
-                # 8-bit projections: the same norm also gives the rows in 8 bits
+                # 8-bit projections: the addition, the norm and its rows in 8 bits
                 x, x8 = mx8.norm_quantize(h, norm.weight, norm.eps, None if delta is None else delta.contiguous())
             elif delta is None:
                 x = norm(h)

@@ -70,8 +70,9 @@ def dequantize(q: Quantized, dtype: torch.dtype = torch.bfloat16) -> torch.Tenso
 
 def norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: torch.Tensor | None = None,
                   rows: bool = True):
-    """(y, Quantized): y = rmsnorm(x) of the rows x [..., dim], or with delta the residual addition first, x <- x + delta in
-    place (add_rmsnorm), and quantize(y). Without rows, y is not written and None."""
+    """(y, Quantized): y = the RMS norm of the rows x [..., dim], or with delta of the residual addition, x <- x + delta in
+    place, and quantize(y). Rows are the formula's, rounded to x's type: a border between two codes is no place for a float32
+    sum's error (RMSNorm's rows may be a step of that type off). Without rows, y is not written and None."""
     _no_gradient(x, weight, delta)
     y, codes, scales = _abi.rmsnorm_mx8(x, weight, eps, delta, rows)
     return y, Quantized(codes, scales)

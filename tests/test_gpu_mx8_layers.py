@@ -34,12 +34,12 @@ def stack(gpu, names, layers=8):
 
 def separate(s, h, cache):
     """AttentionStack.forward from separate calls: the residual addition, the norm and the quantization one by one."""
-    from dsv41 import _abi, mx8
+    from dsv41 import mx8
     from dsv41.model import SharedState
     start, shared = cache.offset, SharedState()
     h = h.clone()
     for layer, norm in zip(s.layers, s.norms):
-        x = _abi.rmsnorm(h, norm.weight, norm.eps)
+        x, _ = mx8.norm_quantize(h, norm.weight, norm.eps)
         if isinstance(layer.wo_b, mx8.MX8Linear):
             h = layer(x, start, cache, shared, residual=h)
         else:
