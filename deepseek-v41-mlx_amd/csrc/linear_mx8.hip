@@ -60,9 +60,9 @@ struct Mx8Side {
   bf16_t* y;
   int n, tile;
 };
-__device__ __forceinline__ Mx8Side side_of(const Mx8Args& a, int tile) {
-  const int i = tile >= a.tiles0;
-  return Mx8Side{a.w[i], a.ws[i], a.y[i], a.n[i], tile - (i ? a.tiles0 : 0)};
+__device__ __forceinline__ Mx8Side side_of(const Mx8Args& a, int tile, int split = 1) {      // split: parts of the call's tiles
+  const int i = tile >= split * a.tiles0;
+  return Mx8Side{a.w[i], a.ws[i], a.y[i], a.n[i], tile - (i ? split * a.tiles0 : 0)};
 }
 
 __device__ __forceinline__ i32x8 join(i32x4 lo, i32x4 hi) {
@@ -652,9 +652,10 @@ struct Mx8Ring {
 };
 
 template <int WR, int WM, int GR, int GM, int NS>
-__device__ __forceinline__ void multiply_ring_tile(const Mx8Args& a, TileAt tile, uint8_t* lds) {
+__device__ __forceinline__ void multiply_ring_tile(const Mx8Args& a, TileAt tile, uint8_t* lds, int split = 1) {
   using C = Mx8Ring<WR, WM, GR, GM, NS>;
-  const Mx8Side s = side_of(a, tile.w);
+  const Mx8Side s = side_of(a, tile.w, split);
+  if (split > 1 && (s.tile * C::TR >= s.n || tile.m * C::TM >= a.rows)) return;       // a part behind the end
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wr = (wave % GR) * 32 * WR, wm = (wave / GR) * 32 * WM;
   const int kb = a.k / 32, steps = a.k / 128;
@@ -815,22 +816,32 @@ __global__ __launch_bounds__(64 * GR * GM, 1) void mx8_ring_kernel(Mx8Args a) {
   multiply_ring_tile<WR, WM, GR, GM, NS>(a, tile_at(a, (int)gridDim.x), lds);
 }
 
-// Tiles of 256 x 256 in whole rounds of the 256 CUs, and what is left (`rest` tiles, half a round at most) as two tiles of
-// 256 x 128 each over a ring: the last round takes little more than half of a whole one's time. 8,192 rows 8192 -> 5120 (2 1/2
-// rounds): 297 -> 283 us; 4,096 rows (1 1/4): 185 -> 152, by tiles of 192 x 256 170.
-__global__ __launch_bounds__(512, 1) void mx8_halves_kernel(Mx8Args a) {
+// Tiles of 256 x 256 in whole rounds of the 256 CUs, and what is left in parts over a ring: half a round or less as two tiles of
+// 256 x 128 each, a quarter or less as four of 128 x 128, so that the last round takes half or a third of a whole one's time.
+// 8,192 rows 8192 -> 5120 (2 1/2 rounds): 297 -> 283 us; 4,096 rows (1 1/4) 189 -> 157 in halves, 154 in quarters, by tiles
+// of 192 x 256 170.
+template <int PARTS>
+__global__ __launch_bounds__(512, 1) void mx8_parts_kernel(Mx8Args a) {
   using Whole = Mx8Tile<4, 2, 2, 4>;
   using Half = Mx8Ring<2, 2, 4, 2, 3>;
+  using Quarter = Mx8Ring<2, 1, 2, 4, 4>;
   static_assert(Whole::NT == Half::NT && Whole::TR == Half::TR && Whole::TM == 2 * Half::TM, "two halves make a tile");
-  __shared__ __align__(16) uint8_t lds[Whole::LDS > Half::LDS ? Whole::LDS : Half::LDS];
+  static_assert(Whole::NT == Quarter::NT && Whole::TR == 2 * Quarter::TR && Whole::TM == 2 * Quarter::TM, "four quarters do");
+  constexpr int RING = PARTS == 2 ? Half::LDS : Quarter::LDS;
+  __shared__ __align__(16) uint8_t lds[Whole::LDS > RING ? Whole::LDS : RING];
   if ((int)blockIdx.x < a.whole) {
     multiply_tile<4, 2, 2, 4>(a, tile_at(a, a.whole), lds);
-  } else {
-    const int b = (int)blockIdx.x - a.whole, unit = a.whole + b / 16 * 8 + b % 8;      // both halves on one XCD
-    if (unit >= a.tiles * a.mtiles) return;
-    TileAt tile = tile_of(a, unit);
-    tile.m = 2 * tile.m + b / 8 % 2;
+    return;
+  }
+  const int b = (int)blockIdx.x - a.whole, part = b / 8 % PARTS, unit = a.whole + b / (8 * PARTS) * 8 + b % 8;   // parts on one XCD
+  if (unit >= a.tiles * a.mtiles) return;
+  TileAt tile = tile_of(a, unit);
+  tile.m = 2 * tile.m + part % 2;
+  if constexpr (PARTS == 2) {
     if (tile.m * Half::TM < a.rows) multiply_ring_tile<2, 2, 4, 2, 3>(a, tile, lds);
+  } else {
+    tile.w = 2 * tile.w + part / 2;
+    multiply_ring_tile<2, 1, 2, 4, 4>(a, tile, lds, 2);
   }
 }
 
@@ -863,12 +874,14 @@ static int64_t tiles_of(const Mx8Args& a, int tr, int tm) {
   return (int64_t)((a.n[0] + tr - 1) / tr + (a.n[1] + tr - 1) / tr) * ((a.rows + tm - 1) / tm);
 }
 
-// Whole rounds of 256 x 256 tiles, and half a round or less.
-static bool holds_halves(const Mx8Args& a) {
+// Whole rounds of 256 x 256 tiles, and a part of a round that takes PARTS workgroups a tile.
+template <int PARTS>
+static bool holds_parts(const Mx8Args& a) {
   const int64_t tiles = tiles_of(a, 256, 256);
-  return holds_ring<4, 2, 2, 4>(a) && tiles > 256 && tiles % 256 > 0 && tiles % 256 <= 128;
+  return holds_ring<4, 2, 2, 4>(a) && tiles > 256 && tiles % 256 > 0 && tiles % 256 * PARTS <= 256;
 }
-static bool launch_halves(const Mx8Args& args, hipStream_t stream) {
+template <int PARTS>
+static bool launch_parts(const Mx8Args& args, hipStream_t stream) {
   Mx8Args a = args;
   a.tiles0 = (a.n[0] + 255) / 256;
   a.tiles = a.tiles0 + (a.n[1] + 255) / 256;
@@ -877,7 +890,7 @@ static bool launch_halves(const Mx8Args& args, hipStream_t stream) {
   const int64_t tiles = (int64_t)a.tiles * a.mtiles, rest = tiles % 256;
   if (tiles * 512 >= (1ll << 32) - (1 << 20)) return false;
   a.whole = (int)(tiles - rest);
-  hipLaunchKernelGGL(mx8_halves_kernel, dim3((unsigned)(a.whole + (rest + 7) / 8 * 16)), dim3(512), 0, stream, a);
+  hipLaunchKernelGGL(mx8_parts_kernel<PARTS>, dim3((unsigned)(a.whole + (rest + 7) / 8 * 8 * PARTS)), dim3(512), 0, stream, a);
   return true;
 }
 
@@ -885,13 +898,13 @@ static bool launch_halves(const Mx8Args& args, hipStream_t stream) {
 
 static bool any(const Mx8Args&) { return true; }
 
-// A tile shape, the ranges of k that one workgroup's waves share out, workgroups that a CU holds, and what a call's time
+// A tile shape, the ranges of k that one workgroup's waves share out (parts of the last tiles for kind 3), workgroups that a CU holds, and what a call's time
 // was measured to consist of, in us: 1 + per round of all CUs + per round and step + per tile of a CU + per tile and step +
 // per GB that tiles read + per 10 MB of results. Fitted to 290 to 420 sizes for each (1 to 8,192 rows, k 256 to 8,192, n 512
 // to 32,768): 9 of 10 estimates are within 10 to 15 % of the time (rows of odd widths, stored by the value, take up to a third
 // longer than estimated, whatever the shape).
 struct Mx8Shape {
-  int kind, tr, tm, ranges, held;      // kind 0: few rows, 1: tiles, 2: tiles over a ring, 3: tiles, the last in halves
+  int kind, tr, tm, ranges, held;      // kind 0: few rows, 1: tiles, 2: tiles over a ring, 3: tiles, the last in parts
   float us[7];
   bool (*launch)(const Mx8Args&, hipStream_t);
   bool (*takes)(const Mx8Args&);
@@ -913,9 +926,10 @@ static const Mx8Shape kShapes[] = {
     {2, 128, 64, 1, 1, {2.53f, 1.46f, 0.32f, 0.f, 0.f, 6.83f, 1.64f}, launch_ring<1, 1, 4, 2, 4>, holds_ring<1, 1, 4, 2>},
     {2, 128, 128, 1, 1, {2.33f, 2.59f, 0.426f, 0.f, 0.f, 10.9f, 0.786f}, launch_ring<2, 1, 2, 4, 4>, holds_ring<2, 1, 2, 4>},
     {2, 256, 128, 1, 1, {1.43f, 0.f, 0.646f, 5.26f, 0.f, 12.9f, 0.237f}, launch_ring<2, 2, 4, 2, 3>, holds_ring<2, 2, 4, 2>},
-    {3, 256, 256, 1, 1, {0.f, 0.f, 0.f, 9.14f, 1.19f, 9.09f, 0.658f}, launch_halves, holds_halves},
+    {3, 256, 256, 2, 1, {0.f, 0.f, 0.f, 9.14f, 1.19f, 9.09f, 0.658f}, launch_parts<2>, holds_parts<2>},
+    {3, 256, 256, 4, 1, {0.f, 0.f, 0.f, 9.14f, 1.19f, 9.09f, 0.658f}, launch_parts<4>, holds_parts<4>},
 };
-static const Mx8Shape& kHalf = kShapes[15];      // what the last shape's halves are
+static const Mx8Shape &kQuarter = kShapes[14], &kHalf = kShapes[15];      // what the last tiles' parts are
 
 
 // The shape whose estimate is the least: over those sizes 0.4 % slower than the best of them in the mean, 2.3 % at most for 19
@@ -924,7 +938,8 @@ static const Mx8Shape& shape_of(const Mx8Args& a) {
   const float out = 2.0f * (float)a.rows * (float)(a.n[0] + a.n[1]) * 1e-7f;
   auto rounds_of = [&](const Mx8Shape& s, int64_t tiles) {
     const int64_t cu = (tiles + 255) / 256, rounds = (cu + s.held - 1) / s.held;
-    const float steps = (float)((a.k / 128 + s.ranges - 1) / s.ranges);
+    const int ranges = s.kind == 0 ? s.ranges : 1;
+    const float steps = (float)((a.k / 128 + ranges - 1) / ranges);
     const float gb = (float)tiles * (float)(s.tr + s.tm) * (float)a.k * 1e-9f;
     return (float)rounds * (s.us[1] + steps * s.us[2]) + (float)cu * (s.us[3] + steps * s.us[4]) + gb * s.us[5];
   };
@@ -933,7 +948,7 @@ static const Mx8Shape& shape_of(const Mx8Args& a) {
   for (const Mx8Shape& s : kShapes) {
     if (!s.takes(a)) continue;
     const int64_t tiles = tiles_of(a, s.tr, s.tm), rest = s.kind == 3 ? tiles % 256 : 0;
-    const float us = s.us[0] + out * s.us[6] + rounds_of(s, tiles - rest) + (rest ? rounds_of(kHalf, 2 * rest) : 0.0f);
+    const float us = s.us[0] + out * s.us[6] + rounds_of(s, tiles - rest) + (rest ? rounds_of(s.ranges == 2 ? kHalf : kQuarter, s.ranges * rest) : 0.0f);
     if (&s == kShapes || us < least) best = &s, least = us;
   }
   return *best;

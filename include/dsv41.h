@@ -658,8 +658,8 @@ int dsv41_linear_mx8_pair(const uint8_t* x, const uint8_t* x_scales, const uint8
                           int32_t n0, int32_t n1, int32_t scale_rows, hipStream_t stream);
 
 /* How those two calls split their work (n1 0 for the single product) where the scales are aligned to words, for tests and
- * profiles: the kernel (0 few rows, 1 tiles, 2 tiles over a ring, 3 whole rounds of tiles and the rest in halves), weight
- * rows and activation rows of a tile, ranges of k that a workgroup's waves share out. */
+ * profiles: the kernel (0 few rows, 1 tiles, 2 tiles over a ring, 3 whole rounds of tiles and the rest in parts), weight
+ * rows and activation rows of a tile, ranges of k that a workgroup's waves share out (kernel 3: parts of a tile). */
 int dsv41_linear_mx8_plan(int32_t rows, int32_t k, int32_t n0, int32_t n1, int32_t plan[4]);
 
 /* ---------------------------------------------------------------- cached sequences --

@@ -83,7 +83,7 @@ def test_products_past_32_bits(gpu, k, n):
 
 
 @pytest.mark.parametrize("rows,k,n0,n1,kernel", [(600, 288, 3008, 1111, 1), (2048, 544, 264, 8000, 1), (400, 512, 1280, 520, 2),
-                                                 (400, 512, 1281, 521, 2), (1300, 1024, 6017, 6600, 3), (2100, 640, 5000, 2571, 3)])
+                                                 (400, 512, 1281, 521, 2), (1300, 1024, 7017, 6600, 3), (1300, 1024, 6017, 6700, 3), (2100, 640, 5000, 2571, 3)])
 def test_a_pair_over_tiles(gpu, rows, k, n0, n1, kernel):
     from dsv41 import _abi, mx8
     assert _abi.linear_mx8_plan(rows, k, n0, n1).kernel == kernel
@@ -98,7 +98,7 @@ def test_a_pair_over_tiles(gpu, rows, k, n0, n1, kernel):
     assert all((h[rows * n:] == 7.0).all() for h, n in zip(held, (n0, n1)))
 
 
-@pytest.mark.parametrize("rows,k,n", [(1410, 640, 11001), (130, 640, 5449), (2353, 384, 5019)])
+@pytest.mark.parametrize("rows,k,n", [(1410, 640, 11001), (1281, 1024, 14001), (130, 640, 5449), (2353, 384, 5019)])
 def test_nothing_beyond_large_outputs_is_written(gpu, rows, k, n):
     from dsv41 import _abi
     x, w = operands(rows, k, n, 64)

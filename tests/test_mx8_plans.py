@@ -10,7 +10,7 @@ def test_the_tested_sizes_take_every_shape():
     few = {(0, 16, 16, 8), (0, 32, 16, 2), (0, 32, 16, 8), (0, 32, 32, 4), (0, 32, 48, 8), (0, 64, 32, 8), (0, 64, 64, 8),
            (0, 64, 96, 4)}
     many = {(1, 64, 64, 1), (1, 128, 128, 1), (1, 192, 256, 1), (1, 256, 256, 1)}
-    ring = {(2, 64, 64, 1), (2, 128, 64, 1), (2, 128, 128, 1), (2, 256, 128, 1), (3, 256, 256, 1)}
+    ring = {(2, 64, 64, 1), (2, 128, 64, 1), (2, 128, 128, 1), (2, 256, 128, 1), (3, 256, 256, 2), (3, 256, 256, 4)}
     plans = [_abi.linear_mx8_plan(*size) for size in SIZES]
     assert {tuple(p) for p in plans} == few | many | ring
     for shape in many | ring:                  # with a part of a pair of steps and without, and with a part of a step
