@@ -32,7 +32,7 @@ struct Mx8Args {
   int n[2];              // a second product of the same rows, or 0
   int tiles0, tiles;     // weight tiles of the first product and of both
   int mtiles, panel;     // tiles of x's rows, and how many of them one weight tile meets before the next
-  int whole;             // tiles that are multiplied whole, where others are in halves
+  int whole;             // tiles that are multiplied whole, where others are in parts
   int rows, k, shift, act;
 };
 

@@ -1480,17 +1480,20 @@ ACTIVATIONS = {"none": 0, None: 0, "relu": 1, "silu": 2, "gelu": 3}
 _U8 = torch.uint8
 
 
+_MX8_WIDTH = 1 << 31                          # channels are 32-bit numbers below
+
+
 def _mx8_rows(name, x):
     """(rows, channels, dtype code, device) of a float tensor of whole 32-channel blocks, contiguous, on the GPU."""
     try:
         k = x.shape[-1]
-        if x.is_cuda and k and k % 32 == 0 and x.is_contiguous():
+        if x.is_cuda and 0 < k < _MX8_WIDTH and k % 32 == 0 and x.is_contiguous():
             return x.numel() // k, k, _DTYPES[x.dtype], x.device
     except (AttributeError, IndexError, KeyError):
         pass
     _gpu(name, x)                              # say what is wrong
-    if x.dim() < 1 or x.shape[-1] == 0 or x.shape[-1] % 32:
-        raise ValueError(f"{name}: x {tuple(x.shape)} must have whole blocks of 32 channels")
+    if x.dim() < 1 or not 0 < x.shape[-1] < _MX8_WIDTH or x.shape[-1] % 32:
+        raise ValueError(f"{name}: x {tuple(x.shape)} must have whole blocks of 32 channels, fewer than 2^31 in a row")
     _contig(name, x)
     k = x.shape[-1]
     return x.numel() // k, k, dtype_code(x, name), x.device
@@ -1543,15 +1546,16 @@ def _mx8_pair(name, codes, scales):
     """Checks that codes and scales are uint8 tensors in one piece on one GPU, of whole blocks."""
     try:
         if (codes.dtype is scales.dtype is _U8 and codes.is_cuda and codes.get_device() == scales.get_device()
-                and codes.is_contiguous() and scales.is_contiguous() and codes.shape[-1] and codes.shape[-1] % 32 == 0):
+                and codes.is_contiguous() and scales.is_contiguous() and 0 < codes.shape[-1] < _MX8_WIDTH
+                and codes.shape[-1] % 32 == 0):
             return
     except (AttributeError, IndexError):
         pass
     _gpu(name, codes, scales)                  # say what is wrong
     if codes.dtype != _U8 or scales.dtype != _U8:
         raise ValueError(f"{name}: codes and scales must be uint8, got {codes.dtype} and {scales.dtype}")
-    if codes.dim() < 1 or codes.shape[-1] == 0 or codes.shape[-1] % 32:
-        raise ValueError(f"{name}: codes {tuple(codes.shape)} must have whole blocks of 32 channels")
+    if codes.dim() < 1 or not 0 < codes.shape[-1] < _MX8_WIDTH or codes.shape[-1] % 32:
+        raise ValueError(f"{name}: codes {tuple(codes.shape)} must have whole blocks of 32 channels, fewer than 2^31 in a row")
     _contig(name, codes, scales)
     _one_device(name, codes, scales)
 
@@ -1641,7 +1645,10 @@ def _linear_mx8_args(name, x, x_scales, w, w_scales):
         per = 32
     else:
         raise ValueError(f"{name}: scales {tuple(w_scales.shape)} do not go with a weight {tuple(w.shape)}")
-    return x.numel() // k, k, n, per
+    rows = x.numel() // k
+    if rows > 1 << 20 or n > 1 << 24 or k > 1 << 20:
+        raise ValueError(f"{name}: {rows} rows and {k} channels are up to 2^20, {n} outputs up to 2^24")
+    return rows, k, n, per
 
 
 class MX8Plan(typing.NamedTuple):

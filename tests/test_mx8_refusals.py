@@ -73,6 +73,17 @@ def test_quantization_checks_its_rows(host_abi):
     _refused(lambda: A.quant_mx8(x, x.view(U8).view(-1)[:192].view(3, 64), both[:6].view(3, 2)), "overlaps")
 
 
+def test_widths_are_32_bit_numbers(host_abi):
+    """A row of 2^32 + 32 channels (memory that is asked for and never touched) is none of 32."""
+    k = (1 << 32) + 32
+    wide, scales = torch.empty(1, k, dtype=U8), torch.empty(1, k // 32, dtype=U8)
+    _refused(lambda: host_abi.dequant_mx8(wide, scales), "fewer than")
+    del wide
+    x = torch.empty(1, k, dtype=BF)
+    _refused(lambda: host_abi.quant_mx8(x), "fewer than")
+    _refused(lambda: host_abi.rmsnorm_mx8(x, torch.ones(32), 1e-6), "fewer than")
+
+
 def test_reading_back_checks_its_codes(host_abi):
     A = host_abi
     c, s = torch.zeros(40, 64, dtype=U8), torch.zeros(40, 2, dtype=U8)
@@ -142,6 +153,8 @@ def test_products_check_their_operands(host_abi):
     _refused(call(x=x[0, 0], x_scales=xs[0, 0]), "whole blocks")
     _refused(call(w=w[None]), "must be")
     _refused(call(w=w[:0], w_scales=ws[:0]), "contract")
+    many = torch.zeros((1 << 20) + 1, 32, dtype=U8), torch.zeros((1 << 20) + 1, 1, dtype=U8)
+    _refused(lambda: A.linear_mx8(*many, torch.zeros(4, 32, dtype=U8), torch.zeros(1, 1, dtype=U8)), "2\\^20")
     _refused(call(bias=torch.zeros(39)), "bias")
     _refused(call(bias=torch.zeros(40, dtype=BF)), "bias")
     _refused(call(activation="tanh"), "activation")
