@@ -82,7 +82,6 @@ template <> struct Eight<float> {
   __device__ __forceinline__ void load(const float* p) {
     a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
   }
-  __device__ __forceinline__ void load_past(const float* p) { a = past_l2<f32x4>(p), b = past_l2<f32x4>(p + 4); }
   __device__ __forceinline__ void store_past(float* p) const { past_l2(p, a), past_l2(p + 4, b); }
   __device__ __forceinline__ void get(float* v) const {
 #pragma unroll

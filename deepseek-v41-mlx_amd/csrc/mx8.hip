@@ -132,8 +132,8 @@ __device__ __forceinline__ void scale_rows(float* v, const float* g, float hi, f
 // type -- what every other reader of the row gets -- and that row's blocks in 8 bits. Everything between stays in registers, so
 // every tensor crosses the bus once. A value in 8 bits has steps of an eighth: a normed value that is rounded to the other side
 // of a border is a whole step off. So the squares are summed in float64 and the products carried past float32 where it
-// matters: bf16 rows are the formula's values rounded (through float32), whatever the order of the sum. In float32 a value in
-// some 500,000 came out a step of 8 bits off. It costs 32,768 rows of 1,280 alone 26.6 -> 30.0 us, 8,192 rows of 8,192 with the
+// matters: bf16 rows are the formula's values rounded (through float32), whatever the order of the sum. In float32 one value
+// in a few million came out a step of 8 bits off. It costs 32,768 rows of 1,280 alone 26.6 -> 30.0 us, 8,192 rows of 8,192 with the
 // addition and the row kept 115.6 -> 116.9, one row of 5,120 3.4 -> 3.6.
 // Thread t holds eights t, t + 256 .. of a row, C of them. WAVE: one wave takes the row (dim at most 2,048), its lanes four
 // times 64 eights, without a barrier.
