@@ -635,30 +635,32 @@ __global__ __launch_bounds__(64 * GR * GM, (Mx8Tile<WR, WM, GR, GM>::LDS <= 80 *
 // ------------------------------------------------------------------ tiles on few workgroups
 
 // The same tile over a ring of NS steps: a workgroup that has its CU to itself waits for the memory's answer every step
-// (about 1 us whatever the tile) unless several steps are on their way. For rows of whole steps, four at least, whose
-// scales lie on words: scales come by copies too, four steps of a row at a time.
-template <int WR, int WM, int GR, int GM, int NS>
+// (about 1 us whatever the tile) unless several steps are on their way. For rows of four steps and more: scales come by copies
+// too, four steps of a row at a time; three where they lie off words or the last step is a part of one (ANY).
+template <int WR, int WM, int GR, int GM, int NS, bool ANY = false>
 struct Mx8Ring {
   static constexpr int NWV = GR * GM, NT = 64 * NWV;
   static constexpr int TR = 32 * WR * GR, TM = 32 * WM * GM, ROWS = TR + TM;
   static constexpr int kW = TR / 8 / NWV, kX = TM / 8 / NWV, kCopies = kW + kX;   // copies of 8 rows per wave and step
   static constexpr int CODES = NS * ROWS * 128;
   static constexpr int PITCH = 32 * WR * 4 + 16;        // bytes of a row of results on their way out, padded for the banks
-  static constexpr int RING = CODES + 2 * ROWS * 16, OUT = NWV * 32 * PITCH;
+  static constexpr int RING = CODES + 2 * ROWS * 16 + (ANY ? 16 : 0), OUT = NWV * 32 * PITCH;      // ANY: a word more is read
   static constexpr int LDS = RING > OUT ? RING : OUT;
   static_assert(TR % (8 * NWV) == 0 && TM % (8 * NWV) == 0 && NWV % 2 == 0, "whole copies, in turn over the waves");
   static_assert(TR % 64 == 0 && TM % 64 == 0 && ROWS <= 64 * NWV, "one copy of 64 rows' scales per wave");
   static_assert(kCopies * (NS - 1) <= 63 && NS >= 3 && NS <= 4, "vmcnt holds 6 bits; scales land in time");
 };
 
-template <int WR, int WM, int GR, int GM, int NS>
+template <int WR, int WM, int GR, int GM, int NS, bool ANY = false>
 __device__ __forceinline__ void multiply_ring_tile(const Mx8Args& a, TileAt tile, uint8_t* lds, int split = 1) {
-  using C = Mx8Ring<WR, WM, GR, GM, NS>;
+  using C = Mx8Ring<WR, WM, GR, GM, NS, ANY>;
   const Mx8Side s = side_of(a, tile.w, split);
   if (split > 1 && (s.tile * C::TR >= s.n || tile.m * C::TM >= a.rows)) return;       // a part behind the end
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   const int wr = (wave % GR) * 32 * WR, wm = (wave / GR) * 32 * WM;
-  const int kb = a.k / 32, steps = a.k / 128;
+  // ANY: the last step lies back from the row's end, whole, and its first `again` blocks, which the step before has, are
+  // multiplied as zeros
+  const int kb = a.k / 32, steps = ANY ? (a.k + 127) / 128 : a.k / 128, again = 4 * steps - kb;
   // The last tile of a side lies back from its end, whole: rows that the tile before owns are multiplied and not stored.
   const int own_r = s.tile * C::TR, r0 = min(own_r, s.n - C::TR);
   const int own_m = tile.m * C::TM, m0 = min(own_m, a.rows - C::TM);
@@ -684,20 +686,27 @@ __device__ __forceinline__ void multiply_ring_tile(const Mx8Args& a, TileAt tile
       else dma16_at<(NS * C::TR + 8 * C::NWV * (c - C::kW)) * 128>(xnext + (uint64_t)(c - C::kW) * pitch, off, xdst);
     }, std::make_integer_sequence<int, C::kCopies>{});
     if (last == C::kCopies) {
-      const uint64_t by = ahead > 0 ? 128 : 0;
+      const uint64_t by = ahead > 0 ? (ANY && ahead == 1 ? 128 - 32 * again : 128) : 0;
       wnext += by, xnext += by, --ahead;
       into = into + 1 < NS ? into + 1 : 0;
     }
   };
-  // scales: 64 rows per wave (one without any of its own repeats the last), the words of steps 4 f .. 4 f + 3 of a row side
-  // by side; the last four steps where fewer are left
-  const int srow = 64 * min(uwave, C::ROWS / 64 - 1);
+  // scales: 64 rows per wave (one without any of its own repeats the last), the words of kGroup steps of a row side by side; the
+  // last kGroup steps where fewer are left. ANY: 16 bytes from the word on that a row's first scale byte lies in hold three
+  // steps' whatever its place; the last 16 end with the word that the row's last byte lies in. So no copy touches a word
+  // without a byte of its row.
+  constexpr int kGroup = ANY ? 3 : 4;
+  const int srow = 64 * min(uwave, C::ROWS / 64 - 1), lastg = (steps - 1) / kGroup;
   const bool of_w = srow < C::TR;
   const int from = of_w ? r0 + srow : m0 + srow - C::TR, shift = of_w ? a.shift : 0;
-  const uint64_t sbase = uniform(reinterpret_cast<uint64_t>(of_w ? s.ws : a.xs) + (uint64_t)(from >> shift) * (uint64_t)kb);
-  const uint32_t soff = (uint32_t)(((from + lane) >> shift) - (from >> shift)) * (uint32_t)kb;
+  const uint64_t sfrom = uniform(reinterpret_cast<uint64_t>(of_w ? s.ws : a.xs) + (uint64_t)(from >> shift) * (uint64_t)kb);
+  const uint64_t sbase = ANY ? sfrom & ~3ull : sfrom;
+  const uint32_t sat = (uint32_t)(((from + lane) >> shift) - (from >> shift)) * (uint32_t)kb + (uint32_t)(sfrom - sbase);
+  const uint32_t soff = ANY ? sat & ~3u : sat, slast = ((sat + (uint32_t)kb + 3u) & ~3u) - 16u;
   auto copy_scales = [&](int f) {
-    dma16_sgpr(sbase + (uint64_t)(4 * min(4 * f, steps - 4)), soff, lds0 + (uint32_t)(C::CODES + (f & 1) * C::ROWS * 16 + srow * 16));
+    const uint32_t to = lds0 + (uint32_t)(C::CODES + (f & 1) * C::ROWS * 16 + srow * 16);
+    if constexpr (ANY) dma16_sgpr(sbase + (uint64_t)(f < lastg ? 12 * f : 0), f < lastg ? soff : slast, to);
+    else dma16_sgpr(sbase + (uint64_t)(4 * min(4 * f, steps - 4)), soff, to);
   };
 
   // LDS addresses of this lane's row in both operands, for each half step and each half of a fragment's 32 bytes, in the
@@ -742,13 +751,43 @@ __device__ __forceinline__ void multiply_ring_tile(const Mx8Args& a, TileAt tile
       else wf[f - WM] = frag(wadr[h], 32 * (f - WM) * 128);
     }
   };
-  // step kt's scale words (blocks 0 .. 3)
+  // step kt's scale words (blocks 0 .. 3). ANY: from two words, at the place of this lane's row
+  int wlow[WR], xlow[WM];                               // where a row's first scale byte lies in its word
+  if constexpr (ANY) {
+#pragma unroll
+    for (int i = 0; i < WR; ++i)
+      wlow[i] = (int)((reinterpret_cast<uintptr_t>(s.ws) + (uintptr_t)((r0 + wr + 32 * i + l32) >> a.shift) * (uintptr_t)kb) & 3u);
+#pragma unroll
+    for (int j = 0; j < WM; ++j)
+      xlow[j] = (int)((reinterpret_cast<uintptr_t>(a.xs) + (uintptr_t)(m0 + wm + 32 * j + l32) * (uintptr_t)kb) & 3u);
+  }
   auto read_scales = [&](int kt, uint32_t (&wsc)[WR], uint32_t (&xsc)[WM]) {
-    const uint32_t by = (uint32_t)(((kt >> 2) & 1) * C::ROWS * 16 + 4 * (kt - min(kt & ~3, steps - 4)));
+    if constexpr (ANY) {
+      const int now = min(kt, steps - 1), f = now / 3, byte = now == steps - 1 ? kb - 4 : 4 * now;      // in the row
+      auto word = [&](uint32_t adr, int low) {
+        const uint32_t at = (uint32_t)(byte + low - (f < lastg ? 12 * f : ((low + kb + 3) & ~3) - 16));
+        const uint32_t p = adr + (uint32_t)((f & 1) * C::ROWS * 16) + (at & ~3u);
+        return __builtin_amdgcn_alignbyte(*(lds_u32)(uintptr_t)(p + 4u), *(lds_u32)(uintptr_t)p, at);
+      };
 #pragma unroll
-    for (int j = 0; j < WM; ++j) xsc[j] = *(lds_u32)(uintptr_t)(xsadr + by + (uint32_t)(16 * 32 * j));
+      for (int j = 0; j < WM; ++j) xsc[j] = word(xsadr + (uint32_t)(16 * 32 * j), xlow[j]);
 #pragma unroll
-    for (int i = 0; i < WR; ++i) wsc[i] = *(lds_u32)(uintptr_t)(wsadr + by + (uint32_t)(16 * 32 * i));
+      for (int i = 0; i < WR; ++i) wsc[i] = word(wsadr + (uint32_t)(16 * 32 * i), wlow[i]);
+    } else {
+      const uint32_t by = (uint32_t)(((kt >> 2) & 1) * C::ROWS * 16 + 4 * (kt - min(kt & ~3, steps - 4)));
+#pragma unroll
+      for (int j = 0; j < WM; ++j) xsc[j] = *(lds_u32)(uintptr_t)(xsadr + by + (uint32_t)(16 * 32 * j));
+#pragma unroll
+      for (int i = 0; i < WR; ++i) wsc[i] = *(lds_u32)(uintptr_t)(wsadr + by + (uint32_t)(16 * 32 * i));
+    }
+  };
+  // the weight's codes of the blocks that the last step has again as zeros: a fragment's halves are blocks 0 and 1, 2 and 3
+  auto once = [&](int kt, int half, int i, i32x8 (&wf)[WR]) {
+    if constexpr (ANY) {
+      const int n = kt == steps - 1 ? again - 2 * half : 0, lo = n > 0 ? 0 : -1, hi = n > 1 ? 0 : -1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) wf[i][e] &= lo, wf[i][4 + e] &= hi;
+    }
   };
 
   f32x16 acc[WR][WM];
@@ -777,6 +816,7 @@ __device__ __forceinline__ void multiply_ring_tile(const Mx8Args& a, TileAt tile
 #pragma unroll
     for (int i = 0; i < WR; ++i) {
       read(1, i * kFrags / WR, (i + 1) * kFrags / WR, w1, x1);
+      once(kt, 0, i, w0);
 #pragma unroll
       for (int j = 0; j < WM; ++j) {
         acc[i][j] = mfma_mx8<0>(w0[i], x0[j], acc[i][j], wsc[i], xsc[j]);
@@ -788,14 +828,16 @@ __device__ __forceinline__ void multiply_ring_tile(const Mx8Args& a, TileAt tile
     // this wave has read the stage and its copies of the next step have landed; then every wave's
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * C::kCopies) : "memory");
     __syncthreads();
-    // the scales of the four steps after the next four: that buffer was last read two steps ago
-    if ((kt & 3) == 0) copy_scales((kt >> 2) + 1);
+    // the scales of the steps after the next kGroup: that buffer was last read two steps ago, and they land two steps before
+    // they are read, at the latest with the wait then
+    if (kt % kGroup == 0) copy_scales(kt / kGroup + 1);
     // the stage takes step kt + NS, and the next step's first half is read, while the second half is multiplied
 #pragma unroll
     for (int i = 0; i < WR; ++i) {
       issue(i * C::kCopies / WR, (i + 1) * C::kCopies / WR);
       read(0, i * kFrags / WR, (i + 1) * kFrags / WR, w0, x0);
       if (i == 0) read_scales(kt + 1, wsn, xsn);
+      once(kt, 1, i, w1);
 #pragma unroll
       for (int j = 0; j < WM; ++j) {
         acc[i][j] = mfma_mx8<2>(w1[i], x1[j], acc[i][j], wsc[i], xsc[j]);
@@ -810,10 +852,10 @@ __device__ __forceinline__ void multiply_ring_tile(const Mx8Args& a, TileAt tile
   store_tile<C, WR, WM>(a, s, lds, acc, own_r, r0 + wr, own_m, m0 + wm);
 }
 
-template <int WR, int WM, int GR, int GM, int NS>
+template <int WR, int WM, int GR, int GM, int NS, bool ANY>
 __global__ __launch_bounds__(64 * GR * GM, 1) void mx8_ring_kernel(Mx8Args a) {
-  __shared__ __align__(16) uint8_t lds[Mx8Ring<WR, WM, GR, GM, NS>::LDS];
-  multiply_ring_tile<WR, WM, GR, GM, NS>(a, tile_at(a, (int)gridDim.x), lds);
+  __shared__ __align__(16) uint8_t lds[Mx8Ring<WR, WM, GR, GM, NS, ANY>::LDS];
+  multiply_ring_tile<WR, WM, GR, GM, NS, ANY>(a, tile_at(a, (int)gridDim.x), lds);
 }
 
 // Tiles of 256 x 256 in whole rounds of the 256 CUs, and what is left in parts over a ring: half a round or less as two tiles of
@@ -852,16 +894,23 @@ static bool holds(const Mx8Args& a) {
   return a.rows >= C::TM && a.n[0] >= C::TR && (a.n[1] == 0 || a.n[1] >= C::TR);
 }
 
-// The same, and rows that the ring's kernel takes.
+// The same, and rows that the ring's kernel takes. Rows of whole steps whose scales lie on words have a kernel of their own: the
+// other one's shifts and masks cost 777 rows 2304 -> 1111 8.6 -> 10.9 us, 300 rows 2048 -> 8192 15.0 -> 16.7. Where rows are no
+// whole lines, copies straddle two besides: 300 rows 2272 -> 8192 take 21.4 us (29.4 in tiles of two steps), 777 rows 2336 -> 1111
+// 11.2 (13.5 as few rows).
 template <int WR, int WM, int GR, int GM>
 static bool holds_ring(const Mx8Args& a) {
+  return holds<WR, WM, GR, GM>(a) && a.k >= 512;
+}
+static bool on_steps(const Mx8Args& a) {
   auto on_words = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; };
-  return holds<WR, WM, GR, GM>(a) && a.k % 128 == 0 && a.k >= 512 && on_words(a.xs) && on_words(a.ws[0]) && on_words(a.ws[1]);
+  return a.k % 128 == 0 && on_words(a.xs) && on_words(a.ws[0]) && on_words(a.ws[1]);
 }
 template <int WR, int WM, int GR, int GM, int NS>
 static bool launch_ring(const Mx8Args& a, hipStream_t stream) {
   using C = Mx8Ring<WR, WM, GR, GM, NS>;
-  return launch_tiles(mx8_ring_kernel<WR, WM, GR, GM, NS>, a, C::TR, C::TM, C::NT, stream);
+  if (on_steps(a)) return launch_tiles(mx8_ring_kernel<WR, WM, GR, GM, NS, false>, a, C::TR, C::TM, C::NT, stream);
+  return launch_tiles(mx8_ring_kernel<WR, WM, GR, GM, NS, true>, a, C::TR, C::TM, C::NT, stream);
 }
 
 template <int WR, int WM, int GR, int GM>
@@ -878,7 +927,7 @@ static int64_t tiles_of(const Mx8Args& a, int tr, int tm) {
 template <int PARTS>
 static bool holds_parts(const Mx8Args& a) {
   const int64_t tiles = tiles_of(a, 256, 256);
-  return holds_ring<4, 2, 2, 4>(a) && tiles > 256 && tiles % 256 > 0 && tiles % 256 * PARTS <= 256;
+  return holds_ring<4, 2, 2, 4>(a) && on_steps(a) && tiles > 256 && tiles % 256 > 0 && tiles % 256 * PARTS <= 256;
 }
 template <int PARTS>
 static bool launch_parts(const Mx8Args& args, hipStream_t stream) {
@@ -939,7 +988,7 @@ static const Mx8Shape& shape_of(const Mx8Args& a) {
   auto rounds_of = [&](const Mx8Shape& s, int64_t tiles) {
     const int64_t cu = (tiles + 255) / 256, rounds = (cu + s.held - 1) / s.held;
     const int ranges = s.kind == 0 ? s.ranges : 1;
-    const float steps = (float)((a.k / 128 + ranges - 1) / ranges);
+    const float steps = (float)(((s.kind == 2 ? a.k + 127 : a.k) / 128 + ranges - 1) / ranges);
     const float gb = (float)tiles * (float)(s.tr + s.tm) * (float)a.k * 1e-9f;
     return (float)rounds * (s.us[1] + steps * s.us[2]) + (float)cu * (s.us[3] + steps * s.us[4]) + gb * s.us[5];
   };

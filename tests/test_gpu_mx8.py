@@ -340,17 +340,19 @@ def test_every_tile_shape(gpu, rows, k, n):
     assert torch.equal(got, mx8.MX8Linear(*w)(x))
 
 
-def test_scales_off_words(gpu):
-    """Scales that begin anywhere in memory: the kernels that copy them by words are not for those."""
+@pytest.mark.parametrize("per", [1, 32])
+@pytest.mark.parametrize("rows,k,n", [(444, 640, 4912), (300, 544, 1701), (130, 672, 5449), (141, 608, 10917), (259, 1056, 13625),
+                                      (79, 3392, 905), (1324, 1024, 11017)])
+def test_scales_off_words(gpu, rows, k, n, per):
+    """Scales that begin anywhere in memory, in tensors that end with their last byte."""
     from dsv41 import _abi
-    x, w = operands(444, 640, 4912, 27)
-    assert _abi.linear_mx8_plan(444, 640, 4912).kernel == 2
+    x, w = operands(rows, k, n, 27, per)
     want = product(x, w)
     for off in (1, 2, 3):
-        held = [torch.zeros(t.numel() + 8, dtype=torch.uint8, device=gpu) for t in (x.scales, w.scales)]
+        held = [torch.full((t.numel() + off * (i + 1),), 255, dtype=torch.uint8, device=gpu) for i, t in enumerate((x.scales, w.scales))]
         for i, (h, t) in enumerate(zip(held, (x.scales, w.scales))):
-            h[off * (i + 1):off * (i + 1) + t.numel()] = t.flatten()
-        xs, ws = (h[off * (i + 1):off * (i + 1) + t.numel()].view(t.shape) for i, (h, t) in enumerate(zip(held, (x.scales, w.scales))))
+            h[off * (i + 1):] = t.flatten()
+        xs, ws = (h[off * (i + 1):].view(t.shape) for i, (h, t) in enumerate(zip(held, (x.scales, w.scales))))
         check(_abi.linear_mx8(x.codes, xs, w.codes, ws), *want)
 
 
