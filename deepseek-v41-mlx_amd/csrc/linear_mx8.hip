@@ -69,6 +69,16 @@ __device__ __forceinline__ i32x8 join(i32x4 lo, i32x4 hi) {
   return i32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
+// v (1 + erf(v / sqrt 2)) / 2 by Abramowitz and Stegun's formula 7.1.26, erfc(a) = (a1 t + .. + a5 t^5) exp(-a^2) with
+// t = 1 / (1 + p a), within 1.5e-7; the left tail comes from erfc itself, without 1 - erf's cancellation (8,192 rows 2304 -> 1112:
+// 42.2 -> 38.8 us).
+__device__ __forceinline__ float gelu(float v) {
+  const float a = fabsf(v), t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * 0.70710678f * a);
+  const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * p * __expf(-0.5f * v * v);
+  return v * (v >= 0.0f ? 1.0f - tail : tail);
+}
+
 // v[e] = act(v[e]), the choice outside of the values. SiLU takes the hardware's exponential and reciprocal: their errors, some
 // |v| 2^-24 of the result and 0 for v under -87 (exp(87) and more has no normal reciprocal), lie far under its rounding to bf16.
 // 8,192 rows 2304 -> 1112 with SiLU: 44.2 -> 33.4 us (none: 32.0).
@@ -82,7 +92,7 @@ __device__ __forceinline__ void activate(V& v, int act) {
     for (int e = 0; e < N; ++e) v[e] = v[e] * __builtin_amdgcn_rcpf(1.0f + __expf(-v[e]));
   } else if (act == ACT_GELU) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) v[e] = 0.5f * v[e] * (1.0f + erff(v[e] * 0.70710678f));
+    for (int e = 0; e < N; ++e) v[e] = gelu(v[e]);
   }
 }
 

@@ -323,6 +323,28 @@ def test_epilogues(gpu, rows, k, n, act, per, bias, residual):
         assert lin(x, activation=act, residual=r, out=r) is r and torch.equal(r, got)
 
 
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_activations_alone(gpu, act, rows):
+    """Products of zeros, so that the bias is what is activated: values of every size, both signs, in aligned rows and not."""
+    from dsv41 import mx8
+    g = torch.Generator().manual_seed(25)
+    v = torch.cat([torch.randn(4000, generator=g) * torch.exp2(torch.randint(-20, 5, (4000,), generator=g).float()),
+                   torch.linspace(-120, 120, 4801), torch.tensor([0.0, -0.0, 1e30, -1e30, 3e38, -3e38, 1e-30, -1e-30])])
+    for n in (v.numel(), v.numel() - v.numel() % 8):
+        w = mx8.Quantized(torch.zeros(n, 64, dtype=torch.uint8, device=gpu), torch.full((n, 2), 127, dtype=torch.uint8, device=gpu))
+        x = mx8.Quantized(torch.zeros(rows, 64, dtype=torch.uint8, device=gpu), torch.full((rows, 2), 127, dtype=torch.uint8, device=gpu))
+        got = mx8.MX8Linear(*w, v[-n:].to(gpu))(x, activation=act).double().cpu()
+        d = v[-n:].double()
+        want = {"relu": d.clamp(min=0), "silu": d * torch.sigmoid(d), "gelu": 0.5 * d * torch.special.erfc(-d * math.sqrt(0.5))}[act]
+        # bf16's half step; gelu's formula is 1.5e-7 off in erf, so 0.75e-7 |v|, and as much again for float32's roundings; silu's
+        # exponential is |v| + 2 steps of 2^-24 off and its reciprocal 0 from exp(87) on, where v / exp(87) is under 2e-36
+        near = want.abs() * HALF[BF] + {"relu": 0.0, "silu": 2e-36, "gelu": 1.5e-7}[act] * d.abs().clamp(max=1e3 if act == "gelu" else 1.0)
+        if act == "silu":
+            near = near + want.abs() * (d.abs() + 4.0) * 2.0 ** -24
+        assert ((got - want).abs() <= near).all(), (d[(got - want).abs() > near][:8], got[0][((got - want).abs() > near)[0]][:8])
+
+
 @pytest.mark.parametrize("rows,k,n", SIZES)
 def test_every_tile_shape(gpu, rows, k, n):
     """Each shape's products, its last tiles where nothing divides, and its epilogue with the residual stream in place; the
