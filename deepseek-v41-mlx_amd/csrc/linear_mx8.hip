@@ -98,8 +98,7 @@ __device__ __forceinline__ void activate(V& v, int act) {
 
 // The epilogue of N outputs at row[e], j[e], in float32 and rounded once, for rows of a width that does not align them: all
 // are read (they lie in the tensor), and those with mine[e] are written. The loads stand together, in front of what waits for
-// them, and a wave's lanes take outputs side by side: 8,192 rows 2304 -> 1111 with bias, SiLU and a residual 109 -> 53 us (1112:
-// 43), 777 rows 16.4 -> 9.6.
+// them, and a wave's lanes take outputs side by side: 8,192 rows 2304 -> 1111 with bias, SiLU and a residual 109 -> 53 us.
 template <int N>
 __device__ __forceinline__ void finish_each(const Mx8Args& a, const Mx8Side& s, const int (&row)[N], const int (&j)[N],
                                             const bool (&mine)[N], float (&v)[N]) {
@@ -143,23 +142,19 @@ __device__ __forceinline__ void finish4(const Mx8Args& a, const Mx8Side& s, int 
   *reinterpret_cast<uint2*>(s.y + at) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
 }
 
-// The same for eight outputs j .. j + 7 of a row, j and the width multiples of 8.
-__device__ __forceinline__ void finish8(const Mx8Args& a, const Mx8Side& s, int64_t m, int j, float (&v)[8]) {
-  const int64_t at = m * s.n + j;
+// The same for eight outputs from `at` on, aligned, with their bias b and residual r.
+__device__ __forceinline__ void finish8(const Mx8Args& a, const Mx8Side& s, int64_t at, const float (&b)[8], const Eight<bf16_t>& r,
+                                        float (&v)[8]) {
   if (a.bias) {
-    float b[8];
-    load8(a.bias + j, b);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += b[e];
   }
   activate<8>(v, a.act);
   if (a.residual) {
-    Eight<bf16_t> held;
-    held.load_past(a.residual + at);
-    float r[8];
-    held.get(r);
+    float f[8];
+    r.get(f);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += r[e];
+    for (int e = 0; e < 8; ++e) v[e] += f[e];
   }
   // past the L2, which keeps the operands that the other tiles read (999 rows 1280 -> 32768: 59 -> 52 us, 8,192 rows 1280 ->
   // 8192: 110 -> 93)
@@ -380,19 +375,42 @@ template <typename C, int WR, int WM>
 __device__ __forceinline__ void store_tile(const Mx8Args& a, const Mx8Side& s, uint8_t* lds, const f32x16 (&acc)[WR][WM], int own_r,
                                            int n0, int own_m, int m0) {
   constexpr int COLS = 32 * WR, LPR = 4 * WR, RPT = 64 / LPR;     // outputs of a wave's row, lanes per row, rows at a time
+  constexpr int kTurns = (32 + RPT - 1) / RPT;
   const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
   uint8_t* const mine = lds + (threadIdx.x >> 6) * 32 * C::PITCH;
+  const bool aligned = (s.n & 7) == 0;
+  const int n = n0 + 8 * (lane % LPR);
+  float b[8];
+  if (a.bias && aligned) load8(a.bias + n, b);
+  __syncthreads();                         // the ring is done with; from here on each wave keeps to its own part
 #pragma unroll
   for (int j = 0; j < WM; ++j) {
-    __syncthreads();
+    // the residual's rows are on their way while the sums cross LDS (8,192 rows 8192 -> 5120 301 -> 289 us, 999 rows 1280 ->
+    // 32768 76 -> 64)
+    Eight<bf16_t> held[kTurns];
+    if (a.residual && aligned) {
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t)
+        held[t].load_past(a.residual + (int64_t)(m0 + 32 * j + min(lane / LPR + RPT * t, 31)) * s.n + n);
+    }
 #pragma unroll
     for (int i = 0; i < WR; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<f32x4*>(mine + l32 * C::PITCH + (32 * i + 8 * q + 4 * g) * 4) =
             f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-    __syncthreads();
-    if ((s.n & 7) != 0) {                  // rows that are not aligned to eight outputs: a value per lane, in the row's order
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (aligned) {
+#pragma unroll
+      for (int t = 0; t < kTurns; ++t) {
+        const int r = lane / LPR + RPT * t, m = m0 + 32 * j + r;
+        if (r < 32 && lane < LPR * RPT && m >= own_m && n >= own_r) {      // own_r is a multiple of 8 here, or n0 on
+          float v[8];
+          load8(reinterpret_cast<const float*>(mine + r * C::PITCH) + 8 * (lane % LPR), v);
+          finish8(a, s, (int64_t)m * s.n + n, b, held[t], v);
+        }
+      }
+    } else {                               // a value per lane, in the row's order
 #pragma unroll 1
       for (int q = lane; q < 32 * COLS; q += 64 * 8) {
         int row[8], col[8];
@@ -406,17 +424,8 @@ __device__ __forceinline__ void store_tile(const Mx8Args& a, const Mx8Side& s, u
         }
         finish_each(a, s, row, col, own, v);
       }
-      continue;
     }
-    const int n = n0 + 8 * (lane % LPR);
-#pragma unroll 1
-    for (int r = lane / LPR; r < 32; r += RPT) {
-      const int m = m0 + 32 * j + r;
-      if (lane >= LPR * RPT || m < own_m || n < own_r) continue;      // own_r is a multiple of 8 here, or n0 on
-      float v[8];
-      load8(reinterpret_cast<const float*>(mine + r * C::PITCH) + 8 * (lane % LPR), v);
-      finish8(a, s, m, n, v);
-    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");       // read, before the next rows are written
   }
 }
 
