@@ -82,8 +82,10 @@ def test_products_past_32_bits(gpu, k, n):
     check(got[spots[-1]:], y, size, residual=res)
 
 
-@pytest.mark.parametrize("rows,k,n0,n1,kernel", [(600, 288, 3008, 1111, 1), (2048, 544, 264, 8000, 1), (400, 512, 1280, 520, 2),
-                                                 (400, 512, 1281, 521, 2), (1300, 1024, 7017, 6600, 3), (1300, 1024, 6017, 6700, 3), (2100, 640, 5000, 2571, 3)])
+@pytest.mark.parametrize("rows,k,n0,n1,kernel", [(600, 288, 3008, 1111, 1), (2048, 544, 264, 8000, 1), (700, 1056, 5001, 330, 1),
+                                                 (400, 512, 1280, 520, 2), (400, 512, 1281, 521, 2), (400, 544, 1281, 521, 2),
+                                                 (259, 608, 9000, 4625, 2), (1300, 1024, 7017, 6600, 3),
+                                                 (1300, 1024, 6017, 6700, 3), (2100, 640, 5000, 2571, 3)])
 def test_a_pair_over_tiles(gpu, rows, k, n0, n1, kernel):
     from dsv41 import _abi, mx8
     assert _abi.linear_mx8_plan(rows, k, n0, n1).kernel == kernel
