@@ -202,11 +202,10 @@ def _inputs(c, seed):
 
 def prepare(case, seed):
     s = _inputs(case, seed)
-    if own:
-        s["mx8"] = mx8 = _package()
-        if "w" in s and case["op"] != "weight":
-            s["x"] = mx8.Quantized(*s["x"])
-            s["lin"] = [mx8.MX8Linear(codes, scales, s["bias"]) for codes, scales in s["w"]]
+    if own and "w" in s and case["op"] != "weight":
+        mx8 = _package()
+        s["x"] = mx8.Quantized(*s["x"])
+        s["lin"] = [mx8.MX8Linear(codes, scales, s["bias"]) for codes, scales in s["w"]]
     s["case"] = case
     return s
 
@@ -215,7 +214,7 @@ def run(state):
     s, c = state, state["case"]
     op = c["op"]
     if own:
-        mx8 = s["mx8"]
+        mx8 = _package()
         if op == "norm":
             y, q = mx8.norm_quantize(s["x"], s["norm"], EPS, delta=s["delta"], rows=c["keep"])
             return dict(h=s["x"], values=mx8.dequantize(q), **(dict(y=y) if c["keep"] else {}))
