@@ -130,16 +130,32 @@ class Attention(torch.nn.Module):
             self.adapters[name] = AdapterBank(slots, w.shape[1], w.shape[0], rank, w.dtype, w.device)
         return self.adapters
 
+    def check_adapters(self) -> None:
+        """Refuses banks on projections that are in 8 bits by now, whichever came first: their products would leave the
+        adapters out."""
+        for name in self.adapters:
+            if isinstance(getattr(self, name, None), mx8.MX8Linear):
+                raise ValueError(f"{name} is held in 8 bits: adapters go on projections of the activations' type")
+
+    def _may_hold_8_bits(self, name: str) -> None:
+        if name in self.adapters:
+            raise ValueError(f"{name} has adapters: they go on projections of the activations' type")
+        if self.dtype != torch.bfloat16:
+            raise ValueError(f"8-bit projections give bfloat16; this layer's activations are {self.dtype}")
+
+    def __setattr__(self, name, value):
+        if name in QUANTIZED and isinstance(value, mx8.MX8Linear):
+            self._may_hold_8_bits(name)
+        super().__setattr__(name, value)
+
     def quantize_projections(self, names=QUANTIZED) -> dict:
         """Holds the named projections in 8 bits from now on (mx8.MX8Linear.from_linear; one that is stays as it is) and
-        returns them. A checkpoint's own codes and scales go in as attributes: attn.wq_b = MX8Linear(codes, scales)."""
+        returns them. A checkpoint's own codes and scales go in as attributes, under the same conditions:
+        attn.wq_b = MX8Linear(codes, scales)."""
         for name in names:
             if name not in QUANTIZED:
                 raise ValueError(f"8 bits are for {QUANTIZED}, not for {name!r}")
-            if name in self.adapters:
-                raise ValueError(f"{name} has adapters: they go on projections of the activations' type")
-            if self.dtype != torch.bfloat16:
-                raise ValueError(f"8-bit projections give bfloat16; this layer's activations are {self.dtype}")
+            self._may_hold_8_bits(name)
         for name in names:
             lin = getattr(self, name)
             if not isinstance(lin, mx8.MX8Linear):
@@ -208,15 +224,16 @@ class Attention(torch.nn.Module):
         """x [b, n, dim] (post attn_norm), absolute positions [start_pos, start_pos + n). x8: x in 8 bits, where the caller
         has it (mx8.norm_quantize) and takes_quantized. residual: the stream that the output goes on; it is added in wo_b's
         own launch where wo_b is in 8 bits, in place, and returned."""
+        # the batch's adapters, one slot (or none) per sequence
+        ids = getattr(shared, "adapter_ids", None)
+        banks = self.adapters if ids is not None else {}
+        if banks:
+            self.check_adapters()
         bsz, n, _ = x.shape
         rd = self.rope_head_dim
         end_pos = start_pos + n
         cos, sin = self._freqs(end_pos)
         x = x.contiguous()
-
-        # the batch's adapters, one slot (or none) per sequence
-        ids = getattr(shared, "adapter_ids", None)
-        banks = self.adapters if ids is not None else {}
 
         qa, kv_raw = self._input_projections(x, x8, banks, ids)
         # queries: q's rope tail (attention.py:117) is applied by the attention launch as it loads q

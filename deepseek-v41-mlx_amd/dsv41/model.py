@@ -71,8 +71,12 @@ class AttentionStack(torch.nn.Module):
     def forward(self, h: torch.Tensor, cache: ModelCache, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
         """h [b, n, dim] continues the sequence at cache.offset; advances the cache. adapter_ids [b] int32: every
         sequence's slot in the layers' adapter banks (-1: none)."""
-        if adapter_ids is not None and not any(attn.adapters for attn in self.layers):
-            raise ValueError("adapter_ids without adapters (add_adapters)")
+        if adapter_ids is not None:
+            if not any(attn.adapters for attn in self.layers):
+                raise ValueError("adapter_ids without adapters (add_adapters)")
+            for attn in self.layers:           # before any layer has moved its cache on
+                if isinstance(attn, Attention):
+                    attn.check_adapters()
         start_pos = cache.offset
         shared = SharedState()
         shared.adapter_ids = adapter_ids
