@@ -662,6 +662,21 @@ __global__ __launch_bounds__(64 * GR * GM, (Mx8Tile<WR, WM, GR, GM>::LDS <= 80 *
 
 // ------------------------------------------------------------------ tiles on few workgroups
 
+// Rows of whole steps: where the scale word of step kt lies behind a row's first byte in the two buffers of `rows` rows x 16 bytes,
+// four steps each, the last four steps side by side where fewer are left. Steps past the last have its word again.
+constexpr __host__ __device__ __forceinline__ int ring_scales_at(int kt, int steps, int rows) {
+  const int now = kt < steps ? kt : steps - 1, group = now & ~3;
+  return ((now >> 2) & 1) * rows * 16 + 4 * (now - (group < steps - 4 ? group : steps - 4));
+}
+constexpr bool ring_scales_inside(int rows) {
+  for (int steps = 4; steps < 24; ++steps)             // every remainder of eight, with the second buffer and without
+    for (int kt = 0; kt <= steps; ++kt) {
+      const int at = ring_scales_at(kt, steps, rows) % (rows * 16);
+      if (at < 0 || at + 4 > 16) return false;          // in its own row's 16 bytes
+    }
+  return true;
+}
+
 // The same tile over a ring of NS steps: a workgroup that has its CU to itself waits for the memory's answer every step
 // (about 1 us whatever the tile) unless several steps are on their way. For rows of four steps and more: scales come by copies
 // too, four steps of a row at a time; three where they lie off words or the last step is a part of one (ANY).
@@ -676,6 +691,7 @@ struct Mx8Ring {
   static constexpr int LDS = RING > OUT ? RING : OUT;
   static_assert(TR % (8 * NWV) == 0 && TM % (8 * NWV) == 0 && NWV % 2 == 0, "whole copies, in turn over the waves");
   static_assert(TR % 64 == 0 && TM % 64 == 0 && ROWS <= 64 * NWV, "one copy of 64 rows' scales per wave");
+  static_assert(ring_scales_inside(ROWS), "the reads ahead stay in the buffers");
   static_assert(kCopies * (NS - 1) <= 63 && NS >= 3 && NS <= 4, "vmcnt holds 6 bits; scales land in time");
 };
 
@@ -802,7 +818,7 @@ __device__ __forceinline__ void multiply_ring_tile(const Mx8Args& a, TileAt tile
 #pragma unroll
       for (int i = 0; i < WR; ++i) wsc[i] = word(wsadr + (uint32_t)(16 * 32 * i), wlow[i]);
     } else {
-      const uint32_t by = (uint32_t)(((kt >> 2) & 1) * C::ROWS * 16 + 4 * (kt - min(kt & ~3, steps - 4)));
+      const uint32_t by = (uint32_t)ring_scales_at(kt, steps, C::ROWS);
 #pragma unroll
       for (int j = 0; j < WM; ++j) xsc[j] = *(lds_u32)(uintptr_t)(xsadr + by + (uint32_t)(16 * 32 * j));
 #pragma unroll
