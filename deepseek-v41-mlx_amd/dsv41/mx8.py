@@ -106,6 +106,15 @@ class MX8Linear(torch.nn.Module):
         """lin in 8 bits (quantize_weight), its bias kept."""
         return cls(*quantize_weight(lin.weight.detach()), None if lin.bias is None else lin.bias.detach())
 
+    def _apply(self, fn, recurse: bool = True):
+        """Moves as any module's; a cast of the types (module.to(torch.bfloat16)) leaves the bias in float32, as the product
+        takes it and with the bits that it has."""
+        bias = self.bias
+        super()._apply(fn, recurse)
+        if bias is not None and self.bias.dtype != torch.float32:
+            self.bias = bias.to(self.bias.device)
+        return self
+
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
 
