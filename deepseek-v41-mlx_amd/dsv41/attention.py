@@ -42,7 +42,7 @@ from .adapters import AdapterBank, adapter_linear, adapter_linear_pair
 from .compressor import Compressor
 from .config import ModelArgs
 from .indexer import Indexer
-from .layers import RMSNorm, yarn_inv_freqs
+from .layers import RMSNorm, only_the_norm, yarn_inv_freqs
 
 # the projections that take low-rank adapters (Attention.add_adapters)
 ADAPTED = ("wq_a", "wkv", "wq_b", "wo_b")
@@ -237,10 +237,14 @@ class Attention(torch.nn.Module):
 
         qa, kv_raw = self._input_projections(x, x8, banks, ids)
         # queries: q's rope tail (attention.py:117) is applied by the attention launch as it loads q
-        if isinstance(self.wq_b, mx8.MX8Linear):       # the normed rows themselves are for the indexer alone
+        if isinstance(self.wq_b, mx8.MX8Linear) and only_the_norm(self.q_norm):
+            # the normed rows themselves are for the indexer alone
             qr, q8 = mx8.norm_quantize(qa.contiguous(), self.q_norm.weight, self.q_norm.eps,
                                        rows=bool(self.ratio) and self.is_index_source)
             q = self.wq_b(q8)
+        elif isinstance(self.wq_b, mx8.MX8Linear):
+            qr = self.q_norm(qa)
+            q = self.wq_b(qr)
         else:
             qr = self.q_norm(qa)
             q = adapter_linear(self.wq_b, qr, banks.get("wq_b"), ids, wide_only=True)

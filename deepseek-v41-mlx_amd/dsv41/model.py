@@ -15,7 +15,7 @@ from . import _abi, mx8
 from .attention import ADAPTED, QUANTIZED, Attention
 from .cache import ModelCache
 from .config import ModelArgs
-from .layers import RMSNorm
+from .layers import RMSNorm, only_the_norm
 
 
 def _fused_norm_ok(h: torch.Tensor) -> bool:
@@ -94,13 +94,13 @@ class AttentionStack(torch.nn.Module):
                 use.index_src_cache = shared.index_src_cache
                 use.topk_idxs = (torch.full_like(shared.topk_idxs, -1)
                                  if shared.topk_idxs is not None else None)
-            x8 = None
-            if getattr(attn, "takes_quantized", False) and _mx8_norm_ok(h):
+            x8, plain = None, only_the_norm(norm)     # a norm with hooks or of another formula is called itself
+            if plain and getattr(attn, "takes_quantized", False) and _mx8_norm_ok(h):
                 # 8-bit projections: the addition, the norm and its rows in 8 bits
                 x, x8 = mx8.norm_quantize(h, norm.weight, norm.eps, None if delta is None else delta.contiguous())
             elif delta is None:
                 x = norm(h)
-            elif _fused_norm_ok(h):
+            elif plain and _fused_norm_ok(h):
                 x = _abi.add_rmsnorm(h, delta.contiguous(), norm.weight, norm.eps)
             else:
                 h.add_(delta)
