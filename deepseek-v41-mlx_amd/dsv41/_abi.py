@@ -1598,7 +1598,7 @@ def rmsnorm_mx8(x, weight, eps, delta=None, rows=True, out=None, codes=None, sca
             if delta.shape != x.shape or delta.dtype != x.dtype:
                 raise ValueError(f"{name}: delta {tuple(delta.shape)} {delta.dtype} must match x {tuple(x.shape)} {x.dtype}")
             _contig(name, delta)
-        _apart(name, x, "delta", delta)
+        _apart(name, x, "delta or the weight", delta, weight)      # x is written too
     if out is not None and not rows:
         raise ValueError(f"{name}: out given, and rows not asked for")
     if out is codes is scales is None:

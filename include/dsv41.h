@@ -638,8 +638,8 @@ int dsv41_dequant_mx8(const uint8_t* codes, const uint8_t* scales, void* x, int6
 /* The RMS norm of x [rows, dim], or with delta of x <- cast(x + delta), with the normed rows in 8 bits: codes [rows, dim] and
  * scales [rows, dim/32] are dsv41_quant_mx8's of the rows rounded to dtype, which also go to y unless it is NULL. Statistics
  * and products keep more than float32: the rows are the formula's, rounded (dsv41_rmsnorm's and dsv41_add_rmsnorm's may be a
- * step of dtype off). dim at most 16,384, fewer than 2^24 rows. y, codes and scales must not overlap x, delta or
- * each other. */
+ * step of dtype off). dim at most 16,384, fewer than 2^24 rows. y, codes and scales must not overlap x, delta,
+ * weight or each other, nor x delta or weight where delta is given. */
 int dsv41_rmsnorm_mx8(void* x, const void* delta, const float* weight, void* y, uint8_t* codes, uint8_t* scales,
                       int64_t rows, int32_t dim, float eps, int32_t dtype, hipStream_t stream);
 
