@@ -119,16 +119,21 @@ class Attention(torch.nn.Module):
         """Banks of `slots` empty adapters for the named projections, of the weights' type and on their device as they
         are now, kept in self.adapters and returned; a forward whose shared.adapter_ids names a slot per sequence applies
         them."""
+        names = tuple(names)
+        self.check_adapted(names)
+        for name in names:
+            w = getattr(self, name).weight
+            self.adapters[name] = AdapterBank(slots, w.shape[1], w.shape[0], rank, w.dtype, w.device)
+        return self.adapters
+
+    def check_adapted(self, names) -> None:
+        """Refuses names that add_adapters refuses."""
         for name in names:
             if name not in ADAPTED:
                 raise ValueError(f"adapters go on {ADAPTED}, not on {name!r}")
         for name in names:
             if isinstance(getattr(self, name), mx8.MX8Linear):
                 raise ValueError(f"{name} is held in 8 bits: adapters go on projections of the activations' type")
-        for name in names:
-            w = getattr(self, name).weight
-            self.adapters[name] = AdapterBank(slots, w.shape[1], w.shape[0], rank, w.dtype, w.device)
-        return self.adapters
 
     def check_adapters(self) -> None:
         """Refuses banks on projections that are in 8 bits by now, whichever came first: their products would leave the
@@ -152,15 +157,23 @@ class Attention(torch.nn.Module):
         """Holds the named projections in 8 bits from now on (mx8.MX8Linear.from_linear; one that is stays as it is) and
         returns them. A checkpoint's own codes and scales go in as attributes, under the same conditions:
         attn.wq_b = MX8Linear(codes, scales)."""
-        for name in names:
-            if name not in QUANTIZED:
-                raise ValueError(f"8 bits are for {QUANTIZED}, not for {name!r}")
-            self._may_hold_8_bits(name)
+        names = tuple(names)
+        self.check_quantized(names)
         for name in names:
             lin = getattr(self, name)
             if not isinstance(lin, mx8.MX8Linear):
                 setattr(self, name, mx8.MX8Linear.from_linear(lin))
         return {name: getattr(self, name) for name in names}
+
+    def check_quantized(self, names) -> None:
+        """Refuses names that quantize_projections refuses, before any projection is replaced."""
+        for name in names:
+            if name not in QUANTIZED:
+                raise ValueError(f"8 bits are for {QUANTIZED}, not for {name!r}")
+            self._may_hold_8_bits(name)
+            lin = getattr(self, name)
+            if not isinstance(lin, mx8.MX8Linear) and lin.weight.shape[1] % 32:
+                raise ValueError(f"{name} takes {lin.weight.shape[1]} channels: 8 bits need whole blocks of 32")
 
     @property
     def takes_quantized(self) -> bool:

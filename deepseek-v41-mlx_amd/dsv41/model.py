@@ -61,11 +61,17 @@ class AttentionStack(torch.nn.Module):
                           index_format, cache_format, fp8_block_rows)
 
     def add_adapters(self, slots: int, rank: int, names=ADAPTED) -> list:
-        """Attention.add_adapters on every layer; the layers' banks."""
+        """Attention.add_adapters on every layer, or on none where one refuses; the layers' banks."""
+        names = tuple(names)
+        for attn in self.layers:
+            attn.check_adapted(names)
         return [attn.add_adapters(slots, rank, names) for attn in self.layers]
 
     def quantize_projections(self, names=QUANTIZED) -> list:
-        """Attention.quantize_projections on every layer; the layers' 8-bit projections."""
+        """Attention.quantize_projections on every layer, or on none where one refuses; the layers' 8-bit projections."""
+        names = tuple(names)
+        for attn in self.layers:
+            attn.check_quantized(names)
         return [attn.quantize_projections(names) for attn in self.layers]
 
     def forward(self, h: torch.Tensor, cache: ModelCache, adapter_ids: torch.Tensor | None = None) -> torch.Tensor:
