@@ -394,8 +394,8 @@ __device__ __forceinline__ void store_tile(const Mx8Args& a, const Mx8Side& s, u
   __syncthreads();                         // the ring is done with; from here on each wave keeps to its own part
 #pragma unroll
   for (int j = 0; j < WM; ++j) {
-    // the residual's rows are on their way while the sums cross LDS (8,192 rows 8192 -> 5120 301 -> 289 us, 999 rows 1280 ->
-    // 32768 76 -> 64)
+    // the residual's rows are on their way while the sums cross LDS (with each wave on its own here: 8,192 rows 8192 -> 5120
+    // 301 -> 287 us, 999 rows 1280 -> 32768 74 -> 61)
     Eight<bf16_t> held[kTurns];
     if (a.residual && aligned) {
 #pragma unroll
@@ -991,17 +991,20 @@ static bool launch_parts(const Mx8Args& args, hipStream_t stream) {
 
 static bool any(const Mx8Args&) { return true; }
 
-// A tile shape, the ranges of k that one workgroup's waves share out (parts of the last tiles for kind 3), workgroups that a CU holds, and what a call's time
-// was measured to consist of, in us: 1 + per round of all CUs + per round and step + per tile of a CU + per tile and step +
-// per GB that tiles read + per 10 MB of results. Fitted to 290 to 420 sizes for each (1 to 8,192 rows, k 256 to 8,192, n 512
-// to 32,768): 9 of 10 estimates are within 10 to 15 % of the time (rows of odd widths, stored by the value, take up to a third
-// longer than estimated, whatever the shape).
+// A tile shape, the ranges of k that one workgroup's waves share out (parts of the last tiles for kind 3), workgroups that a CU
+// holds, and what a call's time was measured to consist of, in us: 1 + per round of all CUs + per round and step + per tile of a CU
+// + per tile and step + per GB that tiles read + per 10 MB of results. Fitted to 290 to 420 sizes for each (1 to 8,192 rows, k 256
+// to 8,192, n 512 to 32,768, no bias or residual): 9 of 10 estimates of those are within 10 to 15 % of the time (rows of odd
+// widths, stored by the value, take up to a third longer than estimated, whatever the shape).
 struct Mx8Shape {
   int kind, tr, tm, ranges, held;      // kind 0: few rows, 1: tiles, 2: tiles over a ring, 3: tiles, the last in parts
   float us[7];
   bool (*launch)(const Mx8Args&, hipStream_t);
   bool (*takes)(const Mx8Args&);
 };
+// what the last tiles' parts are, and tiles of their own
+static const Mx8Shape kQuarter = {2, 128, 128, 1, 1, {2.33f, 2.59f, 0.426f, 0.f, 0.f, 10.9f, 0.786f}, launch_ring<2, 1, 2, 4, 4>, holds_ring<2, 1, 2, 4>};
+static const Mx8Shape kHalf = {2, 256, 128, 1, 1, {1.43f, 0.f, 0.646f, 5.26f, 0.f, 12.9f, 0.237f}, launch_ring<2, 2, 4, 2, 3>, holds_ring<2, 2, 4, 2>};
 static const Mx8Shape kShapes[] = {
     {0, 16, 16, 8, 2, {2.52f, 0.f, 0.203f, 0.644f, 0.0547f, 19.9f, 0.f}, launch_rows<1, 1, 8, 2>, any},
     {0, 32, 16, 8, 1, {1.78f, 1.45f, 0.f, 0.f, 0.405f, 17.2f, 0.f}, launch_rows<2, 1, 8, 2>, any},
@@ -1017,16 +1020,15 @@ static const Mx8Shape kShapes[] = {
     {1, 256, 256, 1, 1, {0.f, 0.f, 0.f, 9.14f, 1.19f, 9.09f, 0.658f}, launch_many<4, 2, 2, 4>, holds<4, 2, 2, 4>},
     {2, 64, 64, 1, 2, {2.97f, 0.f, 0.0924f, 0.815f, 0.125f, 8.08f, 0.f}, launch_ring<1, 1, 2, 2, 4>, holds_ring<1, 1, 2, 2>},
     {2, 128, 64, 1, 1, {2.53f, 1.46f, 0.32f, 0.f, 0.f, 6.83f, 1.64f}, launch_ring<1, 1, 4, 2, 4>, holds_ring<1, 1, 4, 2>},
-    {2, 128, 128, 1, 1, {2.33f, 2.59f, 0.426f, 0.f, 0.f, 10.9f, 0.786f}, launch_ring<2, 1, 2, 4, 4>, holds_ring<2, 1, 2, 4>},
-    {2, 256, 128, 1, 1, {1.43f, 0.f, 0.646f, 5.26f, 0.f, 12.9f, 0.237f}, launch_ring<2, 2, 4, 2, 3>, holds_ring<2, 2, 4, 2>},
+    kQuarter,
+    kHalf,
     {3, 256, 256, 2, 1, {0.f, 0.f, 0.f, 9.14f, 1.19f, 9.09f, 0.658f}, launch_parts<2>, holds_parts<2>},
     {3, 256, 256, 4, 1, {0.f, 0.f, 0.f, 9.14f, 1.19f, 9.09f, 0.658f}, launch_parts<4>, holds_parts<4>},
 };
-static const Mx8Shape &kQuarter = kShapes[14], &kHalf = kShapes[15];      // what the last tiles' parts are
 
-
-// The shape whose estimate is the least: over those sizes 0.4 % slower than the best of them in the mean, 2.3 % at most for 19
-// of 20, 18 % at worst.
+// The shape whose estimate is the least. On 1,000 other sizes of those ranges, 3 of 10 with a residual, 1 in 4 of a width that is
+// no multiple of 8 and 1 in 5 with a part of a step: 1.0 % slower than the best shape in the mean, 6 % at most for 19 of 20, 39 % at worst
+// (459 rows 384 -> 1392 5.9 us in place of 4.2: widths of three steps, which the ring does not take, are the worst ones).
 static const Mx8Shape& shape_of(const Mx8Args& a) {
   const float out = 2.0f * (float)a.rows * (float)(a.n[0] + a.n[1]) * 1e-7f;
   auto rounds_of = [&](const Mx8Shape& s, int64_t tiles) {

@@ -72,7 +72,7 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, eps: float, delta: torc
                   rows: bool = True):
     """(y, Quantized): y = the RMS norm of the rows x [..., dim], or with delta of the residual addition, x <- x + delta in
     place, and quantize(y). Rows are the formula's, rounded to x's type: a border between two codes is no place for a float32
-    sum's error (RMSNorm's rows may be a step of that type off). Without rows, y is not written and None."""
+    sum's error (RMSNorm's rows may be a step of that type off). eps counts as float32. Without rows, y is not written and None."""
     _no_gradient(x, weight, delta)
     y, codes, scales = _abi.rmsnorm_mx8(x, weight, eps, delta, rows)
     return y, Quantized(codes, scales)
