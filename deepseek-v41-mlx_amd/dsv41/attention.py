@@ -132,14 +132,14 @@ class Attention(torch.nn.Module):
             if name not in ADAPTED:
                 raise ValueError(f"adapters go on {ADAPTED}, not on {name!r}")
         for name in names:
-            if isinstance(getattr(self, name), mx8.MX8Linear):
+            if self.in_8_bits(name):
                 raise ValueError(f"{name} is held in 8 bits: adapters go on projections of the activations' type")
 
     def check_adapters(self) -> None:
         """Refuses banks on projections that are in 8 bits by now, whichever came first: their products would leave the
         adapters out."""
         for name in self.adapters:
-            if isinstance(getattr(self, name, None), mx8.MX8Linear):
+            if self.in_8_bits(name):
                 raise ValueError(f"{name} is held in 8 bits: adapters go on projections of the activations' type")
 
     def _may_hold_8_bits(self, name: str) -> None:
@@ -160,9 +160,8 @@ class Attention(torch.nn.Module):
         names = tuple(names)
         self.check_quantized(names)
         for name in names:
-            lin = getattr(self, name)
-            if not isinstance(lin, mx8.MX8Linear):
-                setattr(self, name, mx8.MX8Linear.from_linear(lin))
+            if not self.in_8_bits(name):
+                setattr(self, name, mx8.MX8Linear.from_linear(getattr(self, name)))
         return {name: getattr(self, name) for name in names}
 
     def check_quantized(self, names) -> None:
@@ -171,22 +170,30 @@ class Attention(torch.nn.Module):
             if name not in QUANTIZED:
                 raise ValueError(f"8 bits are for {QUANTIZED}, not for {name!r}")
             self._may_hold_8_bits(name)
-            lin = getattr(self, name)
-            if not isinstance(lin, mx8.MX8Linear) and lin.weight.shape[1] % 32:
-                raise ValueError(f"{name} takes {lin.weight.shape[1]} channels: 8 bits need whole blocks of 32")
+            k = 0 if self.in_8_bits(name) else getattr(self, name).weight.shape[1]
+            if k % 32:
+                raise ValueError(f"{name} takes {k} channels: 8 bits need whole blocks of 32")
 
     @property
     def takes_quantized(self) -> bool:
         """Whether both projections of the layer's input are in 8 bits: the rows in 8 bits (forward's x8) are used."""
-        return isinstance(self.wq_a, mx8.MX8Linear) and isinstance(self.wkv, mx8.MX8Linear)
+        held = self._modules
+        return isinstance(held.get("wq_a"), mx8.MX8Linear) and isinstance(held.get("wkv"), mx8.MX8Linear)
+
+    def in_8_bits(self, name: str) -> bool:
+        """Whether this projection is held in 8 bits. (Looked up where modules are kept: as an attribute each takes 1.5 us of
+        the host's time, in every layer of a token.)"""
+        return isinstance(self._modules.get(name), mx8.MX8Linear)
 
     def _input_projections(self, x, x8, banks, ids):
         """wq_a and wkv of the layer's input, in one launch where they are of one kind."""
-        if self.takes_quantized:
+        held = self._modules
+        a8, kv8 = isinstance(held.get("wq_a"), mx8.MX8Linear), isinstance(held.get("wkv"), mx8.MX8Linear)
+        if a8 and kv8:
             return mx8.linear_pair(self.wq_a, self.wkv, mx8.quantize(x) if x8 is None else x8)
-        if isinstance(self.wq_a, mx8.MX8Linear):
+        if a8:
             return self.wq_a(x), adapter_linear(self.wkv, x, banks.get("wkv"), ids)
-        if isinstance(self.wkv, mx8.MX8Linear):
+        if kv8:
             return adapter_linear(self.wq_a, x, banks.get("wq_a"), ids), self.wkv(x)
         # wq_a and wkv read the same rows: one launch at decode row counts
         return adapter_linear_pair(self.wq_a, self.wkv, x, banks.get("wq_a"), banks.get("wkv"), ids)
@@ -250,12 +257,14 @@ class Attention(torch.nn.Module):
 
         qa, kv_raw = self._input_projections(x, x8, banks, ids)
         # queries: q's rope tail (attention.py:117) is applied by the attention launch as it loads q
-        if isinstance(self.wq_b, mx8.MX8Linear) and only_the_norm(self.q_norm):
+        held = self._modules
+        b8 = isinstance(held.get("wq_b"), mx8.MX8Linear)
+        if b8 and only_the_norm(self.q_norm):
             # the normed rows themselves are for the indexer alone
             qr, q8 = mx8.norm_quantize(qa.contiguous(), self.q_norm.weight, self.q_norm.eps,
                                        rows=bool(self.ratio) and self.is_index_source)
             q = self.wq_b(q8)
-        elif isinstance(self.wq_b, mx8.MX8Linear):
+        elif b8:
             qr = self.q_norm(qa)
             q = self.wq_b(qr)
         else:
@@ -331,7 +340,7 @@ class Attention(torch.nn.Module):
         # wo_b at 33-64 rows: 128-row tiles over 4 contraction ranges and their reduce (24.4 + 4.5
         # us at 64 rows against 28.9 us for the library; the 40-layer token 5.748 against 5.78 ms)
         o = self._wo_a(o.view(bsz, n, -1), x.dtype)
-        if isinstance(self.wo_b, mx8.MX8Linear):
+        if isinstance(held.get("wo_b"), mx8.MX8Linear):
             return self.wo_b(o, residual=residual, out=residual)
         y = adapter_linear(self.wo_b, o, banks.get("wo_b"), ids, wide_only=True)
         return y if residual is None else residual.add_(y)

@@ -29,13 +29,17 @@ class RMSNorm(torch.nn.Module):
         return _abi.rmsnorm(x.contiguous(), self.weight, self.eps)
 
 
+_module = torch.nn.modules.module
+
+
 def only_the_norm(norm: torch.nn.Module) -> bool:
-    """Whether calling norm is RMSNorm's formula alone (no hooks, no forward of its own), so that a launch that holds more
-    than the norm may stand in for the module."""
-    mod = torch.nn.modules.module
-    return (getattr(type(norm), "forward", None) is RMSNorm.forward and "forward" not in norm.__dict__
-            and not (norm._forward_hooks or norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks
-                     or mod._global_forward_hooks or mod._global_forward_pre_hooks))
+    """Whether calling norm is RMSNorm's formula alone (no forward hooks, no forward of its own), so that a launch that holds
+    more than the norm may stand in for the module."""
+    if type(norm) is not RMSNorm:
+        return False
+    own = norm.__dict__
+    return not (own["_forward_hooks"] or own["_forward_pre_hooks"] or "forward" in own
+                or _module._global_forward_hooks or _module._global_forward_pre_hooks)
 
 
 # Decode row counts (at most 128 rows of bf16 activations): the projections that take

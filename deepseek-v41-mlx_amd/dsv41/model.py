@@ -112,7 +112,7 @@ class AttentionStack(torch.nn.Module):
                 h.add_(delta)
                 x = norm(h)
             given = () if x8 is None else (x8,)
-            if isinstance(getattr(attn, "wo_b", None), mx8.MX8Linear):
+            if isinstance(attn._modules.get("wo_b"), mx8.MX8Linear):
                 h, delta = attn(x, start_pos, cache, use, *given, residual=h), None    # added in wo_b's launch, in place
             else:
                 delta = attn(x, start_pos, cache, use, *given)
