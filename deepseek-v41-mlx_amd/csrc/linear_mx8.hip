@@ -1099,6 +1099,8 @@ extern "C" int dsv41_linear_mx8_plan(int32_t rows, int32_t k, int32_t n0, int32_
   DSV41_REQUIRE(plan, DSV41_E_ARG, "%s: null plan", what);
   DSV41_REQUIRE(rows > 0 && k > 0 && k % 32 == 0 && n0 > 0 && n1 >= 0, DSV41_E_SHAPE, "%s: rows %d, k %d, n %d + %d", what, rows,
                 k, n0, n1);
+  DSV41_REQUIRE(k <= (1 << 20) && n0 <= (1 << 24) && n1 <= (1 << 24) && rows <= (1 << 20), DSV41_E_SHAPE,
+                "%s: rows %d and k %d up to 2^20, n %d + %d up to 2^24", what, rows, k, n0, n1);
   Mx8Args a{};
   a.rows = rows, a.k = k, a.n[0] = n0, a.n[1] = n1;
   const Mx8Shape& s = shape_of(a);

@@ -1662,6 +1662,8 @@ class MX8Plan(typing.NamedTuple):
 
 def linear_mx8_plan(rows, k, n0, n1=0) -> MX8Plan:
     plan = (ctypes.c_int32 * 4)()
+    if rows > 1 << 20 or max(n0, n1) > 1 << 24 or k > 1 << 20:      # before they are cut to 32 bits
+        raise ValueError(f"dsv41_linear_mx8_plan: {rows} rows and {k} channels are up to 2^20, {n0} + {n1} outputs up to 2^24")
     _call("dsv41_linear_mx8_plan", rows, k, n0, n1, ctypes.addressof(plan))
     return MX8Plan(*plan)
 
