@@ -647,7 +647,8 @@ int dsv41_rmsnorm_mx8(void* x, const void* delta, const float* weight, void* y, 
  * an epilogue): x codes [rows, k] with scales [rows, k/32], w codes [n, k] with scales [n, k/32] (scale_rows 1) or
  * [ceil(n/32), k/32] (32); bias [n] float32 or NULL; act 0 none, 1 relu, 2 silu, 3 gelu (by erf); residual [rows, n] bf16 or
  * NULL, which may be y itself. Float32 accumulation over the matrix instruction's sums, which cut off of eight neighbouring
- * products what lies under 2^-13 of the largest; one rounding. Any n; rows and k at most 2^20. Scales may
+ * products what lies under 2^-13 of the largest; one rounding. n at most 2^24, rows and k at most 2^20; sizes whose tiles
+ * need 2^32 threads and more are refused (outputs of 500 GB, or 34 GB where one of a pair has fewer than 64 columns). Scales may
  * begin at any byte; the aligned words that hold their first and last bytes are read whole. */
 int dsv41_linear_mx8(const uint8_t* x, const uint8_t* x_scales, const uint8_t* w, const uint8_t* w_scales,
                      const float* bias, const void* residual, void* y, int32_t rows, int32_t k, int32_t n,
